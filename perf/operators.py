@@ -167,9 +167,10 @@ def prepare(case, seed):
         s["kv"] = amdc.Kv({"f16": amdc.TYPE_F16, "bf16": amdc.TYPE_BF16}[case["type"]], n_kv, hd, page, n_pages, s["k"].data_ptr(), s["v"].data_ptr(), n, pages.shape[1],
                           pages.data_ptr(), s["len"].data_ptr())
         s["qt"] = amdc.TYPE_F32 if qty == torch.float32 else s["kv"].type
-        if case["op"] == "decode":
+        if case["op"] != "append":
             # the workspace of a serving loop: made once, cleared once
-            s["ws"] = torch.zeros((amdc.attn_ws_bytes(s["kv"], n_q, case["T"]),), dtype=torch.uint8, device="cuda")
+            size = amdc.attn_decode_ws(s["kv"], n_q, case["T"]) if case["op"] == "decode" else amdc.attn_prefill_ws(s["kv"], n_q, rows)
+            s["ws"] = torch.zeros((size,), dtype=torch.uint8, device="cuda")
     return s
 
 
@@ -202,8 +203,8 @@ def _calls(s):
         amdc.attn_decode(s["kv"], s["q"].data_ptr(), s["y"].data_ptr(), s["qt"], n_q, case["T"], n_q * hd, n_q * hd, 1.0 / math.sqrt(hd), s["ws"].data_ptr(), s["ws"].numel(),
                          window=case["window"], stream=stream)
     else:
-        amdc.attn_prefill(s["kv"], s["q"].data_ptr(), s["y"].data_ptr(), s["qt"], n_q, s["rows"], n_q * hd, n_q * hd, 1.0 / math.sqrt(hd), cu=s["cu"].data_ptr(),
-                          window=case["window"], stream=stream)
+        amdc.attn_prefill(s["kv"], s["q"].data_ptr(), s["y"].data_ptr(), s["qt"], n_q, s["rows"], n_q * hd, n_q * hd, 1.0 / math.sqrt(hd), s["ws"].data_ptr(), s["ws"].numel(),
+                          cu=s["cu"].data_ptr(), window=case["window"], stream=stream)
     return s["y"]
 
 
