@@ -127,17 +127,28 @@ ABI = {
     "amdc_chain_check": (C.c_int, [_P]),
     "amdc_chain_destroy": (C.c_int, [_P]),
     "amdc_gemv_norm": (C.c_int, [C.c_int, _P, _P, _P, _U32, _U32, _P, _P, _P, _P, _P, C.c_float, _P]),
+    "amdc_kv_bytes": (C.c_size_t, [C.c_int, _U32, _U32, _U32, _U32]),
+    "amdc_kv_check": (C.c_int, []),
+    "amdc_kv_append": (C.c_int, [_P, _P, _P, _P, _P, C.c_int, _U32, _U32, _U32, _U32, _U32, _U32, _P, _P, _U32, C.c_int, _P]),
     "amdc_chain_record_begin": (C.c_int, [_P]),
     "amdc_chain_record_end": (C.c_int, [_P, C.c_int, C.POINTER(_P)]),
 }
 
 CHAIN_QUANT, CHAIN_GEMV, CHAIN_GEMV_X, CHAIN_RMSNORM_Q8, CHAIN_SWIGLU_Q8 = 0, 1, 2, 3, 4
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+ROPE_NONE, ROPE_PAIRS, ROPE_HALVES = 0, 1, 2
 
 
 class ChainOp(C.Structure):
     """amdc_chain_op of include/amdc_q4.h."""
     _fields_ = [("type", C.c_int), ("kind", C.c_int), ("sync", C.c_int), ("rows", _U32), ("nb", _U32),
                 ("w", _P), ("x", _P), ("q", _P), ("xq", _P), ("y", _P), ("bias", _P), ("res", _P), ("eps", C.c_float)]
+
+
+class KvStruct(C.Structure):
+    """amdc_kv of include/amdc_q4.h."""
+    _fields_ = [("type", C.c_int), ("n_kv", _U32), ("hd", _U32), ("page", _U32), ("n_pages", _U32), ("k", _P), ("v", _P),
+                ("n_seq", _U32), ("max_pages", _U32), ("pages", _P), ("len", _P)]
 
 
 class AmdcError(RuntimeError):
@@ -445,6 +456,35 @@ def gemv_norm(kind, w, xq, y, rows, nb, nw, ny, eps, nq=None, bias=None, res=Non
 def swiglu_q8(a, b, n, q=None, T=1, as_=0, qs=0, stream=None):
     """amdc_swiglu_q8: a = silu(a) b in place and, when q is given, its Q8 copy."""
     _check(lib().amdc_swiglu_q8(_p(a), _p(b), n, _p(q), T, as_, qs, stream))
+
+
+def kv_bytes(type, n_kv, hd, page, n_pages):
+    """Bytes of each of a paged cache's two pools."""
+    n = lib().amdc_kv_bytes(type, n_kv, hd, page, n_pages)
+    if not n:
+        raise AmdcError(f"type {type}: {n_kv} heads of {hd}, {n_pages} pages of {page} are not supported")
+    return n
+
+
+class Kv:
+    """amdc_kv: a layer's paged cache (the pools k and v, kv_bytes() each) and the batch it is used with (the page table
+    `pages`, n_seq rows of max_pages, and the lengths `len`, all in device memory)."""
+
+    def __init__(self, type, n_kv, hd, page, n_pages, k, v, n_seq, max_pages, pages, len):
+        self.type, self.n_kv, self.hd, self.page, self.n_pages, self.n_seq, self.max_pages = type, n_kv, hd, page, n_pages, n_seq, max_pages
+        self.held = (k, v, pages, len)  # device buffers live as long as this
+        self.s = KvStruct(type, n_kv, hd, page, n_pages, _p(k), _p(v), n_seq, max_pages, _p(pages), _p(len))
+        self.ref = C.byref(self.s)
+
+
+def kv_check():
+    """Waits for the device; raises if a cache operator since the last check met a page, a length or a row outside its bounds."""
+    _check(lib().amdc_kv_check())
+
+
+def kv_append(kv, k, v, q, qo, qt, n_q, T, ks, vs, qs=0, qos=0, cu=None, freq=None, n_rot=0, rope=ROPE_NONE, stream=None):
+    """amdc_kv_append: the new rows' keys (rotated) and values into the cache, and with q the rotated queries to qo."""
+    _check(lib().amdc_kv_append(kv.ref, _p(k), _p(v), _p(q), _p(qo), qt, n_q, T, ks, vs, qs, qos, _p(cu), _p(freq), n_rot, rope, stream))
 
 
 def chain_quant(x, q, nb, sync=True):

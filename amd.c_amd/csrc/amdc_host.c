@@ -288,7 +288,8 @@ enum {
   K_SWIGLU_V,
   K_RMSNORM_R,
   K_GEMVS8, /* amdc_gemv_q8_0_s1, _s2, _xs1, (none), amdc_gemv_q6_k_s1, (none), _xs1, (none), then _s1l, _s2l, _xs1l, _xs2l, ... */
-  K_N = K_GEMVS8 + 15
+  K_APPEND = K_GEMVS8 + 15, /* amdc_kv_append_f16, _bf16 */
+  K_N = K_APPEND + 2
 };
 #define KN(s) "amdc_" s
 #define GW(s) "amdc_gemmw_" s
@@ -319,7 +320,7 @@ static const char *const kname[K_N] = {
     KN("quant_q8_v"), KN("swiglu_q8_v"), KN("rmsnorm_q8_r"),
     KN("gemv_q8_0_s1"), KN("gemv_q8_0_s2"), KN("gemv_q8_0_xs1"), KN("gemv_q8_0_xs1"), KN("gemv_q6_k_s1"), KN("gemv_q6_k_s1"), KN("gemv_q6_k_xs1"),
     KN("gemv_q6_k_xs1"), KN("gemv_q8_0_s1l"), KN("gemv_q8_0_s2l"), KN("gemv_q8_0_xs1l"), KN("gemv_q8_0_xs2l"), KN("gemv_q6_k_s1l"),
-    KN("gemv_q6_k_s1l"), KN("gemv_q6_k_xs1l")};
+    KN("gemv_q6_k_s1l"), KN("gemv_q6_k_xs1l"), KN("kv_append_f16"), KN("kv_append_bf16")};
 
 static hipModule_t g_mod;
 static hipFunction_t g_k[K_N];
@@ -352,6 +353,7 @@ static unsigned g_ws_old_n;
  * amdc_op_gemv_noalloc (g_ws_fixed set) every workspace request is served from it, and a request
  * larger than it is an error; otherwise it is unused. */
 static void *g_scratch;
+static u32 *g_kv_bad;    /* the kernels' kv_bad_flag (device address) */
 static u32 *g_split_cnt; /* the kernels' split_count array (device address) */
 static size_t g_scratch_bytes;
 static int g_ws_fixed;
@@ -453,6 +455,9 @@ int amdc_open(const char *hsaco) {
     HIPCALL(H.ModuleGetGlobal((void **)&g_norm_cnt, &cb, g_mod, "norm_count"));
     if (!g_norm_cnt || cb < sizeof(u32)) return fail(AMDC_EHIP, "amdc_kernels.hsaco: no norm_count counter");
     HIPCALL(H.Memset(g_norm_cnt, 0, cb));
+    HIPCALL(H.ModuleGetGlobal((void **)&g_kv_bad, &cb, g_mod, "kv_bad_flag"));
+    if (!g_kv_bad || cb < sizeof(u32)) return fail(AMDC_EHIP, "amdc_kernels.hsaco: no kv_bad_flag");
+    HIPCALL(H.Memset(g_kv_bad, 0, sizeof(u32)));
   }
   HIPCALL(H.DeviceGetAttribute(&g_cus, hipDeviceAttributeMultiprocessorCount, 0));
   if (t_lanes < 0) t_lanes = envi("AMDC_GEMV_L", 0);
@@ -1583,6 +1588,100 @@ int amdc_block_dots(int kind, const void *w, const uint8_t *xq, int32_t *out, ui
   void *args[] = {&w, &xq, &out, &rows, &nb};
   const int k = kind == AMDC_KIND_Q4_K ? K_DOTS_Q4K : kind == AMDC_KIND_Q8_0 ? K_DOTS_Q8 : kind == AMDC_KIND_Q6_K ? K_DOTS_Q6K : K_DOTS_Q4;
   return launch(k, (unsigned)((n + 255u) / 256u), 1, 0, stream, args);
+}
+
+/* ---------------------------------------------------------------- attention over a paged cache */
+
+size_t amdc_kv_bytes(int type, uint32_t n_kv, uint32_t hd, uint32_t page, uint32_t n_pages) {
+  if ((type != AMDC_TYPE_F16 && type != AMDC_TYPE_BF16) || !n_kv || n_kv > 1024u || (hd != 64u && hd != 128u && hd != 256u) || page < 16u ||
+      page > 65536u || (page & (page - 1u)) || !n_pages || n_pages > 0x7FFFFFFFu)
+    return 0;
+  const u64 row = (u64)n_kv * hd * page * 2u;
+  if (n_pages > UINT64_MAX / row) return 0;
+  return (size_t)(row * n_pages);
+}
+
+static u32 log2u(u32 v) { return 31u - (u32)__builtin_clz(v); }
+
+/* The checks that every cache operator shares; the cache as the kernels take it. rows: the rows of the call. */
+static int check_kv(const char *op, const amdc_kv *kv, u32 n_q, u32 T, const int32_t *cu, amdc_kv_dev *d, u32 *rows) {
+  if (!kv) return fail(AMDC_EINVAL, "%s: kv is NULL", op);
+  if (!amdc_kv_bytes(kv->type, kv->n_kv, kv->hd, kv->page, kv->n_pages))
+    return fail(AMDC_EINVAL,
+                "%s: a cache of type %d, %u heads of %u, %u pages of %u (type F16 or BF16, 1 to 1024 heads of 64, 128 or 256, pages of a "
+                "power of two of 16 to 65536 positions)",
+                op, kv->type, kv->n_kv, kv->hd, kv->n_pages, kv->page);
+  if (!kv->k || !kv->v || !kv->pages || !kv->len) return fail(AMDC_EINVAL, "%s: null pointer in kv", op);
+  if (!aligned16(kv->k) || !aligned16(kv->v)) return fail(AMDC_EINVAL, "%s: the pools k and v must be 16-byte aligned", op);
+  if (!vec_rows(kv->pages, 0, 4u) || !vec_rows(kv->len, 0, 4u) || !vec_rows(cu, 0, 4u)) return fail(AMDC_EINVAL, "%s: pages, len and cu must be 4-byte aligned", op);
+  if (!kv->n_seq || !kv->max_pages || kv->n_seq > (1u << 20) || (u64)kv->max_pages * kv->page >= (1ull << 31))
+    return fail(AMDC_EINVAL, "%s: %u sequences of up to %u pages of %u (1 to 2^20 sequences, under 2^31 positions)", op, kv->n_seq, kv->max_pages, kv->page);
+  if (!n_q || n_q % kv->n_kv || n_q / kv->n_kv > 128u)
+    return fail(AMDC_EINVAL, "%s: %u query heads on %u key / value heads (a multiple, at most 128 each)", op, n_q, kv->n_kv);
+  const u64 r = cu ? T : (u64)kv->n_seq * T;
+  if (!T || r > (1u << 22)) return fail(AMDC_EINVAL, "%s: T %u (1 to 2^22 rows in all)", op, T);
+  *rows = (u32)r;
+  *d = (amdc_kv_dev){kv->k, kv->v, kv->pages, kv->len, g_kv_bad, kv->n_kv, kv->n_pages, kv->n_seq, kv->max_pages, log2u(kv->page), kv->max_pages * kv->page};
+  return AMDC_OK;
+}
+
+int amdc_kv_check(void) {
+  NEED_OPEN();
+  u32 bad = 0;
+  HIPCALL(H.DeviceSynchronize());
+  HIPCALL(H.Memcpy(&bad, g_kv_bad, sizeof bad, hipMemcpyDeviceToHost));
+  if (!bad) return AMDC_OK;
+  HIPCALL(H.Memset(g_kv_bad, 0, sizeof bad));
+  return fail(AMDC_EINVAL, "kv_check: a cache operator met %s",
+              bad == AMDC_BAD_PAGE ? "a page outside the pool"
+              : bad == AMDC_BAD_LEN ? "a length over max_pages * page, or under the sequence's number of new tokens"
+                                    : "rows outside 0 .. T (cu)");
+}
+
+/* the arguments of amdc_kv_append_*: AppendArgs of amdc_attn.h */
+typedef struct {
+  const float *k, *v, *q;
+  void *qo;
+  const int32_t *cu;
+  const float *freq;
+  u32 qt, n_q, T, ks, vs, qs, qos, n_rot, rope, lghd, rows, gq, gv, upb, vec;
+} append_args;
+
+int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const float *q, void *qo, int qt, uint32_t n_q, uint32_t T, uint32_t ks,
+                   uint32_t vs, uint32_t qs, uint32_t qos, const int32_t *cu, const float *freq, uint32_t n_rot, int rope, void *stream) {
+  NEED_OPEN();
+  amdc_kv_dev d;
+  u32 rows = 0;
+  if (!q && kv) n_q = kv->n_kv; /* not used */
+  int rc = check_kv("kv_append", kv, n_q, T, cu, &d, &rows);
+  if (rc) return rc;
+  const u32 wk = kv->n_kv * kv->hd, wq = n_q * kv->hd;
+  if (!k || !v) return fail(AMDC_EINVAL, "kv_append: null pointer (k, v)");
+  if (rope != AMDC_ROPE_NONE && rope != AMDC_ROPE_PAIRS && rope != AMDC_ROPE_HALVES) return fail(AMDC_EINVAL, "kv_append: rope %d", rope);
+  if (rope != AMDC_ROPE_NONE && (!freq || !n_rot || n_rot % 2u || n_rot > kv->hd))
+    return fail(AMDC_EINVAL, "kv_append: n_rot %u of heads of %u (even, 2 to hd), freq %s", n_rot, kv->hd, freq ? "given" : "NULL");
+  if (rows > 1u && (ks < wk || vs < wk)) return fail(AMDC_EINVAL, "kv_append: strides ks %u, vs %u under a row's %u values", ks, vs, wk);
+  if (!vec_rows(k, 0, 4u) || !vec_rows(v, 0, 4u) || !vec_rows(freq, 0, 4u)) return fail(AMDC_EINVAL, "kv_append: k, v and freq must be 4-byte aligned");
+  if (q) {
+    if (!qo) return fail(AMDC_EINVAL, "kv_append: q without qo");
+    if (qt != AMDC_TYPE_F32 && qt != kv->type) return fail(AMDC_EINVAL, "kv_append: qo of type %d (F32 or the cache's)", qt);
+    if (rows > 1u && (qs < wq || qos < wq)) return fail(AMDC_EINVAL, "kv_append: strides qs %u, qos %u under a row's %u values", qs, qos, wq);
+    if (!vec_rows(q, 0, 4u) || !vec_rows(qo, 0, qt == AMDC_TYPE_F32 ? 4u : 2u)) return fail(AMDC_EINVAL, "kv_append: q and qo must be aligned to their types");
+    if ((const void *)q == qo && (qt != AMDC_TYPE_F32 || (rows > 1u && qs != qos)))
+      return fail(AMDC_EINVAL, "kv_append: in place (qo = q) needs type F32 and qos = qs");
+  }
+  const u32 lghd = log2u(kv->hd), hpi = 2048u / kv->hd, its = ((q ? n_q : 0u) + kv->n_kv + hpi - 1u) / hpi;
+  const u32 upb = (T + 14u) / 8u, vu = cu ? rows / 8u + 2u * kv->n_seq : kv->n_seq * upb, vn = (wk + 255u) / 256u;
+  /* a row's heads and a group's values over several workgroups until there are two of each to a CU */
+  const u32 want = 2u * (g_cus > 0 ? (u32)g_cus : 256u), gq0 = (want + rows - 1u) / rows, gv0 = (want + vu - 1u) / vu;
+  const u32 gq = gq0 < its ? gq0 : its, gv = gv0 < vn ? gv0 : vn;
+  if ((u64)rows * gq + (u64)vu * gv >= (1u << 24)) return fail(AMDC_EINVAL, "kv_append: %u rows of %u sequences are too many for one call", rows, kv->n_seq);
+  /* which rows are 16-byte aligned: queries, keys, rotated queries */
+  const u32 vec = (vec_rows(q, rows > 1u ? 4u * qs : 0u, 16u) ? 1u : 0u) | (vec_rows(k, rows > 1u ? 4u * ks : 0u, 16u) ? 2u : 0u) |
+                  (vec_rows(qo, rows > 1u ? (qt == AMDC_TYPE_F32 ? 4u : 2u) * qos : 0u, 16u) ? 4u : 0u);
+  append_args a = {k, v, q, qo, cu, freq, (u32)qt, n_q, T, ks, vs, qs, qos, rope ? n_rot : 0u, (u32)rope, lghd, rows, gq, gv, upb, vec};
+  void *args[] = {&d, &a};
+  return launch(K_APPEND + (kv->type == AMDC_TYPE_BF16), rows * gq + vu * gv, 1, 0, stream, args);
 }
 
 int amdc_probe_read(const void *src, size_t nbytes, void *scratch, uint32_t grid, void *stream) {

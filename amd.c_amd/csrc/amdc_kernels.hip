@@ -4133,3 +4133,8 @@ extern "C" __global__ __launch_bounds__(256, 2) void amdc_gemv_q6_k_v16(const ui
                                                                     float *part, u32 tps, u32 *cnt) {
   gemv8_q6k_body<2, 1>(W, xq, y, rows, nb, bias, res, T, xs, ys, rs, part, tps, cnt);
 }
+
+// The error flag of the cache and attention kernels (amdc_kv_check), 0 while all is well
+__device__ __align__(256) u32 kv_bad_flag[64];
+
+#include "amdc_attn.h"

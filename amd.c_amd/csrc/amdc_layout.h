@@ -101,4 +101,13 @@ AMDC_INLINE uint64_t amdc_row_bytes_k(int kind, uint32_t nb) {
   return kind == AMDC_Q8_0 ? amdc_q8_row_bytes(nb) : kind == AMDC_Q6_K ? amdc_q6k_row_bytes(nb) : amdc_row_bytes(nb);
 }
 
+/* The paged cache as the kernels take it (amdc_kv of amdc_q4.h, checked): by value, 8-byte fields first. */
+typedef struct {
+  uint8_t *k, *v;
+  const int32_t *pages, *len;
+  uint32_t *bad; /* the device flag of amdc_kv_check: an AMDC_BAD_* */
+  uint32_t n_kv, n_pages, n_seq, max_pages, lgp /* log2(page) */, cap /* max_pages << lgp */;
+} amdc_kv_dev;
+enum { AMDC_BAD_PAGE = 1, AMDC_BAD_LEN = 2, AMDC_BAD_ROWS = 3 };
+
 #endif

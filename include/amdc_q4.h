@@ -273,6 +273,63 @@ int amdc_op_gemv_noalloc(int kind, const void *w, const uint8_t *xq, float *y, u
  * + h] = sum (q - 32) a over half h (ie_q6k_dots, :384). */
 int amdc_block_dots(int kind, const void *w, const uint8_t *xq, int32_t *out, uint32_t rows, uint32_t nb, void *stream);
 
+/* ---------------------------------------------------------------- attention over a paged cache */
+
+/* What stands between a layer's qkv matrix and its output matrix: the rotation and the cache of
+ * keys and values (the reference's OP_ROPE and OP_KV), and the attention over it (OP_ATTN); the
+ * float type is the GEMVs' f32, or a 16-bit one. */
+enum { AMDC_TYPE_F32 = 0, AMDC_TYPE_F16 = 1, AMDC_TYPE_BF16 = 2 };
+
+/* A layer's paged cache and the batch that it is used with; the pointers are device memory, so that
+ * a captured graph follows what the host writes there. A page holds `page` positions (a power of two,
+ * 16 to 65536) of all n_kv heads of hd (64, 128 or 256) values; k and v are pools of n_pages pages,
+ * 16-byte aligned, amdc_kv_bytes() each, in the order the matrix units read:
+ *   k  [n_pages][n_kv][page / 16][hd / 8][16][8]: position 16 a + c, value 8 b + e at [a][b][c][e]
+ *   v  [n_pages][n_kv][page / 8][hd][8]:          position 8 a + e, value d        at [a][d][e]
+ * Position p of sequence b is at position p % page of page pages[b * max_pages + p / page]; sequences
+ * may share pages that no call writes. len[b] is the number of positions of sequence b with the
+ * new tokens of the call, at most max_pages * page; 0: the sequence takes no part (nothing is
+ * appended, its rows of attention are 0). Nothing behind position len[b] - 1 is used: its values may be
+ * anything, NaN too.
+ *
+ * New tokens are rows: sequence b has m_b of them, its positions len[b] - m_b .. len[b] - 1. With cu NULL
+ * every m_b is T, the rows b T .. b T + T - 1; with cu (n_seq + 1 device integers that do not decrease, the
+ * last at most T) the rows are cu[b] .. cu[b + 1] - 1 and T is the number of rows there is room for; rows that
+ * belong to no sequence are left as they are.
+ *
+ * What only the device sees is checked there: a page outside the pool, a length over
+ * max_pages * page or under the sequence's number of new tokens, rows outside 0 .. T. Such an entry is never
+ * followed: append leaves out the positions concerned, attention gives NaN in the sequence's rows, and
+ * amdc_kv_check() reports it. */
+typedef struct {
+  int type; /* AMDC_TYPE_F16 or AMDC_TYPE_BF16 */
+  uint32_t n_kv, hd, page, n_pages;
+  void *k, *v;
+  uint32_t n_seq, max_pages;
+  const int32_t *pages, *len;
+} amdc_kv;
+
+/* Bytes of each of the two pools; 0 for a geometry that is not supported. */
+size_t amdc_kv_bytes(int type, uint32_t n_kv, uint32_t hd, uint32_t page, uint32_t n_pages);
+/* Synchronizes the device; AMDC_EINVAL and a message if a call since the last check met a page, a length
+ * or a row outside its bounds (see amdc_kv). */
+int amdc_kv_check(void);
+
+/* Appends the new tokens' keys and values to the cache, the keys rotated by their positions, and with q
+ * not NULL writes the rotated queries to qo (type qt: AMDC_TYPE_F32 or the cache's). Rows of k, v (n_kv
+ * heads) and q, qo (n_q heads, a multiple of n_kv) are ks, vs, qs, qos values apart: the qkv matrix's output rows
+ * can be passed as they are. qo may be q itself where the type and the stride are the same.
+ * The rotation turns n_rot / 2 pairs of values of a head (n_rot even, at most hd; the values behind n_rot are
+ * kept) by the angles p freq[i] (freq: n_rot / 2 device floats; the product and its reduction in 64 bits):
+ *   AMDC_ROPE_PAIRS   the pair i is the values 2 i, 2 i + 1
+ *   AMDC_ROPE_HALVES  the pair i is the values i, i + n_rot / 2
+ *   AMDC_ROPE_NONE    no rotation (freq and n_rot are not used)
+ * (a, b) -> (a cos - b sin, a sin + b cos) in f32, rounded once to the result's type. Two calls, or two
+ * sequences of a call, that write the same position race. */
+enum { AMDC_ROPE_NONE = 0, AMDC_ROPE_PAIRS = 1, AMDC_ROPE_HALVES = 2 };
+int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const float *q, void *qo, int qt, uint32_t n_q, uint32_t T, uint32_t ks,
+                   uint32_t vs, uint32_t qs, uint32_t qos, const int32_t *cu, const float *freq, uint32_t n_rot, int rope, void *stream);
+
 /* Tuning knobs (0 = automatic): lanes per row of the GEMV (4..64, power of
  * two); the decode kernel (0: the pipelined one; 1 or 2: the multi-vector
  * kernel with 1 or 2 super-groups of loads per step); workgroups of a GEMV
