@@ -130,6 +130,8 @@ ABI = {
     "amdc_kv_bytes": (C.c_size_t, [C.c_int, _U32, _U32, _U32, _U32]),
     "amdc_kv_check": (C.c_int, []),
     "amdc_kv_append": (C.c_int, [_P, _P, _P, _P, _P, C.c_int, _U32, _U32, _U32, _U32, _U32, _U32, _P, _P, _U32, C.c_int, _P]),
+    "amdc_attn_decode_ws": (C.c_size_t, [_P, _U32, _U32]),
+    "amdc_attn_decode": (C.c_int, [_P, _P, _P, C.c_int, _U32, _U32, _U32, _U32, C.c_float, _U32, _P, _U32, _P, C.c_size_t, _P]),
     "amdc_chain_record_begin": (C.c_int, [_P]),
     "amdc_chain_record_end": (C.c_int, [_P, C.c_int, C.POINTER(_P)]),
 }
@@ -485,6 +487,19 @@ def kv_check():
 def kv_append(kv, k, v, q, qo, qt, n_q, T, ks, vs, qs=0, qos=0, cu=None, freq=None, n_rot=0, rope=ROPE_NONE, stream=None):
     """amdc_kv_append: the new rows' keys (rotated) and values into the cache, and with q the rotated queries to qo."""
     _check(lib().amdc_kv_append(kv.ref, _p(k), _p(v), _p(q), _p(qo), qt, n_q, T, ks, vs, qs, qos, _p(cu), _p(freq), n_rot, rope, stream))
+
+
+def attn_decode_ws(kv, n_q, T):
+    """Bytes of attn_decode's workspace (device memory, cleared to 0 once)."""
+    n = lib().amdc_attn_decode_ws(kv.ref, n_q, T)
+    if not n:
+        raise AmdcError(f"attn_decode: {n_q} query heads, {T} tokens a sequence: not supported")
+    return n
+
+
+def attn_decode(kv, q, y, type, n_q, T, qs, ys, scale, ws, ws_bytes, window=0, q8=None, q8s=0, stream=None):
+    """amdc_attn_decode: the attention of the T newest tokens of every sequence over its cached positions."""
+    _check(lib().amdc_attn_decode(kv.ref, _p(q), _p(y), type, n_q, T, qs, ys, scale, window, _p(q8), q8s, _p(ws), ws_bytes, stream))
 
 
 def chain_quant(x, q, nb, sync=True):

@@ -2,6 +2,8 @@
 // layout); part of amdc_kernels.hip's translation unit.
 //
 //   amdc_kv_append_{f16,bf16}   rotation, keys and values into the cache, rotated queries
+//   amdc_attn_dec_h{64,128,256}_{f16,f16_f32,bf16,bf16_f32}
+//                               attention of a few new tokens per sequence
 
 // ------------------------------------------------------------------ helpers
 
@@ -246,3 +248,472 @@ __device__ __forceinline__ void append_body(const amdc_kv_dev &kv, const AppendA
 APPEND_KERNEL(f16, false)
 APPEND_KERNEL(bf16, true)
 #undef APPEND_KERNEL
+
+// ------------------------------------------------------------------ attention of a few new tokens
+
+template <bool BF>
+__device__ __forceinline__ v4f mfma16(u32x4 a, u32x4 b, v4f c) {
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// x in NP 16-bit parts whose sum is x to 11 NP (f16) or 8 NP (bf16) bits: each part rounds what the parts before it left
+template <bool BF, int NP>
+__device__ __forceinline__ void split8(float (&x)[8], u32x4 (&w)[NP]) {
+#pragma unroll
+  for (int p = 0; p < NP; p++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const u32 v = pack2<BF>(x[2 * i], x[2 * i + 1]);
+      w[p][i] = v;
+      if (p + 1 < NP) x[2 * i] -= lo16<BF>(v), x[2 * i + 1] -= hi16<BF>(v);
+    }
+}
+
+// Eight query values: f32 (as given), or 16 bits widened
+template <bool BF, bool F32>
+__device__ __forceinline__ void load_q8(const void *q, u64 i, bool vec, float (&x)[8]) {
+  if constexpr (F32) load8((const float *)q + i, vec, x);
+  else {
+    u32x4 w;
+    const unsigned short *p = (const unsigned short *)q + i;
+    if (vec) w = *(const u32x4 *)p;
+    else
+#pragma unroll
+      for (int k = 0; k < 4; k++) w[k] = (u32)p[2 * k] | (u32)p[2 * k + 1] << 16;
+#pragma unroll
+    for (int k = 0; k < 4; k++) x[2 * k] = lo16<BF>(w[k]), x[2 * k + 1] = hi16<BF>(w[k]);
+  }
+}
+
+// Four results of a row: to y, and their Q8 copy (eight lanes to a block of 32, all or none of them here)
+template <bool BF, bool F32>
+__device__ __forceinline__ void store_y4(void *y, u64 i, v4f v, bool vec) {
+  if constexpr (F32) {
+    float *d = (float *)y + i;
+    if (vec) *(v4f *)d = v;
+    else
+#pragma unroll
+      for (int k = 0; k < 4; k++) d[k] = v[k];
+  } else {
+    const u32x2 w = {pack2<BF>(v.x, v.y), pack2<BF>(v.z, v.w)};
+    unsigned short *d = (unsigned short *)y + i;
+    if (vec) *(u32x2 *)d = w;
+    else
+#pragma unroll
+      for (int k = 0; k < 4; k++) d[k] = (unsigned short)(w[k >> 1] >> (16 * (k & 1)));
+  }
+}
+
+// Are all of a wave's values finite?
+__device__ __forceinline__ bool wave_finite(v4f c) {
+  const float z = (c.x - c.x) + (c.y - c.y) + (c.z - c.z) + (c.w - c.w); // NaN where one is not
+  return __ballot(!(z == 0.0f)) == 0ull;
+}
+
+// the 16-bit halves of w (positions p, p + 1, ..) that lie outside [lo, hi), as 0
+__device__ __forceinline__ u32x4 seen16(u32x4 w, u32 p, u32 lo, u32 hi) {
+#pragma unroll
+  for (u32 i = 0; i < 4u; i++) {
+    const u32 a = p + 2u * i, b = a + 1u;
+    w[i] &= (a >= lo && a < hi ? 0xFFFFu : 0u) | (b >= lo && b < hi ? 0xFFFF0000u : 0u);
+  }
+  return w;
+}
+
+struct AttnArgs {
+  const void *q;
+  void *y;
+  const int *cu;
+  uint8_t *q8, *ws;
+  float c; // scale log2(e)
+  u32 n_q, G, T, qs, ys, window, q8s, U, vec, ncb;
+};
+
+#define ATTN_CNT 65536u // bytes of counters at the start of the workspace
+#define DEC_FAN 8u      // partial results joined at once
+#define DEC_CMIN 4u     // the shortest chunk, in steps of 32 positions
+
+// T rows of G = n_q / n_kv heads of a sequence read the same keys and values. A workgroup takes 16 of these T G
+// columns (blocks cb of them), one key / value head and one chunk of the sequence's positions; its four waves take
+// the chunk's steps of 32 positions in turn, each with a softmax of its own (maximum m, sum l, weighted sum O), joined at
+// the end in the LDS.
+//
+// Reading the cache bounds it (16 columns cost 2 x 16 x hd flops per 4 hd bytes, 1 / 40 of the matrix rate at the HBM's), so
+// the layout gives every load of a wave whole lines, straight into the matrix units' operands, no LDS between:
+//   S^T = K Q^T  (16x16x32: rows are positions, columns are the query rows): row r of tile t (of two) is position
+//                8 (r / 4) + 4 t + r % 4 of the step, so that a lane's eight scores are the eight positions 8 g .. 8 g + 7
+//                (g = lane / 16) of its column
+//   O^T = V^T P^T: those eight, as 16-bit weights, are the lane's B operand as they stand; the cache keeps a value's eight
+//                positions together, which is the A operand.
+// In f32, queries and weights go in as sums of 16-bit parts (f16: two, 22 bits; bf16: three, 24), one product each, into the
+// same sums; f16 queries are first scaled by a power of two that brings a row's largest value to 2^10 (no overflow, and the second part
+// stays a normal number). f16 weights carry 2^8 (their least normal is 2^-14), the sum l the same factor.
+// The maximum is raised, and O rescaled, only where a score passes it by 6 (weights stay under 2^14): the join needs a common
+// reference, not the largest score.
+//
+// Chunks: the device divides all sequences' steps by the number of units U that the host wants of a head (workgroups per
+// head to fill the CUs), so that chunks are about equal however different the lengths are; every wave finds its unit by a scan over the
+// lengths. A sequence's chunks leave partial results (O, m, l) in the workspace, agent-coherent as split_put's; of
+// every DEC_FAN neighbours the last to arrive joins them, in their order, up a tree, so the result does not depend on
+// who was last.
+//
+// A step that holds positions which not every column sees is multiplied into sums of its own: where these come out finite they are
+// added, as weights of 0 are right; if not (0 times an infinity or a NaN that a column must not see), column by column with the
+// unseen values as 0.
+template <int HD, bool BF, bool F32>
+__device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &a) {
+  constexpr int NP = F32 ? (BF ? 3 : 2) : 1, KS = HD / 32, DT = HD / 16;
+  constexpr u32 NW = 4u, OS = HD + 4u, QD = HD / 4u; // floats between columns of O in the LDS; quads of a row
+  constexpr float BIAS = BF ? 0.0f : 8.0f, RAISE = 6.0f, NINF = -__builtin_inff();
+  constexpr u32 SMQ = NP * HD * 32u, SMO = NW * 16u * OS * 4u, SMB = SMQ > SMO ? SMQ : SMO;
+  __shared__ __attribute__((aligned(16))) uint8_t sm[SMB];
+  __shared__ float s_cq[16], s_m[NW][16], s_l[NW][16], s_L[16], s_M[16];
+  __shared__ u32 s_bad, s_last;
+  const u32 tid = threadIdx.x, lane = tid & 63u, wv = (u32)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), n = lane & 15u, g4 = lane >> 4;
+  u32 x = blockIdx.x;
+  const u32 cb = x % a.ncb;
+  x /= a.ncb;
+  const u32 h = x % kv.n_kv, u = x / kv.n_kv, T = a.T, G = a.G;
+
+  // the unit: sequence b, its chunk ci of nu, of C steps
+  auto trust = [&](int L) { return (u32)L - 1u < kv.cap && (u32)L >= T; }; // 1 .. cap, the new rows among them
+  auto first = [&](u32 L) { return a.window && L - T + 1u > a.window ? L - T + 1u - a.window : 0u; }; // the first position any row sees
+  auto steps = [&](u32 i) {
+    const int L = kv.len[i];
+    return trust(L) ? cdiv((u32)L, 32u) - first((u32)L) / 32u : 1u;
+  };
+  u32 b = 0u, ci = 0u, nu = 1u, slot0 = 0u, C;
+  {
+    u64 total = 0u;
+    for (u32 i = lane; i < kv.n_seq; i += 64u) total += steps(i);
+    if (kv.n_seq > 1u)
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+    else total = __shfl(total, 0);
+    const u64 c = (total + a.U - 1u) / a.U;
+    C = c < DEC_CMIN ? DEC_CMIN : (u32)(c < (1u << 27) ? c : (1u << 27));
+    u32 units = 0u, slots = 0u;
+    bool found = false;
+    for (u32 i0 = 0u; i0 < kv.n_seq && !found; i0 += 64u) {
+      const u32 mine = i0 + lane < kv.n_seq ? cdiv(steps(i0 + lane), C) : 0u;
+      u32 au = mine, as = mine > 1u ? mine : 0u; // inclusive sums: units, and partial results (of sequences of several)
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const u32 pu = (u32)__shfl_up((int)au, o), ps = (u32)__shfl_up((int)as, o);
+        if ((int)lane >= o) au += pu, as += ps;
+      }
+      const u64 hit = __ballot(units + au > u);
+      if (hit) {
+        const int f = __builtin_ctzll(hit);
+        b = i0 + (u32)f;
+        nu = (u32)__shfl((int)mine, f);
+        ci = u - (units + (u32)__shfl((int)au, f) - nu);
+        slot0 = slots + (u32)__shfl((int)as, f) - (nu > 1u ? nu : 0u);
+        found = true;
+      }
+      units += (u32)__shfl((int)au, 63), slots += (u32)__shfl((int)as, 63);
+    }
+    if (!found) return;
+  }
+  b = (u32)__builtin_amdgcn_readfirstlane((int)b), ci = (u32)__builtin_amdgcn_readfirstlane((int)ci);
+  nu = (u32)__builtin_amdgcn_readfirstlane((int)nu), slot0 = (u32)__builtin_amdgcn_readfirstlane((int)slot0);
+
+  const u32 r0 = 16u * cb, nr = T * G - r0 < 16u ? T * G - r0 : 16u; // the block's columns
+  const u32 nbq = a.n_q * HD / 32u;
+  // row r of the block: its query row and head
+  auto at = [&](u32 r, u32 &row, u32 &head) {
+    const u32 t = (r0 + r) / G;
+    row = b * T + t, head = h * G + (r0 + r) - t * G;
+  };
+  auto put = [&](u32 r, u32 d4, v4f v) {
+    u32 row, head;
+    at(r, row, head);
+    if (a.y) store_y4<BF, F32>(a.y, (u64)row * a.ys + (u64)head * HD + 4u * d4, v, a.vec & 2u);
+    if (a.q8) quant_vec4(v, (head * HD + 4u * d4) / 32u, true, a.q8 + (u64)row * a.q8s, nbq);
+  };
+  const int Ls = kv.len[b];
+  if (!trust(Ls)) { // no part: 0; not to be trusted: NaN
+    if (Ls != 0) kv_bad(kv, AMDC_BAD_LEN);
+    const float v = Ls != 0 ? __builtin_nanf("") : 0.0f;
+    for (u32 i = tid; i < nr * QD; i += 256u) put(i / QD, i % QD, (v4f){v, v, v, v});
+    return;
+  }
+  const u32 L = (u32)Ls;
+
+  { // the columns' queries into the LDS, as the B operand: part p, values 8 c .. 8 c + 7, column
+    const u32 col = tid >> 4, c0 = tid & 15u;
+    u32 row, head;
+    at(col < nr ? col : nr - 1u, row, head);
+    const u64 i0 = (u64)row * a.qs + (u64)head * HD;
+    float v[HD > 128 ? 2 : 1][8], big = 0.0f;
+#pragma unroll
+    for (u32 k = 0; 16u * k < HD / 8u; k++) {
+      const u32 c = c0 + 16u * k;
+      if (HD >= 128 || c < HD / 8u) load_q8<BF, F32>(a.q, i0 + 8u * c, a.vec & 1u, v[k]);
+      else
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[k][i] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) big = __builtin_fmaxf(big, __builtin_fabsf(v[k][i]));
+    }
+    float up = 1.0f, down = 1.0f;
+    if (F32 && !BF) {
+      big = __builtin_fmaxf(big, dpp<0xB1>(big));
+      big = __builtin_fmaxf(big, dpp<0x4E>(big));
+      big = __builtin_fmaxf(big, dpp<0x141>(big));
+      big = __builtin_fmaxf(big, dpp<0x140>(big));
+      const u32 e = __builtin_bit_cast(u32, big) >> 23;
+      const u32 k = e < 11u ? 253u : 264u - e; // 2^10 / 2^(e - 127), kept a normal number, as is its inverse
+      up = __builtin_bit_cast(float, k << 23), down = __builtin_bit_cast(float, (254u - k) << 23);
+    }
+    if (c0 == 0u) s_cq[col] = a.c * down;
+#pragma unroll
+    for (u32 k = 0; 16u * k < HD / 8u; k++) {
+      const u32 c = c0 + 16u * k;
+      if (HD < 128 && c >= HD / 8u) break;
+      if (F32 && !BF)
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[k][i] *= up;
+      u32x4 w[NP];
+      split8<BF, NP>(v[k], w);
+#pragma unroll
+      for (int p = 0; p < NP; p++) *(u32x4 *)(sm + ((p * (HD / 8u) + c) * 16u + col) * 16u) = w[p];
+    }
+    if (tid == 0u) s_bad = 0u;
+  }
+  __syncthreads();
+
+  // the lane's column: what it sees, and the block's extremes
+  const u32 tc = (r0 + (n < nr ? n : nr - 1u)) / G, t_a = r0 / G, t_z = (r0 + nr - 1u) / G;
+  auto lo_of = [&](u32 t) { const u32 e = L - T + t + 1u; return a.window && e > a.window ? e - a.window : 0u; };
+  auto hi_of = [&](u32 t) { return L - T + t + 1u; };
+  const u32 lo = lo_of(tc), hi = hi_of(tc), lo_z = lo_of(t_z), hi_a = hi_of(t_a);
+  const float cq = s_cq[n];
+  const u32 s0 = first(L) / 32u + ci * C, send = cdiv(L, 32u), s1 = s0 + C < send ? s0 + C : send;
+  const u64 gb = 32ull * HD, hb = gb << (kv.lgp - 4u); // bytes of 16 positions of a head, of a page of a head
+  const u32 pmask = (1u << kv.lgp) - 1u;
+  const int *table = kv.pages + (u64)b * kv.max_pages;
+
+  v4f O[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++) O[d] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+  float m = NINF, l = 0.0f;
+  u32x4 kr[2 * KS], vr[DT];
+  const u32 koff = g4 * 256u + (8u * ((n >> 2) & 1u) + (n & 3u)) * 16u, voff = (g4 & 1u) * (16u * HD) + n * 16u;
+  int ids = 0; // of the wave's next 32 steps: lane 2 i + j holds the page of the j-th 16 positions of step i
+  bool bad = false;
+  auto get_ids = [&](u32 st) {
+    const u32 s = st + NW * (lane >> 1), p = 32u * s + 16u * (lane & 1u);
+    const bool in = s < s1 && p < L;
+    ids = in ? table[p >> kv.lgp] : 0;
+    if ((u32)ids >= kv.n_pages) bad = true, ids = 0;
+  };
+  auto base = [&](u32 st, u32 i, u32 j) {
+    const u32 id = (u32)__builtin_amdgcn_readlane(ids, (int)(2u * (i & 31u) + j));
+    return ((u64)id * kv.n_kv + h) * hb + (((32u * st + 16u * j) & pmask) >> 4) * gb;
+  };
+  auto load_k = [&](u64 ga, u64 gz) {
+    const uint8_t *p = kv.k + (n & 8u ? gz : ga) + koff;
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+      for (int s = 0; s < KS; s++) kr[t * KS + s] = *(const u32x4 *)(p + 64 * t + 1024 * s);
+  };
+  auto load_v = [&](u64 ga, u64 gz) {
+    const uint8_t *p = kv.v + (g4 & 2u ? gz : ga) + voff;
+#pragma unroll
+    for (int d = 0; d < DT; d++) vr[d] = *(const u32x4 *)(p + 256 * d);
+  };
+  u32 st = s0 + wv;
+  u64 ga = 0u, gz = 0u;
+  if (st < s1) {
+    get_ids(st);
+    ga = base(st, 0u, 0u), gz = base(st, 0u, 1u);
+    load_k(ga, gz), load_v(ga, gz);
+  }
+  for (u32 i = 0u; st < s1; i++, st += NW) {
+    v4f S[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    // heads of 256: the queries are read from the LDS in every step (kept in registers they would spill others)
+    if (HD > 128) __asm__ volatile("" ::: "memory");
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        const u32x4 qf = *(const u32x4 *)(sm + ((p * (HD / 8u) + 4u * s + g4) * 16u + n) * 16u);
+        S[0] = mfma16<BF>(kr[s], qf, S[0]);
+        S[1] = mfma16<BF>(kr[KS + s], qf, S[1]);
+      }
+    const bool more = st + NW < s1;
+    if (more) {
+      if ((i & 31u) == 31u) get_ids(st + NW);
+      ga = base(st + NW, i + 1u, 0u), gz = base(st + NW, i + 1u, 1u);
+      load_k(ga, gz);
+    }
+    const bool edge = 32u * st + 32u > hi_a || 32u * st < lo_z;
+    float sc[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) sc[k] = S[k >> 2][k & 3] * cq;
+    if (edge)
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const u32 p = 32u * st + 8u * g4 + (u32)k;
+        sc[k] = p >= lo && p < hi ? sc[k] : NINF;
+      }
+    float top = sc[0];
+#pragma unroll
+    for (int k = 1; k < 8; k++) top = __builtin_fmaxf(top, sc[k]);
+    if (__ballot(top > m + RAISE)) {
+      top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+      const float nm = __builtin_fmaxf(m, top), f = m == nm ? 1.0f : __builtin_amdgcn_exp2f(m - nm);
+#pragma unroll
+      for (int d = 0; d < DT; d++) O[d] *= f;
+      l *= f;
+      m = nm;
+    }
+    const float ref = BIAS - (m == NINF ? 0.0f : m);
+#pragma unroll
+    for (int k = 0; k < 8; k++) sc[k] = __builtin_amdgcn_exp2f(sc[k] + ref);
+    l += ((sc[0] + sc[1]) + (sc[2] + sc[3])) + ((sc[4] + sc[5]) + (sc[6] + sc[7]));
+    u32x4 pw[NP];
+    split8<BF, NP>(sc, pw);
+    if (!edge) {
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int p = 0; p < NP; p++) O[d] = mfma16<BF>(vr[d], pw[p], O[d]);
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        v4f e = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int p = 0; p < NP; p++) e = mfma16<BF>(vr[d], pw[p], e);
+        if (wave_finite(e)) O[d] += e;
+        else
+          for (u32 t = t_a; t <= t_z; t++) {
+            e = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+            const u32x4 w = seen16(vr[d], 32u * st + 8u * g4, lo_of(t), hi_of(t));
+#pragma unroll
+            for (int p = 0; p < NP; p++) e = mfma16<BF>(w, pw[p], e);
+            if (tc == t) O[d] += e;
+          }
+      }
+    }
+    if (more) load_v(ga, gz);
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (__ballot(bad)) {
+    if (lane == 0u) kv_bad(kv, AMDC_BAD_PAGE), s_bad = 1u;
+  }
+  __syncthreads(); // the queries are read, their place is the waves' results'
+  float *so = (float *)sm;
+#pragma unroll
+  for (int d = 0; d < DT; d++) *(v4f *)(so + (wv * 16u + n) * OS + 16u * d + 4u * g4) = O[d];
+  if (g4 == 0u) s_m[wv][n] = m, s_l[wv][n] = l;
+  __syncthreads();
+  if (tid < 16u) {
+    float M = s_m[0][tid], sum = 0.0f;
+#pragma unroll
+    for (u32 w = 1; w < NW; w++) M = __builtin_fmaxf(M, s_m[w][tid]);
+#pragma unroll
+    for (u32 w = 0; w < NW; w++) {
+      const float f = __builtin_amdgcn_exp2f(s_m[w][tid] - (M == NINF ? 0.0f : M));
+      s_m[w][tid] = f, sum += f * s_l[w][tid];
+    }
+    s_M[tid] = M, s_L[tid] = s_bad ? __builtin_nanf("") : sum;
+  }
+  __syncthreads();
+  auto mine = [&](u32 i) { // quad i of the workgroup's sums
+    const u32 r = i / QD, d4 = i % QD;
+    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (u32 w = 0; w < NW; w++) v += s_m[w][r] * *(const v4f *)(so + (w * 16u + r) * OS + 4u * d4);
+    return v;
+  };
+  if (nu == 1u) {
+    for (u32 i = tid; i < nr * QD; i += 256u) put(i / QD, i % QD, mine(i) / s_L[i / QD]);
+    return;
+  }
+  // partial results: nr rows of O, then m and l of 16 rows
+  const u32 rmax = T * G < 16u ? T * G : 16u, sb = (rmax * HD + 32u) * 4u;
+  uint8_t *parts = a.ws + ATTN_CNT;
+  auto slot = [&](u32 k) { return ((u64)(slot0 + k) * kv.n_kv + h) * a.ncb + cb; };
+  auto part = [&](u32 k) { return rsrc(parts + slot(k) * sb, sb); };
+  {
+    const __amdgpu_buffer_rsrc_t d = part(ci);
+    for (u32 i = tid; i < nr * QD; i += 256u) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, mine(i)), d, 16u * i, 0, CPOL_SC1);
+    if (tid < nr) {
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_M[tid]), d, rmax * HD * 4u + 4u * tid, 0, CPOL_SC1);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_L[tid]), d, rmax * HD * 4u + 64u + 4u * tid, 0, CPOL_SC1);
+    }
+  }
+  u32 k = ci, left = nu, stride = 1u;
+  for (u32 level = 0u;; level++) {
+    const u32 f0 = k / DEC_FAN * DEC_FAN, cnt = left - f0 < DEC_FAN ? left - f0 : DEC_FAN;
+    if (cnt > 1u) {
+      __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this thread's partial results are stored
+      __syncthreads();
+      if (tid == 0u) {
+        u32 *c = (u32 *)a.ws + slot(f0 * stride + level);
+        const bool last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == cnt;
+        if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_last = last;
+      }
+      __syncthreads();
+      if (!s_last) return;
+      // weights of the cnt results of every row, in the LDS (so is free: the results are in the workspace)
+      float *sw = (float *)sm;
+      if (tid < 16u * DEC_FAN) {
+        const u32 r = tid & 15u, j = tid >> 4;
+        const __amdgpu_buffer_rsrc_t d = part((f0 + (j < cnt ? j : 0u)) * stride);
+        const bool in = j < cnt && r < nr;
+        sw[tid] = in ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(d, rmax * HD * 4u + 4u * r, 0, CPOL_SC1)) : NINF;
+        sw[16u * DEC_FAN + tid] = in ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(d, rmax * HD * 4u + 64u + 4u * r, 0, CPOL_SC1)) : 0.0f;
+      }
+      __syncthreads();
+      if (tid < 16u) {
+        float M = NINF, sum = 0.0f;
+#pragma unroll
+        for (u32 j = 0; j < DEC_FAN; j++) M = __builtin_fmaxf(M, sw[16u * j + tid]);
+#pragma unroll
+        for (u32 j = 0; j < DEC_FAN; j++) {
+          const float f = __builtin_amdgcn_exp2f(sw[16u * j + tid] - (M == NINF ? 0.0f : M));
+          sw[16u * j + tid] = f, sum += f * sw[16u * (DEC_FAN + j) + tid];
+        }
+        s_M[tid] = M, s_L[tid] = sum;
+      }
+      __syncthreads();
+      const bool final = left <= DEC_FAN;
+      const __amdgpu_buffer_rsrc_t to = part(f0 * stride);
+      for (u32 i = tid; i < nr * QD; i += 256u) {
+        u32x4 v[DEC_FAN];
+#pragma unroll
+        for (u32 j = 0; j < DEC_FAN; j++) v[j] = __builtin_amdgcn_raw_buffer_load_b128(part((f0 + (j < cnt ? j : 0u)) * stride), 16u * i, 0, CPOL_SC1);
+        v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (u32 j = 0; j < DEC_FAN; j++)
+          if (j < cnt) sum += sw[16u * j + i / QD] * __builtin_bit_cast(v4f, v[j]);
+        if (final) put(i / QD, i % QD, sum / s_L[i / QD]);
+        else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), to, 16u * i, 0, CPOL_SC1);
+      }
+      if (final) return;
+      if (tid < nr) {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_M[tid]), to, rmax * HD * 4u + 4u * tid, 0, CPOL_SC1);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_L[tid]), to, rmax * HD * 4u + 64u + 4u * tid, 0, CPOL_SC1);
+      }
+    }
+    k /= DEC_FAN, left = cdiv(left, DEC_FAN), stride *= DEC_FAN;
+  }
+}
+
+#define DEC_KERNEL(HD, KN, BF, F32) \
+  extern "C" __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void amdc_attn_dec_h##HD##_##KN(amdc_kv_dev kv, AttnArgs a) { dec_body<HD, BF, F32>(kv, a); }
+#define DEC_KERNELS(HD) DEC_KERNEL(HD, f16, false, false) DEC_KERNEL(HD, f16_f32, false, true) DEC_KERNEL(HD, bf16, true, false) DEC_KERNEL(HD, bf16_f32, true, true)
+DEC_KERNELS(64)
+DEC_KERNELS(128)
+DEC_KERNELS(256)
+#undef DEC_KERNELS
+#undef DEC_KERNEL

@@ -289,9 +289,12 @@ enum {
   K_RMSNORM_R,
   K_GEMVS8, /* amdc_gemv_q8_0_s1, _s2, _xs1, (none), amdc_gemv_q6_k_s1, (none), _xs1, (none), then _s1l, _s2l, _xs1l, _xs2l, ... */
   K_APPEND = K_GEMVS8 + 15, /* amdc_kv_append_f16, _bf16 */
-  K_N = K_APPEND + 2
+  K_ATTN_DEC = K_APPEND + 2, /* amdc_attn_dec_h64_f16, _f16_f32, _bf16, _bf16_f32, then h128, h256 */
+  K_N = K_ATTN_DEC + 12
 };
+
 #define KN(s) "amdc_" s
+#define KA(s) KN(s "_f16"), KN(s "_f16_f32"), KN(s "_bf16"), KN(s "_bf16_f32")
 #define GW(s) "amdc_gemmw_" s
 static const char *const kname[K_N] = {
     "amdc_quant_q8",           "amdc_dots_q4_0",          "amdc_dots_q4_k",          "amdc_gemm_q4_k_n128",
@@ -320,7 +323,8 @@ static const char *const kname[K_N] = {
     KN("quant_q8_v"), KN("swiglu_q8_v"), KN("rmsnorm_q8_r"),
     KN("gemv_q8_0_s1"), KN("gemv_q8_0_s2"), KN("gemv_q8_0_xs1"), KN("gemv_q8_0_xs1"), KN("gemv_q6_k_s1"), KN("gemv_q6_k_s1"), KN("gemv_q6_k_xs1"),
     KN("gemv_q6_k_xs1"), KN("gemv_q8_0_s1l"), KN("gemv_q8_0_s2l"), KN("gemv_q8_0_xs1l"), KN("gemv_q8_0_xs2l"), KN("gemv_q6_k_s1l"),
-    KN("gemv_q6_k_s1l"), KN("gemv_q6_k_xs1l"), KN("kv_append_f16"), KN("kv_append_bf16")};
+    KN("gemv_q6_k_s1l"), KN("gemv_q6_k_xs1l"), KN("kv_append_f16"), KN("kv_append_bf16"),
+    KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256")};
 
 static hipModule_t g_mod;
 static hipFunction_t g_k[K_N];
@@ -1682,6 +1686,80 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
   append_args a = {k, v, q, qo, cu, freq, (u32)qt, n_q, T, ks, vs, qs, qos, rope ? n_rot : 0u, (u32)rope, lghd, rows, gq, gv, upb, vec};
   void *args[] = {&d, &a};
   return launch(K_APPEND + (kv->type == AMDC_TYPE_BF16), rows * gq + vu * gv, 1, 0, stream, args);
+}
+
+/* the arguments of the attention kernels: AttnArgs of amdc_attn.h */
+typedef struct {
+  const void *q;
+  void *y;
+  const int32_t *cu;
+  uint8_t *q8, *ws;
+  float c;
+  u32 n_q, G, T, qs, ys, window, q8s, U, vec, ncb;
+} attn_args;
+#define ATTN_CNT 65536u /* bytes of counters at the start of the workspace (amdc_attn.h) */
+
+/* The checks of both attention operators beyond check_kv's. */
+static int check_attn(const char *op, const amdc_kv *kv, const void *q, const void *y, int t, u32 n_q, u32 rows, u32 qs, u32 ys, const uint8_t *q8,
+                      u32 q8s, const void *ws, size_t ws_bytes, size_t need) {
+  if (t != AMDC_TYPE_F32 && t != kv->type) return fail(AMDC_EINVAL, "%s: q and y of type %d (F32 or the cache's)", op, t);
+  const u64 w = (u64)n_q * kv->hd, es = t == AMDC_TYPE_F32 ? 4u : 2u;
+  if (!q || (!y && !q8)) return fail(AMDC_EINVAL, "%s: null pointer (q, or both y and q8)", op);
+  if (!vec_rows(q, 0, (u32)es) || !vec_rows(y, 0, (u32)es)) return fail(AMDC_EINVAL, "%s: q and y must be aligned to their type", op);
+  if (rows > 1u && (qs < w || (y && ys < w))) return fail(AMDC_EINVAL, "%s: strides qs %u, ys %u under a row's %llu values", op, qs, ys, (unsigned long long)w);
+  if (q8 && (!vec_rows(q8, rows > 1u ? q8s : 0u, 4u) || (rows > 1u && q8s < w / 32u * 40u)))
+    return fail(AMDC_EINVAL, "%s: q8 and q8s (%u) must be multiples of 4, q8s at least %llu", op, q8s, (unsigned long long)(w / 32u * 40u));
+  if (!ws || !aligned16(ws) || ws_bytes < need) return fail(AMDC_EINVAL, "%s: a workspace of %zu bytes (16-byte aligned, at least %zu)", op, ws ? ws_bytes : (size_t)0, need);
+  return AMDC_OK;
+}
+/* which rows are 16-byte aligned (8 for 16-bit results): queries, results */
+static u32 attn_vec(const void *q, const void *y, int t, u32 rows, u32 qs, u32 ys) {
+  const u32 es = t == AMDC_TYPE_F32 ? 4u : 2u;
+  return (vec_rows(q, rows > 1u ? es * qs : 0u, 16u) ? 1u : 0u) | (vec_rows(y, rows > 1u ? es * ys : 0u, 4u * es) ? 2u : 0u);
+}
+/* the kernel of a head size, a cache and a query type, in the order of KA */
+static int attn_kernel(int k0, const amdc_kv *kv, int t) {
+  return k0 + (kv->hd == 64u ? 0 : kv->hd == 128u ? 4 : 8) + (kv->type == AMDC_TYPE_BF16 ? 2 : 0) + (t == AMDC_TYPE_F32 ? 1 : 0);
+}
+
+/* A call of the decode kernel: blocks of 16 columns, and chunks wanted of a head (dec_body in amdc_attn.h) so that the workgroups of
+ * all heads fill the CUs; 0 where the call is refused. The partial results of a call are those of sequences of several
+ * chunks, under twice U, and of U + n_seq chunks in all. */
+static u32 dec_units(u32 n_kv, u32 n_q, u32 hd, u32 T, u32 *ncb) {
+  const u64 cols = (u64)T * (n_q / n_kv);
+  if (!T || cols > 128u) return 0;
+  *ncb = (u32)(cols + 15u) / 16u;
+  const u32 cus = g_cus > 0 ? (u32)g_cus : 256u, heads = n_kv * *ncb, wgs = cus * (hd > 128u ? 1u : 2u);
+  u32 U = wgs / heads, most = ATTN_CNT / 8u / heads; /* counters: one to a partial result */
+  if (U > 256u) U = 256u;
+  if (U > most) U = most;
+  return U ? U : 1u;
+}
+
+size_t amdc_attn_decode_ws(const amdc_kv *kv, uint32_t n_q, uint32_t T) {
+  if (!kv || !amdc_kv_bytes(kv->type, kv->n_kv, kv->hd, kv->page, kv->n_pages) || !n_q || n_q % kv->n_kv) return 0;
+  u32 ncb = 0;
+  const u32 U = dec_units(kv->n_kv, n_q, kv->hd, T, &ncb);
+  if (!U) return 0;
+  const u64 slots = U > kv->n_seq ? (u64)U + kv->n_seq : 2ull * U, cols = (u64)T * (n_q / kv->n_kv), r = cols < 16u ? cols : 16u;
+  return (size_t)(ATTN_CNT + slots * kv->n_kv * ncb * (r * kv->hd + 32u) * 4u);
+}
+
+int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
+                     uint32_t window, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream) {
+  NEED_OPEN();
+  amdc_kv_dev d;
+  u32 rows = 0, ncb = 0;
+  int rc = check_kv("attn_decode", kv, n_q, T, NULL, &d, &rows);
+  if (rc) return rc;
+  const u32 U = dec_units(kv->n_kv, n_q, kv->hd, T, &ncb);
+  if (!U) return fail(AMDC_EINVAL, "attn_decode: T %u of %u query heads to a key / value head (at most 128 together)", T, n_q / kv->n_kv);
+  if ((rc = check_attn("attn_decode", kv, q, y, t, n_q, rows, qs, ys, q8, q8s, ws, ws_bytes, amdc_attn_decode_ws(kv, n_q, T)))) return rc;
+  const u64 grid = ((u64)U + kv->n_seq) * kv->n_kv * ncb;
+  if (grid >= (1u << 24)) return fail(AMDC_EINVAL, "attn_decode: %u sequences of %u heads are too many for one call", kv->n_seq, kv->n_kv);
+  attn_args a = {q, y, NULL, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, U, attn_vec(q, y, t, rows, qs, ys), ncb};
+  void *args[] = {&d, &a};
+  return launch(attn_kernel(K_ATTN_DEC, kv, t), (unsigned)grid, 1, 0, stream, args);
 }
 
 int amdc_probe_read(const void *src, size_t nbytes, void *scratch, uint32_t grid, void *stream) {

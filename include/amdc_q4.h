@@ -330,6 +330,24 @@ enum { AMDC_ROPE_NONE = 0, AMDC_ROPE_PAIRS = 1, AMDC_ROPE_HALVES = 2 };
 int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const float *q, void *qo, int qt, uint32_t n_q, uint32_t T, uint32_t ks,
                    uint32_t vs, uint32_t qs, uint32_t qos, const int32_t *cu, const float *freq, uint32_t n_rot, int rope, void *stream);
 
+/* Attention of the T new tokens of every sequence (T = 1: decode; few: a verify step; T times n_q / n_kv at
+ * most 128) over its cached positions, theirs included (append first): for row t of sequence b, head i
+ *   y = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q.k_j),  head i reads key / value head i / (n_q / n_kv),
+ * over the positions j <= len[b] - T + t, with window not 0 the last `window` of them only. q and y have type
+ * t (AMDC_TYPE_F32 or the cache's), rows qs and ys values apart. Queries are used as they are given; in f32, the
+ * scores, weights, sums and y keep f32's accuracy (the products run on the 16-bit matrix units in parts); in a
+ * 16-bit type the weights are rounded to it. With q8 not NULL also the Q8 copy of the rows (n_q hd values), q8s
+ * bytes apart, for the output matrix: the bits of amdc_quant_q8 of the f32 result (before y's rounding).
+ * A value (or key) that a row does not see may be anything, NaN too, also where another row sees it. Of those that
+ * it sees, a value that is not finite makes its place of the row infinite or NaN, a key that is not finite the row NaN.
+ * ws: amdc_attn_decode_ws(kv, n_q, T) bytes of device memory, 16-byte aligned, cleared to 0 once before the first use
+ * with any call (the calls leave its counters at 0); calls that share it must not overlap on the device, calls with
+ * workspaces of their own may. The size does not depend on the lengths. Nothing is allocated: every call can be
+ * captured. The result does not depend on the order in which workgroups run. */
+size_t amdc_attn_decode_ws(const amdc_kv *kv, uint32_t n_q, uint32_t T);
+int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
+                     uint32_t window, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream);
+
 /* Tuning knobs (0 = automatic): lanes per row of the GEMV (4..64, power of
  * two); the decode kernel (0: the pipelined one; 1 or 2: the multi-vector
  * kernel with 1 or 2 super-groups of loads per step); workgroups of a GEMV
