@@ -132,6 +132,8 @@ ABI = {
     "amdc_kv_append": (C.c_int, [_P, _P, _P, _P, _P, C.c_int, _U32, _U32, _U32, _U32, _U32, _U32, _P, _P, _U32, C.c_int, _P]),
     "amdc_attn_decode_ws": (C.c_size_t, [_P, _U32, _U32]),
     "amdc_attn_decode": (C.c_int, [_P, _P, _P, C.c_int, _U32, _U32, _U32, _U32, C.c_float, _U32, _P, _U32, _P, C.c_size_t, _P]),
+    "amdc_attn_prefill_ws": (C.c_size_t, [_P, _U32, _U32]),
+    "amdc_attn_prefill": (C.c_int, [_P, _P, _P, C.c_int, _U32, _U32, _U32, _U32, C.c_float, _U32, _P, _P, _U32, _P, C.c_size_t, _P]),
     "amdc_chain_record_begin": (C.c_int, [_P]),
     "amdc_chain_record_end": (C.c_int, [_P, C.c_int, C.POINTER(_P)]),
 }
@@ -500,6 +502,19 @@ def attn_decode_ws(kv, n_q, T):
 def attn_decode(kv, q, y, type, n_q, T, qs, ys, scale, ws, ws_bytes, window=0, q8=None, q8s=0, stream=None):
     """amdc_attn_decode: the attention of the T newest tokens of every sequence over its cached positions."""
     _check(lib().amdc_attn_decode(kv.ref, _p(q), _p(y), type, n_q, T, qs, ys, scale, window, _p(q8), q8s, _p(ws), ws_bytes, stream))
+
+
+def attn_prefill_ws(kv, n_q, rows):
+    """Bytes of attn_prefill's workspace for `rows` rows in all (device memory, cleared to 0 once)."""
+    n = lib().amdc_attn_prefill_ws(kv.ref, n_q, rows)
+    if not n:
+        raise AmdcError(f"attn_prefill: {n_q} query heads, {rows} rows: not supported")
+    return n
+
+
+def attn_prefill(kv, q, y, type, n_q, T, qs, ys, scale, ws, ws_bytes, cu=None, window=0, q8=None, q8s=0, stream=None):
+    """amdc_attn_prefill: causal attention of the new rows of every sequence (packed by cu, or T each) over its cached positions."""
+    _check(lib().amdc_attn_prefill(kv.ref, _p(q), _p(y), type, n_q, T, qs, ys, scale, window, _p(cu), _p(q8), q8s, _p(ws), ws_bytes, stream))
 
 
 def chain_quant(x, q, nb, sync=True):

@@ -4,6 +4,8 @@
 //   amdc_kv_append_{f16,bf16}   rotation, keys and values into the cache, rotated queries
 //   amdc_attn_dec_h{64,128,256}_{f16,f16_f32,bf16,bf16_f32}
 //                               attention of a few new tokens per sequence
+//   amdc_attn_pre_h{64,128,256}_{f16,f16_f32,bf16,bf16_f32}
+//                               attention of prompts and prompt chunks
 
 // ------------------------------------------------------------------ helpers
 
@@ -61,9 +63,7 @@ __device__ __forceinline__ SeqRows seq_rows(const amdc_kv_dev &kv, const int *cu
 template <bool BF>
 __device__ __forceinline__ u32 pack2(float a, float b) {
   if constexpr (BF) {
-    u32 r;
-    __asm__("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
+    return __builtin_bit_cast(u32, __builtin_convertvector((v2f){a, b}, b2)); // v_cvt_pk_bf16_f32
   } else {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(u32, (h2){(_Float16)a, (_Float16)b});
@@ -360,8 +360,8 @@ struct AttnArgs {
 // who was last.
 //
 // A step that holds positions which not every column sees is multiplied into sums of its own: where these come out finite they are
-// added, as weights of 0 are right; if not (0 times an infinity or a NaN that a column must not see), column by column with the
-// unseen values as 0.
+// added, as weights of 0 are right; if not (0 times an infinity or a NaN that a column must not see), again with what no column sees as
+// 0, and if that is not enough token by token with what it does not see as 0.
 template <int HD, bool BF, bool F32>
 __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &a) {
   constexpr int NP = F32 ? (BF ? 3 : 2) : 1, KS = HD / 32, DT = HD / 16;
@@ -506,8 +506,8 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
   bool bad = false;
   auto get_ids = [&](u32 st) {
     const u32 s = st + NW * (lane >> 1), p = 32u * s + 16u * (lane & 1u);
-    const bool in = s < s1 && p < L;
-    ids = in ? table[p >> kv.lgp] : 0;
+    const bool in = s < s1; // behind the last position: the last page again
+    ids = in ? table[(p < L ? p : L - 1u) >> kv.lgp] : 0;
     if ((u32)ids >= kv.n_pages) bad = true, ids = 0;
   };
   auto base = [&](u32 st, u32 i, u32 j) {
@@ -590,13 +590,17 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
         v4f e = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int p = 0; p < NP; p++) e = mfma16<BF>(vr[d], pw[p], e);
+        auto again = [&](u32 from, u32 to) {
+          e = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+          const u32x4 w = seen16(vr[d], 32u * st + 8u * g4, from, to);
+#pragma unroll
+          for (int p = 0; p < NP; p++) e = mfma16<BF>(w, pw[p], e);
+        };
+        if (!wave_finite(e)) again(lo_of(t_a), hi_of(t_z)); // without what no column sees: the common case behind the last position
         if (wave_finite(e)) O[d] += e;
         else
           for (u32 t = t_a; t <= t_z; t++) {
-            e = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-            const u32x4 w = seen16(vr[d], 32u * st + 8u * g4, lo_of(t), hi_of(t));
-#pragma unroll
-            for (int p = 0; p < NP; p++) e = mfma16<BF>(w, pw[p], e);
+            again(lo_of(t), hi_of(t));
             if (tc == t) O[d] += e;
           }
       }
@@ -717,3 +721,411 @@ DEC_KERNELS(128)
 DEC_KERNELS(256)
 #undef DEC_KERNELS
 #undef DEC_KERNEL
+
+// ------------------------------------------------------------------ attention of prompts
+
+template <bool BF>
+__device__ __forceinline__ v16f mfma32(u32x4 a, u32x4 b, v16f c) {
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+#define PRE_BM 128u     // query rows of a workgroup
+#define PRE_MAXSPLIT 8u // parts that a tile's positions are split into at most
+#define PRE_MINTILES 4u // tiles of positions that a part has at least
+
+// The new tokens of a sequence and the G heads that share a key / value head are its rows (token t, head g: t G + g). A workgroup
+// takes PRE_BM consecutive rows, its waves W = 32 or 16 each, and goes through tiles of BN positions that the LDS holds twice: while the
+// waves work on one tile the next is loaded into the other half, straight from the cache (the layout is the one the LDS wants; every
+// load moves 1 KB, and every read of an operand, 16 bytes a lane, meets no bank twice).
+// The matrix work bounds it (4 hd flops to a row and position), and next to it the exponentials:
+//   S^T = K Q^T   (32x32x16; columns are query rows): row r of a group of 32 positions is position
+//                 16 (r / 16) + 8 (r / 4 % 2) + 4 (r / 8 % 2) + r % 4, so that the lane's registers 8 s .. 8 s + 7 are the positions
+//                 16 s + 8 (lane / 32) .. + 7 of its row; W = 16 is dec_body's arrangement (16x16x32)
+//   O^T = V^T P^T: and so, as 16-bit weights, the B operand of step s; a value's eight positions are the A operand.
+// A row's maximum and sum are in the two (four) lanes that hold its scores: no reduction over the wave. W = 32 reads each operand
+// from the LDS for twice as many rows; W = 16 needs half the registers for O and the queries. Parts in f32, the raised maximum, the
+// factor 2^8 and the steps at the edges are dec_body's.
+// Rows are dealt from the last tile of the last sequence down: the longest first. Where all rows make fewer workgroups than the CUs
+// hold (a short chunk of a long prompt), a tile's positions are split over a.U workgroups; their partial results go through the
+// workspace, joined by the last to arrive in the order of the positions.
+template <int HD, bool BF, bool F32, u32 W>
+__device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &a) {
+  typedef typename std::conditional<W == 32u, v16f, v4f>::type acc; // of a matrix instruction: W x W / 64
+  constexpr int NP = F32 ? (BF ? 3 : 2) : 1, NA = W == 32u ? 16 : 4, DT = HD / W;
+  constexpr u32 TT = W == 32u ? 1u : 2u, KS = HD / (W == 32u ? 16u : 32u), PF = W / 16u; // of 32 positions: score tiles, steps over hd, weight operands
+  constexpr u32 NW = PRE_BM / W, NTH = 64u * NW, BN = HD > 128 ? 32u : 64u, MT = BN / 32u, TB = BN * HD * 2u, QD = HD / 4u;
+  constexpr u32 PG = HD / 16u, PW = BN / 16u * PG / NW; // KB of a group of 16 positions (keys, then values), and of a tile for each wave
+  constexpr float BIAS = BF ? 0.0f : 8.0f, RAISE = 6.0f, NINF = -__builtin_inff();
+  constexpr bool FULL = HD > 128 && NP > 2; // of registers: the queries' last part stays in the LDS
+  constexpr int QR = FULL ? NP - 1 : NP;
+  __shared__ u32x4 s_q[FULL ? KS : 1][FULL ? NTH : 1]; // step, thread
+  __shared__ __attribute__((aligned(16))) uint8_t sm[2][2][TB]; // half, keys / values
+  __shared__ u32 s_bad, s_last;
+  const u32 tid = threadIdx.x, lane = tid & 63u, wv = (u32)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), n = lane & (W - 1u), gg = lane / W;
+  auto zero = []() {
+    acc z;
+#pragma unroll
+    for (int i = 0; i < NA; i++) z[i] = 0.0f;
+    return z;
+  };
+  auto mfma = [](u32x4 x, u32x4 y, acc c) {
+    if constexpr (W == 32u) return mfma32<BF>(x, y, c);
+    else return mfma16<BF>(x, y, c);
+  };
+  auto over = [](float v, auto f) { // f over the lanes of a row
+    if (W == 16u) v = f(v, __shfl_xor(v, 16));
+    return f(v, __shfl_xor(v, 32));
+  };
+  auto maxf = [](float x, float y) { return __builtin_fmaxf(x, y); };
+  auto addf = [](float x, float y) { return x + y; };
+  const u32 G = a.G, h = blockIdx.x % kv.n_kv;
+  u32 x = blockIdx.x / kv.n_kv;
+  const u32 sp = x % a.U, unit = a.ncb - 1u - x / a.U;
+  u32 b, ti;
+  if (a.cu) {
+    auto base = [&](u32 i) { const int c = a.cu[i]; return (c < 0 ? 0u : (u32)c * G / PRE_BM) + i; };
+    b = find_seq(kv.n_seq, unit, base);
+    ti = unit - base(b);
+  } else {
+    const u32 per = cdiv(a.T * G, PRE_BM);
+    b = unit / per, ti = unit - b * per;
+  }
+  SeqRows s = seq_rows(kv, a.cu, a.T, b);
+  s.row0 = (u32)__builtin_amdgcn_readfirstlane((int)s.row0), s.m = (u32)__builtin_amdgcn_readfirstlane((int)s.m), s.len = (u32)__builtin_amdgcn_readfirstlane((int)s.len);
+  const u32 R = s.m * G, r0 = ti * PRE_BM;
+  if (r0 >= R) return;
+  const u32 nr = R - r0 < PRE_BM ? R - r0 : PRE_BM, nbq = a.n_q * HD / 32u;
+  auto at = [&](u32 r, u32 &row, u32 &head) { // row r of the workgroup
+    const u32 t = (r0 + r) / G;
+    row = s.row0 + t, head = h * G + (r0 + r) - t * G;
+  };
+  auto put = [&](u32 r, u32 d4, v4f v) {
+    u32 row, head;
+    at(r, row, head);
+    if (a.y) store_y4<BF, F32>(a.y, (u64)row * a.ys + (u64)head * HD + 4u * d4, v, a.vec & 2u);
+    if (a.q8) quant_vec4(v, (head * HD + 4u * d4) / 32u, true, a.q8 + (u64)row * a.q8s, nbq);
+  };
+  if (!s.len) { // no part: 0; not to be trusted: NaN
+    const float v = s.bad ? __builtin_nanf("") : 0.0f;
+    if (sp == 0u)
+      for (u32 i = tid; i < nr * QD; i += NTH) put(i / QD, i % QD, (v4f){v, v, v, v});
+    return;
+  }
+  const u32 L = s.len, m0 = L - s.m;
+  auto lo_of = [&](u32 t) { const u32 e = m0 + t + 1u; return a.window && e > a.window ? e - a.window : 0u; };
+  auto hi_of = [&](u32 t) { return m0 + t + 1u; };
+
+  // the tiles of positions [jb, je) of this workgroup
+  const u32 j0 = lo_of(r0 / G) / BN, j1 = cdiv(hi_of((r0 + nr - 1u) / G), BN);
+  const u32 most = (j1 - j0) / PRE_MINTILES, ns = most < 1u ? 1u : most < a.U ? most : a.U;
+  if (sp >= ns) return;
+  const u32 jb = j0 + (j1 - j0) * sp / ns, je = j0 + (j1 - j0) * (sp + 1u) / ns;
+
+  // the wave's rows and the lane's
+  const u32 w0 = W * wv, wr = nr > w0 ? (nr - w0 < W ? nr - w0 : W) : 0u; // 0: only loads
+  const u32 rc = wr ? w0 + (n < wr ? n : wr - 1u) : 0u;
+  const u32 tc = (r0 + rc) / G, t_a = (u32)__builtin_amdgcn_readfirstlane((int)((r0 + (wr ? w0 : 0u)) / G)),
+            t_z = (u32)__builtin_amdgcn_readfirstlane((int)((r0 + (wr ? w0 + wr - 1u : 0u)) / G));
+  const u32 lo = lo_of(tc), hi = hi_of(tc), lo_a = lo_of(t_a), lo_z = lo_of(t_z), hi_a = hi_of(t_a), hi_z = hi_of(t_z);
+
+  // loads: wave wv moves the pieces wv PW .. of a tile, all of one group of positions
+  const u32 grp = wv * PW / PG, pc0 = wv * PW % PG;
+  const u64 gb = 32ull * HD, hb = gb << (kv.lgp - 4u);
+  const u32 pmask = (1u << kv.lgp) - 1u;
+  const int *table = kv.pages + (u64)b * kv.max_pages;
+  int ids = 0; // of the group of tiles jt .. jt + 63
+  bool bad = false;
+  // the first position of the wave's group of tile j; behind the sequence's last group that one again
+  auto place = [&](u32 j) { const u32 p = BN * j + 16u * grp, e = (L - 1u) & ~15u; return p < e ? p : e; };
+  auto get_ids = [&](u32 jt) {
+    const u32 p = place(jt + lane);
+    const bool in = jt + lane < je;
+    ids = in ? table[p >> kv.lgp] : 0;
+    if ((u32)ids >= kv.n_pages) bad = true, ids = 0;
+  };
+  auto issue = [&](u32 j, u32 half) {
+    if (((j - jb) & 63u) == 0u) get_ids(j);
+    const u32 p = place(j);
+    const u64 o64 = ((u64)(u32)__builtin_amdgcn_readlane(ids, (int)((j - jb) & 63u)) * kv.n_kv + h) * hb + ((p & pmask) >> 4) * gb;
+    const u64 off = (u64)(u32)__builtin_amdgcn_readfirstlane((int)(u32)(o64 >> 32)) << 32 | (u32)__builtin_amdgcn_readfirstlane((int)(u32)o64);
+    const __amdgpu_buffer_rsrc_t rk = rsrc(kv.k + off, (u32)gb), rv = rsrc(kv.v + off, (u32)gb);
+#pragma unroll
+    for (u32 i = 0; i < PW; i++) {
+      const u32 c = pc0 + i;
+      const bool val = c >= PG / 2u;
+      const u32 o = 1024u * (val ? c - PG / 2u : c);
+      lds_load16(val ? rv : rk, (__attribute__((address_space(3))) void *)(sm[half][val] + grp * (u32)gb + o), o + 16u * lane);
+    }
+  };
+  if (tid == 0u) s_bad = 0u;
+  issue(jb, 0u);
+
+  // the lane's query row: values HD / KS k + 8 gg .. + 7 of step k
+  u32x4 qf[QR][KS];
+  float cq = a.c;
+  {
+    u32 row, head;
+    at(rc, row, head);
+    const u64 i0 = (u64)row * a.qs + (u64)head * HD + 8u * gg;
+    float up = 1.0f;
+    if (F32 && !BF) {
+      float big = 0.0f;
+#pragma unroll
+      for (u32 k = 0; k < KS; k++) {
+        float v[8];
+        load_q8<BF, F32>(a.q, i0 + HD / KS * k, a.vec & 1u, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) big = __builtin_fmaxf(big, __builtin_fabsf(v[i]));
+      }
+      big = over(big, maxf);
+      const u32 e = __builtin_bit_cast(u32, big) >> 23, k = e < 11u ? 253u : 264u - e;
+      up = __builtin_bit_cast(float, k << 23), cq *= __builtin_bit_cast(float, (254u - k) << 23);
+    }
+#pragma unroll
+    for (u32 k = 0; k < KS; k++) {
+      float v[8];
+      if (FULL) __asm__ volatile("" ::: "memory");
+      load_q8<BF, F32>(a.q, i0 + HD / KS * k, a.vec & 1u, v);
+      if (F32 && !BF)
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= up;
+      u32x4 w[NP];
+      split8<BF, NP>(v, w);
+#pragma unroll
+      for (int p = 0; p < QR; p++) qf[p][k] = w[p];
+      if (FULL) s_q[k][tid] = w[NP - 1]; // read by this thread alone
+    }
+  }
+
+  acc O[DT];
+#pragma unroll
+  for (int d = 0; d < DT; d++) O[d] = zero();
+  float m = NINF, l = 0.0f;
+  const u32 koff = (W == 32u ? (n >> 4) * (u32)gb + (8u * ((n >> 2) & 1u) + 4u * ((n >> 3) & 1u) + (n & 3u)) * 16u
+                             : (n >> 3) * (u32)gb + (8u * ((n >> 2) & 1u) + (n & 3u)) * 16u) + gg * 256u,
+            voff = (gg * HD + n) * 16u;
+  // N groups of 32 positions from p0 on, keys at kt and values at vt in the LDS; EDGE: not every row sees all of them
+  auto tile = [&](auto edge, auto groups, const uint8_t *kt, const uint8_t *vt, u32 p0) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge)::value;
+    constexpr u32 N = decltype(groups)::value, NS = 8u * PF; // scores of a lane in 32 positions: 32 / PF f + 8 gg + 0 .. 7 for f < PF
+    float S[N * NS];
+#pragma unroll
+    for (u32 t = 0; t < N; t++) {
+      acc c[TT];
+#pragma unroll
+      for (u32 u = 0; u < TT; u++) c[u] = zero();
+#pragma unroll
+      for (u32 k = 0; k < KS; k++) {
+        if (FULL && k % 2u == 0u) __asm__ volatile("" ::: "memory"); // few operands at a time: the registers are full
+#pragma unroll
+        for (u32 u = 0; u < TT; u++) {
+          const u32x4 kf = *(const u32x4 *)(kt + t * 2u * (u32)gb + 32u * HD / KS * k + 64u * u);
+#pragma unroll
+          for (int p = 0; p < QR; p++) c[u] = mfma(kf, qf[p][k], c[u]);
+          if (FULL) c[u] = mfma(kf, s_q[k][tid], c[u]);
+        }
+      }
+#pragma unroll
+      for (u32 i = 0; i < NS; i++) S[NS * t + i] = c[i / NA][i % NA] * cq;
+    }
+    float top = NINF;
+#pragma unroll
+    for (u32 i = 0; i < N * NS; i++) {
+      if (EDGE) {
+        const u32 p = p0 + 32u * (i / NS) + 32u / PF * (i % NS / 8u) + 8u * gg + (i & 7u);
+        S[i] = p >= lo && p < hi ? S[i] : NINF;
+      }
+      top = __builtin_fmaxf(top, S[i]);
+    }
+    if (__ballot(top > m + RAISE)) {
+      const float nm = __builtin_fmaxf(m, over(top, maxf)), f = m == nm ? 1.0f : __builtin_amdgcn_exp2f(m - nm);
+#pragma unroll
+      for (int d = 0; d < DT; d++) O[d] *= f;
+      l *= f;
+      m = nm;
+    }
+    const float ref = BIAS - (m == NINF ? 0.0f : m);
+    u32x4 pw[NP][PF * N];
+#pragma unroll
+    for (u32 k = 0; k < PF * N; k++) {
+      float v[8];
+#pragma unroll
+      for (u32 i = 0; i < 8u; i++) v[i] = __builtin_amdgcn_exp2f(S[8u * k + i] + ref);
+      l += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+      u32x4 w[NP];
+      split8<BF, NP>(v, w);
+#pragma unroll
+      for (int p = 0; p < NP; p++) pw[p][k] = w[p];
+    }
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+      if (FULL && d % 4 == 0) __asm__ volatile("" ::: "memory");
+      acc e = EDGE ? zero() : O[d];
+#pragma unroll
+      for (u32 k = 0; k < PF * N; k++) {
+        const u32x4 vf = *(const u32x4 *)(vt + 64u * HD / PF * k + 16u * W * d);
+#pragma unroll
+        for (int p = 0; p < NP; p++) e = mfma(vf, pw[p][k], e);
+      }
+      if (EDGE) {
+        auto finite = [&]() {
+          float z = 0.0f;
+#pragma unroll
+          for (int i = 0; i < NA; i++) z += e[i] - e[i]; // NaN where one is not
+          return __ballot(!(z == 0.0f)) == 0ull;
+        };
+        auto again = [&](u32 from, u32 to) {
+          e = zero();
+#pragma unroll
+          for (u32 k = 0; k < PF * N; k++) {
+            const u32x4 vf = seen16(*(const u32x4 *)(vt + 64u * HD / PF * k + 16u * W * d), p0 + 32u / PF * k + 8u * gg, from, to);
+#pragma unroll
+            for (int p = 0; p < NP; p++) e = mfma(vf, pw[p][k], e);
+          }
+        };
+        if (!finite()) again(lo_a, hi_z); // without what no row sees: the common case behind the last position
+        if (finite()) O[d] += e;
+        else
+          for (u32 t = t_a; t <= t_z; t++) {
+            again(lo_of(t), hi_of(t));
+            if (tc == t) O[d] += e;
+          }
+      } else O[d] = e;
+    }
+  };
+  for (u32 j = jb; j < je; j++) {
+    const u32 half = (j - jb) & 1u, p0 = BN * j;
+    vm_wait(0u);  // this tile has landed ...
+    v8_barrier(); // ... every wave's part, and every wave is done with the other half
+    if (j + 1u < je) issue(j + 1u, half ^ 1u);
+    const uint8_t *kt = sm[half][0] + koff, *vt = sm[half][1] + voff;
+    if (!wr || p0 >= hi_z || p0 + BN <= lo_a) continue;
+    if (p0 + BN <= hi_a && p0 >= lo_z) tile(std::false_type(), std::integral_constant<u32, MT>(), kt, vt, p0);
+    else // an edge, 32 positions at a time
+      for (u32 t = 0; t < MT; t++)
+        if (p0 + 32u * t < hi_z && p0 + 32u * t + 32u > lo_a)
+          tile(std::true_type(), std::integral_constant<u32, 1u>(), kt + t * 2u * (u32)gb, vt + t * 64u * HD, p0 + 32u * t);
+  }
+  l = over(l, addf);
+  if (__ballot(bad) && lane == 0u) kv_bad(kv, AMDC_BAD_PAGE), s_bad = 1u;
+  __syncthreads();
+  if (s_bad) l = __builtin_nanf("");
+
+  auto quad = [&](int d, u32 i) { return (v4f){O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]}; }; // values W d + 8 i + 4 gg .. + 3
+  if (ns == 1u) {
+    u32 row, head;
+    at(rc, row, head);
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+      O[d] *= inv;
+      if (a.y && n < wr)
+#pragma unroll
+        for (u32 i = 0; i < NA / 4u; i++) store_y4<BF, F32>(a.y, (u64)row * a.ys + (u64)head * HD + W * d + 8u * i + 4u * gg, quad(d, i), a.vec & 2u);
+    }
+    if (a.q8)
+#pragma unroll
+      for (int blk = 0; blk < HD / 32; blk++) { // amdc_quant_q8's d, q and sum of a block, spread over the lanes of the row
+        constexpr int BT = 32 / W;
+        float big = 0.0f;
+#pragma unroll
+        for (int i = 0; i < BT * NA; i++) big = __builtin_fmaxf(big, __builtin_fabsf(O[blk * BT + i / NA][i % NA]));
+        const float dd = over(big, maxf) / 127.0f;
+        u32 sum = 0u, w[BT * NA / 4];
+#pragma unroll
+        for (int i = 0; i < BT * NA / 4; i++) {
+          int qi[4];
+          q8_round4(quad(blk * BT + 4 * i / NA, i % (NA / 4)), dd, qi);
+          sum += (u32)qi[0] + (u32)qi[1] + (u32)qi[2] + (u32)qi[3];
+          w[i] = (u32)(qi[0] & 255) | (u32)(qi[1] & 255) << 8 | (u32)(qi[2] & 255) << 16 | (u32)qi[3] << 24;
+        }
+        if (W == 16u) sum += (u32)__shfl_xor((int)sum, 16);
+        sum += (u32)__shfl_xor((int)sum, 32);
+        if (n < wr) {
+          uint8_t *to = a.q8 + (u64)row * a.q8s;
+          const u32 at_blk = head * (HD / 32) + blk;
+#pragma unroll
+          for (u32 i = 0; i < BT * NA / 4; i++) *(u32 *)(to + 32u * at_blk + W * (4u * i / NA) + 8u * (i % (NA / 4)) + 4u * gg) = w[i];
+          if (gg == 0u) ((float *)(to + 32u * nbq))[at_blk] = dd, ((u32 *)(to + 36u * nbq))[at_blk] = sum;
+        }
+      }
+    return;
+  }
+  // partial results: PRE_BM rows of O, then their m and l
+  constexpr u32 SB = (PRE_BM * HD + 2u * PRE_BM) * 4u, OM = PRE_BM * HD * 4u;
+  const u64 cell = (u64)unit * kv.n_kv + h;
+  uint8_t *parts = a.ws + ATTN_CNT + cell * a.U * SB;
+  {
+    const __amdgpu_buffer_rsrc_t d = rsrc(parts + sp * SB, SB);
+    if (n < wr) {
+#pragma unroll
+      for (int k = 0; k < DT; k++)
+#pragma unroll
+        for (u32 i = 0; i < NA / 4u; i++)
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, quad(k, i)), d, ((w0 + n) * HD + W * k + 8u * i + 4u * gg) * 4u, 0, CPOL_SC1);
+      if (gg == 0u) {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, m), d, OM + 4u * (w0 + n), 0, CPOL_SC1);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, l), d, OM + 4u * (PRE_BM + w0 + n), 0, CPOL_SC1);
+      }
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this thread's partial results are stored
+  __syncthreads();
+  if (tid == 0u) {
+    u32 *c = (u32 *)a.ws + cell;
+    const bool last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == ns;
+    if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_last = last;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  float *sw = (float *)sm; // [part][row], then the rows' sums
+  if (tid < PRE_BM) {
+    float mm[PRE_MAXSPLIT], ll[PRE_MAXSPLIT], M = NINF, sum = 0.0f;
+#pragma unroll
+    for (u32 k = 0; k < PRE_MAXSPLIT; k++) {
+      const __amdgpu_buffer_rsrc_t d = rsrc(parts + (k < ns ? k : 0u) * SB, SB);
+      const bool in = k < ns && tid < nr;
+      mm[k] = in ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(d, OM + 4u * tid, 0, CPOL_SC1)) : NINF;
+      ll[k] = in ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(d, OM + 4u * (PRE_BM + tid), 0, CPOL_SC1)) : 0.0f;
+    }
+#pragma unroll
+    for (u32 k = 0; k < PRE_MAXSPLIT; k++) M = __builtin_fmaxf(M, mm[k]);
+#pragma unroll
+    for (u32 k = 0; k < PRE_MAXSPLIT; k++) {
+      const float f = __builtin_amdgcn_exp2f(mm[k] - (M == NINF ? 0.0f : M));
+      sw[k * PRE_BM + tid] = f, sum += f * ll[k];
+    }
+    sw[PRE_MAXSPLIT * PRE_BM + tid] = sum;
+  }
+  __syncthreads();
+  for (u32 i = tid; i < nr * QD; i += NTH) {
+    const u32 r = i / QD;
+    u32x4 v[PRE_MAXSPLIT];
+#pragma unroll
+    for (u32 k = 0; k < PRE_MAXSPLIT; k++) v[k] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(parts + (k < ns ? k : 0u) * SB, SB), 16u * i, 0, CPOL_SC1);
+    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (u32 k = 0; k < PRE_MAXSPLIT; k++)
+      if (k < ns) sum += sw[k * PRE_BM + r] * __builtin_bit_cast(v4f, v[k]);
+    put(r, i % QD, sum / sw[PRE_MAXSPLIT * PRE_BM + r]);
+  }
+}
+
+#define PRE_KERNEL(HD, KN, BF, F32, W, OCC) \
+  extern "C" __global__ __launch_bounds__(8192 / W, OCC) void amdc_attn_pre_h##HD##_##KN(amdc_kv_dev kv, AttnArgs a) { pre_body<HD, BF, F32, W>(kv, a); }
+PRE_KERNEL(64, f16, false, false, 32, 2)
+PRE_KERNEL(64, f16_f32, false, true, 32, 2)
+PRE_KERNEL(64, bf16, true, false, 32, 2)
+PRE_KERNEL(64, bf16_f32, true, true, 32, 2)
+PRE_KERNEL(128, f16, false, false, 32, 2)
+PRE_KERNEL(128, f16_f32, false, true, 32, 1)
+PRE_KERNEL(128, bf16, true, false, 32, 2)
+PRE_KERNEL(128, bf16_f32, true, true, 32, 1)
+PRE_KERNEL(256, f16, false, false, 16, 2)
+PRE_KERNEL(256, f16_f32, false, true, 16, 2)
+PRE_KERNEL(256, bf16, true, false, 16, 2)
+PRE_KERNEL(256, bf16_f32, true, true, 16, 2)
+#undef PRE_KERNEL

@@ -290,7 +290,8 @@ enum {
   K_GEMVS8, /* amdc_gemv_q8_0_s1, _s2, _xs1, (none), amdc_gemv_q6_k_s1, (none), _xs1, (none), then _s1l, _s2l, _xs1l, _xs2l, ... */
   K_APPEND = K_GEMVS8 + 15, /* amdc_kv_append_f16, _bf16 */
   K_ATTN_DEC = K_APPEND + 2, /* amdc_attn_dec_h64_f16, _f16_f32, _bf16, _bf16_f32, then h128, h256 */
-  K_N = K_ATTN_DEC + 12
+  K_ATTN_PRE = K_ATTN_DEC + 12, /* amdc_attn_pre_h64_f16, .. */
+  K_N = K_ATTN_PRE + 12
 };
 
 #define KN(s) "amdc_" s
@@ -324,7 +325,8 @@ static const char *const kname[K_N] = {
     KN("gemv_q8_0_s1"), KN("gemv_q8_0_s2"), KN("gemv_q8_0_xs1"), KN("gemv_q8_0_xs1"), KN("gemv_q6_k_s1"), KN("gemv_q6_k_s1"), KN("gemv_q6_k_xs1"),
     KN("gemv_q6_k_xs1"), KN("gemv_q8_0_s1l"), KN("gemv_q8_0_s2l"), KN("gemv_q8_0_xs1l"), KN("gemv_q8_0_xs2l"), KN("gemv_q6_k_s1l"),
     KN("gemv_q6_k_s1l"), KN("gemv_q6_k_xs1l"), KN("kv_append_f16"), KN("kv_append_bf16"),
-    KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256")};
+    KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256"),
+    KA("attn_pre_h64"), KA("attn_pre_h128"), KA("attn_pre_h256")};
 
 static hipModule_t g_mod;
 static hipFunction_t g_k[K_N];
@@ -1717,6 +1719,8 @@ static u32 attn_vec(const void *q, const void *y, int t, u32 rows, u32 qs, u32 y
   const u32 es = t == AMDC_TYPE_F32 ? 4u : 2u;
   return (vec_rows(q, rows > 1u ? es * qs : 0u, 16u) ? 1u : 0u) | (vec_rows(y, rows > 1u ? es * ys : 0u, 4u * es) ? 2u : 0u);
 }
+/* launch of a prompt kernel: 32 rows to a wave, or 16 for heads of 256 (pre_body in amdc_attn.h) */
+static int launch_pre(int k, u32 hd, unsigned g, void *stream, void **args) { return launch_nt(k, g, 1, hd > 128u ? 512u : 256u, 0, stream, args); }
 /* the kernel of a head size, a cache and a query type, in the order of KA */
 static int attn_kernel(int k0, const amdc_kv *kv, int t) {
   return k0 + (kv->hd == 64u ? 0 : kv->hd == 128u ? 4 : 8) + (kv->type == AMDC_TYPE_BF16 ? 2 : 0) + (t == AMDC_TYPE_F32 ? 1 : 0);
@@ -1760,6 +1764,41 @@ int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t 
   attn_args a = {q, y, NULL, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, U, attn_vec(q, y, t, rows, qs, ys), ncb};
   void *args[] = {&d, &a};
   return launch(attn_kernel(K_ATTN_DEC, kv, t), (unsigned)grid, 1, 0, stream, args);
+}
+
+/* A call of the prompt kernel: tiles of PRE_BM rows of a head at most, and the parts that a tile's positions are split into where
+ * the tiles of all heads are fewer than the CUs hold (pre_body in amdc_attn.h). */
+#define PRE_BM 128u
+#define PRE_MAXSPLIT 8u
+static u32 pre_tiles(const amdc_kv *kv, u32 n_q, u32 rows, int ragged, u32 T, u32 *parts) {
+  const u32 G = n_q / kv->n_kv;
+  const u64 tiles = ragged ? (u64)rows * G / PRE_BM + kv->n_seq : (u64)kv->n_seq * (((u64)T * G + PRE_BM - 1u) / PRE_BM);
+  const u64 wgs = tiles * kv->n_kv, want = (g_cus > 0 ? (u32)g_cus : 256u) * (kv->hd > 128u ? 1u : 2u);
+  *parts = wgs >= want ? 1u : want / wgs < PRE_MAXSPLIT ? (u32)(want / wgs) : PRE_MAXSPLIT;
+  return tiles < (1u << 24) ? (u32)tiles : 1u << 24;
+}
+
+size_t amdc_attn_prefill_ws(const amdc_kv *kv, uint32_t n_q, uint32_t rows) {
+  if (!kv || !amdc_kv_bytes(kv->type, kv->n_kv, kv->hd, kv->page, kv->n_pages) || !n_q || n_q % kv->n_kv || !rows || rows > (1u << 22)) return 0;
+  /* rows dealt to the sequences in any way: fewer tiles mean more parts of each, under `want` workgroups in all */
+  const u64 want = (g_cus > 0 ? (u32)g_cus : 256u) * (kv->hd > 128u ? 1u : 2u);
+  return (size_t)(ATTN_CNT + want * (PRE_BM * kv->hd + 2u * PRE_BM) * 4u);
+}
+
+int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
+                      uint32_t window, const int32_t *cu, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream) {
+  NEED_OPEN();
+  amdc_kv_dev d;
+  u32 rows = 0, parts = 0;
+  int rc = check_kv("attn_prefill", kv, n_q, T, cu, &d, &rows);
+  if (rc) return rc;
+  if ((rc = check_attn("attn_prefill", kv, q, y, t, n_q, rows, qs, ys, q8, q8s, ws, ws_bytes, amdc_attn_prefill_ws(kv, n_q, rows)))) return rc;
+  const u32 tiles = pre_tiles(kv, n_q, rows, cu != NULL, T, &parts);
+  const u64 grid = (u64)tiles * parts * kv->n_kv;
+  if (grid >= (1u << 24)) return fail(AMDC_EINVAL, "attn_prefill: %u rows of %u sequences and %u heads are too many for one call", rows, kv->n_seq, kv->n_kv);
+  attn_args a = {q, y, cu, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, parts, attn_vec(q, y, t, rows, qs, ys), tiles};
+  void *args[] = {&d, &a};
+  return launch_pre(attn_kernel(K_ATTN_PRE, kv, t), kv->hd, (unsigned)grid, stream, args);
 }
 
 int amdc_probe_read(const void *src, size_t nbytes, void *scratch, uint32_t grid, void *stream) {

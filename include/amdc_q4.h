@@ -299,8 +299,8 @@ enum { AMDC_TYPE_F32 = 0, AMDC_TYPE_F16 = 1, AMDC_TYPE_BF16 = 2 };
  *
  * What only the device sees is checked there: a page outside the pool, a length over
  * max_pages * page or under the sequence's number of new tokens, rows outside 0 .. T. Such an entry is never
- * followed: append leaves out the positions concerned, attention gives NaN in the sequence's rows, and
- * amdc_kv_check() reports it. */
+ * followed: append leaves out the positions concerned, attention gives NaN in the sequence's rows (rows outside
+ * 0 .. T: writes none of the sequence), and amdc_kv_check() reports it. */
 typedef struct {
   int type; /* AMDC_TYPE_F16 or AMDC_TYPE_BF16 */
   uint32_t n_kv, hd, page, n_pages;
@@ -347,6 +347,13 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
 size_t amdc_attn_decode_ws(const amdc_kv *kv, uint32_t n_q, uint32_t T);
 int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
                      uint32_t window, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream);
+
+/* The same for any numbers of new tokens: whole prompts, or chunks at the end of what is cached, of different
+ * lengths packed into one call (cu), or T rows of every sequence (cu NULL). ws: amdc_attn_prefill_ws(kv, n_q, rows)
+ * bytes, rows = T with cu, n_seq T without; under the rules of amdc_attn_decode's. */
+size_t amdc_attn_prefill_ws(const amdc_kv *kv, uint32_t n_q, uint32_t rows);
+int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
+                      uint32_t window, const int32_t *cu, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream);
 
 /* Tuning knobs (0 = automatic): lanes per row of the GEMV (4..64, power of
  * two); the decode kernel (0: the pipelined one; 1 or 2: the multi-vector
