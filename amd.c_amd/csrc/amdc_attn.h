@@ -251,6 +251,9 @@ APPEND_KERNEL(bf16, true)
 
 // ------------------------------------------------------------------ attention of a few new tokens
 
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+
 template <bool BF>
 __device__ __forceinline__ v4f mfma16(u32x4 a, u32x4 b, v4f c) {
   typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -313,9 +316,10 @@ __device__ __forceinline__ bool wave_finite(v4f c) {
 }
 
 // the 16-bit halves of w (positions p, p + 1, ..) that lie outside [lo, hi), as 0
-__device__ __forceinline__ u32x4 seen16(u32x4 w, u32 p, u32 lo, u32 hi) {
+template <class V>
+__device__ __forceinline__ V seen16(V w, u32 p, u32 lo, u32 hi) {
 #pragma unroll
-  for (u32 i = 0; i < 4u; i++) {
+  for (u32 i = 0; i < sizeof(V) / 4u; i++) {
     const u32 a = p + 2u * i, b = a + 1u;
     w[i] &= (a >= lo && a < hi ? 0xFFFFu : 0u) | (b >= lo && b < hi ? 0xFFFF0000u : 0u);
   }
@@ -328,53 +332,81 @@ struct AttnArgs {
   const int *cu;
   uint8_t *q8, *ws;
   float c; // scale log2(e)
-  u32 n_q, G, T, qs, ys, window, q8s, U, vec, ncb;
+  u32 n_q, G, T, qs, ys, window, q8s, U, vec, ncb, fit;
 };
 
 #define ATTN_CNT 65536u // bytes of counters at the start of the workspace
 #define DEC_FAN 8u      // partial results joined at once
-#define DEC_CMIN 4u     // the shortest chunk, in steps of 32 positions
+#define DEC_CMIN 512u   // the shortest chunk, in positions
+#define DEC_NT 327680u  // the bytes of a chunk from which its loads are nontemporal
 
-// T rows of G = n_q / n_kv heads of a sequence read the same keys and values. A workgroup takes 16 of these T G
-// columns (blocks cb of them), one key / value head and one chunk of the sequence's positions; its four waves take
-// the chunk's steps of 32 positions in turn, each with a softmax of its own (maximum m, sum l, weighted sum O), joined at
+// The sum of v over the wave, in every lane, and the inclusive sums of v up to each lane
+__device__ __forceinline__ u32 wave_scan(u32 v) {
+  // row_shr 1, 2, 4, 8 inside rows of 16, then the rows' last lanes onto the rows behind (row_bcast 15 and 31)
+  v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
+  v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);
+  v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+__device__ __forceinline__ u32 lane_of(u32 v, u32 lane) { return (u32)__builtin_amdgcn_readlane((int)v, (int)lane); }
+
+// N weights or queries in NP parts, the operands of a step of 32 (N = 8) or 16 (4) positions
+template <bool BF, int NP, int N>
+__device__ __forceinline__ void split_n(float (&x)[N], u32 (&w)[NP][N / 2]) {
+#pragma unroll
+  for (int p = 0; p < NP; p++)
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) {
+      const u32 v = pack2<BF>(x[2 * i], x[2 * i + 1]);
+      w[p][i] = v;
+      if (p + 1 < NP) x[2 * i] -= lo16<BF>(v), x[2 * i + 1] -= hi16<BF>(v);
+    }
+}
+
+// T rows of G = n_q / n_kv heads of a sequence read the same keys and values. A workgroup takes 16 NC of these T G
+// columns (blocks cb of them), one key / value head and one chunk of the sequence's positions; its NW waves take
+// the chunk's steps of SP positions in turn, each with a softmax of its own (maximum m, sum l, weighted sum O), joined at
 // the end in the LDS.
 //
 // Reading the cache bounds it (16 columns cost 2 x 16 x hd flops per 4 hd bytes, 1 / 40 of the matrix rate at the HBM's), so
 // the layout gives every load of a wave whole lines, straight into the matrix units' operands, no LDS between:
-//   S^T = K Q^T  (16x16x32: rows are positions, columns are the query rows): row r of tile t (of two) is position
+//   S^T = K Q^T  (16x16x32: rows are positions, columns are the query rows). SP = 32: row r of tile t (of two) is position
 //                8 (r / 4) + 4 t + r % 4 of the step, so that a lane's eight scores are the eight positions 8 g .. 8 g + 7
-//                (g = lane / 16) of its column
-//   O^T = V^T P^T: those eight, as 16-bit weights, are the lane's B operand as they stand; the cache keeps a value's eight
-//                positions together, which is the A operand.
+//                (g = lane / 16) of its column. SP = 16, for heads of 256, whose O and loads in flight fill the registers at half
+//                the step: row r is position r, a lane's four scores are 4 g .. 4 g + 3
+//   O^T = V^T P^T: those, as 16-bit weights, are the lane's B operand (16x16x32, or 16x16x16) as they stand; the cache keeps a
+//                value's eight positions together, which is the A operand.
 // In f32, queries and weights go in as sums of 16-bit parts (f16: two, 22 bits; bf16: three, 24), one product each, into the
 // same sums; f16 queries are first scaled by a power of two that brings a row's largest value to 2^10 (no overflow, and the second part
 // stays a normal number). f16 weights carry 2^8 (their least normal is 2^-14), the sum l the same factor.
 // The maximum is raised, and O rescaled, only where a score passes it by 6 (weights stay under 2^14): the join needs a common
 // reference, not the largest score.
 //
-// Chunks: the device divides all sequences' steps by the number of units U that the host wants of a head (workgroups per
-// head to fill the CUs), so that chunks are about equal however different the lengths are; every wave finds its unit by a scan over the
-// lengths. A sequence's chunks leave partial results (O, m, l) in the workspace, agent-coherent as split_put's; of
-// every DEC_FAN neighbours the last to arrive joins them, in their order, up a tree, so the result does not depend on
-// who was last.
+// Chunks: the device divides all sequences' steps by the number of units U that the host wants of a head, so that chunks are
+// about equal however different the lengths are; every wave finds its unit by a scan over the lengths. A sequence's chunks
+// leave partial results (O, m, l) in the workspace, agent-coherent as split_put's; of every DEC_FAN neighbours the last to arrive
+// joins them, in their order, up a tree, so the result does not depend on who was last.
 //
 // A step that holds positions which not every column sees is multiplied into sums of its own: where these come out finite they are
 // added, as weights of 0 are right; if not (0 times an infinity or a NaN that a column must not see), again with what no column sees as
 // 0, and if that is not enough token by token with what it does not see as 0.
-template <int HD, bool BF, bool F32>
+template <int HD, bool BF, bool F32, u32 NC, u32 NW>
 __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &a) {
   constexpr int NP = F32 ? (BF ? 3 : 2) : 1, KS = HD / 32, DT = HD / 16;
-  constexpr u32 NW = 4u, OS = HD + 4u, QD = HD / 4u; // floats between columns of O in the LDS; quads of a row
+  constexpr u32 SP = HD > 128 || (NC > 1u && HD > 64) ? 16u : 32u, SL = SP / 4u, TT = SP / 16u, R = 16u * NC, NTH = 64u * NW; // positions of a step, scores of a lane, score tiles
+  constexpr u32 OS = HD + 4u, QD = HD / 4u; // floats between columns of O in the LDS; quads of a row
   constexpr float BIAS = BF ? 0.0f : 8.0f, RAISE = 6.0f, NINF = -__builtin_inff();
-  constexpr u32 SMQ = NP * HD * 32u, SMO = NW * 16u * OS * 4u, SMB = SMQ > SMO ? SMQ : SMO;
+  constexpr u32 NS = NW > 4u && HD * NC > 256 ? 4u : NW, SMQ = NP * HD * 2u * R, SMO = NS * R * OS * 4u, SMB = SMQ > SMO ? SMQ : SMO;
+  typedef u32 op __attribute__((ext_vector_type(SL / 2))); // SL 16-bit values
   __shared__ __attribute__((aligned(16))) uint8_t sm[SMB];
-  __shared__ float s_cq[16], s_m[NW][16], s_l[NW][16], s_L[16], s_M[16];
+  __shared__ float s_cq[R], s_m[NW][R], s_l[NW][R], s_L[R], s_M[R];
   __shared__ u32 s_bad, s_last;
   const u32 tid = threadIdx.x, lane = tid & 63u, wv = (u32)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), n = lane & 15u, g4 = lane >> 4;
-  u32 x = blockIdx.x;
-  const u32 cb = x % a.ncb;
-  x /= a.ncb;
+  // the blocks of columns of a unit are 8 workgroups apart: on one XCD, whose L2 the second to read finds the cache in
+  const u32 cb = blockIdx.x / 8u % a.ncb, x = blockIdx.x / (8u * a.ncb) * 8u + (blockIdx.x & 7u);
   const u32 h = x % kv.n_kv, u = x / kv.n_kv, T = a.T, G = a.G;
 
   // the unit: sequence b, its chunk ci of nu, of C steps
@@ -382,45 +414,49 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
   auto first = [&](u32 L) { return a.window && L - T + 1u > a.window ? L - T + 1u - a.window : 0u; }; // the first position any row sees
   auto steps = [&](u32 i) {
     const int L = kv.len[i];
-    return trust(L) ? cdiv((u32)L, 32u) - first((u32)L) / 32u : 1u;
+    return trust(L) ? cdiv((u32)L, SP) - first((u32)L) / SP : 1u;
   };
-  u32 b = 0u, ci = 0u, nu = 1u, slot0 = 0u, C;
-  {
-    u64 total = 0u;
+  u32 b = 0u, ci = u, nu, slot0 = 0u, C;
+  if (kv.n_seq == 1u) {
+    const u32 all = steps(0u), c = cdiv(all, a.U);
+    C = c < DEC_CMIN / SP ? DEC_CMIN / SP : c;
+    nu = cdiv(all, C);
+    if (u >= nu) return;
+  } else {
+    u32 total = 0u;
     for (u32 i = lane; i < kv.n_seq; i += 64u) total += steps(i);
-    if (kv.n_seq > 1u)
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
-    else total = __shfl(total, 0);
-    const u64 c = (total + a.U - 1u) / a.U;
-    C = c < DEC_CMIN ? DEC_CMIN : (u32)(c < (1u << 27) ? c : (1u << 27));
+    total = lane_of(wave_scan(total), 63u);
+    const u32 c = cdiv(total, a.U);
+    C = c < DEC_CMIN / SP ? DEC_CMIN / SP : c;
+    // one round of workgroups: the chunks made longer until the units are no more than U
+    for (u32 k = 0u; k < 4u && a.fit; k++) {
+      u32 all = 0u;
+      for (u32 i = lane; i < kv.n_seq; i += 64u) all += cdiv(steps(i), C);
+      all = lane_of(wave_scan(all), 63u);
+      if (all <= a.U) break;
+      C += 1u + (u32)((float)C * (float)(all - a.U) / (float)a.U);
+    }
     u32 units = 0u, slots = 0u;
     bool found = false;
+    nu = 1u;
     for (u32 i0 = 0u; i0 < kv.n_seq && !found; i0 += 64u) {
       const u32 mine = i0 + lane < kv.n_seq ? cdiv(steps(i0 + lane), C) : 0u;
-      u32 au = mine, as = mine > 1u ? mine : 0u; // inclusive sums: units, and partial results (of sequences of several)
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const u32 pu = (u32)__shfl_up((int)au, o), ps = (u32)__shfl_up((int)as, o);
-        if ((int)lane >= o) au += pu, as += ps;
-      }
+      const u32 au = wave_scan(mine), as = wave_scan(mine > 1u ? mine : 0u); // units, and partial results (of sequences of several)
       const u64 hit = __ballot(units + au > u);
       if (hit) {
-        const int f = __builtin_ctzll(hit);
-        b = i0 + (u32)f;
-        nu = (u32)__shfl((int)mine, f);
-        ci = u - (units + (u32)__shfl((int)au, f) - nu);
-        slot0 = slots + (u32)__shfl((int)as, f) - (nu > 1u ? nu : 0u);
+        const u32 f = (u32)__builtin_ctzll(hit);
+        b = i0 + f, nu = lane_of(mine, f);
+        ci = u - (units + lane_of(au, f) - nu);
+        slot0 = slots + lane_of(as, f) - (nu > 1u ? nu : 0u);
         found = true;
       }
-      units += (u32)__shfl((int)au, 63), slots += (u32)__shfl((int)as, 63);
+      units += lane_of(au, 63u), slots += lane_of(as, 63u);
     }
     if (!found) return;
   }
-  b = (u32)__builtin_amdgcn_readfirstlane((int)b), ci = (u32)__builtin_amdgcn_readfirstlane((int)ci);
-  nu = (u32)__builtin_amdgcn_readfirstlane((int)nu), slot0 = (u32)__builtin_amdgcn_readfirstlane((int)slot0);
+  nu = (u32)__builtin_amdgcn_readfirstlane((int)nu);
 
-  const u32 r0 = 16u * cb, nr = T * G - r0 < 16u ? T * G - r0 : 16u; // the block's columns
+  const u32 r0 = R * cb, nr = T * G - r0 < R ? T * G - r0 : R; // the block's columns
   const u32 nbq = a.n_q * HD / 32u;
   // row r of the block: its query row and head
   auto at = [&](u32 r, u32 &row, u32 &head) {
@@ -433,225 +469,311 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
     if (a.y) store_y4<BF, F32>(a.y, (u64)row * a.ys + (u64)head * HD + 4u * d4, v, a.vec & 2u);
     if (a.q8) quant_vec4(v, (head * HD + 4u * d4) / 32u, true, a.q8 + (u64)row * a.q8s, nbq);
   };
-  const int Ls = kv.len[b];
+  const int Ls = __builtin_amdgcn_readfirstlane(kv.len[b]);
   if (!trust(Ls)) { // no part: 0; not to be trusted: NaN
     if (Ls != 0) kv_bad(kv, AMDC_BAD_LEN);
     const float v = Ls != 0 ? __builtin_nanf("") : 0.0f;
-    for (u32 i = tid; i < nr * QD; i += 256u) put(i / QD, i % QD, (v4f){v, v, v, v});
+    for (u32 i = tid; i < nr * QD; i += NTH) put(i / QD, i % QD, (v4f){v, v, v, v});
     return;
   }
   const u32 L = (u32)Ls;
 
-  { // the columns' queries into the LDS, as the B operand: part p, values 8 c .. 8 c + 7, column
-    const u32 col = tid >> 4, c0 = tid & 15u;
+  // the columns' queries, loaded before the cache (loads complete in order): thread (column, one of 16) holds values
+  // 8 c .. 8 c + 7 for c = c0, c0 + 16
+  constexpr u32 QE = (16u * R + NTH - 1u) / NTH, QK = HD > 128 ? 2u : 1u;
+  float qv[QE][QK][8];
+#pragma unroll
+  for (u32 e = 0; e < QE; e++) {
+    const u32 col = (tid + NTH * e) >> 4, c0 = tid & 15u;
     u32 row, head;
     at(col < nr ? col : nr - 1u, row, head);
-    const u64 i0 = (u64)row * a.qs + (u64)head * HD;
-    float v[HD > 128 ? 2 : 1][8], big = 0.0f;
 #pragma unroll
-    for (u32 k = 0; 16u * k < HD / 8u; k++) {
+    for (u32 k = 0; k < QK; k++) {
       const u32 c = c0 + 16u * k;
-      if (HD >= 128 || c < HD / 8u) load_q8<BF, F32>(a.q, i0 + 8u * c, a.vec & 1u, v[k]);
-      else
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[k][i] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; i++) big = __builtin_fmaxf(big, __builtin_fabsf(v[k][i]));
+      load_q8<BF, F32>(a.q, (u64)row * a.qs + (u64)head * HD + 8u * (c < HD / 8u ? c : 0u), a.vec & 1u, qv[e][k]);
     }
+  }
+  __asm__ volatile("" ::: "memory");
+
+  // the steps of the wave: every NW-th of the chunk's [s0, s1)
+  const u32 s0 = first(L) / SP + ci * C, send = cdiv(L, SP), s1 = s0 + C < send ? s0 + C : send;
+  const u64 gb = 32ull * HD, hb = gb << (kv.lgp - 4u); // bytes of 16 positions of a head, of a page of a head
+  const u32 pmask = (1u << kv.lgp) - 1u;
+  const int *table = kv.pages + (u64)b * kv.max_pages;
+  u32x4 kr[TT * KS];
+  op vr[DT];
+  const u32 koff = SP == 32u ? g4 * 256u + (8u * ((n >> 2) & 1u) + (n & 3u)) * 16u : g4 * 256u + n * 16u;
+  const u32 voff = SP == 32u ? (g4 & 1u) * (16u * HD) + n * 16u : (g4 >> 1) * (16u * HD) + n * 16u + (g4 & 1u) * 8u;
+  int ids = 0; // of the wave's next 64 / TT steps: lane TT i + j holds the page of the j-th 16 positions of step i
+  bool bad = false;
+  auto get_ids = [&](u32 st) {
+    const u32 s = st + NW * (lane / TT), p = SP * s + 16u * (lane % TT);
+    const bool in = s < s1; // behind the last position: the last page again
+    ids = in ? table[(p < L ? p : L - 1u) >> kv.lgp] : 0;
+    if ((u32)ids >= kv.n_pages) bad = true, ids = 0;
+  };
+  auto base = [&](u32 st, u32 i, u32 j) {
+    const u32 id = lane_of((u32)ids, TT * (i & (64u / TT - 1u)) + j);
+    return ((u64)id * kv.n_kv + h) * hb + (((SP * st + 16u * j) & pmask) >> 4) * gb;
+  };
+  // one round of long chunks: the cache is read once, all of it in the same time, and more than stays in the last-level cache. (The
+  // comments in the assembly keep the compiler from making the two branches one, of ordinary loads.)
+  const bool nt = a.fit && a.ncb == 1u && C * SP >= DEC_NT / (4u * HD);
+  auto load_k = [&](u64 ga, u64 gz) {
+    const uint8_t *p = kv.k + (SP == 32u && n & 8u ? gz : ga) + koff;
+    auto at = [&](u32 i) { return (const u32x4 *)(p + 64u * (i / KS) + 1024u * (i % KS)); };
+    if (nt) {
+      __asm__ volatile("; nontemporal");
+#pragma unroll
+      for (u32 i = 0; i < TT * KS; i++) kr[i] = __builtin_nontemporal_load(at(i));
+      __asm__ volatile("; nontemporal");
+    } else {
+      __asm__ volatile("; cached");
+#pragma unroll
+      for (u32 i = 0; i < TT * KS; i++) kr[i] = *at(i);
+      __asm__ volatile("; cached");
+    }
+  };
+  auto load_v = [&](u64 ga, u64 gz) {
+    const uint8_t *p = kv.v + (SP == 32u && g4 & 2u ? gz : ga) + voff;
+    if (nt) {
+      __asm__ volatile("; nontemporal");
+#pragma unroll
+      for (int d = 0; d < DT; d++) vr[d] = __builtin_nontemporal_load((const op *)(p + 256 * d));
+      __asm__ volatile("; nontemporal");
+    } else {
+      __asm__ volatile("; cached");
+#pragma unroll
+      for (int d = 0; d < DT; d++) vr[d] = *(const op *)(p + 256 * d);
+      __asm__ volatile("; cached");
+    }
+  };
+  u32 st = s0 + wv;
+  u64 ga = 0u, gz = 0u;
+  if (st < s1) {
+    get_ids(st);
+    ga = base(st, 0u, 0u), gz = base(st, 0u, TT - 1u);
+    load_k(ga, gz), load_v(ga, gz);
+  }
+
+  // the queries into the LDS, as the B operand: part p, values 8 c .. 8 c + 7, column
+#pragma unroll
+  for (u32 e = 0; e < QE; e++) {
+    const u32 col = (tid + NTH * e) >> 4, c0 = tid & 15u;
+    float big = 0.0f;
+#pragma unroll
+    for (u32 k = 0; k < QK; k++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) big = __builtin_fmaxf(big, __builtin_fabsf(qv[e][k][i]));
     float up = 1.0f, down = 1.0f;
     if (F32 && !BF) {
       big = __builtin_fmaxf(big, dpp<0xB1>(big));
       big = __builtin_fmaxf(big, dpp<0x4E>(big));
       big = __builtin_fmaxf(big, dpp<0x141>(big));
       big = __builtin_fmaxf(big, dpp<0x140>(big));
-      const u32 e = __builtin_bit_cast(u32, big) >> 23;
-      const u32 k = e < 11u ? 253u : 264u - e; // 2^10 / 2^(e - 127), kept a normal number, as is its inverse
+      const u32 ex = __builtin_bit_cast(u32, big) >> 23;
+      const u32 k = ex < 11u ? 253u : 264u - ex; // 2^10 / 2^(ex - 127), kept a normal number, as is its inverse
       up = __builtin_bit_cast(float, k << 23), down = __builtin_bit_cast(float, (254u - k) << 23);
     }
+    if (col >= R) continue;
     if (c0 == 0u) s_cq[col] = a.c * down;
 #pragma unroll
-    for (u32 k = 0; 16u * k < HD / 8u; k++) {
+    for (u32 k = 0; k < QK; k++) {
       const u32 c = c0 + 16u * k;
-      if (HD < 128 && c >= HD / 8u) break;
+      if (c >= HD / 8u) continue;
       if (F32 && !BF)
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[k][i] *= up;
-      u32x4 w[NP];
-      split8<BF, NP>(v[k], w);
+        for (int i = 0; i < 8; i++) qv[e][k][i] *= up;
+      u32 w[NP][4];
+      split_n<BF, NP>(qv[e][k], w);
 #pragma unroll
-      for (int p = 0; p < NP; p++) *(u32x4 *)(sm + ((p * (HD / 8u) + c) * 16u + col) * 16u) = w[p];
+      for (int p = 0; p < NP; p++) *(u32x4 *)(sm + ((p * (HD / 8u) + c) * R + col) * 16u) = (u32x4){w[p][0], w[p][1], w[p][2], w[p][3]};
     }
-    if (tid == 0u) s_bad = 0u;
   }
-  __syncthreads();
+  if (tid == 0u) s_bad = 0u;
+  v8_barrier(); // not __syncthreads: the first keys and values stay in flight
 
-  // the lane's column: what it sees, and the block's extremes
-  const u32 tc = (r0 + (n < nr ? n : nr - 1u)) / G, t_a = r0 / G, t_z = (r0 + nr - 1u) / G;
+  // the lane's columns: what they see, and the block's extremes
+  const u32 t_a = r0 / G, t_z = (r0 + nr - 1u) / G;
   auto lo_of = [&](u32 t) { const u32 e = L - T + t + 1u; return a.window && e > a.window ? e - a.window : 0u; };
   auto hi_of = [&](u32 t) { return L - T + t + 1u; };
-  const u32 lo = lo_of(tc), hi = hi_of(tc), lo_z = lo_of(t_z), hi_a = hi_of(t_a);
-  const float cq = s_cq[n];
-  const u32 s0 = first(L) / 32u + ci * C, send = cdiv(L, 32u), s1 = s0 + C < send ? s0 + C : send;
-  const u64 gb = 32ull * HD, hb = gb << (kv.lgp - 4u); // bytes of 16 positions of a head, of a page of a head
-  const u32 pmask = (1u << kv.lgp) - 1u;
-  const int *table = kv.pages + (u64)b * kv.max_pages;
-
-  v4f O[DT];
+  u32 tc[NC];
+  float cq[NC], m[NC], l[NC];
+  v4f O[NC][DT];
 #pragma unroll
-  for (int d = 0; d < DT; d++) O[d] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-  float m = NINF, l = 0.0f;
-  u32x4 kr[2 * KS], vr[DT];
-  const u32 koff = g4 * 256u + (8u * ((n >> 2) & 1u) + (n & 3u)) * 16u, voff = (g4 & 1u) * (16u * HD) + n * 16u;
-  int ids = 0; // of the wave's next 32 steps: lane 2 i + j holds the page of the j-th 16 positions of step i
-  bool bad = false;
-  auto get_ids = [&](u32 st) {
-    const u32 s = st + NW * (lane >> 1), p = 32u * s + 16u * (lane & 1u);
-    const bool in = s < s1; // behind the last position: the last page again
-    ids = in ? table[(p < L ? p : L - 1u) >> kv.lgp] : 0;
-    if ((u32)ids >= kv.n_pages) bad = true, ids = 0;
-  };
-  auto base = [&](u32 st, u32 i, u32 j) {
-    const u32 id = (u32)__builtin_amdgcn_readlane(ids, (int)(2u * (i & 31u) + j));
-    return ((u64)id * kv.n_kv + h) * hb + (((32u * st + 16u * j) & pmask) >> 4) * gb;
-  };
-  auto load_k = [&](u64 ga, u64 gz) {
-    const uint8_t *p = kv.k + (n & 8u ? gz : ga) + koff;
+  for (u32 c = 0; c < NC; c++) {
+    tc[c] = (r0 + (16u * c + n < nr ? 16u * c + n : nr - 1u)) / G;
+    cq[c] = s_cq[16u * c + n], m[c] = NINF, l[c] = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 2; t++)
-#pragma unroll
-      for (int s = 0; s < KS; s++) kr[t * KS + s] = *(const u32x4 *)(p + 64 * t + 1024 * s);
-  };
-  auto load_v = [&](u64 ga, u64 gz) {
-    const uint8_t *p = kv.v + (g4 & 2u ? gz : ga) + voff;
-#pragma unroll
-    for (int d = 0; d < DT; d++) vr[d] = *(const u32x4 *)(p + 256 * d);
-  };
-  u32 st = s0 + wv;
-  u64 ga = 0u, gz = 0u;
-  if (st < s1) {
-    get_ids(st);
-    ga = base(st, 0u, 0u), gz = base(st, 0u, 1u);
-    load_k(ga, gz), load_v(ga, gz);
+    for (int d = 0; d < DT; d++) O[c][d] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
   }
+  const u32 lo_z = lo_of(t_z), hi_a = hi_of(t_a);
+  auto mfma_v = [](op v, op p, v4f c) {
+    if constexpr (SP == 32u) return mfma16<BF>(v, p, c);
+    else if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s4, v), __builtin_bit_cast(s4, p), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(h4, v), __builtin_bit_cast(h4, p), c, 0, 0, 0);
+  };
   for (u32 i = 0u; st < s1; i++, st += NW) {
-    v4f S[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-    // heads of 256: the queries are read from the LDS in every step (kept in registers they would spill others)
-    if (HD > 128) __asm__ volatile("" ::: "memory");
+    v4f S[NC][TT];
 #pragma unroll
-    for (int s = 0; s < KS; s++)
+    for (u32 c = 0; c < NC; c++)
 #pragma unroll
-      for (int p = 0; p < NP; p++) {
-        const u32x4 qf = *(const u32x4 *)(sm + ((p * (HD / 8u) + 4u * s + g4) * 16u + n) * 16u);
-        S[0] = mfma16<BF>(kr[s], qf, S[0]);
-        S[1] = mfma16<BF>(kr[KS + s], qf, S[1]);
-      }
+      for (u32 t = 0; t < TT; t++) S[c][t] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+    // heads of 256, or two column tiles: the queries are read from the LDS in every step (kept in registers they would spill others)
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      if ((HD > 128 || NC > 1u) && s % 2 == 0) __asm__ volatile("" ::: "memory");
+#pragma unroll
+      for (u32 c = 0; c < NC; c++)
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          const u32x4 qf = *(const u32x4 *)(sm + ((p * (HD / 8u) + 4u * s + g4) * R + 16u * c + n) * 16u);
+#pragma unroll
+          for (u32 t = 0; t < TT; t++) S[c][t] = mfma16<BF>(kr[t * KS + s], qf, S[c][t]);
+        }
+    }
     const bool more = st + NW < s1;
     if (more) {
-      if ((i & 31u) == 31u) get_ids(st + NW);
-      ga = base(st + NW, i + 1u, 0u), gz = base(st + NW, i + 1u, 1u);
+      if ((i & (64u / TT - 1u)) == 64u / TT - 1u) get_ids(st + NW);
+      ga = base(st + NW, i + 1u, 0u), gz = base(st + NW, i + 1u, TT - 1u);
       load_k(ga, gz);
     }
-    const bool edge = 32u * st + 32u > hi_a || 32u * st < lo_z;
-    float sc[8];
+    const bool edge = SP * st + SP > hi_a || SP * st < lo_z;
+    op pw[NC][NP];
 #pragma unroll
-    for (int k = 0; k < 8; k++) sc[k] = S[k >> 2][k & 3] * cq;
-    if (edge)
+    for (u32 c = 0; c < NC; c++) {
+      float sc[SL], top = NINF;
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const u32 p = 32u * st + 8u * g4 + (u32)k;
-        sc[k] = p >= lo && p < hi ? sc[k] : NINF;
+      for (u32 k = 0; k < SL; k++) sc[k] = S[c][k >> 2][k & 3u] * cq[c];
+      if (edge) {
+        const u32 lo = lo_of(tc[c]), hi = hi_of(tc[c]);
+#pragma unroll
+        for (u32 k = 0; k < SL; k++) {
+          const u32 p = SP * st + SL * g4 + k;
+          sc[k] = p >= lo && p < hi ? sc[k] : NINF;
+        }
       }
-    float top = sc[0];
 #pragma unroll
-    for (int k = 1; k < 8; k++) top = __builtin_fmaxf(top, sc[k]);
-    if (__ballot(top > m + RAISE)) {
-      top = __builtin_fmaxf(top, __shfl_xor(top, 16));
-      top = __builtin_fmaxf(top, __shfl_xor(top, 32));
-      const float nm = __builtin_fmaxf(m, top), f = m == nm ? 1.0f : __builtin_amdgcn_exp2f(m - nm);
+      for (u32 k = 0; k < SL; k++) top = __builtin_fmaxf(top, sc[k]);
+      if (__ballot(top > m[c] + RAISE)) {
+        top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+        top = __builtin_fmaxf(top, __shfl_xor(top, 32));
+        const float nm = __builtin_fmaxf(m[c], top), f = m[c] == nm ? 1.0f : __builtin_amdgcn_exp2f(m[c] - nm);
 #pragma unroll
-      for (int d = 0; d < DT; d++) O[d] *= f;
-      l *= f;
-      m = nm;
+        for (int d = 0; d < DT; d++) O[c][d] *= f;
+        l[c] *= f;
+        m[c] = nm;
+      }
+      const float ref = BIAS - (m[c] == NINF ? 0.0f : m[c]);
+#pragma unroll
+      for (u32 k = 0; k < SL; k++) sc[k] = __builtin_amdgcn_exp2f(sc[k] + ref);
+#pragma unroll
+      for (u32 k = 0; k < SL; k += 4u) l[c] += (sc[k] + sc[k + 1u]) + (sc[k + 2u] + sc[k + 3u]);
+      u32 w[NP][SL / 2];
+      split_n<BF, NP>(sc, w);
+#pragma unroll
+      for (int p = 0; p < NP; p++)
+#pragma unroll
+        for (u32 k = 0; k < SL / 2u; k++) pw[c][p][k] = w[p][k];
     }
-    const float ref = BIAS - (m == NINF ? 0.0f : m);
-#pragma unroll
-    for (int k = 0; k < 8; k++) sc[k] = __builtin_amdgcn_exp2f(sc[k] + ref);
-    l += ((sc[0] + sc[1]) + (sc[2] + sc[3])) + ((sc[4] + sc[5]) + (sc[6] + sc[7]));
-    u32x4 pw[NP];
-    split8<BF, NP>(sc, pw);
     if (!edge) {
 #pragma unroll
       for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int p = 0; p < NP; p++) O[d] = mfma16<BF>(vr[d], pw[p], O[d]);
+        for (u32 c = 0; c < NC; c++)
+#pragma unroll
+          for (int p = 0; p < NP; p++) O[c][d] = mfma_v(vr[d], pw[c][p], O[c][d]);
     } else {
 #pragma unroll
-      for (int d = 0; d < DT; d++) {
-        v4f e = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (u32 c = 0; c < NC; c++)
 #pragma unroll
-        for (int p = 0; p < NP; p++) e = mfma16<BF>(vr[d], pw[p], e);
-        auto again = [&](u32 from, u32 to) {
-          e = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-          const u32x4 w = seen16(vr[d], 32u * st + 8u * g4, from, to);
+        for (int d = 0; d < DT; d++) {
+          v4f e = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int p = 0; p < NP; p++) e = mfma16<BF>(w, pw[p], e);
-        };
-        if (!wave_finite(e)) again(lo_of(t_a), hi_of(t_z)); // without what no column sees: the common case behind the last position
-        if (wave_finite(e)) O[d] += e;
-        else
-          for (u32 t = t_a; t <= t_z; t++) {
-            again(lo_of(t), hi_of(t));
-            if (tc == t) O[d] += e;
-          }
-      }
+          for (int p = 0; p < NP; p++) e = mfma_v(vr[d], pw[c][p], e);
+          auto again = [&](u32 from, u32 to) {
+            e = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+            const op w = seen16(vr[d], SP * st + SL * g4, from, to);
+#pragma unroll
+            for (int p = 0; p < NP; p++) e = mfma_v(w, pw[c][p], e);
+          };
+          if (!wave_finite(e)) again(lo_of(t_a), hi_of(t_z)); // without what no column sees: the common case behind the last position
+          if (wave_finite(e)) O[c][d] += e;
+          else
+            for (u32 t = t_a; t <= t_z; t++) {
+              again(lo_of(t), hi_of(t));
+              if (tc[c] == t) O[c][d] += e;
+            }
+        }
     }
     if (more) load_v(ga, gz);
   }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
   if (__ballot(bad)) {
     if (lane == 0u) kv_bad(kv, AMDC_BAD_PAGE), s_bad = 1u;
   }
-  __syncthreads(); // the queries are read, their place is the waves' results'
-  float *so = (float *)sm;
+  // the waves' sums brought to one reference and added: NS of them through the LDS (the others' onto the first NS' before)
 #pragma unroll
-  for (int d = 0; d < DT; d++) *(v4f *)(so + (wv * 16u + n) * OS + 16u * d + 4u * g4) = O[d];
-  if (g4 == 0u) s_m[wv][n] = m, s_l[wv][n] = l;
-  __syncthreads();
-  if (tid < 16u) {
-    float M = s_m[0][tid], sum = 0.0f;
-#pragma unroll
-    for (u32 w = 1; w < NW; w++) M = __builtin_fmaxf(M, s_m[w][tid]);
-#pragma unroll
-    for (u32 w = 0; w < NW; w++) {
-      const float f = __builtin_amdgcn_exp2f(s_m[w][tid] - (M == NINF ? 0.0f : M));
-      s_m[w][tid] = f, sum += f * s_l[w][tid];
-    }
-    s_M[tid] = M, s_L[tid] = s_bad ? __builtin_nanf("") : sum;
+  for (u32 c = 0; c < NC; c++) {
+    l[c] += __shfl_xor(l[c], 16);
+    l[c] += __shfl_xor(l[c], 32);
+    if (g4 == 0u) s_m[wv][16u * c + n] = m[c], s_l[wv][16u * c + n] = l[c];
   }
+  __syncthreads(); // and the queries are read, their place is the sums'
+  float *so = (float *)sm;
+  auto give = [&](u32 to) {
+#pragma unroll
+    for (u32 c = 0; c < NC; c++)
+#pragma unroll
+      for (int d = 0; d < DT; d++) *(v4f *)(so + (to * R + 16u * c + n) * OS + 16u * d + 4u * g4) = O[c][d];
+  };
+#pragma unroll
+  for (u32 c = 0; c < NC; c++) {
+    float M = s_m[0][16u * c + n];
+#pragma unroll
+    for (u32 w = 1; w < NW; w++) M = __builtin_fmaxf(M, s_m[w][16u * c + n]);
+    const float ref = M == NINF ? 0.0f : M, f = __builtin_amdgcn_exp2f(m[c] - ref);
+#pragma unroll
+    for (int d = 0; d < DT; d++) O[c][d] *= f;
+    if (wv == 0u && g4 == 0u) {
+      float sum = 0.0f;
+#pragma unroll
+      for (u32 w = 0; w < NW; w++) sum += __builtin_amdgcn_exp2f(s_m[w][16u * c + n] - ref) * s_l[w][16u * c + n];
+      s_M[16u * c + n] = M, s_L[16u * c + n] = s_bad ? __builtin_nanf("") : sum;
+    }
+  }
+  if (NW > NS) {
+    if (wv >= NS) give(wv - NS);
+    __syncthreads();
+    if (wv < NS)
+#pragma unroll
+      for (u32 c = 0; c < NC; c++)
+#pragma unroll
+        for (int d = 0; d < DT; d++) O[c][d] += *(const v4f *)(so + (wv * R + 16u * c + n) * OS + 16u * d + 4u * g4);
+  }
+  if (wv < NS) give(wv);
   __syncthreads();
   auto mine = [&](u32 i) { // quad i of the workgroup's sums
     const u32 r = i / QD, d4 = i % QD;
-    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+    v4f v = *(const v4f *)(so + r * OS + 4u * d4);
 #pragma unroll
-    for (u32 w = 0; w < NW; w++) v += s_m[w][r] * *(const v4f *)(so + (w * 16u + r) * OS + 4u * d4);
+    for (u32 w = 1; w < NS; w++) v += *(const v4f *)(so + (w * R + r) * OS + 4u * d4);
     return v;
   };
   if (nu == 1u) {
-    for (u32 i = tid; i < nr * QD; i += 256u) put(i / QD, i % QD, mine(i) / s_L[i / QD]);
+    for (u32 i = tid; i < nr * QD; i += NTH) put(i / QD, i % QD, mine(i) / s_L[i / QD]);
     return;
   }
-  // partial results: nr rows of O, then m and l of 16 rows
-  const u32 rmax = T * G < 16u ? T * G : 16u, sb = (rmax * HD + 32u) * 4u;
+  // partial results: rmax rows of O, then m and l of R rows
+  const u32 rmax = T * G < R ? T * G : R, om = rmax * HD * 4u, sb = om + 8u * R;
   uint8_t *parts = a.ws + ATTN_CNT;
   auto slot = [&](u32 k) { return ((u64)(slot0 + k) * kv.n_kv + h) * a.ncb + cb; };
   auto part = [&](u32 k) { return rsrc(parts + slot(k) * sb, sb); };
   {
     const __amdgpu_buffer_rsrc_t d = part(ci);
-    for (u32 i = tid; i < nr * QD; i += 256u) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, mine(i)), d, 16u * i, 0, CPOL_SC1);
+    for (u32 i = tid; i < nr * QD; i += NTH) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, mine(i)), d, 16u * i, 0, CPOL_SC1);
     if (tid < nr) {
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_M[tid]), d, rmax * HD * 4u + 4u * tid, 0, CPOL_SC1);
-      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_L[tid]), d, rmax * HD * 4u + 64u + 4u * tid, 0, CPOL_SC1);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_M[tid]), d, om + 4u * tid, 0, CPOL_SC1);
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_L[tid]), d, om + 4u * (R + tid), 0, CPOL_SC1);
     }
   }
   u32 k = ci, left = nu, stride = 1u;
@@ -668,57 +790,65 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
       }
       __syncthreads();
       if (!s_last) return;
-      // weights of the cnt results of every row, in the LDS (so is free: the results are in the workspace)
+      // a thread's first quads of the cnt results, then the weights of every row's results in the LDS (so is free: the
+      // results are in the workspace)
+      u32x4 v[DEC_FAN];
+      auto get = [&](u32 i) {
+#pragma unroll
+        for (u32 j = 0; j < DEC_FAN; j++) v[j] = __builtin_amdgcn_raw_buffer_load_b128(part((f0 + (j < cnt ? j : 0u)) * stride), 16u * i, 0, CPOL_SC1);
+      };
+      if (tid < nr * QD) get(tid);
       float *sw = (float *)sm;
-      if (tid < 16u * DEC_FAN) {
-        const u32 r = tid & 15u, j = tid >> 4;
-        const __amdgpu_buffer_rsrc_t d = part((f0 + (j < cnt ? j : 0u)) * stride);
+      for (u32 e = tid; e < R * DEC_FAN; e += NTH) {
+        const u32 r = e % R, j = e / R;
+        const uint8_t *d = parts + slot((f0 + (j < cnt ? j : 0u)) * stride) * sb + om + 4u * r;
         const bool in = j < cnt && r < nr;
-        sw[tid] = in ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(d, rmax * HD * 4u + 4u * r, 0, CPOL_SC1)) : NINF;
-        sw[16u * DEC_FAN + tid] = in ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(d, rmax * HD * 4u + 64u + 4u * r, 0, CPOL_SC1)) : 0.0f;
+        sw[e] = in ? __hip_atomic_load((const float *)d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : NINF;
+        sw[R * DEC_FAN + e] = in ? __hip_atomic_load((const float *)(d + 4u * R), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f;
       }
       __syncthreads();
-      if (tid < 16u) {
+      if (tid < R) {
         float M = NINF, sum = 0.0f;
 #pragma unroll
-        for (u32 j = 0; j < DEC_FAN; j++) M = __builtin_fmaxf(M, sw[16u * j + tid]);
+        for (u32 j = 0; j < DEC_FAN; j++) M = __builtin_fmaxf(M, sw[R * j + tid]);
 #pragma unroll
         for (u32 j = 0; j < DEC_FAN; j++) {
-          const float f = __builtin_amdgcn_exp2f(sw[16u * j + tid] - (M == NINF ? 0.0f : M));
-          sw[16u * j + tid] = f, sum += f * sw[16u * (DEC_FAN + j) + tid];
+          const float f = __builtin_amdgcn_exp2f(sw[R * j + tid] - (M == NINF ? 0.0f : M));
+          sw[R * j + tid] = f, sum += f * sw[R * (DEC_FAN + j) + tid];
         }
         s_M[tid] = M, s_L[tid] = sum;
       }
       __syncthreads();
       const bool final = left <= DEC_FAN;
       const __amdgpu_buffer_rsrc_t to = part(f0 * stride);
-      for (u32 i = tid; i < nr * QD; i += 256u) {
-        u32x4 v[DEC_FAN];
-#pragma unroll
-        for (u32 j = 0; j < DEC_FAN; j++) v[j] = __builtin_amdgcn_raw_buffer_load_b128(part((f0 + (j < cnt ? j : 0u)) * stride), 16u * i, 0, CPOL_SC1);
+      for (u32 i = tid; i < nr * QD; i += NTH) {
+        if (i != tid) get(i);
         v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (u32 j = 0; j < DEC_FAN; j++)
-          if (j < cnt) sum += sw[16u * j + i / QD] * __builtin_bit_cast(v4f, v[j]);
+          if (j < cnt) sum += sw[R * j + i / QD] * __builtin_bit_cast(v4f, v[j]);
         if (final) put(i / QD, i % QD, sum / s_L[i / QD]);
         else __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), to, 16u * i, 0, CPOL_SC1);
       }
       if (final) return;
       if (tid < nr) {
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_M[tid]), to, rmax * HD * 4u + 4u * tid, 0, CPOL_SC1);
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_L[tid]), to, rmax * HD * 4u + 64u + 4u * tid, 0, CPOL_SC1);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_M[tid]), to, om + 4u * tid, 0, CPOL_SC1);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, s_L[tid]), to, om + 4u * (R + tid), 0, CPOL_SC1);
       }
     }
     k /= DEC_FAN, left = cdiv(left, DEC_FAN), stride *= DEC_FAN;
   }
 }
 
-#define DEC_KERNEL(HD, KN, BF, F32) \
-  extern "C" __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void amdc_attn_dec_h##HD##_##KN(amdc_kv_dev kv, AttnArgs a) { dec_body<HD, BF, F32>(kv, a); }
-#define DEC_KERNELS(HD) DEC_KERNEL(HD, f16, false, false) DEC_KERNEL(HD, f16_f32, false, true) DEC_KERNEL(HD, bf16, true, false) DEC_KERNEL(HD, bf16_f32, true, true)
-DEC_KERNELS(64)
-DEC_KERNELS(128)
-DEC_KERNELS(256)
+#define DEC_KERNEL(HD, KN, TAG, BF, F32, NC) \
+  extern "C" __global__ __launch_bounds__(512, 2) void amdc_attn_dec_h##HD##_##KN##TAG(amdc_kv_dev kv, AttnArgs a) { dec_body<HD, BF, F32, NC, 8u>(kv, a); }
+#define DEC_KERNELS(HD, TAG, NC) \
+  DEC_KERNEL(HD, f16, TAG, false, false, NC) DEC_KERNEL(HD, f16_f32, TAG, false, true, NC) DEC_KERNEL(HD, bf16, TAG, true, false, NC) DEC_KERNEL(HD, bf16_f32, TAG, true, true, NC)
+DEC_KERNELS(64, , 1u)
+DEC_KERNELS(128, , 1u)
+DEC_KERNELS(256, , 1u)
+DEC_KERNELS(64, _n2, 2u)
+DEC_KERNELS(128, _n2, 2u)
 #undef DEC_KERNELS
 #undef DEC_KERNEL
 

@@ -290,11 +290,13 @@ enum {
   K_GEMVS8, /* amdc_gemv_q8_0_s1, _s2, _xs1, (none), amdc_gemv_q6_k_s1, (none), _xs1, (none), then _s1l, _s2l, _xs1l, _xs2l, ... */
   K_APPEND = K_GEMVS8 + 15, /* amdc_kv_append_f16, _bf16 */
   K_ATTN_DEC = K_APPEND + 2, /* amdc_attn_dec_h64_f16, _f16_f32, _bf16, _bf16_f32, then h128, h256 */
-  K_ATTN_PRE = K_ATTN_DEC + 12, /* amdc_attn_pre_h64_f16, .. */
+  K_ATTN_DEC2 = K_ATTN_DEC + 12, /* amdc_attn_dec_h64_f16_n2, .. */
+  K_ATTN_PRE = K_ATTN_DEC2 + 8, /* amdc_attn_pre_h64_f16, .. */
   K_N = K_ATTN_PRE + 12
 };
 
 #define KN(s) "amdc_" s
+#define KA2(s) KN(s "_f16_n2"), KN(s "_f16_f32_n2"), KN(s "_bf16_n2"), KN(s "_bf16_f32_n2")
 #define KA(s) KN(s "_f16"), KN(s "_f16_f32"), KN(s "_bf16"), KN(s "_bf16_f32")
 #define GW(s) "amdc_gemmw_" s
 static const char *const kname[K_N] = {
@@ -325,7 +327,7 @@ static const char *const kname[K_N] = {
     KN("gemv_q8_0_s1"), KN("gemv_q8_0_s2"), KN("gemv_q8_0_xs1"), KN("gemv_q8_0_xs1"), KN("gemv_q6_k_s1"), KN("gemv_q6_k_s1"), KN("gemv_q6_k_xs1"),
     KN("gemv_q6_k_xs1"), KN("gemv_q8_0_s1l"), KN("gemv_q8_0_s2l"), KN("gemv_q8_0_xs1l"), KN("gemv_q8_0_xs2l"), KN("gemv_q6_k_s1l"),
     KN("gemv_q6_k_s1l"), KN("gemv_q6_k_xs1l"), KN("kv_append_f16"), KN("kv_append_bf16"),
-    KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256"),
+    KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256"), KA2("attn_dec_h64"), KA2("attn_dec_h128"),
     KA("attn_pre_h64"), KA("attn_pre_h128"), KA("attn_pre_h256")};
 
 static hipModule_t g_mod;
@@ -1697,7 +1699,7 @@ typedef struct {
   const int32_t *cu;
   uint8_t *q8, *ws;
   float c;
-  u32 n_q, G, T, qs, ys, window, q8s, U, vec, ncb;
+  u32 n_q, G, T, qs, ys, window, q8s, U, vec, ncb, fit;
 } attn_args;
 #define ATTN_CNT 65536u /* bytes of counters at the start of the workspace (amdc_attn.h) */
 
@@ -1726,44 +1728,53 @@ static int attn_kernel(int k0, const amdc_kv *kv, int t) {
   return k0 + (kv->hd == 64u ? 0 : kv->hd == 128u ? 4 : 8) + (kv->type == AMDC_TYPE_BF16 ? 2 : 0) + (t == AMDC_TYPE_F32 ? 1 : 0);
 }
 
-/* A call of the decode kernel: blocks of 16 columns, and chunks wanted of a head (dec_body in amdc_attn.h) so that the workgroups of
- * all heads fill the CUs; 0 where the call is refused. The partial results of a call are those of sequences of several
- * chunks, under twice U, and of U + n_seq chunks in all. */
-static u32 dec_units(u32 n_kv, u32 n_q, u32 hd, u32 T, u32 *ncb) {
+/* A call of the decode kernel (dec_body in amdc_attn.h): the columns of a block, R, and their blocks, ncb; and the chunks wanted of a
+ * head, U, of a workgroup each (0 where the call is refused). One workgroup is resident on a CU. Where the sequences leave room (fit),
+ * one round: U chunks of a head fill the CUs, and no more. Else twice that, so that long sequences among short ones are spread
+ * (MI355X, us at U x 1, 2, 3, 4: 64 sequences of 30 to 16000, 32 / 8 heads of 128 152, 136, 133, 134; 16 of 200 to 2500, 32 / 32
+ * heads - 61, 63, 67; one of 60001 in rounds 54, 62, 67).
+ * Blocks of 32 columns from 17 on, where their registers suffice (heads of up to 128; 8 sequences of 900 to 6000, T = 8, 32 / 8 heads of
+ * 128: 31 us, 35 in two blocks of 16). The partial results of a call are those of sequences of several chunks, under twice U,
+ * and of U + n_seq chunks in all. */
+static u32 dec_units(u32 n_kv, u32 n_q, u32 hd, u32 T, u32 n_seq, u32 *R, u32 *ncb, u32 *fit) {
   const u64 cols = (u64)T * (n_q / n_kv);
   if (!T || cols > 128u) return 0;
-  *ncb = (u32)(cols + 15u) / 16u;
-  const u32 cus = g_cus > 0 ? (u32)g_cus : 256u, heads = n_kv * *ncb, wgs = cus * (hd > 128u ? 1u : 2u);
-  u32 U = wgs / heads, most = ATTN_CNT / 8u / heads; /* counters: one to a partial result */
-  if (U > 256u) U = 256u;
+  *R = cols > 16u && hd <= 128u ? 32u : 16u;
+  *ncb = (u32)(cols + *R - 1u) / *R;
+  const u32 cus = g_cus > 0 ? (u32)g_cus : 256u, heads = n_kv * *ncb;
+  u32 U = cus / heads, most = ATTN_CNT / 8u / heads; /* counters: one to a partial result */
+  *fit = 2u * n_seq <= U;
+  if (!*fit) U = cus * 2u / heads;
   if (U > most) U = most;
   return U ? U : 1u;
 }
 
 size_t amdc_attn_decode_ws(const amdc_kv *kv, uint32_t n_q, uint32_t T) {
   if (!kv || !amdc_kv_bytes(kv->type, kv->n_kv, kv->hd, kv->page, kv->n_pages) || !n_q || n_q % kv->n_kv) return 0;
-  u32 ncb = 0;
-  const u32 U = dec_units(kv->n_kv, n_q, kv->hd, T, &ncb);
+  u32 ncb = 0, R = 0, fit;
+  const u32 U = dec_units(kv->n_kv, n_q, kv->hd, T, kv->n_seq, &R, &ncb, &fit);
   if (!U) return 0;
-  const u64 slots = U > kv->n_seq ? (u64)U + kv->n_seq : 2ull * U, cols = (u64)T * (n_q / kv->n_kv), r = cols < 16u ? cols : 16u;
-  return (size_t)(ATTN_CNT + slots * kv->n_kv * ncb * (r * kv->hd + 32u) * 4u);
+  const u64 slots = U > kv->n_seq ? (u64)U + kv->n_seq : 2ull * U, cols = (u64)T * (n_q / kv->n_kv), r = cols < R ? cols : R;
+  return (size_t)(ATTN_CNT + slots * kv->n_kv * ncb * (r * kv->hd + 2u * R) * 4u);
 }
 
 int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
                      uint32_t window, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream) {
   NEED_OPEN();
   amdc_kv_dev d;
-  u32 rows = 0, ncb = 0;
+  u32 rows = 0, ncb = 0, R = 0, fit = 0;
   int rc = check_kv("attn_decode", kv, n_q, T, NULL, &d, &rows);
   if (rc) return rc;
-  const u32 U = dec_units(kv->n_kv, n_q, kv->hd, T, &ncb);
+  const u32 U = dec_units(kv->n_kv, n_q, kv->hd, T, kv->n_seq, &R, &ncb, &fit);
   if (!U) return fail(AMDC_EINVAL, "attn_decode: T %u of %u query heads to a key / value head (at most 128 together)", T, n_q / kv->n_kv);
   if ((rc = check_attn("attn_decode", kv, q, y, t, n_q, rows, qs, ys, q8, q8s, ws, ws_bytes, amdc_attn_decode_ws(kv, n_q, T)))) return rc;
-  const u64 grid = ((u64)U + kv->n_seq) * kv->n_kv * ncb;
-  if (grid >= (1u << 24)) return fail(AMDC_EINVAL, "attn_decode: %u sequences of %u heads are too many for one call", kv->n_seq, kv->n_kv);
-  attn_args a = {q, y, NULL, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, U, attn_vec(q, y, t, rows, qs, ys), ncb};
+  /* the workgroups of a unit's blocks of columns are 8 apart */
+  const u64 grid = (((u64)U + kv->n_seq) * kv->n_kv + 7u) / 8u * 8u * ncb;
+  if (grid >= (1u << 23) || (u64)kv->n_seq * d.cap >= (1ull << 36))
+    return fail(AMDC_EINVAL, "attn_decode: %u sequences of %u heads and up to %u positions are too many for one call", kv->n_seq, kv->n_kv, d.cap);
+  attn_args a = {q, y, NULL, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, U, attn_vec(q, y, t, rows, qs, ys), ncb, fit};
   void *args[] = {&d, &a};
-  return launch(attn_kernel(K_ATTN_DEC, kv, t), (unsigned)grid, 1, 0, stream, args);
+  return launch_nt(attn_kernel(R > 16u ? K_ATTN_DEC2 : K_ATTN_DEC, kv, t), (unsigned)grid, 1, 512u, 0, stream, args);
 }
 
 /* A call of the prompt kernel: tiles of PRE_BM rows of a head at most, and the parts that a tile's positions are split into where
@@ -1796,7 +1807,7 @@ int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t
   const u32 tiles = pre_tiles(kv, n_q, rows, cu != NULL, T, &parts);
   const u64 grid = (u64)tiles * parts * kv->n_kv;
   if (grid >= (1u << 24)) return fail(AMDC_EINVAL, "attn_prefill: %u rows of %u sequences and %u heads are too many for one call", rows, kv->n_seq, kv->n_kv);
-  attn_args a = {q, y, cu, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, parts, attn_vec(q, y, t, rows, qs, ys), tiles};
+  attn_args a = {q, y, cu, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, parts, attn_vec(q, y, t, rows, qs, ys), tiles, 0};
   void *args[] = {&d, &a};
   return launch_pre(attn_kernel(K_ATTN_PRE, kv, t), kv->hd, (unsigned)grid, stream, args);
 }

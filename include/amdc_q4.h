@@ -343,7 +343,7 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
  * ws: amdc_attn_decode_ws(kv, n_q, T) bytes of device memory, 16-byte aligned, cleared to 0 once before the first use
  * with any call (the calls leave its counters at 0); calls that share it must not overlap on the device, calls with
  * workspaces of their own may. The size does not depend on the lengths. Nothing is allocated: every call can be
- * captured. The result does not depend on the order in which workgroups run. */
+ * captured. The result does not depend on the order in which workgroups run. n_seq max_pages page is under 2^36. */
 size_t amdc_attn_decode_ws(const amdc_kv *kv, uint32_t n_q, uint32_t T);
 int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
                      uint32_t window, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream);

@@ -97,13 +97,18 @@ CASES = [
     (F16, F16, 12, 12, 64, 16, 16, 0, (16, 17, 90)),
     (BF16, BF16, 8, 8, 128, 16, 1, 0, tuple(20 + 37 * i % 400 for i in range(150))),  # over 128 sequences
     (F16, F16, 4, 1, 128, 16, 1, 0, tuple(1 + (i * i * 7) % 3000 for i in range(70))),
+    (F16, F32, 2, 1, 128, 64, 1, 0, (190_000,)),  # chunks long enough for nontemporal loads
+    (BF16, BF16, 6, 1, 256, 16, 1, 0, (90_000, 33_000)),
+    (F16, F16, 32, 1, 128, 16, 1, 0, (5000, 1, 300)),  # one block of 32 columns, split
+    (BF16, F32, 20, 1, 64, 16, 3, 0, (3000, 70)),  # blocks of 32 and 28
+    (F16, F16, 128, 128, 64, 16, 1, 0, (700, 31)),  # more heads than CUs leave room for
 ]
 
 
 @pytest.mark.parametrize("i", range(len(CASES)))
 def test_decode(dev, i):
     ty, t, n_q, n_kv, hd, page, T, window, lens = CASES[i]
-    print(CASES[i], flush=True)
+    print(CASES[i] if len(lens) < 20 else CASES[i][:-1], flush=True)
     c = Case(dev, 200 + i, ty, n_q, n_kv, hd, page, lens, (T,) * len(lens)).fill_all().upload()
     Call(c, t, T, window).launch().check()
 
