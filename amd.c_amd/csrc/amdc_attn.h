@@ -4,11 +4,12 @@
 //   amdc_kv_append_{f16,bf16}   rotation, keys and values into the cache, rotated queries
 //   amdc_attn_dec_h{64,128,256}_{f16,f16_f32,bf16,bf16_f32}
 //                               attention of a few new tokens per sequence
-//   amdc_attn_pre_h{64,128,256}_{f16,f16_f32,bf16,bf16_f32}
+//   amdc_attn_pre_h{64,128,256}_{f16,f16_f32,bf16,bf16_f32}, amdc_attn_join_{f32,f16,bf16}
 //                               attention of prompts and prompt chunks
 
 // ------------------------------------------------------------------ helpers
 
+__device__ __forceinline__ u32 uniform(u32 v) { return (u32)__builtin_amdgcn_readfirstlane((int)v); }
 // n / d rounded up
 __device__ __forceinline__ u32 cdiv(u32 n, u32 d) { return (n + d - 1u) / d; }
 
@@ -125,19 +126,21 @@ __device__ __forceinline__ void load8(const float *p, bool vec, float (&x)[8]) {
   }
 }
 
-// Workgroups 0 .. rows gq - 1: queries and keys, gq of them to a row. The row's n_rot / 2 angles once, into the LDS, then
-// eight values a thread: a key's eight are 16 bytes of the cache. Where the pairs are halves apart a thread reads the
-// other eight as well (from the L1) instead of trading them.
-// The others: values, gv workgroups to a group of eight positions of a sequence, aligned as the cache is (for ragged
-// rows, cu[b] / 8 + 2 b is a first group of b's that leaves room for its floor(m / 8) + 2 at most). A thread reads one
-// value of up to eight rows and stores them as 16 bytes, or where the group is not full the new ones alone.
+// Reading and writing bound it. Queries and keys: the first nrw workgroups, a wave to a row (or gq waves, where the rows are few). The
+// row's n_rot / 2 angles once, into the wave's part of the LDS, then eight values a lane, whole heads at a time: a key's eight are 16
+// bytes of the cache. Where the pairs are halves apart a lane reads the other eight as well (from the L1) instead of trading them.
+// Values: the other workgroups, gv of them to a group of eight positions of a sequence, aligned as the cache is (for ragged rows,
+// cu[b] / 8 + 2 b is a first group of b's that leaves room for its floor(m / 8) + 2 at most). A thread reads one value (four, where the
+// rows are aligned) of up to eight rows and stores each value's positions as 16 bytes, or where the group is not full the new ones alone.
+// Measured on MI355X: 8657 rows of 32 + 8 + 8 heads of 128 (319 MB) 79 us; a workgroup to a row 87, three to a row 110.
 template <bool BF>
 __device__ __forceinline__ void append_body(const amdc_kv_dev &kv, const AppendArgs &a) {
-  __shared__ float s_cos[128], s_sin[128];
-  const u32 hd = 1u << a.lghd, tid = threadIdx.x, nrw = a.rows * a.gq;
+  __shared__ float s_cos[4][128], s_sin[4][128];
+  const u32 hd = 1u << a.lghd, tid = threadIdx.x, nrw = cdiv(a.rows * a.gq, 4u);
   const u64 gb = 32ull << a.lghd, lgg = kv.lgp - 4u; // bytes of 16 positions of a head, log2 of such groups in a page
   if (blockIdx.x < nrw) {
-    const u32 row = blockIdx.x / a.gq, part = blockIdx.x - row * a.gq;
+    const u32 lane = tid & 63u, wv = uniform(tid >> 6), w = 4u * blockIdx.x + wv, row = w / a.gq, part = w - row * a.gq;
+    if (row >= a.rows) return;
     const u32 b = a.cu ? find_seq(kv.n_seq, row, [&](u32 i) { const int c = a.cu[i]; return c < 0 ? 0u : (u32)c; }) : row / a.T;
     const SeqRows s = seq_rows(kv, a.cu, a.T, b);
     if (!s.len || row < s.row0 || row - s.row0 >= s.m) return;
@@ -147,53 +150,52 @@ __device__ __forceinline__ void append_body(const amdc_kv_dev &kv, const AppendA
     if (!ok) kv_bad(kv, AMDC_BAD_PAGE);
     const u32 half = a.n_rot >> 1;
     if (a.rope) {
-      if (tid < half) sincos64((double)pos * (double)a.freq[tid], s_sin[tid], s_cos[tid]);
-      __syncthreads();
+      for (u32 i = lane; i < half; i += 64u) sincos64((double)pos * (double)a.freq[i], s_sin[wv][i], s_cos[wv][i]);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); // the wave's own LDS: in order, once the compiler keeps them so
+      __builtin_amdgcn_wave_barrier();
     }
-    const u32 nq = a.q ? a.n_q : 0u, nh = nq + kv.n_kv, hpi = 2048u >> a.lghd;
-    const u32 slot = pos & ((1u << kv.lgp) - 1u), c = tid & ((hd >> 3) - 1u);
+    const u32 nq = a.q ? a.n_q : 0u, nh = nq + kv.n_kv, hpi = 512u >> a.lghd;
+    const u32 slot = pos & ((1u << kv.lgp) - 1u), c = lane & ((hd >> 3) - 1u);
     for (u32 h0 = part * hpi; h0 < nh; h0 += a.gq * hpi) {
-      const u32 h = h0 + (tid >> (a.lghd - 3u));
-      const bool on = h < nh;
+      const u32 h = h0 + (lane >> (a.lghd - 3u));
+      if (h >= nh) break;
       float x[8];
-      if (on) {
-        const float *src = h < nq ? a.q + (u64)row * a.qs + (u64)h * hd : a.k + (u64)row * a.ks + (u64)(h - nq) * hd;
-        load8(src + 8u * c, a.vec & (h < nq ? 1u : 2u), x);
-        if (a.rope == 1u) { // pairs
+      const float *src = h < nq ? a.q + (u64)row * a.qs + (u64)h * hd : a.k + (u64)row * a.ks + (u64)(h - nq) * hd;
+      load8(src + 8u * c, a.vec & (h < nq ? 1u : 2u), x);
+      if (a.rope == 1u) { // pairs
 #pragma unroll
-          for (u32 i = 0; i < 8u; i += 2u) {
-            const u32 e = 8u * c + i;
-            if (e < a.n_rot) {
-              const float cs = s_cos[e >> 1], sn = s_sin[e >> 1], u = x[i], w = x[i + 1u];
-              x[i] = u * cs - w * sn, x[i + 1u] = u * sn + w * cs;
-            }
+        for (u32 i = 0; i < 8u; i += 2u) {
+          const u32 e = 8u * c + i;
+          if (e < a.n_rot) {
+            const float cs = s_cos[wv][e >> 1], sn = s_sin[wv][e >> 1], u = x[i], v = x[i + 1u];
+            x[i] = u * cs - v * sn, x[i + 1u] = u * sn + v * cs;
           }
-        } else if (a.rope == 2u && 8u * c < a.n_rot) { // halves
-          float o[8];
-          if (!(half & 7u)) load8(src + (8u * c < half ? 8u * c + half : 8u * c - half), a.vec & (h < nq ? 1u : 2u), o);
-          else
-#pragma unroll
-            for (u32 i = 0; i < 8u; i++) {
-              const u32 e = 8u * c + i;
-              o[i] = e < a.n_rot ? src[e < half ? e + half : e - half] : 0.0f;
-            }
+        }
+      } else if (a.rope == 2u && 8u * c < a.n_rot) { // halves
+        float o[8];
+        if (!(half & 7u)) load8(src + (8u * c < half ? 8u * c + half : 8u * c - half), a.vec & (h < nq ? 1u : 2u), o);
+        else
 #pragma unroll
           for (u32 i = 0; i < 8u; i++) {
             const u32 e = 8u * c + i;
-            if (e < a.n_rot) {
-              const u32 f = e < half ? e : e - half;
-              const float cs = s_cos[f], sn = s_sin[f];
-              x[i] = e < half ? x[i] * cs - o[i] * sn : o[i] * sn + x[i] * cs;
-            }
+            o[i] = e < a.n_rot ? src[e < half ? e + half : e - half] : 0.0f;
+          }
+#pragma unroll
+        for (u32 i = 0; i < 8u; i++) {
+          const u32 e = 8u * c + i;
+          if (e < a.n_rot) {
+            const u32 f = e < half ? e : e - half;
+            const float cs = s_cos[wv][f], sn = s_sin[wv][f];
+            x[i] = e < half ? x[i] * cs - o[i] * sn : o[i] * sn + x[i] * cs;
           }
         }
       }
-      if (a.q == (const float *)a.qo) __syncthreads(); // queries in place: every read of these heads before the first write
-      if (!on) continue;
+      // queries in place: a head is one wave's, in one pass, and all of the wave's reads are back before its first write
+      if (a.q == (const float *)a.qo) __builtin_amdgcn_s_waitcnt(0x0F70);
       if (h >= nq) {
         if (!ok) continue;
-        const u32x4 w = {pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]), pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7])};
-        *(u32x4 *)(kv.k + (((((u64)(u32)id * kv.n_kv + (h - nq)) << lgg) + (slot >> 4)) * gb + 256u * c + 16u * (slot & 15u))) = w;
+        const u32x4 v = {pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]), pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7])};
+        *(u32x4 *)(kv.k + (((((u64)(u32)id * kv.n_kv + (h - nq)) << lgg) + (slot >> 4)) * gb + 256u * c + 16u * (slot & 15u))) = v;
       } else if (a.qt == 0u) {
         float *d = (float *)a.qo + (u64)row * a.qos + (u64)h * hd + 8u * c;
         if (a.vec & 4u) ((v4f *)d)[0] = (v4f){x[0], x[1], x[2], x[3]}, ((v4f *)d)[1] = (v4f){x[4], x[5], x[6], x[7]};
@@ -201,12 +203,12 @@ __device__ __forceinline__ void append_body(const amdc_kv_dev &kv, const AppendA
 #pragma unroll
           for (int i = 0; i < 8; i++) d[i] = x[i];
       } else {
-        const u32x4 w = {pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]), pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7])};
+        const u32x4 v = {pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]), pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7])};
         unsigned short *d = (unsigned short *)a.qo + (u64)row * a.qos + (u64)h * hd + 8u * c;
-        if (a.vec & 4u) *(u32x4 *)d = w;
+        if (a.vec & 4u) *(u32x4 *)d = v;
         else
 #pragma unroll
-          for (int i = 0; i < 8; i++) d[i] = (unsigned short)(w[i >> 1] >> (16 * (i & 1)));
+          for (int i = 0; i < 8; i++) d[i] = (unsigned short)(v[i >> 1] >> (16 * (i & 1)));
       }
     }
     return;
@@ -228,18 +230,35 @@ __device__ __forceinline__ void append_body(const amdc_kv_dev &kv, const AppendA
   if ((u32)id >= kv.n_pages) return; // flagged by the row's own workgroup
   const u32 g = (p0 & ((1u << kv.lgp) - 1u)) >> 3, n = kv.n_kv << a.lghd;
   const float *src = a.v + (u64)(s.row0 + (p0 + j0 - start)) * a.vs;
+  auto put8 = [&](uint8_t *to, u32x4 w) { // a value's eight positions, or the new ones of them
+    if (j1 - j0 == 8u) *(u32x4 *)to = w;
+    else
+#pragma unroll
+      for (u32 j = 0; j < 8u; j++)
+        if (j >= j0 && j < j1) ((unsigned short *)to)[j] = (unsigned short)(w[j >> 1] >> (16u * (j & 1u)));
+  };
+  if (a.vec & 8u) { // four values a thread
+    for (u32 i = 4u * (part * 256u + tid); i < n; i += a.gv * 1024u) {
+      const u32 h = i >> a.lghd, d = i & (hd - 1u);
+      v4f x[8];
+#pragma unroll
+      for (u32 j = 0; j < 8u; j++) x[j] = j >= j0 && j < j1 ? *(const v4f *)(src + (u64)(j - j0) * a.vs + i) : (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+      uint8_t *to = kv.v + (((((u64)(u32)id * kv.n_kv + h) << (lgg + 1u)) + g) * (gb >> 1) + 16u * d);
+#pragma unroll
+      for (u32 e = 0; e < 4u; e++) {
+        const u32x4 w = {pack2<BF>(x[0][e], x[1][e]), pack2<BF>(x[2][e], x[3][e]), pack2<BF>(x[4][e], x[5][e]), pack2<BF>(x[6][e], x[7][e])};
+        put8(to + 16u * e, w);
+      }
+    }
+    return;
+  }
   for (u32 i = part * 256u + tid; i < n; i += a.gv * 256u) {
     const u32 h = i >> a.lghd, d = i & (hd - 1u);
     float x[8];
 #pragma unroll
     for (u32 j = 0; j < 8u; j++) x[j] = j >= j0 && j < j1 ? src[(u64)(j - j0) * a.vs + i] : 0.0f;
     const u32x4 w = {pack2<BF>(x[0], x[1]), pack2<BF>(x[2], x[3]), pack2<BF>(x[4], x[5]), pack2<BF>(x[6], x[7])};
-    uint8_t *to = kv.v + (((((u64)(u32)id * kv.n_kv + h) << (lgg + 1u)) + g) * (gb >> 1) + 16u * d);
-    if (j1 - j0 == 8u) *(u32x4 *)to = w;
-    else
-#pragma unroll
-      for (u32 j = 0; j < 8u; j++)
-        if (j >= j0 && j < j1) ((unsigned short *)to)[j] = (unsigned short)(w[j >> 1] >> (16u * (j & 1u)));
+    put8(kv.v + (((((u64)(u32)id * kv.n_kv + h) << (lgg + 1u)) + g) * (gb >> 1) + 16u * d), w);
   }
 }
 
@@ -691,19 +710,27 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
           v4f e = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int p = 0; p < NP; p++) e = mfma_v(vr[d], pw[c][p], e);
-          auto again = [&](u32 from, u32 to) {
-            e = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
-            const op w = seen16(vr[d], SP * st + SL * g4, from, to);
+          if (!wave_finite(e)) { // again: without what no column sees (the common case behind the last position), then token by token
+            v4f g = {0.0f, 0.0f, 0.0f, 0.0f};
+            bool whole = true;
+            for (u32 t = t_a;;) {
+              e = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+              const op w = seen16(vr[d], SP * st + SL * g4, whole ? lo_of(t_a) : lo_of(t), whole ? hi_of(t_z) : hi_of(t));
 #pragma unroll
-            for (int p = 0; p < NP; p++) e = mfma_v(w, pw[c][p], e);
-          };
-          if (!wave_finite(e)) again(lo_of(t_a), hi_of(t_z)); // without what no column sees: the common case behind the last position
-          if (wave_finite(e)) O[c][d] += e;
-          else
-            for (u32 t = t_a; t <= t_z; t++) {
-              again(lo_of(t), hi_of(t));
-              if (tc[c] == t) O[c][d] += e;
+              for (int p = 0; p < NP; p++) e = mfma_v(w, pw[c][p], e);
+              if (whole && wave_finite(e)) {
+                g = e;
+                break;
+              }
+              if (!whole) {
+                if (tc[c] == t) g = e;
+                if (t++ == t_z) break;
+              }
+              whole = false;
             }
+            e = g;
+          }
+          O[c][d] += e;
         }
     }
     if (more) load_v(ga, gz);
@@ -854,6 +881,14 @@ DEC_KERNELS(128, _n2, 2u)
 
 // ------------------------------------------------------------------ attention of prompts
 
+// c and the two 16-bit values of w
+template <bool BF>
+__device__ __forceinline__ float sum2(u32 w, float c) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  if constexpr (BF) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w), __builtin_bit_cast(b2, 0x3F803F80u), c, false);
+  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), __builtin_bit_cast(h2, 0x3C003C00u), c, false);
+}
+
 template <bool BF>
 __device__ __forceinline__ v16f mfma32(u32x4 a, u32x4 b, v16f c) {
   typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -862,8 +897,37 @@ __device__ __forceinline__ v16f mfma32(u32x4 a, u32x4 b, v16f c) {
 }
 
 #define PRE_BM 128u     // query rows of a workgroup
-#define PRE_MAXSPLIT 8u // parts that a tile's positions are split into at most
 #define PRE_MINTILES 4u // tiles of positions that a part has at least
+#define PRE_SB(hd) ((PRE_BM * (hd) + 2u * PRE_BM) * 4u) // bytes of a partial result
+
+// The rows of a unit (a tile of PRE_BM rows of a sequence) and the tiles of BN positions [j0, j1) that they see, in ns parts
+struct PreUnit {
+  SeqRows s;
+  u32 b, r0, nr, j0, j1, ns;
+};
+__device__ __forceinline__ PreUnit pre_unit(const amdc_kv_dev &kv, const AttnArgs &a, u32 unit, u32 BN) {
+  PreUnit p;
+  u32 ti;
+  if (a.cu) {
+    auto base = [&](u32 i) { const int c = a.cu[i]; return (c < 0 ? 0u : (u32)c * a.G / PRE_BM) + i; };
+    p.b = find_seq(kv.n_seq, unit, base);
+    ti = unit - base(p.b);
+  } else {
+    const u32 per = cdiv(a.T * a.G, PRE_BM);
+    p.b = unit / per, ti = unit - p.b * per;
+  }
+  p.s = seq_rows(kv, a.cu, a.T, p.b);
+  p.s.row0 = uniform(p.s.row0), p.s.m = uniform(p.s.m), p.s.len = uniform(p.s.len);
+  const u32 R = p.s.m * a.G;
+  p.r0 = ti * PRE_BM;
+  p.nr = p.r0 >= R ? 0u : R - p.r0 < PRE_BM ? R - p.r0 : PRE_BM;
+  if (!p.nr || !p.s.len) return p;
+  const u32 m0 = p.s.len - p.s.m, e = m0 + p.r0 / a.G + 1u;
+  p.j0 = (a.window && e > a.window ? e - a.window : 0u) / BN, p.j1 = cdiv(m0 + (p.r0 + p.nr - 1u) / a.G + 1u, BN);
+  const u32 most = (p.j1 - p.j0) / PRE_MINTILES;
+  p.ns = most < 1u ? 1u : most < a.U ? most : a.U;
+  return p;
+}
 
 // The new tokens of a sequence and the G heads that share a key / value head are its rows (token t, head g: t G + g). A workgroup
 // takes PRE_BM consecutive rows, its waves W = 32 or 16 each, and goes through tiles of BN positions that the LDS holds twice: while the
@@ -879,20 +943,20 @@ __device__ __forceinline__ v16f mfma32(u32x4 a, u32x4 b, v16f c) {
 // factor 2^8 and the steps at the edges are dec_body's.
 // Rows are dealt from the last tile of the last sequence down: the longest first. Where all rows make fewer workgroups than the CUs
 // hold (a short chunk of a long prompt), a tile's positions are split over a.U workgroups; their partial results go through the
-// workspace, joined by the last to arrive in the order of the positions.
-template <int HD, bool BF, bool F32, u32 W>
+// workspace and amdc_attn_join_*, a launch of its own (joined by the last workgroup to arrive, 128 rows of four parts took it 18 us).
+template <int HD, bool BF, bool F32, u32 W, u32 BN>
 __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &a) {
   typedef typename std::conditional<W == 32u, v16f, v4f>::type acc; // of a matrix instruction: W x W / 64
   constexpr int NP = F32 ? (BF ? 3 : 2) : 1, NA = W == 32u ? 16 : 4, DT = HD / W;
   constexpr u32 TT = W == 32u ? 1u : 2u, KS = HD / (W == 32u ? 16u : 32u), PF = W / 16u; // of 32 positions: score tiles, steps over hd, weight operands
-  constexpr u32 NW = PRE_BM / W, NTH = 64u * NW, BN = HD > 128 ? 32u : 64u, MT = BN / 32u, TB = BN * HD * 2u, QD = HD / 4u;
+  constexpr u32 NW = PRE_BM / W, NTH = 64u * NW, MT = BN / 32u, TB = BN * HD * 2u, QD = HD / 4u;
   constexpr u32 PG = HD / 16u, PW = BN / 16u * PG / NW; // KB of a group of 16 positions (keys, then values), and of a tile for each wave
   constexpr float BIAS = BF ? 0.0f : 8.0f, RAISE = 6.0f, NINF = -__builtin_inff();
-  constexpr bool FULL = HD > 128 && NP > 2; // of registers: the queries' last part stays in the LDS
+  constexpr bool FULL = HD > 128 && NP > 1; // of registers: the queries' last part stays in the LDS
   constexpr int QR = FULL ? NP - 1 : NP;
   __shared__ u32x4 s_q[FULL ? KS : 1][FULL ? NTH : 1]; // step, thread
   __shared__ __attribute__((aligned(16))) uint8_t sm[2][2][TB]; // half, keys / values
-  __shared__ u32 s_bad, s_last;
+  __shared__ u32 s_bad;
   const u32 tid = threadIdx.x, lane = tid & 63u, wv = (u32)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), n = lane & (W - 1u), gg = lane / W;
   auto zero = []() {
     acc z;
@@ -913,20 +977,10 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
   const u32 G = a.G, h = blockIdx.x % kv.n_kv;
   u32 x = blockIdx.x / kv.n_kv;
   const u32 sp = x % a.U, unit = a.ncb - 1u - x / a.U;
-  u32 b, ti;
-  if (a.cu) {
-    auto base = [&](u32 i) { const int c = a.cu[i]; return (c < 0 ? 0u : (u32)c * G / PRE_BM) + i; };
-    b = find_seq(kv.n_seq, unit, base);
-    ti = unit - base(b);
-  } else {
-    const u32 per = cdiv(a.T * G, PRE_BM);
-    b = unit / per, ti = unit - b * per;
-  }
-  SeqRows s = seq_rows(kv, a.cu, a.T, b);
-  s.row0 = (u32)__builtin_amdgcn_readfirstlane((int)s.row0), s.m = (u32)__builtin_amdgcn_readfirstlane((int)s.m), s.len = (u32)__builtin_amdgcn_readfirstlane((int)s.len);
-  const u32 R = s.m * G, r0 = ti * PRE_BM;
-  if (r0 >= R) return;
-  const u32 nr = R - r0 < PRE_BM ? R - r0 : PRE_BM, nbq = a.n_q * HD / 32u;
+  const PreUnit pu = pre_unit(kv, a, unit, BN);
+  const SeqRows &s = pu.s;
+  const u32 r0 = pu.r0, nr = pu.nr, nbq = a.n_q * HD / 32u;
+  if (!nr) return;
   auto at = [&](u32 r, u32 &row, u32 &head) { // row r of the workgroup
     const u32 t = (r0 + r) / G;
     row = s.row0 + t, head = h * G + (r0 + r) - t * G;
@@ -948,10 +1002,9 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
   auto hi_of = [&](u32 t) { return m0 + t + 1u; };
 
   // the tiles of positions [jb, je) of this workgroup
-  const u32 j0 = lo_of(r0 / G) / BN, j1 = cdiv(hi_of((r0 + nr - 1u) / G), BN);
-  const u32 most = (j1 - j0) / PRE_MINTILES, ns = most < 1u ? 1u : most < a.U ? most : a.U;
+  const u32 ns = pu.ns;
   if (sp >= ns) return;
-  const u32 jb = j0 + (j1 - j0) * sp / ns, je = j0 + (j1 - j0) * (sp + 1u) / ns;
+  const u32 jb = pu.j0 + (pu.j1 - pu.j0) * sp / ns, je = pu.j0 + (pu.j1 - pu.j0) * (sp + 1u) / ns;
 
   // the wave's rows and the lane's
   const u32 w0 = W * wv, wr = nr > w0 ? (nr - w0 < W ? nr - w0 : W) : 0u; // 0: only loads
@@ -964,7 +1017,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
   const u32 grp = wv * PW / PG, pc0 = wv * PW % PG;
   const u64 gb = 32ull * HD, hb = gb << (kv.lgp - 4u);
   const u32 pmask = (1u << kv.lgp) - 1u;
-  const int *table = kv.pages + (u64)b * kv.max_pages;
+  const int *table = kv.pages + (u64)pu.b * kv.max_pages;
   int ids = 0; // of the group of tiles jt .. jt + 63
   bool bad = false;
   // the first position of the wave's group of tile j; behind the sequence's last group that one again
@@ -994,35 +1047,31 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
 
   // the lane's query row: values HD / KS k + 8 gg .. + 7 of step k
   u32x4 qf[QR][KS];
-  float cq = a.c;
+  float cq = __builtin_fabsf(a.c); // a negative scale's sign goes to the queries: the largest product is the largest score
   {
     u32 row, head;
     at(rc, row, head);
     const u64 i0 = (u64)row * a.qs + (u64)head * HD + 8u * gg;
-    float up = 1.0f;
+    float up = a.c < 0.0f ? -1.0f : 1.0f, v[KS][8];
+#pragma unroll
+    for (u32 k = 0; k < KS; k++) load_q8<BF, F32>(a.q, i0 + HD / KS * k, a.vec & 1u, v[k]);
     if (F32 && !BF) {
       float big = 0.0f;
 #pragma unroll
-      for (u32 k = 0; k < KS; k++) {
-        float v[8];
-        load_q8<BF, F32>(a.q, i0 + HD / KS * k, a.vec & 1u, v);
+      for (u32 k = 0; k < KS; k++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) big = __builtin_fmaxf(big, __builtin_fabsf(v[i]));
-      }
+        for (int i = 0; i < 8; i++) big = __builtin_fmaxf(big, __builtin_fabsf(v[k][i]));
       big = over(big, maxf);
       const u32 e = __builtin_bit_cast(u32, big) >> 23, k = e < 11u ? 253u : 264u - e;
-      up = __builtin_bit_cast(float, k << 23), cq *= __builtin_bit_cast(float, (254u - k) << 23);
+      up *= __builtin_bit_cast(float, k << 23), cq *= __builtin_bit_cast(float, (254u - k) << 23);
     }
+    cq = __builtin_fmaxf(cq, 0x1p-126f); // scale 0: a score of 0, also of -infinity (what is not seen) not NaN
 #pragma unroll
     for (u32 k = 0; k < KS; k++) {
-      float v[8];
-      if (FULL) __asm__ volatile("" ::: "memory");
-      load_q8<BF, F32>(a.q, i0 + HD / KS * k, a.vec & 1u, v);
-      if (F32 && !BF)
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= up;
+      for (int i = 0; i < 8; i++) v[k][i] *= up;
       u32x4 w[NP];
-      split8<BF, NP>(v, w);
+      split8<BF, NP>(v[k], w);
 #pragma unroll
       for (int p = 0; p < QR; p++) qf[p][k] = w[p];
       if (FULL) s_q[k][tid] = w[NP - 1]; // read by this thread alone
@@ -1058,8 +1107,11 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
         }
       }
 #pragma unroll
-      for (u32 i = 0; i < NS; i++) S[NS * t + i] = c[i / NA][i % NA] * cq;
+      for (u32 i = 0; i < NS; i++) S[NS * t + i] = c[i / NA][i % NA];
     }
+    // the softmax before the other wave's matrix products, which then run beside it (MI355X, us: 2 x 4096 rows of 32 / 8 heads of 64
+    // 184, without 198; of 128 322, 323)
+    __builtin_amdgcn_s_setprio(1);
     float top = NINF;
 #pragma unroll
     for (u32 i = 0; i < N * NS; i++) {
@@ -1069,8 +1121,8 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
       }
       top = __builtin_fmaxf(top, S[i]);
     }
-    if (__ballot(top > m + RAISE)) {
-      const float nm = __builtin_fmaxf(m, over(top, maxf)), f = m == nm ? 1.0f : __builtin_amdgcn_exp2f(m - nm);
+    if (__ballot(top * cq > m + RAISE)) {
+      const float nm = __builtin_fmaxf(m, over(top, maxf) * cq), f = m == nm ? 1.0f : __builtin_amdgcn_exp2f(m - nm);
 #pragma unroll
       for (int d = 0; d < DT; d++) O[d] *= f;
       l *= f;
@@ -1082,13 +1134,24 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
     for (u32 k = 0; k < PF * N; k++) {
       float v[8];
 #pragma unroll
-      for (u32 i = 0; i < 8u; i++) v[i] = __builtin_amdgcn_exp2f(S[8u * k + i] + ref);
-      l += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+      for (u32 i = 0; i < 8u; i++) v[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[8u * k + i], cq, ref));
+      if (NP > 1) l += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
       u32x4 w[NP];
       split8<BF, NP>(v, w);
 #pragma unroll
       for (int p = 0; p < NP; p++) pw[p][k] = w[p];
+      if (NP == 1) // the sum of the rounded weights, the ones that the values get
+#pragma unroll
+        for (int i = 0; i < 4; i++) l = sum2<BF>(w[0][i], l);
     }
+    auto finite = [&](const acc &e) {
+      float z = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NA; i++) z += e[i] - e[i]; // NaN where one is not
+      return __ballot(!(z == 0.0f)) == 0ull;
+    };
+    u32 redo = 0u;
+    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int d = 0; d < DT; d++) {
       if (FULL && d % 4 == 0) __asm__ volatile("" ::: "memory");
@@ -1099,31 +1162,38 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
 #pragma unroll
         for (int p = 0; p < NP; p++) e = mfma(vf, pw[p][k], e);
       }
-      if (EDGE) {
-        auto finite = [&]() {
-          float z = 0.0f;
-#pragma unroll
-          for (int i = 0; i < NA; i++) z += e[i] - e[i]; // NaN where one is not
-          return __ballot(!(z == 0.0f)) == 0ull;
-        };
-        auto again = [&](u32 from, u32 to) {
-          e = zero();
+      if (!EDGE) O[d] = e;
+      else if (finite(e)) O[d] += e;
+      else redo |= 1u << d;
+    }
+    if (EDGE)
+      while (redo) { // the d-th W values again: without what no row sees (the common case behind the last position), then row by row
+        const u32 d = (u32)__builtin_ctz(redo);
+        redo &= redo - 1u;
+        acc g = zero();
+        bool whole = true;
+        for (u32 t = t_a;;) {
+          acc e = zero();
 #pragma unroll
           for (u32 k = 0; k < PF * N; k++) {
-            const u32x4 vf = seen16(*(const u32x4 *)(vt + 64u * HD / PF * k + 16u * W * d), p0 + 32u / PF * k + 8u * gg, from, to);
+            const u32x4 vf = seen16(*(const u32x4 *)(vt + 64u * HD / PF * k + 16u * W * d), p0 + 32u / PF * k + 8u * gg, whole ? lo_a : lo_of(t), whole ? hi_z : hi_of(t));
 #pragma unroll
             for (int p = 0; p < NP; p++) e = mfma(vf, pw[p][k], e);
           }
-        };
-        if (!finite()) again(lo_a, hi_z); // without what no row sees: the common case behind the last position
-        if (finite()) O[d] += e;
-        else
-          for (u32 t = t_a; t <= t_z; t++) {
-            again(lo_of(t), hi_of(t));
-            if (tc == t) O[d] += e;
+          if (whole && finite(e)) {
+            g = e;
+            break;
           }
-      } else O[d] = e;
-    }
+          if (!whole) {
+            if (tc == t) g = e;
+            if (t++ == t_z) break;
+          }
+          whole = false;
+        }
+#pragma unroll
+        for (int i = 0; i < DT; i++)
+          if (d == (u32)i) O[i] += g;
+      }
   };
   for (u32 j = jb; j < je; j++) {
     const u32 half = (j - jb) & 1u, p0 = BN * j;
@@ -1183,79 +1253,90 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
       }
     return;
   }
-  // partial results: PRE_BM rows of O, then their m and l
-  constexpr u32 SB = (PRE_BM * HD + 2u * PRE_BM) * 4u, OM = PRE_BM * HD * 4u;
-  const u64 cell = (u64)unit * kv.n_kv + h;
-  uint8_t *parts = a.ws + ATTN_CNT + cell * a.U * SB;
-  {
-    const __amdgpu_buffer_rsrc_t d = rsrc(parts + sp * SB, SB);
-    if (n < wr) {
+  // a partial result: PRE_BM rows of O, then their m and l
+  float *part = (float *)(a.ws + ATTN_CNT + (((u64)unit * kv.n_kv + h) * a.U + sp) * PRE_SB(HD));
+  if (n < wr) {
 #pragma unroll
-      for (int k = 0; k < DT; k++)
+    for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (u32 i = 0; i < NA / 4u; i++)
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, quad(k, i)), d, ((w0 + n) * HD + W * k + 8u * i + 4u * gg) * 4u, 0, CPOL_SC1);
-      if (gg == 0u) {
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, m), d, OM + 4u * (w0 + n), 0, CPOL_SC1);
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, l), d, OM + 4u * (PRE_BM + w0 + n), 0, CPOL_SC1);
-      }
-    }
-  }
-  __builtin_amdgcn_s_waitcnt(0x0F70); // vmcnt(0): this thread's partial results are stored
-  __syncthreads();
-  if (tid == 0u) {
-    u32 *c = (u32 *)a.ws + cell;
-    const bool last = __hip_atomic_fetch_add(c, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u == ns;
-    if (last) __hip_atomic_store(c, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_last = last;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  float *sw = (float *)sm; // [part][row], then the rows' sums
-  if (tid < PRE_BM) {
-    float mm[PRE_MAXSPLIT], ll[PRE_MAXSPLIT], M = NINF, sum = 0.0f;
-#pragma unroll
-    for (u32 k = 0; k < PRE_MAXSPLIT; k++) {
-      const __amdgpu_buffer_rsrc_t d = rsrc(parts + (k < ns ? k : 0u) * SB, SB);
-      const bool in = k < ns && tid < nr;
-      mm[k] = in ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(d, OM + 4u * tid, 0, CPOL_SC1)) : NINF;
-      ll[k] = in ? __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(d, OM + 4u * (PRE_BM + tid), 0, CPOL_SC1)) : 0.0f;
-    }
-#pragma unroll
-    for (u32 k = 0; k < PRE_MAXSPLIT; k++) M = __builtin_fmaxf(M, mm[k]);
-#pragma unroll
-    for (u32 k = 0; k < PRE_MAXSPLIT; k++) {
-      const float f = __builtin_amdgcn_exp2f(mm[k] - (M == NINF ? 0.0f : M));
-      sw[k * PRE_BM + tid] = f, sum += f * ll[k];
-    }
-    sw[PRE_MAXSPLIT * PRE_BM + tid] = sum;
-  }
-  __syncthreads();
-  for (u32 i = tid; i < nr * QD; i += NTH) {
-    const u32 r = i / QD;
-    u32x4 v[PRE_MAXSPLIT];
-#pragma unroll
-    for (u32 k = 0; k < PRE_MAXSPLIT; k++) v[k] = __builtin_amdgcn_raw_buffer_load_b128(rsrc(parts + (k < ns ? k : 0u) * SB, SB), 16u * i, 0, CPOL_SC1);
-    v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (u32 k = 0; k < PRE_MAXSPLIT; k++)
-      if (k < ns) sum += sw[k * PRE_BM + r] * __builtin_bit_cast(v4f, v[k]);
-    put(r, i % QD, sum / sw[PRE_MAXSPLIT * PRE_BM + r]);
+      for (u32 i = 0; i < NA / 4u; i++) *(v4f *)(part + (w0 + n) * HD + W * d + 8u * i + 4u * gg) = quad(d, i);
+    if (gg == 0u) part[PRE_BM * HD + w0 + n] = m, part[PRE_BM * (HD + 1u) + w0 + n] = l;
   }
 }
 
-#define PRE_KERNEL(HD, KN, BF, F32, W, OCC) \
-  extern "C" __global__ __launch_bounds__(8192 / W, OCC) void amdc_attn_pre_h##HD##_##KN(amdc_kv_dev kv, AttnArgs a) { pre_body<HD, BF, F32, W>(kv, a); }
-PRE_KERNEL(64, f16, false, false, 32, 2)
-PRE_KERNEL(64, f16_f32, false, true, 32, 2)
-PRE_KERNEL(64, bf16, true, false, 32, 2)
-PRE_KERNEL(64, bf16_f32, true, true, 32, 2)
-PRE_KERNEL(128, f16, false, false, 32, 2)
-PRE_KERNEL(128, f16_f32, false, true, 32, 1)
-PRE_KERNEL(128, bf16, true, false, 32, 2)
-PRE_KERNEL(128, bf16_f32, true, true, 32, 1)
-PRE_KERNEL(256, f16, false, false, 16, 2)
-PRE_KERNEL(256, f16_f32, false, true, 16, 2)
-PRE_KERNEL(256, bf16, true, false, 16, 2)
-PRE_KERNEL(256, bf16_f32, true, true, 16, 2)
+// The parts of a split tile joined in the order of their positions: 16 of its rows, JOIN_N parts' loads in flight a thread
+#define JOIN_N 8u
+template <bool BF, bool F32>
+__device__ __forceinline__ void join_body(const amdc_kv_dev &kv, const AttnArgs &a, u32 hd, u32 BN) {
+  __shared__ float s_M[16], s_L[16], s_w[JOIN_N][16];
+  const u32 tid = threadIdx.x, qd = hd / 4u, nbq = a.n_q * hd / 32u;
+  const u32 h = blockIdx.x % kv.n_kv, x = blockIdx.x / kv.n_kv, unit = x / (PRE_BM / 16u), f = x % (PRE_BM / 16u) * 16u;
+  const PreUnit pu = pre_unit(kv, a, unit, BN);
+  if (f >= pu.nr || !pu.s.len || pu.ns == 1u) return; // nothing to join: the rows are written
+  const u32 nr = pu.nr - f < 16u ? pu.nr - f : 16u, ns = pu.ns, pf = PRE_SB(hd) / 4u; // floats of a partial result
+  const float *parts = (const float *)(a.ws + ATTN_CNT) + ((u64)unit * kv.n_kv + h) * a.U * pf, *ml = parts + PRE_BM * hd + f;
+  if (tid < 16u) {
+    const u32 r = tid < nr ? tid : 0u;
+    float M = -__builtin_inff(), sum = 0.0f;
+    for (u32 k = 0u; k < ns; k++) M = __builtin_fmaxf(M, ml[k * pf + r]);
+    const float ref = M == -__builtin_inff() ? 0.0f : M;
+    for (u32 k = 0u; k < ns; k++) sum += __builtin_amdgcn_exp2f(ml[k * pf + r] - ref) * ml[k * pf + PRE_BM + r];
+    s_M[tid] = ref, s_L[tid] = sum;
+  }
+  v4f v[4]; // quads tid, tid + 256, .. of the 16 rows: at most 4
+#pragma unroll
+  for (u32 i = 0; i < 4u; i++) v[i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
+  for (u32 k0 = 0u; k0 < ns; k0 += JOIN_N) {
+    __syncthreads();
+    if (tid < 16u * JOIN_N) {
+      const u32 r = tid & 15u, k = k0 + (tid >> 4);
+      s_w[tid >> 4][r] = k < ns && r < nr ? __builtin_amdgcn_exp2f(ml[k * pf + r] - s_M[r]) : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (u32 i = 0; i < 4u; i++) {
+      const u32 e = tid + 256u * i;
+      if (e >= nr * qd) break;
+      v4f w[JOIN_N];
+#pragma unroll
+      for (u32 k = 0; k < JOIN_N; k++) w[k] = *(const v4f *)(parts + (u64)(k0 + k < ns ? k0 + k : k0) * pf + f * hd + 4u * e);
+#pragma unroll
+      for (u32 k = 0; k < JOIN_N; k++)
+        if (k0 + k < ns) v[i] += s_w[k][e / qd] * w[k];
+    }
+  }
+#pragma unroll
+  for (u32 i = 0; i < 4u; i++) {
+    const u32 e = tid + 256u * i;
+    if (e >= nr * qd) break;
+    const u32 r = e / qd, d4 = e - r * qd, t = (pu.r0 + f + r) / a.G, row = pu.s.row0 + t, head = h * a.G + (pu.r0 + f + r) - t * a.G;
+    const v4f y = v[i] / s_L[r];
+    if (a.y) store_y4<BF, F32>(a.y, (u64)row * a.ys + (u64)head * hd + 4u * d4, y, a.vec & 2u);
+    if (a.q8) quant_vec4(y, (head * hd + 4u * d4) / 32u, true, a.q8 + (u64)row * a.q8s, nbq);
+  }
+}
+extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f32(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<false, true>(kv, a, hd, bn); }
+extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f16(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<false, false>(kv, a, hd, bn); }
+extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_bf16(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<true, false>(kv, a, hd, bn); }
+
+#ifndef PRE_P
+#define PRE_P 64, 2, 64, 2
+#endif
+#define PRE_KERNEL(HD, KN, BF, F32, W, BN, OCC) \
+  extern "C" __global__ __launch_bounds__(8192 / W, OCC) void amdc_attn_pre_h##HD##_##KN(amdc_kv_dev kv, AttnArgs a) { pre_body<HD, BF, F32, W, BN>(kv, a); }
+#define PRE_PAIR2(B1, O1, B2, O2) \
+PRE_KERNEL(64, f16, false, false, 32, B1, O1) \
+PRE_KERNEL(64, bf16, true, false, 32, B1, O1) \
+PRE_KERNEL(128, f16, false, false, 32, B2, O2) \
+PRE_KERNEL(128, bf16, true, false, 32, B2, O2)
+#define PRE_PAIR(...) PRE_PAIR2(__VA_ARGS__)
+PRE_PAIR(PRE_P)
+PRE_KERNEL(64, f16_f32, false, true, 32, 64, 2)
+PRE_KERNEL(64, bf16_f32, true, true, 32, 64, 2)
+PRE_KERNEL(128, f16_f32, false, true, 32, 64, 1)
+PRE_KERNEL(128, bf16_f32, true, true, 32, 64, 1)
+PRE_KERNEL(256, f16, false, false, 16, 32, 2)
+PRE_KERNEL(256, f16_f32, false, true, 16, 32, 2)
+PRE_KERNEL(256, bf16, true, false, 16, 32, 2)
+PRE_KERNEL(256, bf16_f32, true, true, 16, 32, 2)
 #undef PRE_KERNEL

@@ -292,7 +292,8 @@ enum {
   K_ATTN_DEC = K_APPEND + 2, /* amdc_attn_dec_h64_f16, _f16_f32, _bf16, _bf16_f32, then h128, h256 */
   K_ATTN_DEC2 = K_ATTN_DEC + 12, /* amdc_attn_dec_h64_f16_n2, .. */
   K_ATTN_PRE = K_ATTN_DEC2 + 8, /* amdc_attn_pre_h64_f16, .. */
-  K_N = K_ATTN_PRE + 12
+  K_ATTN_JOIN = K_ATTN_PRE + 12, /* amdc_attn_join_f32, _f16, _bf16: in the order of AMDC_TYPE_* */
+  K_N = K_ATTN_JOIN + 3
 };
 
 #define KN(s) "amdc_" s
@@ -328,7 +329,8 @@ static const char *const kname[K_N] = {
     KN("gemv_q6_k_xs1"), KN("gemv_q8_0_s1l"), KN("gemv_q8_0_s2l"), KN("gemv_q8_0_xs1l"), KN("gemv_q8_0_xs2l"), KN("gemv_q6_k_s1l"),
     KN("gemv_q6_k_s1l"), KN("gemv_q6_k_xs1l"), KN("kv_append_f16"), KN("kv_append_bf16"),
     KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256"), KA2("attn_dec_h64"), KA2("attn_dec_h128"),
-    KA("attn_pre_h64"), KA("attn_pre_h128"), KA("attn_pre_h256")};
+    KA("attn_pre_h64"), KA("attn_pre_h128"), KA("attn_pre_h256"),
+    KN("attn_join_f32"), KN("attn_join_f16"), KN("attn_join_bf16")};
 
 static hipModule_t g_mod;
 static hipFunction_t g_k[K_N];
@@ -1678,18 +1680,19 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
     if ((const void *)q == qo && (qt != AMDC_TYPE_F32 || (rows > 1u && qs != qos)))
       return fail(AMDC_EINVAL, "kv_append: in place (qo = q) needs type F32 and qos = qs");
   }
-  const u32 lghd = log2u(kv->hd), hpi = 2048u / kv->hd, its = ((q ? n_q : 0u) + kv->n_kv + hpi - 1u) / hpi;
-  const u32 upb = (T + 14u) / 8u, vu = cu ? rows / 8u + 2u * kv->n_seq : kv->n_seq * upb, vn = (wk + 255u) / 256u;
-  /* a row's heads and a group's values over several workgroups until there are two of each to a CU */
-  const u32 want = 2u * (g_cus > 0 ? (u32)g_cus : 256u), gq0 = (want + rows - 1u) / rows, gv0 = (want + vu - 1u) / vu;
+  const u32 lghd = log2u(kv->hd), hpi = 512u / kv->hd, its = ((q ? n_q : 0u) + kv->n_kv + hpi - 1u) / hpi;
+  const int v4 = vec_rows(v, rows > 1u ? 4u * vs : 0u, 16u);
+  const u32 upb = (T + 14u) / 8u, vu = cu ? rows / 8u + 2u * kv->n_seq : kv->n_seq * upb, vn = v4 ? (wk + 1023u) / 1024u : (wk + 255u) / 256u;
+  /* a row's heads over several waves until there are eight to a CU, a group's values over several workgroups until there are two */
+  const u32 cus = g_cus > 0 ? (u32)g_cus : 256u, gq0 = (8u * cus + rows - 1u) / rows, gv0 = (2u * cus + vu - 1u) / vu;
   const u32 gq = gq0 < its ? gq0 : its, gv = gv0 < vn ? gv0 : vn;
-  if ((u64)rows * gq + (u64)vu * gv >= (1u << 24)) return fail(AMDC_EINVAL, "kv_append: %u rows of %u sequences are too many for one call", rows, kv->n_seq);
-  /* which rows are 16-byte aligned: queries, keys, rotated queries */
+  if ((u64)rows * gq >= (1u << 24) || (u64)vu * gv >= (1u << 23)) return fail(AMDC_EINVAL, "kv_append: %u rows of %u sequences are too many for one call", rows, kv->n_seq);
+  /* which rows are 16-byte aligned: queries, keys, rotated queries, values */
   const u32 vec = (vec_rows(q, rows > 1u ? 4u * qs : 0u, 16u) ? 1u : 0u) | (vec_rows(k, rows > 1u ? 4u * ks : 0u, 16u) ? 2u : 0u) |
-                  (vec_rows(qo, rows > 1u ? (qt == AMDC_TYPE_F32 ? 4u : 2u) * qos : 0u, 16u) ? 4u : 0u);
+                  (vec_rows(qo, rows > 1u ? (qt == AMDC_TYPE_F32 ? 4u : 2u) * qos : 0u, 16u) ? 4u : 0u) | (v4 ? 8u : 0u);
   append_args a = {k, v, q, qo, cu, freq, (u32)qt, n_q, T, ks, vs, qs, qos, rope ? n_rot : 0u, (u32)rope, lghd, rows, gq, gv, upb, vec};
   void *args[] = {&d, &a};
-  return launch(K_APPEND + (kv->type == AMDC_TYPE_BF16), rows * gq + vu * gv, 1, 0, stream, args);
+  return launch(K_APPEND + (kv->type == AMDC_TYPE_BF16), (rows * gq + 3u) / 4u + vu * gv, 1, 0, stream, args);
 }
 
 /* the arguments of the attention kernels: AttnArgs of amdc_attn.h */
@@ -1780,20 +1783,23 @@ int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t 
 /* A call of the prompt kernel: tiles of PRE_BM rows of a head at most, and the parts that a tile's positions are split into where
  * the tiles of all heads are fewer than the CUs hold (pre_body in amdc_attn.h). */
 #define PRE_BM 128u
-#define PRE_MAXSPLIT 8u
+#define PRE_MINTILES 4u
+#define PRE_BN(hd) ((hd) > 128u ? 32u : 64u) /* positions of a tile */
+static u32 pre_want(u32 hd) { return (g_cus > 0 ? (u32)g_cus : 256u) * (hd > 128u ? 1u : 2u); }
 static u32 pre_tiles(const amdc_kv *kv, u32 n_q, u32 rows, int ragged, u32 T, u32 *parts) {
   const u32 G = n_q / kv->n_kv;
-  const u64 tiles = ragged ? (u64)rows * G / PRE_BM + kv->n_seq : (u64)kv->n_seq * (((u64)T * G + PRE_BM - 1u) / PRE_BM);
-  const u64 wgs = tiles * kv->n_kv, want = (g_cus > 0 ? (u32)g_cus : 256u) * (kv->hd > 128u ? 1u : 2u);
-  *parts = wgs >= want ? 1u : want / wgs < PRE_MAXSPLIT ? (u32)(want / wgs) : PRE_MAXSPLIT;
+  const u64 tiles = ragged ? ((u64)rows * G + PRE_BM - 1u) / PRE_BM + kv->n_seq - 1u : (u64)kv->n_seq * (((u64)T * G + PRE_BM - 1u) / PRE_BM);
+  const u64 wgs = tiles * kv->n_kv, want = pre_want(kv->hd);
+  /* parts of at least PRE_MINTILES tiles of the most positions that the table holds; 1: no join */
+  const u64 most = (u64)kv->max_pages * kv->page / (PRE_MINTILES * PRE_BN(kv->hd));
+  *parts = wgs < want && most > 1u ? (u32)(want / wgs < most ? want / wgs : most) : 1u;
   return tiles < (1u << 24) ? (u32)tiles : 1u << 24;
 }
 
 size_t amdc_attn_prefill_ws(const amdc_kv *kv, uint32_t n_q, uint32_t rows) {
   if (!kv || !amdc_kv_bytes(kv->type, kv->n_kv, kv->hd, kv->page, kv->n_pages) || !n_q || n_q % kv->n_kv || !rows || rows > (1u << 22)) return 0;
-  /* rows dealt to the sequences in any way: fewer tiles mean more parts of each, under `want` workgroups in all */
-  const u64 want = (g_cus > 0 ? (u32)g_cus : 256u) * (kv->hd > 128u ? 1u : 2u);
-  return (size_t)(ATTN_CNT + want * (PRE_BM * kv->hd + 2u * PRE_BM) * 4u);
+  /* under pre_want partial results, however the rows are dealt to the sequences */
+  return (size_t)(ATTN_CNT + (u64)pre_want(kv->hd) * (PRE_BM * kv->hd + 2u * PRE_BM) * 4u);
 }
 
 int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
@@ -1809,7 +1815,10 @@ int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t
   if (grid >= (1u << 24)) return fail(AMDC_EINVAL, "attn_prefill: %u rows of %u sequences and %u heads are too many for one call", rows, kv->n_seq, kv->n_kv);
   attn_args a = {q, y, cu, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, parts, attn_vec(q, y, t, rows, qs, ys), tiles, 0};
   void *args[] = {&d, &a};
-  return launch_pre(attn_kernel(K_ATTN_PRE, kv, t), kv->hd, (unsigned)grid, stream, args);
+  if ((rc = launch_pre(attn_kernel(K_ATTN_PRE, kv, t), kv->hd, (unsigned)grid, stream, args)) || parts == 1u) return rc;
+  const u32 bn = PRE_BN(kv->hd);
+  void *ja[] = {&d, &a, (void *)&kv->hd, (void *)&bn};
+  return launch(K_ATTN_JOIN + t, tiles * (PRE_BM / 16u) * kv->n_kv, 1, 0, stream, ja);
 }
 
 int amdc_probe_read(const void *src, size_t nbytes, void *scratch, uint32_t grid, void *stream) {

@@ -9,7 +9,7 @@ import pytest
 HERE = os.path.dirname(os.path.abspath(__file__))
 
 APPEND = dict(k=4096, v=4096, q=4096, qo=8192, qt=0, n_q=8, T=3, ks=512, vs=512, qs=512, qos=512, cu=None, freq=4096, n_rot=64, rope=1)
-KV = dict(type=1, n_kv=2, hd=64, page=16, n_pages=9, k=4096, v=4096, n_seq=2, max_pages=4, pages=4096, len=4096)
+KV = dict(type=1, n_kv=2, hd=64, page=16, n_pages=9, k=4096, v=4096, n_seq=2, max_pages=40, pages=4096, len=4096)
 
 BAD = {
     "append": [("kv", dict(type=0)), ("kv", dict(type=3)), ("kv", dict(n_kv=0)), ("kv", dict(n_kv=1025)), ("kv", dict(hd=96)), ("kv", dict(page=8)), ("kv", dict(page=48)),
@@ -77,9 +77,11 @@ def test_refused(stub, op):
 
 @pytest.mark.parametrize("op", sorted(BASE))
 def test_taken(stub, op):
-    """One launch each, and no allocation: every call can be captured."""
+    """One launch each (prompts: and one that joins, where few rows are split over the positions), and no allocation: every call can be
+    captured."""
     for change, got in zip(GOOD[op], calls(stub, op, [(None, c) for c in GOOD[op]])):
-        assert got == ("", 1, 0), change
+        split = op == "prefill" and change.get("T", 3) < 4000
+        assert got == ("", 2 if split else 1, 0), change
 
 
 def test_kv_bytes():
