@@ -249,8 +249,8 @@ class DevBuf:
 
 
 def _p(x):
-    if x is None:
-        return None
+    if x is None or x.__class__ is int:
+        return x
     return x.ptr if isinstance(x, (DevBuf, DevMat)) else int(x)
 
 

@@ -1319,21 +1319,18 @@ extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f32(amdc_kv_dev
 extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f16(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<false, false>(kv, a, hd, bn); }
 extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_bf16(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<true, false>(kv, a, hd, bn); }
 
-#ifndef PRE_P
-#define PRE_P 64, 2, 64, 2
-#endif
+// Rows of a wave, positions of a tile, workgroups a CU wanted of the registers (MI355X, us). Heads of 128, 16-bit: 64 positions 1204 for
+// 12000 rows of 32 / 8 heads, 32 positions (half the scores' registers) 1342. Heads of 256: 32 rows a wave, one wave a SIMD, 144 where 16
+// rows, two waves, take 110 (256 rows over 5000 positions, 24 / 4 heads, f32)
 #define PRE_KERNEL(HD, KN, BF, F32, W, BN, OCC) \
   extern "C" __global__ __launch_bounds__(8192 / W, OCC) void amdc_attn_pre_h##HD##_##KN(amdc_kv_dev kv, AttnArgs a) { pre_body<HD, BF, F32, W, BN>(kv, a); }
-#define PRE_PAIR2(B1, O1, B2, O2) \
-PRE_KERNEL(64, f16, false, false, 32, B1, O1) \
-PRE_KERNEL(64, bf16, true, false, 32, B1, O1) \
-PRE_KERNEL(128, f16, false, false, 32, B2, O2) \
-PRE_KERNEL(128, bf16, true, false, 32, B2, O2)
-#define PRE_PAIR(...) PRE_PAIR2(__VA_ARGS__)
-PRE_PAIR(PRE_P)
+PRE_KERNEL(64, f16, false, false, 32, 64, 2)
 PRE_KERNEL(64, f16_f32, false, true, 32, 64, 2)
+PRE_KERNEL(64, bf16, true, false, 32, 64, 2)
 PRE_KERNEL(64, bf16_f32, true, true, 32, 64, 2)
+PRE_KERNEL(128, f16, false, false, 32, 64, 2)
 PRE_KERNEL(128, f16_f32, false, true, 32, 64, 1)
+PRE_KERNEL(128, bf16, true, false, 32, 64, 2)
 PRE_KERNEL(128, bf16_f32, true, true, 32, 64, 1)
 PRE_KERNEL(256, f16, false, false, 16, 32, 2)
 PRE_KERNEL(256, f16_f32, false, true, 16, 32, 2)

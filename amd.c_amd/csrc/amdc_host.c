@@ -1713,6 +1713,7 @@ static int check_attn(const char *op, const amdc_kv *kv, const void *q, const vo
   const u64 w = (u64)n_q * kv->hd, es = t == AMDC_TYPE_F32 ? 4u : 2u;
   if (!q || (!y && !q8)) return fail(AMDC_EINVAL, "%s: null pointer (q, or both y and q8)", op);
   if (!vec_rows(q, 0, (u32)es) || !vec_rows(y, 0, (u32)es)) return fail(AMDC_EINVAL, "%s: q and y must be aligned to their type", op);
+  if (q == y) return fail(AMDC_EINVAL, "%s: y cannot be written over q", op);
   if (rows > 1u && (qs < w || (y && ys < w))) return fail(AMDC_EINVAL, "%s: strides qs %u, ys %u under a row's %llu values", op, qs, ys, (unsigned long long)w);
   if (q8 && (!vec_rows(q8, rows > 1u ? q8s : 0u, 4u) || (rows > 1u && q8s < w / 32u * 40u)))
     return fail(AMDC_EINVAL, "%s: q8 and q8s (%u) must be multiples of 4, q8s at least %llu", op, q8s, (unsigned long long)(w / 32u * 40u));
@@ -1773,7 +1774,7 @@ int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t 
   if ((rc = check_attn("attn_decode", kv, q, y, t, n_q, rows, qs, ys, q8, q8s, ws, ws_bytes, amdc_attn_decode_ws(kv, n_q, T)))) return rc;
   /* the workgroups of a unit's blocks of columns are 8 apart */
   const u64 grid = (((u64)U + kv->n_seq) * kv->n_kv + 7u) / 8u * 8u * ncb;
-  if (grid >= (1u << 23) || (u64)kv->n_seq * d.cap >= (1ull << 36))
+  if (grid >= (1u << 23) || (u64)kv->n_seq * d.cap >= (1ull << 35)) /* the kernel counts all steps of 16 in 32 bits */
     return fail(AMDC_EINVAL, "attn_decode: %u sequences of %u heads and up to %u positions are too many for one call", kv->n_seq, kv->n_kv, d.cap);
   attn_args a = {q, y, NULL, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, U, attn_vec(q, y, t, rows, qs, ys), ncb, fit};
   void *args[] = {&d, &a};
@@ -1812,7 +1813,7 @@ int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t
   if ((rc = check_attn("attn_prefill", kv, q, y, t, n_q, rows, qs, ys, q8, q8s, ws, ws_bytes, amdc_attn_prefill_ws(kv, n_q, rows)))) return rc;
   const u32 tiles = pre_tiles(kv, n_q, rows, cu != NULL, T, &parts);
   const u64 grid = (u64)tiles * parts * kv->n_kv;
-  if (grid >= (1u << 24)) return fail(AMDC_EINVAL, "attn_prefill: %u rows of %u sequences and %u heads are too many for one call", rows, kv->n_seq, kv->n_kv);
+  if (grid >= (1u << 23)) return fail(AMDC_EINVAL, "attn_prefill: %u rows of %u sequences and %u heads are too many for one call", rows, kv->n_seq, kv->n_kv);
   attn_args a = {q, y, cu, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, parts, attn_vec(q, y, t, rows, qs, ys), tiles, 0};
   void *args[] = {&d, &a};
   if ((rc = launch_pre(attn_kernel(K_ATTN_PRE, kv, t), kv->hd, (unsigned)grid, stream, args)) || parts == 1u) return rc;

@@ -23,7 +23,7 @@
  * GEMV and its per-tile arrival counters, amdc_gemv_*_x with q8 NULL above the fused size) share it: work of
  * theirs queued on different streams, or in graphs replayed on them, must be
  * ordered (one stream, or an event between), or their results race. The same
- * holds for amdc_op_gemv_noalloc and its fixed workspace. */
+ * holds for amdc_op_gemv_noalloc and its fixed workspace. The attention operators take a workspace of the caller's instead. */
 #ifndef AMDC_Q4_H
 #define AMDC_Q4_H
 
@@ -334,7 +334,7 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
  * most 128) over its cached positions, theirs included (append first): for row t of sequence b, head i
  *   y = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q.k_j),  head i reads key / value head i / (n_q / n_kv),
  * over the positions j <= len[b] - T + t, with window not 0 the last `window` of them only. q and y have type
- * t (AMDC_TYPE_F32 or the cache's), rows qs and ys values apart. Queries are used as they are given; in f32, the
+ * t (AMDC_TYPE_F32 or the cache's), rows qs and ys values apart, and do not overlap. Queries are used as they are given; in f32, the
  * scores, weights, sums and y keep f32's accuracy (the products run on the 16-bit matrix units in parts); in a
  * 16-bit type the weights are rounded to it. With q8 not NULL also the Q8 copy of the rows (n_q hd values), q8s
  * bytes apart, for the output matrix: the bits of amdc_quant_q8 of the f32 result (before y's rounding).
@@ -343,7 +343,7 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
  * ws: amdc_attn_decode_ws(kv, n_q, T) bytes of device memory, 16-byte aligned, cleared to 0 once before the first use
  * with any call (the calls leave its counters at 0); calls that share it must not overlap on the device, calls with
  * workspaces of their own may. The size does not depend on the lengths. Nothing is allocated: every call can be
- * captured. The result does not depend on the order in which workgroups run. n_seq max_pages page is under 2^36. */
+ * captured. The result does not depend on the order in which workgroups run. n_seq max_pages page is under 2^35. */
 size_t amdc_attn_decode_ws(const amdc_kv *kv, uint32_t n_q, uint32_t T);
 int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
                      uint32_t window, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream);
