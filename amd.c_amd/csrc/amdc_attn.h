@@ -527,8 +527,9 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
   bool bad = false;
   auto get_ids = [&](u32 st) {
     const u32 s = st + NW * (lane / TT), p = SP * s + 16u * (lane % TT);
-    const bool in = s < s1; // behind the last position: the last page again
-    ids = in ? table[(p < L ? p : L - 1u) >> kv.lgp] : 0;
+    ids = s < s1 ? table[(p < L ? p : L - 1u) >> kv.lgp] : 0; // behind the last position: the last page again
+  };
+  auto check_ids = [&]() {
     if ((u32)ids >= kv.n_pages) bad = true, ids = 0;
   };
   auto base = [&](u32 st, u32 i, u32 j) {
@@ -569,13 +570,8 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
   };
   u32 st = s0 + wv;
   u64 ga = 0u, gz = 0u;
-  if (st < s1) {
-    get_ids(st);
-    ga = base(st, 0u, 0u), gz = base(st, 0u, TT - 1u);
-    load_k(ga, gz), load_v(ga, gz);
-  }
-
-  // the queries into the LDS, as the B operand: part p, values 8 c .. 8 c + 7, column
+  get_ids(st);
+  // the queries into the LDS before the cache is asked for (after it, the compiler would wait for both), as the B operand: part p, values 8 c .. 8 c + 7, column
 #pragma unroll
   for (u32 e = 0; e < QE; e++) {
     const u32 col = (tid + NTH * e) >> 4, c0 = tid & 15u;
@@ -608,6 +604,11 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
 #pragma unroll
       for (int p = 0; p < NP; p++) *(u32x4 *)(sm + ((p * (HD / 8u) + c) * R + col) * 16u) = (u32x4){w[p][0], w[p][1], w[p][2], w[p][3]};
     }
+  }
+  check_ids();
+  if (st < s1) {
+    ga = base(st, 0u, 0u), gz = base(st, 0u, TT - 1u);
+    load_k(ga, gz), load_v(ga, gz);
   }
   if (tid == 0u) s_bad = 0u;
   v8_barrier(); // not __syncthreads: the first keys and values stay in flight
@@ -653,7 +654,7 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
     }
     const bool more = st + NW < s1;
     if (more) {
-      if ((i & (64u / TT - 1u)) == 64u / TT - 1u) get_ids(st + NW);
+      if ((i & (64u / TT - 1u)) == 64u / TT - 1u) get_ids(st + NW), check_ids();
       ga = base(st + NW, i + 1u, 0u), gz = base(st + NW, i + 1u, TT - 1u);
       load_k(ga, gz);
     }
@@ -950,12 +951,14 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
   constexpr int NP = F32 ? (BF ? 3 : 2) : 1, NA = W == 32u ? 16 : 4, DT = HD / W;
   constexpr u32 TT = W == 32u ? 1u : 2u, KS = HD / (W == 32u ? 16u : 32u), PF = W / 16u; // of 32 positions: score tiles, steps over hd, weight operands
   constexpr u32 NW = PRE_BM / W, NTH = 64u * NW, MT = BN / 32u, TB = BN * HD * 2u, QD = HD / 4u;
+  // the keys' groups of 16 positions in the LDS: W = 16 reads two at once, 16 banks apart
+  constexpr u32 GS = 32u * HD + (W == 16u ? 64u : 0u), KB = BN / 16u * GS;
   constexpr u32 PG = HD / 16u, PW = BN / 16u * PG / NW; // KB of a group of 16 positions (keys, then values), and of a tile for each wave
   constexpr float BIAS = BF ? 0.0f : 8.0f, RAISE = 6.0f, NINF = -__builtin_inff();
   constexpr bool FULL = HD > 128 && NP > 1; // of registers: the queries' last part stays in the LDS
   constexpr int QR = FULL ? NP - 1 : NP;
   __shared__ u32x4 s_q[FULL ? KS : 1][FULL ? NTH : 1]; // step, thread
-  __shared__ __attribute__((aligned(16))) uint8_t sm[2][2][TB]; // half, keys / values
+  __shared__ __attribute__((aligned(16))) uint8_t sm[2][KB + TB]; // half: keys, values
   __shared__ u32 s_bad;
   const u32 tid = threadIdx.x, lane = tid & 63u, wv = (u32)__builtin_amdgcn_readfirstlane((int)(tid >> 6)), n = lane & (W - 1u), gg = lane / W;
   auto zero = []() {
@@ -1039,7 +1042,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
       const u32 c = pc0 + i;
       const bool val = c >= PG / 2u;
       const u32 o = 1024u * (val ? c - PG / 2u : c);
-      lds_load16(val ? rv : rk, (__attribute__((address_space(3))) void *)(sm[half][val] + grp * (u32)gb + o), o + 16u * lane);
+      lds_load16(val ? rv : rk, (__attribute__((address_space(3))) void *)(sm[half] + (val ? KB + grp * (u32)gb : grp * GS) + o), o + 16u * lane);
     }
   };
   if (tid == 0u) s_bad = 0u;
@@ -1082,8 +1085,8 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
 #pragma unroll
   for (int d = 0; d < DT; d++) O[d] = zero();
   float m = NINF, l = 0.0f;
-  const u32 koff = (W == 32u ? (n >> 4) * (u32)gb + (8u * ((n >> 2) & 1u) + 4u * ((n >> 3) & 1u) + (n & 3u)) * 16u
-                             : (n >> 3) * (u32)gb + (8u * ((n >> 2) & 1u) + (n & 3u)) * 16u) + gg * 256u,
+  const u32 koff = (W == 32u ? (n >> 4) * GS + (8u * ((n >> 2) & 1u) + 4u * ((n >> 3) & 1u) + (n & 3u)) * 16u
+                             : (n >> 3) * GS + (8u * ((n >> 2) & 1u) + (n & 3u)) * 16u) + gg * 256u,
             voff = (gg * HD + n) * 16u;
   // N groups of 32 positions from p0 on, keys at kt and values at vt in the LDS; EDGE: not every row sees all of them
   auto tile = [&](auto edge, auto groups, const uint8_t *kt, const uint8_t *vt, u32 p0) __attribute__((always_inline)) {
@@ -1100,7 +1103,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
         if (FULL && k % 2u == 0u) __asm__ volatile("" ::: "memory"); // few operands at a time: the registers are full
 #pragma unroll
         for (u32 u = 0; u < TT; u++) {
-          const u32x4 kf = *(const u32x4 *)(kt + t * 2u * (u32)gb + 32u * HD / KS * k + 64u * u);
+          const u32x4 kf = *(const u32x4 *)(kt + t * 2u * GS + 32u * HD / KS * k + 64u * u);
 #pragma unroll
           for (int p = 0; p < QR; p++) c[u] = mfma(kf, qf[p][k], c[u]);
           if (FULL) c[u] = mfma(kf, s_q[k][tid], c[u]);
@@ -1200,13 +1203,13 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
     vm_wait(0u);  // this tile has landed ...
     v8_barrier(); // ... every wave's part, and every wave is done with the other half
     if (j + 1u < je) issue(j + 1u, half ^ 1u);
-    const uint8_t *kt = sm[half][0] + koff, *vt = sm[half][1] + voff;
+    const uint8_t *kt = sm[half] + koff, *vt = sm[half] + KB + voff;
     if (!wr || p0 >= hi_z || p0 + BN <= lo_a) continue;
     if (p0 + BN <= hi_a && p0 >= lo_z) tile(std::false_type(), std::integral_constant<u32, MT>(), kt, vt, p0);
     else // an edge, 32 positions at a time
       for (u32 t = 0; t < MT; t++)
         if (p0 + 32u * t < hi_z && p0 + 32u * t + 32u > lo_a)
-          tile(std::true_type(), std::integral_constant<u32, 1u>(), kt + t * 2u * (u32)gb, vt + t * 64u * HD, p0 + 32u * t);
+          tile(std::true_type(), std::integral_constant<u32, 1u>(), kt + t * 2u * GS, vt + t * 64u * HD, p0 + 32u * t);
   }
   l = over(l, addf);
   if (__ballot(bad) && lane == 0u) kv_bad(kv, AMDC_BAD_PAGE), s_bad = 1u;
