@@ -897,6 +897,12 @@ __device__ __forceinline__ v16f mfma32(u32x4 a, u32x4 b, v16f c) {
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
+// lds_load16 with a scalar offset too: one lane offset for every piece of a tile
+__device__ __forceinline__ void lds_load16s(__amdgpu_buffer_rsrc_t rs, __attribute__((address_space(3))) void *d, u32 voff, u32 soff) {
+  const u32 m = __builtin_amdgcn_readfirstlane((u32)(__UINTPTR_TYPE__)d);
+  __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m), "v"(voff), "s"(rs), "s"(soff) : "memory");
+}
+
 #define PRE_BM 128u     // query rows of a workgroup
 #define PRE_MINTILES 4u // tiles of positions that a part has at least
 #define PRE_SB(hd) ((PRE_BM * (hd) + 2u * PRE_BM) * 4u) // bytes of a partial result
@@ -1018,31 +1024,27 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
 
   // loads: wave wv moves the pieces wv PW .. of a tile, all of one group of positions
   const u32 grp = wv * PW / PG, pc0 = wv * PW % PG;
-  const u64 gb = 32ull * HD, hb = gb << (kv.lgp - 4u);
+  constexpr u32 GB = 32u * HD; // bytes of a group: a power of two
   const u32 pmask = (1u << kv.lgp) - 1u;
   const int *table = kv.pages + (u64)pu.b * kv.max_pages;
-  int ids = 0; // of the group of tiles jt .. jt + 63
+  u32 at16 = 0u; // where in the pools, in groups, the wave's group of tiles jt .. jt + 63 is (a lane each)
   bool bad = false;
-  // the first position of the wave's group of tile j; behind the sequence's last group that one again
-  auto place = [&](u32 j) { const u32 p = BN * j + 16u * grp, e = (L - 1u) & ~15u; return p < e ? p : e; };
   auto get_ids = [&](u32 jt) {
-    const u32 p = place(jt + lane);
-    const bool in = jt + lane < je;
-    ids = in ? table[p >> kv.lgp] : 0;
-    if ((u32)ids >= kv.n_pages) bad = true, ids = 0;
+    // behind the last tile that one again, behind the sequence's last group of positions that one
+    const u32 j = jt + lane < je ? jt + lane : je - 1u, f = BN * j + 16u * grp, e = (L - 1u) & ~15u, p = f < e ? f : e;
+    u32 id = (u32)table[p >> kv.lgp];
+    if (id >= kv.n_pages) bad = true, id = 0u;
+    at16 = ((id * kv.n_kv + h) << (kv.lgp - 4u)) + ((p & pmask) >> 4);
   };
   auto issue = [&](u32 j, u32 half) {
     if (((j - jb) & 63u) == 0u) get_ids(j);
-    const u32 p = place(j);
-    const u64 o64 = ((u64)(u32)__builtin_amdgcn_readlane(ids, (int)((j - jb) & 63u)) * kv.n_kv + h) * hb + ((p & pmask) >> 4) * gb;
-    const u64 off = (u64)(u32)__builtin_amdgcn_readfirstlane((int)(u32)(o64 >> 32)) << 32 | (u32)__builtin_amdgcn_readfirstlane((int)(u32)o64);
-    const __amdgpu_buffer_rsrc_t rk = rsrc(kv.k + off, (u32)gb), rv = rsrc(kv.v + off, (u32)gb);
+    const u64 off = (u64)lane_of(at16, (j - jb) & 63u) * GB;
 #pragma unroll
     for (u32 i = 0; i < PW; i++) {
       const u32 c = pc0 + i;
       const bool val = c >= PG / 2u;
       const u32 o = 1024u * (val ? c - PG / 2u : c);
-      lds_load16(val ? rv : rk, (__attribute__((address_space(3))) void *)(sm[half] + (val ? KB + grp * (u32)gb : grp * GS) + o), o + 16u * lane);
+      lds_load16s(rsrc((val ? kv.v : kv.k) + off, GB), (__attribute__((address_space(3))) void *)(sm[half] + (val ? KB + grp * GB : grp * GS) + o), 16u * lane, o);
     }
   };
   if (tid == 0u) s_bad = 0u;

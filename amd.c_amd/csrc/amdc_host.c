@@ -1607,7 +1607,7 @@ size_t amdc_kv_bytes(int type, uint32_t n_kv, uint32_t hd, uint32_t page, uint32
       page > 65536u || (page & (page - 1u)) || !n_pages || n_pages > 0x7FFFFFFFu)
     return 0;
   const u64 row = (u64)n_kv * hd * page * 2u;
-  if (n_pages > UINT64_MAX / row) return 0;
+  if ((u64)n_kv * (page / 16u) * n_pages >= (1ull << 32)) return 0; /* the kernels number groups of 16 positions in 32 bits: 8 TB and more */
   return (size_t)(row * n_pages);
 }
 

@@ -88,6 +88,6 @@ def test_kv_bytes():
     import amdc
     assert amdc.kv_bytes(1, 8, 128, 16, 10) == 8 * 128 * 16 * 10 * 2
     assert amdc.kv_bytes(2, 4, 256, 64, 3) == 4 * 256 * 64 * 3 * 2
-    for bad in ((0, 8, 128, 16, 1), (1, 8, 80, 16, 1), (1, 8, 128, 24, 1), (1, 0, 128, 16, 1), (1, 8, 128, 16, 0)):
+    for bad in ((0, 8, 128, 16, 1), (1, 8, 80, 16, 1), (1, 8, 128, 24, 1), (1, 0, 128, 16, 1), (1, 8, 128, 16, 0), (1, 8, 64, 64, 1 << 27)):
         with pytest.raises(amdc.AmdcError):
             amdc.kv_bytes(*bad)
