@@ -1271,33 +1271,37 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
 
 // The parts of a split tile joined in the order of their positions: 16 of its rows, JOIN_N parts' loads in flight a thread
 #define JOIN_N 8u
+#define PRE_MAXPARTS 64u
 template <bool BF, bool F32>
 __device__ __forceinline__ void join_body(const amdc_kv_dev &kv, const AttnArgs &a, u32 hd, u32 BN) {
-  __shared__ float s_M[16], s_L[16], s_w[JOIN_N][16];
+  __shared__ float s_w[PRE_MAXPARTS][16], s_l[PRE_MAXPARTS][16], s_L[16]; // of every part and row: m, then its weight; l
   const u32 tid = threadIdx.x, qd = hd / 4u, nbq = a.n_q * hd / 32u;
   const u32 h = blockIdx.x % kv.n_kv, x = blockIdx.x / kv.n_kv, unit = x / (PRE_BM / 16u), f = x % (PRE_BM / 16u) * 16u;
   const PreUnit pu = pre_unit(kv, a, unit, BN);
   if (f >= pu.nr || !pu.s.len || pu.ns == 1u) return; // nothing to join: the rows are written
   const u32 nr = pu.nr - f < 16u ? pu.nr - f : 16u, ns = pu.ns, pf = PRE_SB(hd) / 4u; // floats of a partial result
   const float *parts = (const float *)(a.ws + ATTN_CNT) + ((u64)unit * kv.n_kv + h) * a.U * pf, *ml = parts + PRE_BM * hd + f;
-  if (tid < 16u) {
-    const u32 r = tid < nr ? tid : 0u;
-    float M = -__builtin_inff(), sum = 0.0f;
-    for (u32 k = 0u; k < ns; k++) M = __builtin_fmaxf(M, ml[k * pf + r]);
-    const float ref = M == -__builtin_inff() ? 0.0f : M;
-    for (u32 k = 0u; k < ns; k++) sum += __builtin_amdgcn_exp2f(ml[k * pf + r] - ref) * ml[k * pf + PRE_BM + r];
-    s_M[tid] = ref, s_L[tid] = sum;
+  for (u32 e = tid; e < 16u * ns; e += 256u) {
+    const u32 r = e & 15u, k = e >> 4;
+    const float *p = ml + (u64)k * pf + (r < nr ? r : 0u);
+    s_w[k][r] = p[0], s_l[k][r] = p[PRE_BM];
   }
+  __syncthreads();
+  if (tid < 16u) {
+    float M = -__builtin_inff(), sum = 0.0f;
+    for (u32 k = 0u; k < ns; k++) M = __builtin_fmaxf(M, s_w[k][tid]);
+    const float ref = M == -__builtin_inff() ? 0.0f : M;
+    for (u32 k = 0u; k < ns; k++) {
+      const float w = __builtin_amdgcn_exp2f(s_w[k][tid] - ref);
+      s_w[k][tid] = w, sum += w * s_l[k][tid];
+    }
+    s_L[tid] = sum;
+  }
+  __syncthreads();
   v4f v[4]; // quads tid, tid + 256, .. of the 16 rows: at most 4
 #pragma unroll
   for (u32 i = 0; i < 4u; i++) v[i] = (v4f){0.0f, 0.0f, 0.0f, 0.0f};
   for (u32 k0 = 0u; k0 < ns; k0 += JOIN_N) {
-    __syncthreads();
-    if (tid < 16u * JOIN_N) {
-      const u32 r = tid & 15u, k = k0 + (tid >> 4);
-      s_w[tid >> 4][r] = k < ns && r < nr ? __builtin_amdgcn_exp2f(ml[k * pf + r] - s_M[r]) : 0.0f;
-    }
-    __syncthreads();
 #pragma unroll
     for (u32 i = 0; i < 4u; i++) {
       const u32 e = tid + 256u * i;
@@ -1307,7 +1311,7 @@ __device__ __forceinline__ void join_body(const amdc_kv_dev &kv, const AttnArgs 
       for (u32 k = 0; k < JOIN_N; k++) w[k] = *(const v4f *)(parts + (u64)(k0 + k < ns ? k0 + k : k0) * pf + f * hd + 4u * e);
 #pragma unroll
       for (u32 k = 0; k < JOIN_N; k++)
-        if (k0 + k < ns) v[i] += s_w[k][e / qd] * w[k];
+        if (k0 + k < ns) v[i] += s_w[k0 + k][e / qd] * w[k];
     }
   }
 #pragma unroll

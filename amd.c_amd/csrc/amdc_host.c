@@ -1785,6 +1785,7 @@ int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t 
  * the tiles of all heads are fewer than the CUs hold (pre_body in amdc_attn.h). */
 #define PRE_BM 128u
 #define PRE_MINTILES 4u
+#define PRE_MAXPARTS 64u
 #define PRE_BN(hd) ((hd) > 128u ? 32u : 64u) /* positions of a tile */
 static u32 pre_want(u32 hd) { return (g_cus > 0 ? (u32)g_cus : 256u) * (hd > 128u ? 1u : 2u); }
 static u32 pre_tiles(const amdc_kv *kv, u32 n_q, u32 rows, int ragged, u32 T, u32 *parts) {
@@ -1793,7 +1794,9 @@ static u32 pre_tiles(const amdc_kv *kv, u32 n_q, u32 rows, int ragged, u32 T, u3
   const u64 wgs = tiles * kv->n_kv, want = pre_want(kv->hd);
   /* parts of at least PRE_MINTILES tiles of the most positions that the table holds; 1: no join */
   const u64 most = (u64)kv->max_pages * kv->page / (PRE_MINTILES * PRE_BN(kv->hd));
-  *parts = wgs < want && most > 1u ? (u32)(want / wgs < most ? want / wgs : most) : 1u;
+  u64 p = wgs < want ? want / wgs : 1u;
+  if (p > most) p = most;
+  *parts = p < 2u ? 1u : p < PRE_MAXPARTS ? (u32)p : PRE_MAXPARTS;
   return tiles < (1u << 24) ? (u32)tiles : 1u << 24;
 }
 
