@@ -412,6 +412,11 @@ __device__ __forceinline__ void split_n(float (&x)[N], u32 (&w)[NP][N / 2]) {
 // A step that holds positions which not every column sees is multiplied into sums of its own: where these come out finite they are
 // added, as weights of 0 are right; if not (0 times an infinity or a NaN that a column must not see), again with what no column sees as
 // 0, and if that is not enough token by token with what it does not see as 0.
+//
+// Measured on MI355X (replayed, buffers in turn): 60001 positions, 24 / 4 heads of 256, f16, f32 queries (246 MB) 47.5 us, 5.2 TB/s; 64
+// sequences of 30 to 16000, 32 / 8 heads of 128, bf16 (699 MB) 135 us, 5.2 TB/s; 8 sequences of 900 to 6000, T = 5, 24 / 4 heads of
+// 256 (104 MB, two blocks of columns, the second from the L2) 34 us, 3.1 TB/s; 421 positions, 32 / 32 heads of 128 8.3 us, all latency.
+// A plain read reaches 6.3 TB/s. Four waves a workgroup, two workgroups a CU and loads not ahead of the queries: 54, 151 and 54 us.
 template <int HD, bool BF, bool F32, u32 NC, u32 NW>
 __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &a) {
   constexpr int NP = F32 ? (BF ? 3 : 2) : 1, KS = HD / 32, DT = HD / 16;
@@ -951,6 +956,10 @@ __device__ __forceinline__ PreUnit pre_unit(const amdc_kv_dev &kv, const AttnArg
 // Rows are dealt from the last tile of the last sequence down: the longest first. Where all rows make fewer workgroups than the CUs
 // hold (a short chunk of a long prompt), a tile's positions are split over a.U workgroups; their partial results go through the
 // workspace and amdc_attn_join_*, a launch of its own (joined by the last workgroup to arrive, 128 rows of four parts took it 18 us).
+// Measured on MI355X (replayed): 12000 rows of 32 / 8 heads of 128, bf16, 1.19 ms, 991 TFLOP/s of causal work (a large product: 1210),
+// matrix units busy 52 % of the cycles, vector units 54 %; 11 prompts under a window, heads of 64, f16, 70 to 75 us, 513 TFLOP/s,
+// vector units busy 65 % (the exponentials); a chunk of 256 over 5000, 24 / 4 heads of 256, f32, 85.5 us with its join of 10; 77 rows, 32
+// / 32 heads of 128 12.5 us, latency.
 template <int HD, bool BF, bool F32, u32 W, u32 BN>
 __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &a) {
   typedef typename std::conditional<W == 32u, v16f, v4f>::type acc; // of a matrix instruction: W x W / 64

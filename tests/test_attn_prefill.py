@@ -226,7 +226,7 @@ def test_graph_streams_and_workspaces(dev):
         a.new, a.rows = new, sum(new)
         a.cu = np.array([0, new[0], sum(new)], np.int32)
         a.dcu.upload(a.cu)
-        q = ca.g if hasattr(ca, "g") else np.random.default_rng(step)
+        q = np.random.default_rng(step)
         x = q.standard_normal((ca.rows, ca.w)).astype(np.float32)
         ca.Q.upload(x)
         ca.q = x.astype(np.float64).reshape(ca.q.shape)
