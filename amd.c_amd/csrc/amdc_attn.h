@@ -520,7 +520,7 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
   __asm__ volatile("" ::: "memory");
 
   // the steps of the wave: every NW-th of the chunk's [s0, s1)
-  const u32 s0 = first(L) / SP + ci * C, send = cdiv(L, SP), s1 = s0 + C < send ? s0 + C : send;
+  const u32 seen0 = first(L), s0 = seen0 / SP + ci * C, send = cdiv(L, SP), s1 = s0 + C < send ? s0 + C : send;
   const u64 gb = 32ull * HD, hb = gb << (kv.lgp - 4u); // bytes of 16 positions of a head, of a page of a head
   const u32 pmask = (1u << kv.lgp) - 1u;
   const int *table = kv.pages + (u64)b * kv.max_pages;
@@ -532,7 +532,8 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
   bool bad = false;
   auto get_ids = [&](u32 st) {
     const u32 s = st + NW * (lane / TT), p = SP * s + 16u * (lane % TT);
-    ids = s < s1 ? table[(p < L ? p : L - 1u) >> kv.lgp] : 0; // behind the last position: the last page again
+    // behind the last position that a row sees the last page again, before the first the first: other entries are not looked at
+    ids = s < s1 ? table[(p < seen0 ? seen0 : p < L ? p : L - 1u) >> kv.lgp] : 0;
   };
   auto check_ids = [&]() {
     if ((u32)ids >= kv.n_pages) bad = true, ids = 0;
@@ -1038,9 +1039,10 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
   const int *table = kv.pages + (u64)pu.b * kv.max_pages;
   u32 at16 = 0u; // where in the pools, in groups, the wave's group of tiles jt .. jt + 63 is (a lane each)
   bool bad = false;
+  const u32 seen0 = lo_of(r0 / G) & ~15u;
   auto get_ids = [&](u32 jt) {
-    // behind the last tile that one again, behind the sequence's last group of positions that one
-    const u32 j = jt + lane < je ? jt + lane : je - 1u, f = BN * j + 16u * grp, e = (L - 1u) & ~15u, p = f < e ? f : e;
+    // behind the last tile that one again, behind the sequence's last group of positions that one, before the first that a row sees that
+    const u32 j = jt + lane < je ? jt + lane : je - 1u, f = BN * j + 16u * grp, e = (L - 1u) & ~15u, p = f < seen0 ? seen0 : f < e ? f : e;
     u32 id = (u32)table[p >> kv.lgp];
     if (id >= kv.n_pages) bad = true, id = 0u;
     at16 = ((id * kv.n_kv + h) << (kv.lgp - 4u)) + ((p & pmask) >> 4);

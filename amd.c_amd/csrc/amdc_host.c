@@ -1713,7 +1713,7 @@ static int check_attn(const char *op, const amdc_kv *kv, const void *q, const vo
   const u64 w = (u64)n_q * kv->hd, es = t == AMDC_TYPE_F32 ? 4u : 2u;
   if (!q || (!y && !q8)) return fail(AMDC_EINVAL, "%s: null pointer (q, or both y and q8)", op);
   if (!vec_rows(q, 0, (u32)es) || !vec_rows(y, 0, (u32)es)) return fail(AMDC_EINVAL, "%s: q and y must be aligned to their type", op);
-  if (q == y) return fail(AMDC_EINVAL, "%s: y cannot be written over q", op);
+  if (q == y || q == q8 || y == q8) return fail(AMDC_EINVAL, "%s: q, y and q8 cannot be the same", op);
   if (rows > 1u && (qs < w || (y && ys < w))) return fail(AMDC_EINVAL, "%s: strides qs %u, ys %u under a row's %llu values", op, qs, ys, (unsigned long long)w);
   if (q8 && (!vec_rows(q8, rows > 1u ? q8s : 0u, 4u) || (rows > 1u && q8s < w / 32u * 40u)))
     return fail(AMDC_EINVAL, "%s: q8 and q8s (%u) must be multiples of 4, q8s at least %llu", op, q8s, (unsigned long long)(w / 32u * 40u));

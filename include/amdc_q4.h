@@ -299,8 +299,9 @@ enum { AMDC_TYPE_F32 = 0, AMDC_TYPE_F16 = 1, AMDC_TYPE_BF16 = 2 };
  *
  * What only the device sees is checked there: a page outside the pool, a length over
  * max_pages * page or under the sequence's number of new tokens, rows outside 0 .. T. Such an entry is never
- * followed: append leaves out the positions concerned, attention gives NaN in the sequence's rows (rows outside
- * 0 .. T: writes none of the sequence), and amdc_kv_check() reports it. */
+ * followed: append leaves out the positions concerned, attention gives NaN in the sequence's rows (a page: in those that
+ * see it, at least; rows outside 0 .. T: writes none of the sequence), and amdc_kv_check() reports it. Pages whose positions are
+ * all before the window of every row, or behind the last position, are not looked at: their entries may be anything. */
 typedef struct {
   int type; /* AMDC_TYPE_F16 or AMDC_TYPE_BF16 */
   uint32_t n_kv, hd, page, n_pages;
@@ -318,7 +319,7 @@ int amdc_kv_check(void);
 /* Appends the new tokens' keys and values to the cache, the keys rotated by their positions, and with q
  * not NULL writes the rotated queries to qo (type qt: AMDC_TYPE_F32 or the cache's). Rows of k, v (n_kv
  * heads) and q, qo (n_q heads, a multiple of n_kv) are ks, vs, qs, qos values apart: the qkv matrix's output rows
- * can be passed as they are. qo may be q itself where the type and the stride are the same.
+ * can be passed as they are. qo may be q itself where the type and the stride are the same, and else overlaps no input.
  * The rotation turns n_rot / 2 pairs of values of a head (n_rot even, at most hd; the values behind n_rot are
  * kept) by the angles p freq[i] (freq: n_rot / 2 device floats; the product and its reduction in 64 bits):
  *   AMDC_ROPE_PAIRS   the pair i is the values 2 i, 2 i + 1
@@ -334,12 +335,13 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
  * most 128) over its cached positions, theirs included (append first): for row t of sequence b, head i
  *   y = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q.k_j),  head i reads key / value head i / (n_q / n_kv),
  * over the positions j <= len[b] - T + t, with window not 0 the last `window` of them only. q and y have type
- * t (AMDC_TYPE_F32 or the cache's), rows qs and ys values apart, and do not overlap. Queries are used as they are given; in f32, the
+ * t (AMDC_TYPE_F32 or the cache's), rows qs and ys values apart; q, y and q8 do not overlap. Queries are used as they are given; in f32, the
  * scores, weights, sums and y keep f32's accuracy (the products run on the 16-bit matrix units in parts); in a
  * 16-bit type the weights are rounded to it. With q8 not NULL also the Q8 copy of the rows (n_q hd values), q8s
  * bytes apart, for the output matrix: the bits of amdc_quant_q8 of the f32 result (before y's rounding).
  * A value (or key) that a row does not see may be anything, NaN too, also where another row sees it. Of those that
- * it sees, a value that is not finite makes its place of the row infinite or NaN, a key that is not finite the row NaN.
+ * it sees, a value that is not finite makes its place of the row infinite or NaN, a key that is not finite the row NaN (or, where
+ * the score is -infinity, counts for nothing).
  * ws: amdc_attn_decode_ws(kv, n_q, T) bytes of device memory, 16-byte aligned, cleared to 0 once before the first use
  * with any call (the calls leave its counters at 0); calls that share it must not overlap on the device, calls with
  * workspaces of their own may. The size does not depend on the lengths. Nothing is allocated: every call can be

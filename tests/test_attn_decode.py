@@ -182,6 +182,20 @@ def test_infinities_before_the_window(dev):
     Call(c, F16, 2, window=40).launch().check()
 
 
+@pytest.mark.parametrize("ty,hd,page", [(F16, 64, 16), (BF16, 128, 16), (F16, 128, 32), (F16, 256, 16)])
+def test_pages_before_the_window(dev, ty, hd, page):
+    """Entries of pages that are wholly before every row's window, given back to the pool, may be anything."""
+    lens, T, window = (300, 77, 90, 2000), 2, 40
+    c = Case(dev, 60, ty, 8, 2, hd, page, lens, (T,) * 4).fill_all().upload()
+    gone = c.table.copy()
+    for b, L in enumerate(lens):
+        gone[b, :max(0, L - T + 1 - window) // page] = (-1, 999999, 0x7FFFFFFF, -2 ** 31)[b]
+    c.dtable.upload(gone)
+    for t in (F32, ty):
+        Call(c, t, T, window=window).launch().check()
+    dev.kv_check()
+
+
 def test_extreme_scores(dev):
     """Queries over f16's range (scaled down again by the scale), tiny ones, rows of zero, scores hundreds apart, a negative scale."""
     c = Case(dev, 35, F16, 4, 2, 128, 16, (200, 33), (1, 1)).fill_all().upload()

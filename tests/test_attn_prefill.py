@@ -178,6 +178,20 @@ def test_keys_where_rows_do_not_see(dev):
         assert np.isnan(y[~ok]).all()
 
 
+@pytest.mark.parametrize("ty,hd,page,lens,new", [(F16, 64, 16, (300, 77, 700), (20, 9, 70)), (BF16, 128, 32, (300, 77, 3000), (20, 9, 3)), (F16, 256, 16, (300, 77, 5000), (20, 1, 4))])
+def test_pages_before_the_window(dev, ty, hd, page, lens, new):
+    """Entries of pages that are wholly before every row's window, given back to the pool, may be anything."""
+    window = 40
+    c = Case(dev, 471, ty, 4, 2, hd, page, lens, new).fill_all().upload()
+    gone = c.table.copy()
+    for b, L in enumerate(lens):
+        gone[b, :max(0, L - new[b] + 1 - window) // page] = (-1, 999999, -2 ** 31)[b]
+    c.dtable.upload(gone)
+    for t in (F32, ty):
+        Call(c, t, window=window).launch().check()
+    dev.kv_check()
+
+
 def test_extreme_scores(dev):
     c = Case(dev, 480, F16, 4, 2, 128, 16, (100, 33), (100, 20)).fill_all().upload()
     q = c.g.standard_normal((120, 4 * 128))

@@ -23,15 +23,16 @@ BAD = {
 ATTN = dict(q=4096, y=8192, type=0, n_q=8, T=3, qs=512, ys=512, scale=0.125, ws=4096, ws_bytes=1 << 30, window=0, q8=None, q8s=0)
 ATTN_BAD = [b for b in BAD["append"] if b[0] == "kv"] + [
     (None, c) for c in (dict(q=None), dict(y=None), dict(y=4096), dict(type=2), dict(type=3), dict(n_q=0), dict(n_q=7), dict(T=0), dict(qs=511), dict(ys=511), dict(q=4098), dict(y=8193),
-                        dict(ws=None), dict(ws=4104), dict(ws_bytes=65536), dict(q8=4097, q8s=640), dict(q8=4096, q8s=636), dict(q8=4096, q8s=642))]
+                        dict(ws=None), dict(ws=4104), dict(ws_bytes=65536), dict(q8=12289, q8s=640), dict(q8=12288, q8s=636), dict(q8=12288, q8s=642),
+                        dict(q8=4096, q8s=640), dict(q8=8192, q8s=640))]
 BAD["decode"] = ATTN_BAD + [(None, dict(T=33)), (None, dict(n_q=256, T=2, qs=1 << 14, ys=1 << 14)), ("kv", dict(n_seq=1 << 20, n_kv=128)),
                              ("kv", dict(n_seq=33, max_pages=1 << 26))]
 BAD["prefill"] = ATTN_BAD + [(None, dict(cu=4098)), (None, dict(T=1 << 22)), (None, dict(cu=4096, T=(1 << 22) + 1)), ("kv", dict(n_seq=1 << 20, n_kv=64))]
 BASE = {"append": APPEND, "decode": ATTN, "prefill": ATTN}
 GOOD = {
     "append": [{}, dict(q=None, qo=None, n_q=0, qs=0, qos=0), dict(cu=4096, T=100), dict(rope=0, freq=None, n_rot=0), dict(qt=1), dict(qo=4096), dict(n_q=256, qs=1 << 14, qos=1 << 14)],
-    "decode": [{}, dict(type=1), dict(window=5), dict(y=None, q8=4096, q8s=640), dict(q8=4096, q8s=644), dict(T=32), dict(n_q=256, T=1, qs=1 << 14, ys=1 << 14)],
-    "prefill": [{}, dict(type=1), dict(window=5), dict(cu=4096, T=5000), dict(y=None, q8=4096, q8s=640), dict(q8=4096, q8s=644), dict(T=4000), dict(n_q=256, T=1, qs=1 << 14, ys=1 << 14)],
+    "decode": [{}, dict(type=1), dict(window=5), dict(y=None, q8=12288, q8s=640), dict(q8=12288, q8s=644), dict(T=32), dict(n_q=256, T=1, qs=1 << 14, ys=1 << 14)],
+    "prefill": [{}, dict(type=1), dict(window=5), dict(cu=4096, T=5000), dict(y=None, q8=12288, q8s=640), dict(q8=12288, q8s=644), dict(T=4000), dict(n_q=256, T=1, qs=1 << 14, ys=1 << 14)],
 }
 
 
