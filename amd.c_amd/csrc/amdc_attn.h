@@ -1081,7 +1081,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
       const u32 e = __builtin_bit_cast(u32, big) >> 23, k = e < 11u ? 253u : 264u - e;
       up *= __builtin_bit_cast(float, k << 23), cq *= __builtin_bit_cast(float, (254u - k) << 23);
     }
-    cq = __builtin_fmaxf(cq, 0x1p-126f); // scale 0: a score of 0, also of -infinity (what is not seen) not NaN
+    cq = __builtin_fmaxf(cq, 0x1p-149f); // scale 0: a score of 0 (2^-21 at most), also of -infinity (what is not seen) not NaN
 #pragma unroll
     for (u32 k = 0; k < KS; k++) {
 #pragma unroll
@@ -1341,12 +1341,13 @@ extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_bf16(amdc_kv_de
 
 // Rows of a wave, positions of a tile, workgroups a CU wanted of the registers (MI355X, us). Heads of 128, 16-bit: 64 positions 1204 for
 // 12000 rows of 32 / 8 heads, 32 positions (half the scores' registers) 1342. Heads of 256: 32 rows a wave, one wave a SIMD, 144 where 16
-// rows, two waves, take 110 (256 rows over 5000 positions, 24 / 4 heads, f32)
+// rows, two waves, take 110 (256 rows over 5000 positions, 24 / 4 heads, f32). Heads of 64, 16-bit: three workgroups a CU 76 for 11 prompts
+// under a window, two 81 (with the registers of two); four, of 32 positions, spill, as f32's three do.
 #define PRE_KERNEL(HD, KN, BF, F32, W, BN, OCC) \
   extern "C" __global__ __launch_bounds__(8192 / W, OCC) void amdc_attn_pre_h##HD##_##KN(amdc_kv_dev kv, AttnArgs a) { pre_body<HD, BF, F32, W, BN>(kv, a); }
-PRE_KERNEL(64, f16, false, false, 32, 64, 2)
+PRE_KERNEL(64, f16, false, false, 32, 64, 3)
 PRE_KERNEL(64, f16_f32, false, true, 32, 64, 2)
-PRE_KERNEL(64, bf16, true, false, 32, 64, 2)
+PRE_KERNEL(64, bf16, true, false, 32, 64, 3)
 PRE_KERNEL(64, bf16_f32, true, true, 32, 64, 2)
 PRE_KERNEL(128, f16, false, false, 32, 64, 2)
 PRE_KERNEL(128, f16_f32, false, true, 32, 64, 1)

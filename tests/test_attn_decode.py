@@ -213,6 +213,15 @@ def test_extreme_scores(dev):
     Call(c, BF16, 1, q=q * 1e15, scale=1e-30).launch().check()
 
 
+def test_scales_of_zero_and_near_it(dev):
+    """Scale 0 is the mean, whatever the products; a subnormal scale of products near f32's largest."""
+    c = Case(dev, 61, BF16, 4, 2, 64, 16, (100, 33), (1, 1), amp=1e18).fill_all().upload()
+    q = c.g.standard_normal((2, 4 * 64))
+    for t in (F32, BF16):
+        Call(c, t, 1, q=q * 1e18, scale=0.0).launch().check()
+        Call(c, t, 1, q=q * 1e18, scale=1e-39).launch().check()
+
+
 def test_rising_scores(dev):
     """Scores that grow along the sequence: the maximum is raised again and again."""
     c = Case(dev, 37, F16, 2, 2, 64, 16, (2500,), (1,))

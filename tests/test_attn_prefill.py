@@ -208,6 +208,18 @@ def test_extreme_scores(dev):
     Call(c, F16, q=np.ones((500, 128)), scale=0.5).launch().check(every=7)
 
 
+def test_scales_of_zero_and_near_it(dev):
+    """Scale 0 is the mean, whatever the products; a subnormal scale of products near f32's largest."""
+    c = Case(dev, 482, BF16, 4, 2, 64, 16, (100, 33), (100, 20), amp=1e18).fill_all().upload()
+    q = c.g.standard_normal((120, 4 * 64))
+    for t in (F32, BF16):
+        Call(c, t, q=q * 1e18, scale=0.0).launch().check()
+        Call(c, t, q=q * 1e18, scale=1e-39).launch().check()
+    c = Case(dev, 483, F16, 4, 2, 128, 16, (100, 33), (100, 20)).fill_all().upload()
+    Call(c, F32, scale=0.0, window=30).launch().check()
+    Call(c, F16, scale=0.0).launch().check()
+
+
 def test_offsets_over_4_gib(dev):
     n_pages = 20_000
     size = dev.kv_bytes(BF16, 8, 128, 128, n_pages)
