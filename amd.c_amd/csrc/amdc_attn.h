@@ -1211,18 +1211,28 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
           if (d == (u32)i) O[i] += g;
       }
   };
-  for (u32 j = jb; j < je; j++) {
-    const u32 half = (j - jb) & 1u, p0 = BN * j;
-    vm_wait(0u);  // this tile has landed ...
+  auto step = [&](u32 j) { // to tile j
+    vm_wait(0u);  // it has landed ...
     v8_barrier(); // ... every wave's part, and every wave is done with the other half
-    if (j + 1u < je) issue(j + 1u, half ^ 1u);
-    const uint8_t *kt = sm[half] + koff, *vt = sm[half] + KB + voff;
-    if (!wr || p0 >= hi_z || p0 + BN <= lo_a) continue;
-    if (p0 + BN <= hi_a && p0 >= lo_z) tile(std::false_type(), std::integral_constant<u32, MT>(), kt, vt, p0);
-    else // an edge, 32 positions at a time
-      for (u32 t = 0; t < MT; t++)
-        if (p0 + 32u * t < hi_z && p0 + 32u * t + 32u > lo_a)
-          tile(std::true_type(), std::integral_constant<u32, 1u>(), kt + t * 2u * GS, vt + t * 64u * HD, p0 + 32u * t);
+    if (j + 1u < je) issue(j + 1u, ((j - jb) & 1u) ^ 1u);
+  };
+  // every wave goes through all tiles, those that all of its rows see entirely, j0 .. j1 - 1, in a loop of their own (in one loop with the
+  // others the compiler copies O to other registers and back in every tile)
+  const u32 f0 = wr ? cdiv(lo_z, BN) : je, f1 = wr ? hi_a / BN : je;
+  for (u32 j = jb; j < je;) {
+    for (; j >= f0 && j < f1 && j < je; j++) {
+      step(j);
+      const uint8_t *at = sm[(j - jb) & 1u];
+      tile(std::false_type(), std::integral_constant<u32, MT>(), at + koff, at + KB + voff, BN * j);
+    }
+    if (j >= je) break;
+    step(j);
+    const uint8_t *at = sm[(j - jb) & 1u];
+    const u32 p0 = BN * j++;
+    if (!wr) continue;
+    for (u32 t = 0; t < MT; t++) // an edge, 32 positions at a time
+      if (p0 + 32u * t < hi_z && p0 + 32u * t + 32u > lo_a)
+        tile(std::true_type(), std::integral_constant<u32, 1u>(), at + koff + t * 2u * GS, at + KB + voff + t * 64u * HD, p0 + 32u * t);
   }
   l = over(l, addf);
   if (__ballot(bad) && lane == 0u) kv_bad(kv, AMDC_BAD_PAGE), s_bad = 1u;
