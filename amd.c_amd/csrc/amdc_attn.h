@@ -1167,6 +1167,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
       return __ballot(!(z == 0.0f)) == 0ull;
     };
     u32 redo = 0u;
+    __asm__ volatile("" : "+v"(l)); // summed here: the compiler would keep the weights for it until after the products
     __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int d = 0; d < DT; d++) {
@@ -1241,8 +1242,9 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
 
   auto quad = [&](int d, u32 i) { return (v4f){O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]}; }; // values W d + 8 i + 4 gg .. + 3
   if (ns == 1u) {
-    u32 row, head;
-    at(rc, row, head);
+    u32 row, head, rr = rc;
+    __asm__ volatile("" : "+v"(rr)); // where the row is computed again, not kept in registers since the queries
+    at(rr, row, head);
     const float inv = 1.0f / l;
 #pragma unroll
     for (int d = 0; d < DT; d++) {
@@ -1360,7 +1362,7 @@ PRE_KERNEL(64, f16_f32, false, true, 32, 64, 2)
 PRE_KERNEL(64, bf16, true, false, 32, 64, 3)
 PRE_KERNEL(64, bf16_f32, true, true, 32, 64, 2)
 PRE_KERNEL(128, f16, false, false, 32, 64, 2)
-PRE_KERNEL(128, f16_f32, false, true, 32, 64, 1)
+PRE_KERNEL(128, f16_f32, false, true, 32, 32, 2)
 PRE_KERNEL(128, bf16, true, false, 32, 64, 2)
 PRE_KERNEL(128, bf16_f32, true, true, 32, 64, 1)
 PRE_KERNEL(256, f16, false, false, 16, 32, 2)

@@ -1786,14 +1786,15 @@ int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t 
 #define PRE_BM 128u
 #define PRE_MINTILES 4u
 #define PRE_MAXPARTS 64u
-#define PRE_BN(hd) ((hd) > 128u ? 32u : 64u) /* positions of a tile */
+/* positions of a tile, as PRE_KERNEL of amdc_attn.h has them */
+static u32 pre_bn(const amdc_kv *kv, int t) { return kv->hd > 128u || (kv->hd > 64u && t == AMDC_TYPE_F32 && kv->type == AMDC_TYPE_F16) ? 32u : 64u; }
 static u32 pre_want(u32 hd) { return (g_cus > 0 ? (u32)g_cus : 256u) * (hd > 128u ? 1u : 2u); }
-static u32 pre_tiles(const amdc_kv *kv, u32 n_q, u32 rows, int ragged, u32 T, u32 *parts) {
+static u32 pre_tiles(const amdc_kv *kv, int t, u32 n_q, u32 rows, int ragged, u32 T, u32 *parts) {
   const u32 G = n_q / kv->n_kv;
   const u64 tiles = ragged ? ((u64)rows * G + PRE_BM - 1u) / PRE_BM + kv->n_seq - 1u : (u64)kv->n_seq * (((u64)T * G + PRE_BM - 1u) / PRE_BM);
   const u64 wgs = tiles * kv->n_kv, want = pre_want(kv->hd);
   /* parts of at least PRE_MINTILES tiles of the most positions that the table holds; 1: no join */
-  const u64 most = (u64)kv->max_pages * kv->page / (PRE_MINTILES * PRE_BN(kv->hd));
+  const u64 most = (u64)kv->max_pages * kv->page / (PRE_MINTILES * pre_bn(kv, t));
   u64 p = wgs < want ? want / wgs : 1u;
   if (p > most) p = most;
   *parts = p < 2u ? 1u : p < PRE_MAXPARTS ? (u32)p : PRE_MAXPARTS;
@@ -1814,13 +1815,13 @@ int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t
   int rc = check_kv("attn_prefill", kv, n_q, T, cu, &d, &rows);
   if (rc) return rc;
   if ((rc = check_attn("attn_prefill", kv, q, y, t, n_q, rows, qs, ys, q8, q8s, ws, ws_bytes, amdc_attn_prefill_ws(kv, n_q, rows)))) return rc;
-  const u32 tiles = pre_tiles(kv, n_q, rows, cu != NULL, T, &parts);
+  const u32 tiles = pre_tiles(kv, t, n_q, rows, cu != NULL, T, &parts);
   const u64 grid = (u64)tiles * parts * kv->n_kv;
   if (grid >= (1u << 23)) return fail(AMDC_EINVAL, "attn_prefill: %u rows of %u sequences and %u heads are too many for one call", rows, kv->n_seq, kv->n_kv);
   attn_args a = {q, y, cu, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, parts, attn_vec(q, y, t, rows, qs, ys), tiles, 0};
   void *args[] = {&d, &a};
   if ((rc = launch_pre(attn_kernel(K_ATTN_PRE, kv, t), kv->hd, (unsigned)grid, stream, args)) || parts == 1u) return rc;
-  const u32 bn = PRE_BN(kv->hd);
+  const u32 bn = pre_bn(kv, t);
   void *ja[] = {&d, &a, (void *)&kv->hd, (void *)&bn};
   return launch(K_ATTN_JOIN + t, tiles * (PRE_BM / 16u) * kv->n_kv, 1, 0, stream, ja);
 }
