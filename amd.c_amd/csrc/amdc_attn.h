@@ -971,7 +971,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
   constexpr u32 GS = 32u * HD + (W == 16u ? 64u : 0u), KB = BN / 16u * GS;
   constexpr u32 PG = HD / 16u, PW = BN / 16u * PG / NW; // KB of a group of 16 positions (keys, then values), and of a tile for each wave
   constexpr float BIAS = BF ? 0.0f : 8.0f, RAISE = 6.0f, NINF = -__builtin_inff();
-  constexpr bool FULL = HD > 128 && NP > 1; // of registers: the queries' last part stays in the LDS
+  constexpr bool FULL = HD > 128 && NP > 2; // of registers: the queries' last part stays in the LDS
   constexpr int QR = FULL ? NP - 1 : NP;
   __shared__ u32x4 s_q[FULL ? KS : 1][FULL ? NTH : 1]; // step, thread
   __shared__ __attribute__((aligned(16))) uint8_t sm[2][KB + TB]; // half: keys, values
