@@ -957,10 +957,10 @@ __device__ __forceinline__ PreUnit pre_unit(const amdc_kv_dev &kv, const AttnArg
 // Rows are dealt from the last tile of the last sequence down: the longest first. Where all rows make fewer workgroups than the CUs
 // hold (a short chunk of a long prompt), a tile's positions are split over a.U workgroups; their partial results go through the
 // workspace and amdc_attn_join_*, a launch of its own (joined by the last workgroup to arrive, 128 rows of four parts took it 18 us).
-// Measured on MI355X (replayed): 12000 rows of 32 / 8 heads of 128, bf16, 1.19 ms, 991 TFLOP/s of causal work (a large product: 1210),
-// matrix units busy 52 % of the cycles, vector units 54 %; 11 prompts under a window, heads of 64, f16, 70 to 75 us, 513 TFLOP/s,
-// vector units busy 65 % (the exponentials); a chunk of 256 over 5000, 24 / 4 heads of 256, f32, 85.5 us with its join of 10; 77 rows, 32
-// / 32 heads of 128 12.5 us, latency.
+// Measured on MI355X (replayed; cards differ by 5 %): 12000 rows of 32 / 8 heads of 128, bf16, 1.12 ms, 1050 TFLOP/s of causal work (a
+// large product: 1210), matrix units busy 54 % of the cycles, vector units 42 %, at 1.7 to 1.9 GHz; 11 prompts under a window, heads of
+// 64, f16, 72 us, 530 TFLOP/s, vector units busy 61 % (the exponentials); a chunk of 256 over 5000, 24 / 4 heads of 256, f32, 80 us with
+// its join of 9; 77 rows, 32 / 32 heads of 128 12.2 us, latency.
 template <int HD, bool BF, bool F32, u32 W, u32 BN>
 __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &a) {
   typedef typename std::conditional<W == 32u, v16f, v4f>::type acc; // of a matrix instruction: W x W / 64
@@ -1106,6 +1106,9 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
     constexpr bool EDGE = decltype(edge)::value;
     constexpr u32 N = decltype(groups)::value, NS = 8u * PF; // scores of a lane in 32 positions: 32 / PF f + 8 gg + 0 .. 7 for f < PF
     float S[N * NS];
+    // these products before the other wave's softmax, which then runs beside them (MI355X, us: 2 x 4096 rows of 32 / 8 heads of 128 303,
+    // without 308; both products so 307; heads of 64 173 each)
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (u32 t = 0; t < N; t++) {
       acc c[TT];
@@ -1125,9 +1128,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
 #pragma unroll
       for (u32 i = 0; i < NS; i++) S[NS * t + i] = c[i / NA][i % NA];
     }
-    // the softmax before the other wave's matrix products, which then run beside it (MI355X, us: 2 x 4096 rows of 32 / 8 heads of 64
-    // 184, without 198; of 128 322, 323)
-    __builtin_amdgcn_s_setprio(1);
+    __builtin_amdgcn_s_setprio(0);
     float top = NINF;
 #pragma unroll
     for (u32 i = 0; i < N * NS; i++) {
@@ -1168,7 +1169,6 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
     };
     u32 redo = 0u;
     __asm__ volatile("" : "+v"(l)); // summed here: the compiler would keep the weights for it until after the products
-    __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int d = 0; d < DT; d++) {
       if (FULL && d % 4 == 0) __asm__ volatile("" ::: "memory");
@@ -1351,10 +1351,11 @@ extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f32(amdc_kv_dev
 extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f16(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<false, false>(kv, a, hd, bn); }
 extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_bf16(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<true, false>(kv, a, hd, bn); }
 
-// Rows of a wave, positions of a tile, workgroups a CU wanted of the registers (MI355X, us). Heads of 128, 16-bit: 64 positions 1204 for
-// 12000 rows of 32 / 8 heads, 32 positions (half the scores' registers) 1342. Heads of 256: 32 rows a wave, one wave a SIMD, 144 where 16
-// rows, two waves, take 110 (256 rows over 5000 positions, 24 / 4 heads, f32). Heads of 64, 16-bit: three workgroups a CU 76 for 11 prompts
-// under a window, two 81 (with the registers of two); four, of 32 positions, spill, as f32's three do.
+// Rows of a wave, positions of a tile, workgroups a CU wanted of the registers (MI355X, us; each pair as measured when it was chosen).
+// Heads of 128, 16-bit: two workgroups on tiles of 64 positions; three, on tiles of 32, spill (12000 rows 1084 against 1098, 4096 rows 306
+// against 301). Heads of 128, f32 on f16: two on tiles of 32 505 for 2 x 4096 rows, one on tiles of 64 587; bf16's three parts would spill.
+// Heads of 256: 32 rows a wave, one wave a SIMD, 144 where 16 rows, two waves, took 110 (256 rows over 5000 positions, 24 / 4 heads, f32).
+// Heads of 64, 16-bit: three workgroups a CU 76 for 11 prompts under a window, two 81; four spill, as f32's three do.
 #define PRE_KERNEL(HD, KN, BF, F32, W, BN, OCC) \
   extern "C" __global__ __launch_bounds__(8192 / W, OCC) void amdc_attn_pre_h##HD##_##KN(amdc_kv_dev kv, AttnArgs a) { pre_body<HD, BF, F32, W, BN>(kv, a); }
 PRE_KERNEL(64, f16, false, false, 32, 64, 3)

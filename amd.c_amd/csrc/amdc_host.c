@@ -1736,7 +1736,7 @@ static int attn_kernel(int k0, const amdc_kv *kv, int t) {
  * head, U, of a workgroup each (0 where the call is refused). One workgroup is resident on a CU. Where the sequences leave room (fit),
  * one round: U chunks of a head fill the CUs, and no more. Else twice that, so that long sequences among short ones are spread
  * (MI355X, us at U x 1, 2, 3, 4: 64 sequences of 30 to 16000, 32 / 8 heads of 128 152, 136, 133, 134; 16 of 200 to 2500, 32 / 32
- * heads - 61, 63, 67; one of 60001 in rounds 54, 62, 67).
+ * heads - 61, 63, 67; one of 60001 in rounds 54, 62, 67; measured before the queries went ahead of the cache's loads).
  * Blocks of 32 columns from 17 on, where their registers suffice (heads of up to 128; 8 sequences of 900 to 6000, T = 8, 32 / 8 heads of
  * 128: 31 us, 35 in two blocks of 16). The partial results of a call are those of sequences of several chunks, under twice U,
  * and of U + n_seq chunks in all. */

@@ -22,7 +22,7 @@ def test_kernels(code):  # noqa: F811
     assert mine == set(DEC + PRE + OTHER)
     for k in DEC + PRE:
         assert any(mn.startswith("v_mfma_") for _, mn, _ in funcs[k]), k
-        assert meta[k]["vgpr_count"] <= (512 if k in ("amdc_attn_pre_h128_f16_f32", "amdc_attn_pre_h128_bf16_f32") else 256), "two waves on a SIMD"
+        assert meta[k]["vgpr_count"] <= (512 if k == "amdc_attn_pre_h128_bf16_f32" else 256), "two waves on a SIMD"
 
 
 def test_host_names():
@@ -65,5 +65,6 @@ def test_lds_loads(code, name):  # noqa: F811
             waits += 1 + (int(ops.split()[0], 0) if mn == "s_nop" else 0)
             j -= 1
     assert sum(writes_m0(*x[1:]) for x in ins) == len(loads)
+    # in both loops over tiles: those that every row sees, and the others
     marked = [ops for _, mn, ops in ins if mn == "s_waitcnt" and "expcnt(6)" in ops]
-    assert len(marked) == 1 and "vmcnt(0)" in marked[0], "the wait at the head of a tile"
+    assert len(marked) == 2 and all("vmcnt(0)" in ops for ops in marked), "the wait at the head of a tile"
