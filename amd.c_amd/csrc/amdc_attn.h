@@ -960,7 +960,7 @@ __device__ __forceinline__ PreUnit pre_unit(const amdc_kv_dev &kv, const AttnArg
 // Measured on MI355X (replayed; cards differ by 5 %): 12000 rows of 32 / 8 heads of 128, bf16, 1.12 ms, 1050 TFLOP/s of causal work (a
 // large product: 1210), matrix units busy 54 % of the cycles, vector units 42 %, at 1.7 to 1.9 GHz; 11 prompts under a window, heads of
 // 64, f16, 72 us, 530 TFLOP/s, vector units busy 61 % (the exponentials); a chunk of 256 over 5000, 24 / 4 heads of 256, f32, 80 us with
-// its join of 9; 77 rows, 32 / 32 heads of 128 12.2 us, latency.
+// its join of 11 (profiled); 77 rows, 32 / 32 heads of 128 12.2 us, latency.
 template <int HD, bool BF, bool F32, u32 W, u32 BN>
 __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &a) {
   typedef typename std::conditional<W == 32u, v16f, v4f>::type acc; // of a matrix instruction: W x W / 64
