@@ -1257,9 +1257,9 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
 #pragma unroll
       for (int blk = 0; blk < HD / 32; blk++) { // amdc_quant_q8's d, q and sum of a block, spread over the lanes of the row
         constexpr int BT = 32 / W;
-        float big = 0.0f;
+        float big = __builtin_fabsf(O[blk * BT][0]); // not 0: of values that are all NaN, d is NaN
 #pragma unroll
-        for (int i = 0; i < BT * NA; i++) big = __builtin_fmaxf(big, __builtin_fabsf(O[blk * BT + i / NA][i % NA]));
+        for (int i = 1; i < BT * NA; i++) big = __builtin_fmaxf(big, __builtin_fabsf(O[blk * BT + i / NA][i % NA]));
         const float dd = over(big, maxf) / 127.0f;
         u32 sum = 0u, w[BT * NA / 4];
 #pragma unroll
