@@ -1081,7 +1081,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
       const u32 e = __builtin_bit_cast(u32, big) >> 23, k = e < 11u ? 253u : 264u - e;
       up *= __builtin_bit_cast(float, k << 23), cq *= __builtin_bit_cast(float, (254u - k) << 23);
     }
-    cq = __builtin_fmaxf(cq, 0x1p-149f); // scale 0: a score of 0 (2^-21 at most), also of -infinity (what is not seen) not NaN
+    cq = cq < 0x1p-149f ? 0x1p-149f : cq; // scale 0: a score of 0 (2^-21 at most), also of -infinity (what is not seen) not NaN; a NaN stays one
 #pragma unroll
     for (u32 k = 0; k < KS; k++) {
 #pragma unroll

@@ -337,7 +337,7 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
  * over the positions j <= len[b] - T + t, with window not 0 the last `window` of them only. q and y have type
  * t (AMDC_TYPE_F32 or the cache's), rows qs and ys values apart; q, y and q8 do not overlap. Queries are used as they are given; in f32, the
  * scores, weights, sums and y keep f32's accuracy (the products run on the 16-bit matrix units in parts); in a
- * 16-bit type the weights are rounded to it. With q8 not NULL also the Q8 copy of the rows (n_q hd values), q8s
+ * 16-bit type the weights are rounded to it. A scale that is not finite gives NaN. With q8 not NULL also the Q8 copy of the rows (n_q hd values), q8s
  * bytes apart, for the output matrix: the bits of amdc_quant_q8 of the f32 result (before y's rounding).
  * A value (or key) that a row does not see may be anything, NaN too, also where another row sees it. Of those that
  * it sees, a value that is not finite makes its place of the row infinite or NaN, a key that is not finite the row NaN (or, where
