@@ -996,6 +996,8 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
   const u32 G = a.G, h = blockIdx.x % kv.n_kv;
   u32 x = blockIdx.x / kv.n_kv;
   const u32 sp = x % a.U, unit = a.ncb - 1u - x / a.U;
+  // rows that go past T: no unit need belong to the sequence (one that begins at T has none). The last workgroup's rows are the shortest.
+  if (a.cu && blockIdx.x == gridDim.x - 1u && (u32)a.cu[kv.n_seq] > a.T) kv_bad(kv, AMDC_BAD_ROWS);
   const PreUnit pu = pre_unit(kv, a, unit, BN);
   const SeqRows &s = pu.s;
   const u32 r0 = pu.r0, nr = pu.nr, nbq = a.n_q * HD / 32u;
