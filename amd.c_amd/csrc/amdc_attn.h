@@ -1025,7 +1025,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
   // the tiles of positions [jb, je) of this workgroup
   const u32 ns = pu.ns;
   if (sp >= ns) return;
-  const u32 jb = pu.j0 + (pu.j1 - pu.j0) * sp / ns, je = pu.j0 + (pu.j1 - pu.j0) * (sp + 1u) / ns;
+  const u32 jb = pu.j0 + amdc_part_at(pu.j1 - pu.j0, sp, ns), je = pu.j0 + amdc_part_at(pu.j1 - pu.j0, sp + 1u, ns);
 
   // the wave's rows and the lane's
   const u32 w0 = W * wv, wr = nr > w0 ? (nr - w0 < W ? nr - w0 : W) : 0u; // 0: only loads

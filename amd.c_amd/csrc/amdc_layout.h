@@ -108,6 +108,8 @@ typedef struct {
   uint32_t *bad; /* the device flag of amdc_kv_check: an AMDC_BAD_* */
   uint32_t n_kv, n_pages, n_seq, max_pages, lgp /* log2(page) */, cap /* max_pages << lgp */;
 } amdc_kv_dev;
+/* Where part i of n tiles in `parts` parts begins, floor(n i / parts): n i itself passes 32 bits (2^26 tiles in 64 parts). */
+AMDC_INLINE uint32_t amdc_part_at(uint32_t n, uint32_t i, uint32_t parts) { return n / parts * i + n % parts * i / parts; }
 enum { AMDC_BAD_PAGE = 1, AMDC_BAD_LEN = 2, AMDC_BAD_ROWS = 3 };
 
 #endif
