@@ -293,7 +293,8 @@ enum {
   K_ATTN_DEC2 = K_ATTN_DEC + 12, /* amdc_attn_dec_h64_f16_n2, .. */
   K_ATTN_PRE = K_ATTN_DEC2 + 8, /* amdc_attn_pre_h64_f16, .. */
   K_ATTN_JOIN = K_ATTN_PRE + 12, /* amdc_attn_join_f32, _f16, _bf16: in the order of AMDC_TYPE_* */
-  K_N = K_ATTN_JOIN + 3
+  K_TAKE_FLAG = K_ATTN_JOIN + 3,
+  K_N
 };
 
 #define KN(s) "amdc_" s
@@ -330,7 +331,7 @@ static const char *const kname[K_N] = {
     KN("gemv_q6_k_s1l"), KN("gemv_q6_k_xs1l"), KN("kv_append_f16"), KN("kv_append_bf16"),
     KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256"), KA2("attn_dec_h64"), KA2("attn_dec_h128"),
     KA("attn_pre_h64"), KA("attn_pre_h128"), KA("attn_pre_h256"),
-    KN("attn_join_f32"), KN("attn_join_f16"), KN("attn_join_bf16")};
+    KN("attn_join_f32"), KN("attn_join_f16"), KN("attn_join_bf16"), KN("take_flag")};
 
 static hipModule_t g_mod;
 static hipFunction_t g_k[K_N];
@@ -363,7 +364,7 @@ static unsigned g_ws_old_n;
  * amdc_op_gemv_noalloc (g_ws_fixed set) every workspace request is served from it, and a request
  * larger than it is an error; otherwise it is unused. */
 static void *g_scratch;
-static u32 *g_kv_bad;    /* the kernels' kv_bad_flag (device address) */
+static u32 *g_kv_bad;    /* the kernels' kv_bad_flag (device address); [1]: what amdc_kv_check takes it to */
 static u32 *g_split_cnt; /* the kernels' split_count array (device address) */
 static size_t g_scratch_bytes;
 static int g_ws_fixed;
@@ -466,7 +467,7 @@ int amdc_open(const char *hsaco) {
     if (!g_norm_cnt || cb < sizeof(u32)) return fail(AMDC_EHIP, "amdc_kernels.hsaco: no norm_count counter");
     HIPCALL(H.Memset(g_norm_cnt, 0, cb));
     HIPCALL(H.ModuleGetGlobal((void **)&g_kv_bad, &cb, g_mod, "kv_bad_flag"));
-    if (!g_kv_bad || cb < sizeof(u32)) return fail(AMDC_EHIP, "amdc_kernels.hsaco: no kv_bad_flag");
+    if (!g_kv_bad || cb < 2u * sizeof(u32)) return fail(AMDC_EHIP, "amdc_kernels.hsaco: no kv_bad_flag");
     HIPCALL(H.Memset(g_kv_bad, 0, sizeof(u32)));
   }
   HIPCALL(H.DeviceGetAttribute(&g_cus, hipDeviceAttributeMultiprocessorCount, 0));
@@ -1637,11 +1638,14 @@ static int check_kv(const char *op, const amdc_kv *kv, u32 n_q, u32 T, const int
 
 int amdc_kv_check(void) {
   NEED_OPEN();
-  u32 bad = 0;
+  u32 bad = 0, *took = g_kv_bad + 1;
+  void *args[] = {&g_kv_bad, &took};
   HIPCALL(H.DeviceSynchronize());
-  HIPCALL(H.Memcpy(&bad, g_kv_bad, sizeof bad, hipMemcpyDeviceToHost));
+  /* not read and then cleared: work on another stream, a replayed graph's too, may report in between, and a clearing may run after
+   * what is launched next */
+  HIPCALL(H.ModuleLaunchKernel(g_k[K_TAKE_FLAG], 1, 1, 1, 1, 1, 1, 0, NULL, args, NULL));
+  HIPCALL(H.Memcpy(&bad, took, sizeof bad, hipMemcpyDeviceToHost));
   if (!bad) return AMDC_OK;
-  HIPCALL(H.Memset(g_kv_bad, 0, sizeof bad));
   return fail(AMDC_EINVAL, "kv_check: a cache operator met %s",
               bad == AMDC_BAD_PAGE ? "a page outside the pool"
               : bad == AMDC_BAD_LEN ? "a length over max_pages * page, or under the sequence's number of new tokens"

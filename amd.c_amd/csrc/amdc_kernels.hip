@@ -4136,7 +4136,10 @@ extern "C" __global__ __launch_bounds__(256, 2) void amdc_gemv_q6_k_v16(const ui
   gemv8_q6k_body<2, 1>(W, xq, y, rows, nb, bias, res, T, xs, ys, rs, part, tps, cnt);
 }
 
-// The error flag of the cache and attention kernels (amdc_kv_check), 0 while all is well
+// The error flag of the cache and attention kernels (amdc_kv_check), 0 while all is well; [1]: what amdc_take_flag took
 __device__ __align__(256) u32 kv_bad_flag[64];
+
+// Takes a flag: one exchange, so that a report made at any time is in `to` now or in the flag for the next to take.
+extern "C" __global__ void amdc_take_flag(u32 *flag, u32 *to) { *to = __hip_atomic_exchange(flag, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 #include "amdc_attn.h"

@@ -313,7 +313,8 @@ typedef struct {
 /* Bytes of each of the two pools; 0 for a geometry that is not supported. */
 size_t amdc_kv_bytes(int type, uint32_t n_kv, uint32_t hd, uint32_t page, uint32_t n_pages);
 /* Synchronizes the device; AMDC_EINVAL and a message if a call since the last check met a page, a length
- * or a row outside its bounds (see amdc_kv). */
+ * or a row outside its bounds (see amdc_kv). One flag serves all caches and streams: the message is of one such call
+ * and does not say which; a report made while this runs is kept for the next check. */
 int amdc_kv_check(void);
 
 /* Appends the new tokens' keys and values to the cache, the keys rotated by their positions, and with q
