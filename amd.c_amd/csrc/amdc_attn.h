@@ -106,14 +106,6 @@ __device__ __forceinline__ void sincos64(double a, float &s, float &c) {
 
 // ------------------------------------------------------------------ append
 
-struct AppendArgs {
-  const float *k, *v, *q;
-  void *qo;
-  const int *cu;
-  const float *freq;
-  u32 qt, n_q, T, ks, vs, qs, qos, n_rot, rope, lghd, rows, gq, gv, upb, vec;
-};
-
 // Eight values of a row from p (16-byte aligned where vec)
 __device__ __forceinline__ void load8(const float *p, bool vec, float (&x)[8]) {
   if (vec) {
@@ -134,7 +126,7 @@ __device__ __forceinline__ void load8(const float *p, bool vec, float (&x)[8]) {
 // rows are aligned) of up to eight rows and stores each value's positions as 16 bytes, or where the group is not full the new ones alone.
 // Measured on MI355X: 8657 rows of 32 + 8 + 8 heads of 128 (319 MB) 79 us; a workgroup to a row 87, three to a row 110.
 template <bool BF>
-__device__ __forceinline__ void append_body(const amdc_kv_dev &kv, const AppendArgs &a) {
+__device__ __forceinline__ void append_body(const amdc_kv_dev &kv, const amdc_append_args &a) {
   __shared__ float s_cos[4][128], s_sin[4][128];
   const u32 hd = 1u << a.lghd, tid = threadIdx.x, nrw = cdiv(a.rows * a.gq, 4u);
   const u64 gb = 32ull << a.lghd, lgg = kv.lgp - 4u; // bytes of 16 positions of a head, log2 of such groups in a page
@@ -263,7 +255,7 @@ __device__ __forceinline__ void append_body(const amdc_kv_dev &kv, const AppendA
 }
 
 #define APPEND_KERNEL(KN, BF) \
-  extern "C" __global__ __launch_bounds__(256) void amdc_kv_append_##KN(amdc_kv_dev kv, AppendArgs a) { append_body<BF>(kv, a); }
+  extern "C" __global__ __launch_bounds__(256) void amdc_kv_append_##KN(amdc_kv_dev kv, amdc_append_args a) { append_body<BF>(kv, a); }
 APPEND_KERNEL(f16, false)
 APPEND_KERNEL(bf16, true)
 #undef APPEND_KERNEL
@@ -345,16 +337,6 @@ __device__ __forceinline__ V seen16(V w, u32 p, u32 lo, u32 hi) {
   return w;
 }
 
-struct AttnArgs {
-  const void *q;
-  void *y;
-  const int *cu;
-  uint8_t *q8, *ws;
-  float c; // scale log2(e)
-  u32 n_q, G, T, qs, ys, window, q8s, U, vec, ncb, fit;
-};
-
-#define ATTN_CNT 65536u // bytes of counters at the start of the workspace
 #define DEC_FAN 8u      // partial results joined at once
 #define DEC_CMIN 512u   // the shortest chunk, in positions
 #define DEC_NT 327680u  // the bytes of a chunk from which its loads are nontemporal
@@ -418,7 +400,7 @@ __device__ __forceinline__ void split_n(float (&x)[N], u32 (&w)[NP][N / 2]) {
 // 256 (104 MB, two blocks of columns, the second from the L2) 34 us, 3.1 TB/s; 421 positions, 32 / 32 heads of 128 8.3 us, all latency.
 // A plain read reaches 6.3 TB/s. Four waves a workgroup, two workgroups a CU and loads not ahead of the queries: 54, 151 and 54 us.
 template <int HD, bool BF, bool F32, u32 NC, u32 NW>
-__device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &a) {
+__device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const amdc_attn_args &a) {
   constexpr int NP = F32 ? (BF ? 3 : 2) : 1, KS = HD / 32, DT = HD / 16;
   constexpr u32 SP = HD > 128 || (NC > 1u && HD > 64) ? 16u : 32u, SL = SP / 4u, TT = SP / 16u, R = 16u * NC, NTH = 64u * NW; // positions of a step, scores of a lane, score tiles
   constexpr u32 OS = HD + 4u, QD = HD / 4u; // floats between columns of O in the LDS; quads of a row
@@ -799,7 +781,7 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
   }
   // partial results: rmax rows of O, then m and l of R rows
   const u32 rmax = T * G < R ? T * G : R, om = rmax * HD * 4u, sb = om + 8u * R;
-  uint8_t *parts = a.ws + ATTN_CNT;
+  uint8_t *parts = a.ws + AMDC_ATTN_CNT;
   auto slot = [&](u32 k) { return ((u64)(slot0 + k) * kv.n_kv + h) * a.ncb + cb; };
   auto part = [&](u32 k) { return rsrc(parts + slot(k) * sb, sb); };
   {
@@ -875,7 +857,7 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const AttnArgs &
 }
 
 #define DEC_KERNEL(HD, KN, TAG, BF, F32, NC) \
-  extern "C" __global__ __launch_bounds__(512, 2) void amdc_attn_dec_h##HD##_##KN##TAG(amdc_kv_dev kv, AttnArgs a) { dec_body<HD, BF, F32, NC, 8u>(kv, a); }
+  extern "C" __global__ __launch_bounds__(64u * AMDC_DEC_NW, 2) void amdc_attn_dec_h##HD##_##KN##TAG(amdc_kv_dev kv, amdc_attn_args a) { dec_body<HD, BF, F32, NC, AMDC_DEC_NW>(kv, a); }
 #define DEC_KERNELS(HD, TAG, NC) \
   DEC_KERNEL(HD, f16, TAG, false, false, NC) DEC_KERNEL(HD, f16_f32, TAG, false, true, NC) DEC_KERNEL(HD, bf16, TAG, true, false, NC) DEC_KERNEL(HD, bf16_f32, TAG, true, true, NC)
 DEC_KERNELS(64, , 1u)
@@ -909,41 +891,39 @@ __device__ __forceinline__ void lds_load16s(__amdgpu_buffer_rsrc_t rs, __attribu
   __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m), "v"(voff), "s"(rs), "s"(soff) : "memory");
 }
 
-#define PRE_BM 128u     // query rows of a workgroup
-#define PRE_MINTILES 4u // tiles of positions that a part has at least
-#define PRE_SB(hd) ((PRE_BM * (hd) + 2u * PRE_BM) * 4u) // bytes of a partial result
+#define PRE_SB(hd) ((AMDC_PRE_BM * (hd) + 2u * AMDC_PRE_BM) * 4u) // bytes of a partial result
 
-// The rows of a unit (a tile of PRE_BM rows of a sequence) and the tiles of BN positions [j0, j1) that they see, in ns parts
+// The rows of a unit (a tile of AMDC_PRE_BM rows of a sequence) and the tiles of BN positions [j0, j1) that they see, in ns parts
 struct PreUnit {
   SeqRows s;
   u32 b, r0, nr, j0, j1, ns;
 };
-__device__ __forceinline__ PreUnit pre_unit(const amdc_kv_dev &kv, const AttnArgs &a, u32 unit, u32 BN) {
+__device__ __forceinline__ PreUnit pre_unit(const amdc_kv_dev &kv, const amdc_attn_args &a, u32 unit, u32 BN) {
   PreUnit p;
   u32 ti;
   if (a.cu) {
-    auto base = [&](u32 i) { const int c = a.cu[i]; return (c < 0 ? 0u : (u32)c * a.G / PRE_BM) + i; };
+    auto base = [&](u32 i) { const int c = a.cu[i]; return (c < 0 ? 0u : (u32)c * a.G / AMDC_PRE_BM) + i; };
     p.b = find_seq(kv.n_seq, unit, base);
     ti = unit - base(p.b);
   } else {
-    const u32 per = cdiv(a.T * a.G, PRE_BM);
+    const u32 per = cdiv(a.T * a.G, AMDC_PRE_BM);
     p.b = unit / per, ti = unit - p.b * per;
   }
   p.s = seq_rows(kv, a.cu, a.T, p.b);
   p.s.row0 = uniform(p.s.row0), p.s.m = uniform(p.s.m), p.s.len = uniform(p.s.len);
   const u32 R = p.s.m * a.G;
-  p.r0 = ti * PRE_BM;
-  p.nr = p.r0 >= R ? 0u : R - p.r0 < PRE_BM ? R - p.r0 : PRE_BM;
+  p.r0 = ti * AMDC_PRE_BM;
+  p.nr = p.r0 >= R ? 0u : R - p.r0 < AMDC_PRE_BM ? R - p.r0 : AMDC_PRE_BM;
   if (!p.nr || !p.s.len) return p;
   const u32 m0 = p.s.len - p.s.m, e = m0 + p.r0 / a.G + 1u;
   p.j0 = (a.window && e > a.window ? e - a.window : 0u) / BN, p.j1 = cdiv(m0 + (p.r0 + p.nr - 1u) / a.G + 1u, BN);
-  const u32 most = (p.j1 - p.j0) / PRE_MINTILES;
+  const u32 most = (p.j1 - p.j0) / AMDC_PRE_MINTILES;
   p.ns = most < 1u ? 1u : most < a.U ? most : a.U;
   return p;
 }
 
 // The new tokens of a sequence and the G heads that share a key / value head are its rows (token t, head g: t G + g). A workgroup
-// takes PRE_BM consecutive rows, its waves W = 32 or 16 each, and goes through tiles of BN positions that the LDS holds twice: while the
+// takes AMDC_PRE_BM consecutive rows, its waves W = 32 or 16 each, and goes through tiles of BN positions that the LDS holds twice: while the
 // waves work on one tile the next is loaded into the other half, straight from the cache (the layout is the one the LDS wants; every
 // load moves 1 KB, and every read of an operand, 16 bytes a lane, meets no bank twice).
 // The matrix work bounds it (4 hd flops to a row and position), and next to it the exponentials:
@@ -962,11 +942,11 @@ __device__ __forceinline__ PreUnit pre_unit(const amdc_kv_dev &kv, const AttnArg
 // 64, f16, 72 us, 530 TFLOP/s, vector units busy 61 % (the exponentials); a chunk of 256 over 5000, 24 / 4 heads of 256, f32, 80 us with
 // its join of 11 (profiled); 77 rows, 32 / 32 heads of 128 12.2 us, latency.
 template <int HD, bool BF, bool F32, u32 W, u32 BN>
-__device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &a) {
+__device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const amdc_attn_args &a) {
   typedef typename std::conditional<W == 32u, v16f, v4f>::type acc; // of a matrix instruction: W x W / 64
   constexpr int NP = F32 ? (BF ? 3 : 2) : 1, NA = W == 32u ? 16 : 4, DT = HD / W;
   constexpr u32 TT = W == 32u ? 1u : 2u, KS = HD / (W == 32u ? 16u : 32u), PF = W / 16u; // of 32 positions: score tiles, steps over hd, weight operands
-  constexpr u32 NW = PRE_BM / W, NTH = 64u * NW, MT = BN / 32u, TB = BN * HD * 2u, QD = HD / 4u;
+  constexpr u32 NW = AMDC_PRE_BM / W, NTH = 64u * NW, MT = BN / 32u, TB = BN * HD * 2u, QD = HD / 4u;
   // the keys' groups of 16 positions in the LDS: W = 16 reads two at once, 16 banks apart
   constexpr u32 GS = 32u * HD + (W == 16u ? 64u : 0u), KB = BN / 16u * GS;
   constexpr u32 PG = HD / 16u, PW = BN / 16u * PG / NW; // KB of a group of 16 positions (keys, then values), and of a tile for each wave
@@ -1283,33 +1263,32 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const AttnArgs &
       }
     return;
   }
-  // a partial result: PRE_BM rows of O, then their m and l
-  float *part = (float *)(a.ws + ATTN_CNT + (((u64)unit * kv.n_kv + h) * a.U + sp) * PRE_SB(HD));
+  // a partial result: AMDC_PRE_BM rows of O, then their m and l
+  float *part = (float *)(a.ws + AMDC_ATTN_CNT + (((u64)unit * kv.n_kv + h) * a.U + sp) * PRE_SB(HD));
   if (n < wr) {
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
       for (u32 i = 0; i < NA / 4u; i++) *(v4f *)(part + (w0 + n) * HD + W * d + 8u * i + 4u * gg) = quad(d, i);
-    if (gg == 0u) part[PRE_BM * HD + w0 + n] = m, part[PRE_BM * (HD + 1u) + w0 + n] = l;
+    if (gg == 0u) part[AMDC_PRE_BM * HD + w0 + n] = m, part[AMDC_PRE_BM * (HD + 1u) + w0 + n] = l;
   }
 }
 
 // The parts of a split tile joined in the order of their positions: 16 of its rows, JOIN_N parts' loads in flight a thread
 #define JOIN_N 8u
-#define PRE_MAXPARTS 64u
 template <bool BF, bool F32>
-__device__ __forceinline__ void join_body(const amdc_kv_dev &kv, const AttnArgs &a, u32 hd, u32 BN) {
-  __shared__ float s_w[PRE_MAXPARTS][16], s_l[PRE_MAXPARTS][16], s_L[16]; // of every part and row: m, then its weight; l
+__device__ __forceinline__ void join_body(const amdc_kv_dev &kv, const amdc_attn_args &a, u32 hd, u32 BN) {
+  __shared__ float s_w[AMDC_PRE_MAXPARTS][16], s_l[AMDC_PRE_MAXPARTS][16], s_L[16]; // of every part and row: m, then its weight; l
   const u32 tid = threadIdx.x, qd = hd / 4u, nbq = a.n_q * hd / 32u;
-  const u32 h = blockIdx.x % kv.n_kv, x = blockIdx.x / kv.n_kv, unit = x / (PRE_BM / 16u), f = x % (PRE_BM / 16u) * 16u;
+  const u32 h = blockIdx.x % kv.n_kv, x = blockIdx.x / kv.n_kv, unit = x / (AMDC_PRE_BM / 16u), f = x % (AMDC_PRE_BM / 16u) * 16u;
   const PreUnit pu = pre_unit(kv, a, unit, BN);
   if (f >= pu.nr || !pu.s.len || pu.ns == 1u) return; // nothing to join: the rows are written
   const u32 nr = pu.nr - f < 16u ? pu.nr - f : 16u, ns = pu.ns, pf = PRE_SB(hd) / 4u; // floats of a partial result
-  const float *parts = (const float *)(a.ws + ATTN_CNT) + ((u64)unit * kv.n_kv + h) * a.U * pf, *ml = parts + PRE_BM * hd + f;
+  const float *parts = (const float *)(a.ws + AMDC_ATTN_CNT) + ((u64)unit * kv.n_kv + h) * a.U * pf, *ml = parts + AMDC_PRE_BM * hd + f;
   for (u32 e = tid; e < 16u * ns; e += 256u) {
     const u32 r = e & 15u, k = e >> 4;
     const float *p = ml + (u64)k * pf + (r < nr ? r : 0u);
-    s_w[k][r] = p[0], s_l[k][r] = p[PRE_BM];
+    s_w[k][r] = p[0], s_l[k][r] = p[AMDC_PRE_BM];
   }
   __syncthreads();
   if (tid < 16u) {
@@ -1349,27 +1328,29 @@ __device__ __forceinline__ void join_body(const amdc_kv_dev &kv, const AttnArgs 
     if (a.q8) quant_vec4(y, (head * hd + 4u * d4) / 32u, true, a.q8 + (u64)row * a.q8s, nbq);
   }
 }
-extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f32(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<false, true>(kv, a, hd, bn); }
-extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f16(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<false, false>(kv, a, hd, bn); }
-extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_bf16(amdc_kv_dev kv, AttnArgs a, u32 hd, u32 bn) { join_body<true, false>(kv, a, hd, bn); }
+extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f32(amdc_kv_dev kv, amdc_attn_args a, u32 hd, u32 bn) { join_body<false, true>(kv, a, hd, bn); }
+extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_f16(amdc_kv_dev kv, amdc_attn_args a, u32 hd, u32 bn) { join_body<false, false>(kv, a, hd, bn); }
+extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_bf16(amdc_kv_dev kv, amdc_attn_args a, u32 hd, u32 bn) { join_body<true, false>(kv, a, hd, bn); }
 
 // Rows of a wave, positions of a tile, workgroups a CU wanted of the registers (MI355X, us; each pair as measured when it was chosen).
 // Heads of 128, 16-bit: two workgroups on tiles of 64 positions; three, on tiles of 32, spill (12000 rows 1084 against 1098, 4096 rows 306
 // against 301). Heads of 128, f32 on f16: two on tiles of 32 505 for 2 x 4096 rows, one on tiles of 64 587; bf16's three parts would spill.
 // Heads of 256: 32 rows a wave, one wave a SIMD, 144 where 16 rows, two waves, took 110 (256 rows over 5000 positions, 24 / 4 heads, f32).
 // Heads of 64, 16-bit: three workgroups a CU 76 for 11 prompts under a window, two 81; four spill, as f32's three do.
-#define PRE_KERNEL(HD, KN, BF, F32, W, BN, OCC) \
-  extern "C" __global__ __launch_bounds__(8192 / W, OCC) void amdc_attn_pre_h##HD##_##KN(amdc_kv_dev kv, AttnArgs a) { pre_body<HD, BF, F32, W, BN>(kv, a); }
-PRE_KERNEL(64, f16, false, false, 32, 64, 3)
-PRE_KERNEL(64, f16_f32, false, true, 32, 64, 2)
-PRE_KERNEL(64, bf16, true, false, 32, 64, 3)
-PRE_KERNEL(64, bf16_f32, true, true, 32, 64, 2)
-PRE_KERNEL(128, f16, false, false, 32, 64, 2)
-PRE_KERNEL(128, f16_f32, false, true, 32, 32, 2)
-PRE_KERNEL(128, bf16, true, false, 32, 64, 2)
-PRE_KERNEL(128, bf16_f32, true, true, 32, 64, 1)
-PRE_KERNEL(256, f16, false, false, 16, 32, 2)
-PRE_KERNEL(256, f16_f32, false, true, 16, 32, 2)
-PRE_KERNEL(256, bf16, true, false, 16, 32, 2)
-PRE_KERNEL(256, bf16_f32, true, true, 16, 32, 2)
+#define PRE_KERNEL(HD, KN, BF, F32, OCC) \
+  extern "C" __global__ __launch_bounds__(64u * AMDC_PRE_BM / AMDC_PRE_W(HD), OCC) void amdc_attn_pre_h##HD##_##KN(amdc_kv_dev kv, amdc_attn_args a) { \
+    pre_body<HD, BF, F32, AMDC_PRE_W(HD), AMDC_PRE_BN(HD, BF, F32)>(kv, a); \
+  }
+PRE_KERNEL(64, f16, false, false, 3)
+PRE_KERNEL(64, f16_f32, false, true, 2)
+PRE_KERNEL(64, bf16, true, false, 3)
+PRE_KERNEL(64, bf16_f32, true, true, 2)
+PRE_KERNEL(128, f16, false, false, 2)
+PRE_KERNEL(128, f16_f32, false, true, 2)
+PRE_KERNEL(128, bf16, true, false, 2)
+PRE_KERNEL(128, bf16_f32, true, true, 1)
+PRE_KERNEL(256, f16, false, false, 2)
+PRE_KERNEL(256, f16_f32, false, true, 2)
+PRE_KERNEL(256, bf16, true, false, 2)
+PRE_KERNEL(256, bf16_f32, true, true, 2)
 #undef PRE_KERNEL

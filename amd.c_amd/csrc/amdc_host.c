@@ -1652,15 +1652,6 @@ int amdc_kv_check(void) {
                                     : "rows outside 0 .. T (cu)");
 }
 
-/* the arguments of amdc_kv_append_*: AppendArgs of amdc_attn.h */
-typedef struct {
-  const float *k, *v, *q;
-  void *qo;
-  const int32_t *cu;
-  const float *freq;
-  u32 qt, n_q, T, ks, vs, qs, qos, n_rot, rope, lghd, rows, gq, gv, upb, vec;
-} append_args;
-
 int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const float *q, void *qo, int qt, uint32_t n_q, uint32_t T, uint32_t ks,
                    uint32_t vs, uint32_t qs, uint32_t qos, const int32_t *cu, const float *freq, uint32_t n_rot, int rope, void *stream) {
   NEED_OPEN();
@@ -1694,21 +1685,10 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
   /* which rows are 16-byte aligned: queries, keys, rotated queries, values */
   const u32 vec = (vec_rows(q, rows > 1u ? 4u * qs : 0u, 16u) ? 1u : 0u) | (vec_rows(k, rows > 1u ? 4u * ks : 0u, 16u) ? 2u : 0u) |
                   (vec_rows(qo, rows > 1u ? (qt == AMDC_TYPE_F32 ? 4u : 2u) * qos : 0u, 16u) ? 4u : 0u) | (v4 ? 8u : 0u);
-  append_args a = {k, v, q, qo, cu, freq, (u32)qt, n_q, T, ks, vs, qs, qos, rope ? n_rot : 0u, (u32)rope, lghd, rows, gq, gv, upb, vec};
+  amdc_append_args a = {k, v, q, qo, cu, freq, (u32)qt, n_q, T, ks, vs, qs, qos, rope ? n_rot : 0u, (u32)rope, lghd, rows, gq, gv, upb, vec};
   void *args[] = {&d, &a};
   return launch(K_APPEND + (kv->type == AMDC_TYPE_BF16), (rows * gq + 3u) / 4u + vu * gv, 1, 0, stream, args);
 }
-
-/* the arguments of the attention kernels: AttnArgs of amdc_attn.h */
-typedef struct {
-  const void *q;
-  void *y;
-  const int32_t *cu;
-  uint8_t *q8, *ws;
-  float c;
-  u32 n_q, G, T, qs, ys, window, q8s, U, vec, ncb, fit;
-} attn_args;
-#define ATTN_CNT 65536u /* bytes of counters at the start of the workspace (amdc_attn.h) */
 
 /* The checks of both attention operators beyond check_kv's. */
 static int check_attn(const char *op, const amdc_kv *kv, const void *q, const void *y, int t, u32 n_q, u32 rows, u32 qs, u32 ys, const uint8_t *q8,
@@ -1729,8 +1709,8 @@ static u32 attn_vec(const void *q, const void *y, int t, u32 rows, u32 qs, u32 y
   const u32 es = t == AMDC_TYPE_F32 ? 4u : 2u;
   return (vec_rows(q, rows > 1u ? es * qs : 0u, 16u) ? 1u : 0u) | (vec_rows(y, rows > 1u ? es * ys : 0u, 4u * es) ? 2u : 0u);
 }
-/* launch of a prompt kernel: 32 rows to a wave, or 16 for heads of 256 (pre_body in amdc_attn.h) */
-static int launch_pre(int k, u32 hd, unsigned g, void *stream, void **args) { return launch_nt(k, g, 1, hd > 128u ? 512u : 256u, 0, stream, args); }
+/* launch of a prompt kernel (pre_body in amdc_attn.h) */
+static int launch_pre(int k, u32 hd, unsigned g, void *stream, void **args) { return launch_nt(k, g, 1, 64u * AMDC_PRE_BM / AMDC_PRE_W(hd), 0, stream, args); }
 /* the kernel of a head size, a cache and a query type, in the order of KA */
 static int attn_kernel(int k0, const amdc_kv *kv, int t) {
   return k0 + (kv->hd == 64u ? 0 : kv->hd == 128u ? 4 : 8) + (kv->type == AMDC_TYPE_BF16 ? 2 : 0) + (t == AMDC_TYPE_F32 ? 1 : 0);
@@ -1750,7 +1730,7 @@ static u32 dec_units(u32 n_kv, u32 n_q, u32 hd, u32 T, u32 n_seq, u32 *R, u32 *n
   *R = cols > 16u && hd <= 128u ? 32u : 16u;
   *ncb = (u32)(cols + *R - 1u) / *R;
   const u32 cus = g_cus > 0 ? (u32)g_cus : 256u, heads = n_kv * *ncb;
-  u32 U = cus / heads, most = ATTN_CNT / 8u / heads; /* counters: one to a partial result */
+  u32 U = cus / heads, most = AMDC_ATTN_CNT / 8u / heads; /* counters: one to a partial result */
   *fit = 2u * n_seq <= U;
   if (!*fit) U = cus * 2u / heads;
   if (U > most) U = most;
@@ -1763,7 +1743,7 @@ size_t amdc_attn_decode_ws(const amdc_kv *kv, uint32_t n_q, uint32_t T) {
   const u32 U = dec_units(kv->n_kv, n_q, kv->hd, T, kv->n_seq, &R, &ncb, &fit);
   if (!U) return 0;
   const u64 slots = U > kv->n_seq ? (u64)U + kv->n_seq : 2ull * U, cols = (u64)T * (n_q / kv->n_kv), r = cols < R ? cols : R;
-  return (size_t)(ATTN_CNT + slots * kv->n_kv * ncb * (r * kv->hd + 2u * R) * 4u);
+  return (size_t)(AMDC_ATTN_CNT + slots * kv->n_kv * ncb * (r * kv->hd + 2u * R) * 4u);
 }
 
 int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
@@ -1780,35 +1760,31 @@ int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t 
   const u64 grid = (((u64)U + kv->n_seq) * kv->n_kv + 7u) / 8u * 8u * ncb;
   if (grid >= (1u << 23) || (u64)kv->n_seq * d.cap >= (1ull << 35)) /* the kernel counts all steps of 16 in 32 bits */
     return fail(AMDC_EINVAL, "attn_decode: %u sequences of %u heads and up to %u positions are too many for one call", kv->n_seq, kv->n_kv, d.cap);
-  attn_args a = {q, y, NULL, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, U, attn_vec(q, y, t, rows, qs, ys), ncb, fit};
+  amdc_attn_args a = {q, y, NULL, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, U, attn_vec(q, y, t, rows, qs, ys), ncb, fit};
   void *args[] = {&d, &a};
-  return launch_nt(attn_kernel(R > 16u ? K_ATTN_DEC2 : K_ATTN_DEC, kv, t), (unsigned)grid, 1, 512u, 0, stream, args);
+  return launch_nt(attn_kernel(R > 16u ? K_ATTN_DEC2 : K_ATTN_DEC, kv, t), (unsigned)grid, 1, 64u * AMDC_DEC_NW, 0, stream, args);
 }
 
-/* A call of the prompt kernel: tiles of PRE_BM rows of a head at most, and the parts that a tile's positions are split into where
+/* A call of the prompt kernel: tiles of AMDC_PRE_BM rows of a head at most, and the parts that a tile's positions are split into where
  * the tiles of all heads are fewer than the CUs hold (pre_body in amdc_attn.h). */
-#define PRE_BM 128u
-#define PRE_MINTILES 4u
-#define PRE_MAXPARTS 64u
-/* positions of a tile, as PRE_KERNEL of amdc_attn.h has them */
-static u32 pre_bn(const amdc_kv *kv, int t) { return kv->hd > 128u || (kv->hd > 64u && t == AMDC_TYPE_F32 && kv->type == AMDC_TYPE_F16) ? 32u : 64u; }
+static u32 pre_bn(const amdc_kv *kv, int t) { return AMDC_PRE_BN(kv->hd, kv->type == AMDC_TYPE_BF16, t == AMDC_TYPE_F32); }
 static u32 pre_want(u32 hd) { return (g_cus > 0 ? (u32)g_cus : 256u) * (hd > 128u ? 1u : 2u); }
 static u32 pre_tiles(const amdc_kv *kv, int t, u32 n_q, u32 rows, int ragged, u32 T, u32 *parts) {
   const u32 G = n_q / kv->n_kv;
-  const u64 tiles = ragged ? ((u64)rows * G + PRE_BM - 1u) / PRE_BM + kv->n_seq - 1u : (u64)kv->n_seq * (((u64)T * G + PRE_BM - 1u) / PRE_BM);
+  const u64 tiles = ragged ? ((u64)rows * G + AMDC_PRE_BM - 1u) / AMDC_PRE_BM + kv->n_seq - 1u : (u64)kv->n_seq * (((u64)T * G + AMDC_PRE_BM - 1u) / AMDC_PRE_BM);
   const u64 wgs = tiles * kv->n_kv, want = pre_want(kv->hd);
-  /* parts of at least PRE_MINTILES tiles of the most positions that the table holds; 1: no join */
-  const u64 most = (u64)kv->max_pages * kv->page / (PRE_MINTILES * pre_bn(kv, t));
+  /* parts of at least AMDC_PRE_MINTILES tiles of the most positions that the table holds; 1: no join */
+  const u64 most = (u64)kv->max_pages * kv->page / (AMDC_PRE_MINTILES * pre_bn(kv, t));
   u64 p = wgs < want ? want / wgs : 1u;
   if (p > most) p = most;
-  *parts = p < 2u ? 1u : p < PRE_MAXPARTS ? (u32)p : PRE_MAXPARTS;
+  *parts = p < 2u ? 1u : p < AMDC_PRE_MAXPARTS ? (u32)p : AMDC_PRE_MAXPARTS;
   return tiles < (1u << 24) ? (u32)tiles : 1u << 24;
 }
 
 size_t amdc_attn_prefill_ws(const amdc_kv *kv, uint32_t n_q, uint32_t rows) {
   if (!kv || !amdc_kv_bytes(kv->type, kv->n_kv, kv->hd, kv->page, kv->n_pages) || !n_q || n_q % kv->n_kv || !rows || rows > (1u << 22)) return 0;
   /* under pre_want partial results, however the rows are dealt to the sequences */
-  return (size_t)(ATTN_CNT + (u64)pre_want(kv->hd) * (PRE_BM * kv->hd + 2u * PRE_BM) * 4u);
+  return (size_t)(AMDC_ATTN_CNT + (u64)pre_want(kv->hd) * (AMDC_PRE_BM * kv->hd + 2u * AMDC_PRE_BM) * 4u);
 }
 
 int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
@@ -1822,12 +1798,12 @@ int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t
   const u32 tiles = pre_tiles(kv, t, n_q, rows, cu != NULL, T, &parts);
   const u64 grid = (u64)tiles * parts * kv->n_kv;
   if (grid >= (1u << 23)) return fail(AMDC_EINVAL, "attn_prefill: %u rows of %u sequences and %u heads are too many for one call", rows, kv->n_seq, kv->n_kv);
-  attn_args a = {q, y, cu, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, parts, attn_vec(q, y, t, rows, qs, ys), tiles, 0};
+  amdc_attn_args a = {q, y, cu, q8, ws, scale * 1.4426950408889634f, n_q, n_q / kv->n_kv, T, qs, ys, window, q8s, parts, attn_vec(q, y, t, rows, qs, ys), tiles, 0};
   void *args[] = {&d, &a};
   if ((rc = launch_pre(attn_kernel(K_ATTN_PRE, kv, t), kv->hd, (unsigned)grid, stream, args)) || parts == 1u) return rc;
   const u32 bn = pre_bn(kv, t);
   void *ja[] = {&d, &a, (void *)&kv->hd, (void *)&bn};
-  return launch(K_ATTN_JOIN + t, tiles * (PRE_BM / 16u) * kv->n_kv, 1, 0, stream, ja);
+  return launch(K_ATTN_JOIN + t, tiles * (AMDC_PRE_BM / 16u) * kv->n_kv, 1, 0, stream, ja);
 }
 
 int amdc_probe_read(const void *src, size_t nbytes, void *scratch, uint32_t grid, void *stream) {

@@ -108,6 +108,34 @@ typedef struct {
   uint32_t *bad; /* the device flag of amdc_kv_check: an AMDC_BAD_* */
   uint32_t n_kv, n_pages, n_seq, max_pages, lgp /* log2(page) */, cap /* max_pages << lgp */;
 } amdc_kv_dev;
+/* What the host and the attention kernels both have to know (amdc_attn.h says why each is what it is). */
+#define AMDC_ATTN_CNT 65536u /* bytes of counters at the start of a workspace */
+#define AMDC_DEC_NW 8u       /* waves of a decode workgroup */
+#define AMDC_PRE_BM 128u     /* query rows of a prompt workgroup */
+#define AMDC_PRE_W(hd) ((hd) > 128u ? 16u : 32u)                                               /* of a wave */
+#define AMDC_PRE_BN(hd, bf, f32) ((hd) > 128u || ((hd) > 64u && (f32) && !(bf)) ? 32u : 64u) /* positions of a tile; bf: the cache, f32: the queries */
+#define AMDC_PRE_MINTILES 4u                                                                      /* tiles that a part has at least */
+#define AMDC_PRE_MAXPARTS 64u
+/* The kernels' arguments, by value. */
+typedef struct {
+  const float *k, *v, *q;
+  void *qo;
+  const int32_t *cu;
+  const float *freq;
+  uint32_t qt, n_q, T, ks, vs, qs, qos, n_rot, rope, lghd, rows, gq, gv, upb, vec;
+} amdc_append_args;
+typedef struct {
+  const void *q;
+  void *y;
+  const int32_t *cu;
+  uint8_t *q8, *ws;
+  float c; /* scale log2(e) */
+  uint32_t n_q, G, T, qs, ys, window, q8s;
+  uint32_t U;        /* decode: the chunks wanted of a head; prompts: the parts that a tile's positions are split into at most */
+  uint32_t vec, ncb; /* decode: blocks of columns; prompts: tiles of rows */
+  uint32_t fit;      /* decode: one round of workgroups (prompts: not used) */
+} amdc_attn_args;
+
 /* Where part i of n tiles in `parts` parts begins, floor(n i / parts): n i itself passes 32 bits (2^26 tiles in 64 parts). */
 AMDC_INLINE uint32_t amdc_part_at(uint32_t n, uint32_t i, uint32_t parts) { return n / parts * i + n % parts * i / parts; }
 enum { AMDC_BAD_PAGE = 1, AMDC_BAD_LEN = 2, AMDC_BAD_ROWS = 3 };
