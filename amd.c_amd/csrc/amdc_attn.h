@@ -301,7 +301,7 @@ __device__ __forceinline__ void load_q8(const void *q, u64 i, bool vec, float (&
   }
 }
 
-// Four results of a row: to y, and their Q8 copy (eight lanes to a block of 32, all or none of them here)
+// Four results of a row to y
 template <bool BF, bool F32>
 __device__ __forceinline__ void store_y4(void *y, u64 i, v4f v, bool vec) {
   if constexpr (F32) {
@@ -341,7 +341,7 @@ __device__ __forceinline__ V seen16(V w, u32 p, u32 lo, u32 hi) {
 #define DEC_CMIN 512u   // the shortest chunk, in positions
 #define DEC_NT 327680u  // the bytes of a chunk from which its loads are nontemporal
 
-// The sum of v over the wave, in every lane, and the inclusive sums of v up to each lane
+// The sum of v over the lanes up to this one, itself included (in lane 63: over the wave)
 __device__ __forceinline__ u32 wave_scan(u32 v) {
   // row_shr 1, 2, 4, 8 inside rows of 16, then the rows' last lanes onto the rows behind (row_bcast 15 and 31)
   v += (u32)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);
@@ -372,8 +372,8 @@ __device__ __forceinline__ void split_n(float (&x)[N], u32 (&w)[NP][N / 2]) {
 // the chunk's steps of SP positions in turn, each with a softmax of its own (maximum m, sum l, weighted sum O), joined at
 // the end in the LDS.
 //
-// Reading the cache bounds it (16 columns cost 2 x 16 x hd flops per 4 hd bytes, 1 / 40 of the matrix rate at the HBM's), so
-// the layout gives every load of a wave whole lines, straight into the matrix units' operands, no LDS between:
+// Reading the cache bounds it: 16 columns cost 4 x 16 x hd flops per 4 hd bytes, a key and a value; at the HBM's 6.3 TB/s that is 1 / 12 of a
+// large product's rate (1210 TFLOP/s), in f32's two or three parts 1 / 6 or 1 / 4. So the layout gives every load of a wave whole lines, straight into the matrix units' operands, no LDS between:
 //   S^T = K Q^T  (16x16x32: rows are positions, columns are the query rows). SP = 32: row r of tile t (of two) is position
 //                8 (r / 4) + 4 t + r % 4 of the step, so that a lane's eight scores are the eight positions 8 g .. 8 g + 7
 //                (g = lane / 16) of its column. SP = 16, for heads of 256, whose O and loads in flight fill the registers at half
@@ -395,9 +395,10 @@ __device__ __forceinline__ void split_n(float (&x)[N], u32 (&w)[NP][N / 2]) {
 // added, as weights of 0 are right; if not (0 times an infinity or a NaN that a column must not see), again with what no column sees as
 // 0, and if that is not enough token by token with what it does not see as 0.
 //
-// Measured on MI355X (replayed, buffers in turn): 60001 positions, 24 / 4 heads of 256, f16, f32 queries (246 MB) 47.5 us, 5.2 TB/s; 64
-// sequences of 30 to 16000, 32 / 8 heads of 128, bf16 (699 MB) 135 us, 5.2 TB/s; 8 sequences of 900 to 6000, T = 5, 24 / 4 heads of
-// 256 (104 MB, two blocks of columns, the second from the L2) 34 us, 3.1 TB/s; 421 positions, 32 / 32 heads of 128 8.3 us, all latency.
+// Measured on MI355X (replayed, buffers in turn; cards differ by 5 %): 60001 positions, 24 / 4 heads of 256, f16, f32 queries (246 MB) 47 to
+// 49 us, 5.0 to 5.2 TB/s (bf16, f32 queries 49); 64 sequences of 30 to 16000, 32 / 8 heads of 128, bf16 (699 MB) 135 to 141 us, 5.0 to 5.2 TB/s;
+// 8 sequences of 900 to 6000, T = 5, 24 / 4 heads of 256 (104 MB, two blocks of columns, the second from the L2) 34 us, 3.1 TB/s; 421
+// positions, 32 / 32 heads of 128 8.3 us, all latency.
 // A plain read reaches 6.3 TB/s. Four waves a workgroup, two workgroups a CU and loads not ahead of the queries: 54, 151 and 54 us.
 template <int HD, bool BF, bool F32, u32 NC, u32 NW>
 __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const amdc_attn_args &a) {
@@ -676,7 +677,7 @@ __device__ __forceinline__ void dec_body(const amdc_kv_dev &kv, const amdc_attn_
 #pragma unroll
       for (u32 k = 0; k < SL; k++) sc[k] = __builtin_amdgcn_exp2f(sc[k] + ref);
 #pragma unroll
-      for (u32 k = 0; k < SL; k += 4u) l[c] += (sc[k] + sc[k + 1u]) + (sc[k + 2u] + sc[k + 3u]);
+      for (u32 k = 0; k < SL; k += 4u) l[c] += (sc[k] + sc[k + 1u]) + (sc[k + 2u] + sc[k + 3u]); // before a 16-bit type's rounding (pre_body: after it)
       u32 w[NP][SL / 2];
       split_n<BF, NP>(sc, w);
 #pragma unroll
@@ -937,10 +938,12 @@ __device__ __forceinline__ PreUnit pre_unit(const amdc_kv_dev &kv, const amdc_at
 // Rows are dealt from the last tile of the last sequence down: the longest first. Where all rows make fewer workgroups than the CUs
 // hold (a short chunk of a long prompt), a tile's positions are split over a.U workgroups; their partial results go through the
 // workspace and amdc_attn_join_*, a launch of its own (joined by the last workgroup to arrive, 128 rows of four parts took it 18 us).
-// Measured on MI355X (replayed; cards differ by 5 %): 12000 rows of 32 / 8 heads of 128, bf16, 1.12 ms, 1050 TFLOP/s of causal work (a
-// large product: 1210), matrix units busy 54 % of the cycles, vector units 42 %, at 1.7 to 1.9 GHz; 11 prompts under a window, heads of
-// 64, f16, 72 us, 530 TFLOP/s, vector units busy 61 % (the exponentials); a chunk of 256 over 5000, 24 / 4 heads of 256, f32, 80 us with
-// its join of 11 (profiled); 77 rows, 32 / 32 heads of 128 12.2 us, latency.
+// Measured on MI355X (replayed; cards differ by 5 %): 12000 rows of 32 / 8 heads of 128, bf16, 1.11 ms, 1066 TFLOP/s of causal work (a
+// large product: 1210), matrix units busy 56 % of the cycles, vector units 44 %, at 1.7 to 1.9 GHz; 11 prompts under a window, heads of
+// 64, f16, 71 us, 540 TFLOP/s, matrix units 30 %, vector units 61 %: a tile's scores, softmax and products follow each other in a wave, and
+// the two kinds of units run one after the other more than beside each other; a chunk of 256 over 5000, 24 / 4 heads of 256, f32, 77 to 80
+// us with its join of 11 (profiled); 77 rows, 32 / 32 heads of 128 12.4 us, latency. 2 x 4096 rows, 32 / 8 heads of 128: 286 bf16, 501 f32 on
+// f16, 709 f32 on bf16; 2 x 2048 rows, 24 / 4 heads of 256: 145, 217, 264.
 template <int HD, bool BF, bool F32, u32 W, u32 BN>
 __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const amdc_attn_args &a) {
   typedef typename std::conditional<W == 32u, v16f, v4f>::type acc; // of a matrix instruction: W x W / 64
@@ -1089,7 +1092,7 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const amdc_attn_
     constexpr u32 N = decltype(groups)::value, NS = 8u * PF; // scores of a lane in 32 positions: 32 / PF f + 8 gg + 0 .. 7 for f < PF
     float S[N * NS];
     // these products before the other wave's softmax, which then runs beside them (MI355X, us: 2 x 4096 rows of 32 / 8 heads of 128 303,
-    // without 308; both products so 307; heads of 64 173 each)
+    // without 308, both products so 307; of heads of 64 173, the softmax raised in their place 179)
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (u32 t = 0; t < N; t++) {
@@ -1139,7 +1142,9 @@ __device__ __forceinline__ void pre_body(const amdc_kv_dev &kv, const amdc_attn_
       split8<BF, NP>(v, w);
 #pragma unroll
       for (int p = 0; p < NP; p++) pw[p][k] = w[p];
-      if (NP == 1) // the sum of the rounded weights, the ones that the values get
+      // 16-bit: the sum of the rounded weights, the ones that the values get, two in an instruction (dec_body, which waits for the HBM, sums
+      // them before: either is within the weights' half steps, and the two operators' rows differ by that)
+      if (NP == 1)
 #pragma unroll
         for (int i = 0; i < 4; i++) l = sum2<BF>(w[0][i], l);
     }
@@ -1335,7 +1340,7 @@ extern "C" __global__ __launch_bounds__(256) void amdc_attn_join_bf16(amdc_kv_de
 // Rows of a wave, positions of a tile, workgroups a CU wanted of the registers (MI355X, us; each pair as measured when it was chosen).
 // Heads of 128, 16-bit: two workgroups on tiles of 64 positions; three, on tiles of 32, spill (12000 rows 1084 against 1098, 4096 rows 306
 // against 301). Heads of 128, f32 on f16: two on tiles of 32 505 for 2 x 4096 rows, one on tiles of 64 587; bf16's three parts would spill.
-// Heads of 256: 32 rows a wave, one wave a SIMD, 144 where 16 rows, two waves, took 110 (256 rows over 5000 positions, 24 / 4 heads, f32).
+// Heads of 256: 32 rows a wave, one wave a SIMD, 144 where 16 rows, two waves, took 110 (256 rows over 5000 positions, 24 / 4 heads, f32; 77 now).
 // Heads of 64, 16-bit: three workgroups a CU 76 for 11 prompts under a window, two 81; four spill, as f32's three do.
 #define PRE_KERNEL(HD, KN, BF, F32, OCC) \
   extern "C" __global__ __launch_bounds__(64u * AMDC_PRE_BM / AMDC_PRE_W(HD), OCC) void amdc_attn_pre_h##HD##_##KN(amdc_kv_dev kv, amdc_attn_args a) { \

@@ -338,11 +338,13 @@ int amdc_kv_append(const amdc_kv *kv, const float *k, const float *v, const floa
  * over the positions j <= len[b] - T + t, with window not 0 the last `window` of them only. q and y have type
  * t (AMDC_TYPE_F32 or the cache's), rows qs and ys values apart; q, y and q8 do not overlap. Queries are used as they are given; in f32, the
  * scores, weights, sums and y keep f32's accuracy (the products run on the 16-bit matrix units in parts); in a
- * 16-bit type the weights are rounded to it. A scale that is not finite gives NaN. With q8 not NULL also the Q8 copy of the rows (n_q hd values), q8s
+ * 16-bit type the weights are rounded to it (and decode divides by their sum before the rounding, prompts by that after it: their rows
+ * agree within it, not in bits). A scale that is not finite gives NaN. With q8 not NULL also the Q8 copy of the rows (n_q hd values), q8s
  * bytes apart, for the output matrix: the bits of amdc_quant_q8 of the f32 result (before y's rounding).
  * A value (or key) that a row does not see may be anything, NaN too, also where another row sees it. Of those that
  * it sees, a value that is not finite makes its place of the row infinite or NaN, a key that is not finite the row NaN (or, where
- * the score is -infinity, counts for nothing).
+ * the score is -infinity, counts for nothing). The sums are f32's: a bf16 cache's values over 2^122 / len can pass its range and give
+ * infinities.
  * ws: amdc_attn_decode_ws(kv, n_q, T) bytes of device memory, 16-byte aligned, cleared to 0 once before the first use
  * with any call (the calls leave its counters at 0); calls that share it must not overlap on the device, calls with
  * workspaces of their own may. The size does not depend on the lengths. Nothing is allocated: every call can be
@@ -353,7 +355,8 @@ int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t 
 
 /* The same for any numbers of new tokens: whole prompts, or chunks at the end of what is cached, of different
  * lengths packed into one call (cu), or T rows of every sequence (cu NULL). ws: amdc_attn_prefill_ws(kv, n_q, rows)
- * bytes, rows = T with cu, n_seq T without; under the rules of amdc_attn_decode's. */
+ * bytes, rows = T with cu, n_seq T without; under the rules of amdc_attn_decode's. It has room for the parts that few rows over many
+ * positions are split into, 17 MB for heads of 64 and 34 MB for others, whatever n_q and rows: one serves every chunk. */
 size_t amdc_attn_prefill_ws(const amdc_kv *kv, uint32_t n_q, uint32_t rows);
 int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
                       uint32_t window, const int32_t *cu, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream);
