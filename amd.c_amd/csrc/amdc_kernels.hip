@@ -32,6 +32,7 @@
 //                      command list for these operations)
 //   amdc_kv_append_*, amdc_attn_dec_*, amdc_attn_pre_*, amdc_attn_join_*
 //                      the paged cache and the attention over it (amdc_attn.h)
+//   amdc_take_flag     amdc_kv_check's look at their error flag
 //   amdc_dots_{q4_0,q4_k,q8_0,q6_k}
 //                      the per-block int32 dot products (parity check)
 //   amdc_probe_read, amdc_probe_copy
