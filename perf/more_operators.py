@@ -215,7 +215,7 @@ def _calls(s):
         amdc.norm_res_q8(s["x"].data_ptr(), s["w1"].data_ptr() if case["post"] else None, case["scale"], s["res"].data_ptr(), s["h"].data_ptr(), s["w2"].data_ptr(), y, n, 1e-6,
                          T=case["rows"], xs=4 * n, rs=4 * n, hs=4 * n, ys=4 * n, stream=stream)
         return {"h": s["h"], "y": s["y"]}
-    T = case.get("T", case["new_hi"] if s["each"] or case.get("new_hi") == 1 else None) if op != "prefill" else None
+    T = case["T"] if op == "decode" else case["new_hi"] if op == "conv" and (s["each"] or case["new_hi"] == 1) else None
     if op == "conv":
         ch = case["ch"]
         amdc.conv(s["slots"], s["state"].data_ptr(), s["x"].data_ptr(), s["w"].data_ptr(), s["bias"].data_ptr(), y, s["t"], ch, case["width"], T or s["rows"], ch, ch,
