@@ -134,6 +134,14 @@ ABI = {
     "amdc_attn_decode": (C.c_int, [_P, _P, _P, C.c_int, _U32, _U32, _U32, _U32, C.c_float, _U32, _P, _U32, _P, C.c_size_t, _P]),
     "amdc_attn_prefill_ws": (C.c_size_t, [_P, _U32, _U32]),
     "amdc_attn_prefill": (C.c_int, [_P, _P, _P, C.c_int, _U32, _U32, _U32, _U32, C.c_float, _U32, _P, _P, _U32, _P, C.c_size_t, _P]),
+    "amdc_conv_bytes": (C.c_size_t, [_U32, _U32, _U32]),
+    "amdc_conv": (C.c_int, [_P, _P, _P, _P, _P, _P, C.c_int, _U32, _U32, _U32, _U32, _U32, _P, C.c_int, C.c_int, _P]),
+    "amdc_gdn_bytes": (C.c_size_t, [_U32, _U32, _U32, _U32]),
+    "amdc_gdn_decode": (C.c_int, [_P] * 9 + [C.c_int] + [_U32] * 7 + [C.c_int, _P]),
+    "amdc_gdn_prefill_ws": (C.c_size_t, [_P, _U32, _U32]),
+    "amdc_gdn_prefill": (C.c_int, [_P] * 9 + [C.c_int] + [_U32] * 7 + [_P, _P, C.c_size_t, _P]),
+    "amdc_norm_gate_q8": (C.c_int, [_P, C.c_int, _P, _P, _P, _U32, _U32, C.c_float, C.c_int, _P, _U32, _U32, _U32, _U32, _U32, _P]),
+    "amdc_norm_res_q8": (C.c_int, [_P, _P, C.c_float, _P, _P, _P, _P, _U32, C.c_float, _P, _U32, _U32, _U32, _U32, _U32, _U32, _P]),
     "amdc_chain_record_begin": (C.c_int, [_P]),
     "amdc_chain_record_end": (C.c_int, [_P, C.c_int, C.POINTER(_P)]),
 }
@@ -141,6 +149,9 @@ ABI = {
 CHAIN_QUANT, CHAIN_GEMV, CHAIN_GEMV_X, CHAIN_RMSNORM_Q8, CHAIN_SWIGLU_Q8 = 0, 1, 2, 3, 4
 TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 ROPE_NONE, ROPE_PAIRS, ROPE_HALVES = 0, 1, 2
+ACT_NONE, ACT_SILU = 0, 1
+HEADS_GROUPED, HEADS_TILED = 0, 1
+GATE_SILU, GATE_SIGMOID = 0, 1
 
 
 class ChainOp(C.Structure):
@@ -153,6 +164,17 @@ class KvStruct(C.Structure):
     """amdc_kv of include/amdc_q4.h."""
     _fields_ = [("type", C.c_int), ("n_kv", _U32), ("hd", _U32), ("page", _U32), ("n_pages", _U32), ("k", _P), ("v", _P),
                 ("n_seq", _U32), ("max_pages", _U32), ("pages", _P), ("len", _P)]
+
+
+class SlotsStruct(C.Structure):
+    """amdc_slots of include/amdc_q4.h."""
+    _fields_ = [("n_seq", _U32), ("n_slots", _U32), ("from_", _P), ("to", _P)]
+
+
+class GdnStruct(C.Structure):
+    """amdc_gdn of include/amdc_q4.h."""
+    _fields_ = [("n_k", _U32), ("n_v", _U32), ("dk", _U32), ("dv", _U32), ("order", C.c_int), ("scale", C.c_float), ("eps", C.c_float),
+                ("A", _P), ("dt", _P)]
 
 
 class AmdcError(RuntimeError):
@@ -515,6 +537,76 @@ def attn_prefill_ws(kv, n_q, rows):
 def attn_prefill(kv, q, y, type, n_q, T, qs, ys, scale, ws, ws_bytes, cu=None, window=0, q8=None, q8s=0, stream=None):
     """amdc_attn_prefill: causal attention of the new rows of every sequence (packed by cu, or T each) over its cached positions."""
     _check(lib().amdc_attn_prefill(kv.ref, _p(q), _p(y), type, n_q, T, qs, ys, scale, window, _p(cu), _p(q8), q8s, _p(ws), ws_bytes, stream))
+
+
+class Slots:
+    """amdc_slots: the sequences of a call, the slot of the pools that each starts from (`from_`, -1: zeros) and the one that its new
+    state goes to (`to`, -1: none), both in device memory."""
+
+    def __init__(self, n_seq, n_slots, from_, to):
+        self.n_seq, self.n_slots = n_seq, n_slots
+        self.held = (from_, to)  # device buffers live as long as this
+        self.s = SlotsStruct(n_seq, n_slots, _p(from_), _p(to))
+        self.ref = C.byref(self.s)
+
+
+class Gdn:
+    """amdc_gdn: the heads of a layer's gated delta rule and what its gates learned (A and dt, device memory)."""
+
+    def __init__(self, n_k, n_v, dk, dv, order, scale, eps, A, dt):
+        self.n_k, self.n_v, self.dk, self.dv = n_k, n_v, dk, dv
+        self.held = (A, dt)
+        self.s = GdnStruct(n_k, n_v, dk, dv, order, scale, eps, _p(A), _p(dt))
+        self.ref = C.byref(self.s)
+
+
+def conv_bytes(ch, width, n_slots):
+    """Bytes of a convolution's pool of states."""
+    n = lib().amdc_conv_bytes(ch, width, n_slots)
+    if not n:
+        raise AmdcError(f"conv: {ch} channels, width {width}, {n_slots} slots: not supported")
+    return n
+
+
+def conv(slots, states, x, w, bias, y, type, ch, width, T, xs, ys, cu=None, each=0, act=ACT_SILU, stream=None):
+    """amdc_conv: the causal convolution of the new rows over each channel, and the sequences' new states."""
+    _check(lib().amdc_conv(slots.ref, _p(states), _p(x), _p(w), _p(bias), _p(y), type, ch, width, T, xs, ys, _p(cu), each, act, stream))
+
+
+def gdn_bytes(n_v, dk, dv, n_slots):
+    """Bytes of the delta rule's pool of states."""
+    n = lib().amdc_gdn_bytes(n_v, dk, dv, n_slots)
+    if not n:
+        raise AmdcError(f"gdn: {n_v} heads of {dk} x {dv}, {n_slots} slots: not supported")
+    return n
+
+
+def gdn_decode(gdn, slots, states, q, k, v, a, b, y, type, T, qs, ks, vs, as_, bs, ys, each=0, stream=None):
+    """amdc_gdn_decode: the gated delta rule over the T new tokens of every sequence (each: the state is kept after every one)."""
+    _check(lib().amdc_gdn_decode(gdn.ref, slots.ref, _p(states), _p(q), _p(k), _p(v), _p(a), _p(b), _p(y), type, T, qs, ks, vs, as_, bs, ys, each, stream))
+
+
+def gdn_prefill_ws(gdn, n_seq, rows):
+    """Bytes of gdn_prefill's workspace for `rows` rows in all (device memory)."""
+    n = lib().amdc_gdn_prefill_ws(gdn.ref, n_seq, rows)
+    if not n:
+        raise AmdcError(f"gdn_prefill: {n_seq} sequences, {rows} rows: not supported")
+    return n
+
+
+def gdn_prefill(gdn, slots, states, q, k, v, a, b, y, type, T, qs, ks, vs, as_, bs, ys, ws, ws_bytes, cu=None, stream=None):
+    """amdc_gdn_prefill: the gated delta rule over the new rows of every sequence (packed by cu, or T each)."""
+    _check(lib().amdc_gdn_prefill(gdn.ref, slots.ref, _p(states), _p(q), _p(k), _p(v), _p(a), _p(b), _p(y), type, T, qs, ks, vs, as_, bs, ys, _p(cu), _p(ws), ws_bytes, stream))
+
+
+def norm_gate_q8(x, type, w, z, y, n_h, hd, eps, gate=GATE_SILU, q=None, T=1, xs=0, zs=0, ys=0, qs=0, stream=None):
+    """amdc_norm_gate_q8: y = rmsnorm(x) w gate(z), each head by itself, and, when q is given, its Q8 copy."""
+    _check(lib().amdc_norm_gate_q8(_p(x), type, _p(w), _p(z), _p(y), n_h, hd, eps, gate, _p(q), T, xs, zs, ys, qs, stream))
+
+
+def norm_res_q8(x, w1, scale, res, h, w2, y, n, eps, q=None, T=1, xs=0, rs=0, hs=0, ys=0, qs=0, stream=None):
+    """amdc_norm_res_q8: h = res + scale rmsnorm(x) w1 (w1 None: x itself), y = rmsnorm(h) w2 and, when q is given, its Q8 copy."""
+    _check(lib().amdc_norm_res_q8(_p(x), _p(w1), scale, _p(res), _p(h), _p(w2), _p(y), n, eps, _p(q), T, xs, rs, hs, ys, qs, stream))
 
 
 def chain_quant(x, q, nb, sync=True):

@@ -294,12 +294,17 @@ enum {
   K_ATTN_PRE = K_ATTN_DEC2 + 8, /* amdc_attn_pre_h64_f16, .. */
   K_ATTN_JOIN = K_ATTN_PRE + 12, /* amdc_attn_join_f32, _f16, _bf16: in the order of AMDC_TYPE_* */
   K_TAKE_FLAG = K_ATTN_JOIN + 3,
-  K_N
+  K_CONV, /* amdc_conv_w2_f32, _f16, _bf16, then w3, w4 */
+  K_GDN_REC = K_CONV + 9, /* amdc_gdn_rec_h64_f32, _f16, _bf16, then h128 */
+  K_NORM_GATE = K_GDN_REC + 6, /* amdc_norm_gate_f32, _f16, _bf16 */
+  K_NORM_RES = K_NORM_GATE + 3, /* amdc_norm_res_1, _2, _4, _8 */
+  K_N = K_NORM_RES + 4
 };
 
 #define KN(s) "amdc_" s
 #define KA2(s) KN(s "_f16_n2"), KN(s "_f16_f32_n2"), KN(s "_bf16_n2"), KN(s "_bf16_f32_n2")
 #define KA(s) KN(s "_f16"), KN(s "_f16_f32"), KN(s "_bf16"), KN(s "_bf16_f32")
+#define KT(s) KN(s "_f32"), KN(s "_f16"), KN(s "_bf16")
 #define GW(s) "amdc_gemmw_" s
 static const char *const kname[K_N] = {
     "amdc_quant_q8",           "amdc_dots_q4_0",          "amdc_dots_q4_k",          "amdc_gemm_q4_k_n128",
@@ -331,7 +336,9 @@ static const char *const kname[K_N] = {
     KN("gemv_q6_k_s1l"), KN("gemv_q6_k_xs1l"), KN("kv_append_f16"), KN("kv_append_bf16"),
     KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256"), KA2("attn_dec_h64"), KA2("attn_dec_h128"),
     KA("attn_pre_h64"), KA("attn_pre_h128"), KA("attn_pre_h256"),
-    KN("attn_join_f32"), KN("attn_join_f16"), KN("attn_join_bf16"), KN("take_flag")};
+    KN("attn_join_f32"), KN("attn_join_f16"), KN("attn_join_bf16"), KN("take_flag"),
+    KT("conv_w2"), KT("conv_w3"), KT("conv_w4"), KT("gdn_rec_h64"), KT("gdn_rec_h128"), KT("norm_gate"),
+    KN("norm_res_1"), KN("norm_res_2"), KN("norm_res_4"), KN("norm_res_8")};
 
 static hipModule_t g_mod;
 static hipFunction_t g_k[K_N];
@@ -1649,6 +1656,7 @@ int amdc_kv_check(void) {
   return fail(AMDC_EINVAL, "kv_check: a cache operator met %s",
               bad == AMDC_BAD_PAGE ? "a page outside the pool"
               : bad == AMDC_BAD_LEN ? "a length over max_pages * page, or under the sequence's number of new tokens"
+              : bad == AMDC_BAD_SLOT ? "a slot outside the pool of states"
                                     : "rows outside 0 .. T (cu)");
 }
 
@@ -1804,6 +1812,172 @@ int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t
   const u32 bn = pre_bn(kv, t);
   void *ja[] = {&d, &a, (void *)&kv->hd, (void *)&bn};
   return launch(K_ATTN_JOIN + t, tiles * (AMDC_PRE_BM / 16u) * kv->n_kv, 1, 0, stream, ja);
+}
+
+/* ---------------------------------------------------------------- a linear-attention layer */
+
+/* The checks of sequences, slots and rows that every operator with states shares. rows: the rows of the call. */
+static int check_slots(const char *op, const amdc_slots *sl, const void *states, u32 T, const int32_t *cu, int each, amdc_slots_dev *d, u32 *rows) {
+  if (!sl) return fail(AMDC_EINVAL, "%s: slots is NULL", op);
+  if (!sl->n_seq || sl->n_seq > (1u << 20) || !sl->n_slots || sl->n_slots > 0x7FFFFFFFu)
+    return fail(AMDC_EINVAL, "%s: %u sequences, %u slots (1 to 2^20 sequences, 1 to 2^31 - 1 slots)", op, sl->n_seq, sl->n_slots);
+  if (!sl->from || !sl->to || !states) return fail(AMDC_EINVAL, "%s: null pointer (from, to or the pool)", op);
+  if (!vec_rows(sl->from, 0, 4u) || !vec_rows(sl->to, 0, 4u) || !vec_rows(cu, 0, 4u)) return fail(AMDC_EINVAL, "%s: from, to and cu must be 4-byte aligned", op);
+  if (!aligned16(states)) return fail(AMDC_EINVAL, "%s: the pool must be 16-byte aligned", op);
+  if (each && (cu || T > AMDC_LIN_MAX_T)) return fail(AMDC_EINVAL, "%s: the states after every token of at most %u each, without cu (T %u)", op, AMDC_LIN_MAX_T, T);
+  const u64 r = cu ? T : (u64)sl->n_seq * T;
+  if (!T || r > (1u << 22)) return fail(AMDC_EINVAL, "%s: T %u (1 to 2^22 rows in all)", op, T);
+  *rows = (u32)r;
+  *d = (amdc_slots_dev){sl->from, sl->to, cu, g_kv_bad, sl->n_seq, sl->n_slots, T, each ? 1u : 0u};
+  return AMDC_OK;
+}
+static int type_ok(int t) { return t == AMDC_TYPE_F32 || t == AMDC_TYPE_F16 || t == AMDC_TYPE_BF16; }
+static u32 type_bytes(int t) { return t == AMDC_TYPE_F32 ? 4u : 2u; }
+/* rows of s values of es bytes, aligned to four values */
+static int vec4_rows(const void *p, u32 rows, u32 s, u32 es) { return (((uintptr_t)p | (rows > 1u ? (u64)s * es : 0u)) & (4u * es - 1u)) == 0; }
+
+size_t amdc_conv_bytes(uint32_t ch, uint32_t width, uint32_t n_slots) {
+  if (!ch || ch > (1u << 20) || width < 2u || width > 4u || !n_slots || n_slots > 0x7FFFFFFFu) return 0;
+  return (size_t)n_slots * (width - 1u) * ch * sizeof(float);
+}
+
+int amdc_conv(const amdc_slots *slots, float *states, const float *x, const float *w, const float *bias, void *y, int t, uint32_t ch, uint32_t width,
+              uint32_t T, uint32_t xs, uint32_t ys, const int32_t *cu, int each, int act, void *stream) {
+  NEED_OPEN();
+  amdc_slots_dev d;
+  u32 rows = 0;
+  int rc = check_slots("conv", slots, states, T, cu, each, &d, &rows);
+  if (rc) return rc;
+  if (!amdc_conv_bytes(ch, width, slots->n_slots)) return fail(AMDC_EINVAL, "conv: %u channels, width %u (1 to 2^20 channels, width 2 to 4)", ch, width);
+  if (!x || !w || !y) return fail(AMDC_EINVAL, "conv: null pointer (x, w or y)");
+  if (!type_ok(t)) return fail(AMDC_EINVAL, "conv: y of type %d", t);
+  if (act != AMDC_ACT_NONE && act != AMDC_ACT_SILU) return fail(AMDC_EINVAL, "conv: act %d", act);
+  if (!vec_rows(x, 0, 4u) || !vec_rows(w, 0, 4u) || !vec_rows(bias, 0, 4u) || !vec_rows(y, 0, type_bytes(t))) return fail(AMDC_EINVAL, "conv: x, w, bias and y must be aligned to their types");
+  if ((const void *)x == y) return fail(AMDC_EINVAL, "conv: y cannot be x");
+  if (rows > 1u && (xs < ch || ys < ch)) return fail(AMDC_EINVAL, "conv: strides xs %u, ys %u under a row's %u values", xs, ys, ch);
+  /* workgroups of one wave while the call's are few: they spread over the CUs */
+  const u32 upb = (T + AMDC_CONV_ROWS - 1u) / AMDC_CONV_ROWS;
+  const u64 units = cu ? (u64)rows / AMDC_CONV_ROWS + slots->n_seq : (u64)slots->n_seq * upb;
+  const u32 cols = (ch + 3u) / 4u, nt = units * ((cols + 255u) / 256u) < 4u * (u64)(g_cus > 0 ? g_cus : 256) ? 64u : 256u, cb = (cols + nt - 1u) / nt;
+  if (units * cb >= (1u << 24)) return fail(AMDC_EINVAL, "conv: %u rows of %u sequences and %u channels are too many for one call", rows, slots->n_seq, ch);
+  const u32 vec = (ch % 4u == 0 && vec4_rows(x, rows, xs, 4u) ? 1u : 0u) | (ch % 4u == 0 && vec4_rows(y, rows, ys, type_bytes(t)) ? 2u : 0u);
+  amdc_conv_args a = {states, x, w, bias, y, ch, xs, ys, cb, upb, (u32)act, vec};
+  void *args[] = {&d, &a};
+  return launch_nt(K_CONV + 3 * (int)(width - 2u) + t, (unsigned)(units * cb), 1, nt, 0, stream, args);
+}
+
+size_t amdc_gdn_bytes(uint32_t n_v, uint32_t dk, uint32_t dv, uint32_t n_slots) {
+  if (!n_v || n_v > 1024u || (dk != 64u && dk != 128u) || !dv || dv % 16u || dv > 256u || !n_slots || n_slots > 0x7FFFFFFFu) return 0;
+  return (size_t)n_slots * n_v * dk * dv * sizeof(float);
+}
+
+/* The checks of both forms of the delta rule beyond check_slots'; the arguments as the kernels take them. */
+static int check_gdn(const char *op, const amdc_gdn *g, const amdc_slots *sl, float *states, const void *q, const void *k, const void *v, const float *a, const float *b,
+                     void *y, int t, u32 rows, u32 qs, u32 ks, u32 vs, u32 as, u32 bs, u32 ys, amdc_gdn_args *d) {
+  if (!g) return fail(AMDC_EINVAL, "%s: gdn is NULL", op);
+  if (!g->n_k || !amdc_gdn_bytes(g->n_v, g->dk, g->dv, sl->n_slots) || g->n_v % g->n_k)
+    return fail(AMDC_EINVAL, "%s: %u key heads of %u, %u value heads of %u (1 to 1024, a multiple; keys of 64 or 128, values of a multiple of 16 up to 256)", op, g->n_k, g->dk,
+                g->n_v, g->dv);
+  if (g->order != AMDC_HEADS_GROUPED && g->order != AMDC_HEADS_TILED) return fail(AMDC_EINVAL, "%s: order %d", op, g->order);
+  if (!(g->eps > 0.0f)) return fail(AMDC_EINVAL, "%s: eps %g (above 0)", op, (double)g->eps);
+  if (!type_ok(t)) return fail(AMDC_EINVAL, "%s: q, k, v and y of type %d", op, t);
+  if (!q || !k || !v || !a || !b || !y || !g->A || !g->dt) return fail(AMDC_EINVAL, "%s: null pointer (q, k, v, a, b, y, A or dt)", op);
+  const u32 es = type_bytes(t), wk = g->n_k * g->dk, wv = g->n_v * g->dv;
+  if (!vec_rows(q, 0, es) || !vec_rows(k, 0, es) || !vec_rows(v, 0, es) || !vec_rows(y, 0, es) || !vec_rows(a, 0, 4u) || !vec_rows(b, 0, 4u) || !vec_rows(g->A, 0, 4u) ||
+      !vec_rows(g->dt, 0, 4u))
+    return fail(AMDC_EINVAL, "%s: q, k, v, y, a, b, A and dt must be aligned to their types", op);
+  if (y == q || y == k || y == v) return fail(AMDC_EINVAL, "%s: y cannot be q, k or v", op);
+  if (rows > 1u && (qs < wk || ks < wk || vs < wv || ys < wv || as < g->n_v || bs < g->n_v))
+    return fail(AMDC_EINVAL, "%s: strides qs %u, ks %u, vs %u, as %u, bs %u, ys %u under a row's values (%u, %u, %u)", op, qs, ks, vs, as, bs, ys, wk, wv, g->n_v);
+  const u32 vec = (vec4_rows(v, rows, vs, es) ? 1u : 0u) | (vec4_rows(y, rows, ys, es) ? 2u : 0u);
+  *d = (amdc_gdn_args){states, q, k, v, a, b, g->A, g->dt, y, NULL, g->scale, g->eps, g->n_k, g->n_v, g->dv, g->n_v / g->n_k, g->order == AMDC_HEADS_TILED, qs, ks, vs, as, bs, ys, vec};
+  return AMDC_OK;
+}
+static int launch_rec(const char *op, const amdc_gdn *g, int t, amdc_slots_dev *d, amdc_gdn_args *a, void *stream) {
+  const u64 waves = (u64)d->n_seq * g->n_v * (g->dv / 16u);
+  if (waves >= (1u << 25)) return fail(AMDC_EINVAL, "%s: %u sequences of %u heads of %u are too many for one call", op, d->n_seq, g->n_v, g->dv);
+  void *args[] = {d, a};
+  return launch(K_GDN_REC + (g->dk == 128u ? 3 : 0) + t, (unsigned)((waves + 3u) / 4u), 1, 0, stream, args);
+}
+
+int amdc_gdn_decode(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
+                    uint32_t T, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t as, uint32_t bs, uint32_t ys, int each, void *stream) {
+  NEED_OPEN();
+  amdc_slots_dev d;
+  amdc_gdn_args g;
+  u32 rows = 0;
+  int rc = check_slots("gdn_decode", slots, states, T, NULL, each, &d, &rows);
+  if (rc) return rc;
+  if (T > AMDC_LIN_MAX_T) return fail(AMDC_EINVAL, "gdn_decode: T %u (at most %u; more: gdn_prefill)", T, AMDC_LIN_MAX_T);
+  if ((rc = check_gdn("gdn_decode", gdn, slots, states, q, k, v, a, b, y, t, rows, qs, ks, vs, as, bs, ys, &g))) return rc;
+  return launch_rec("gdn_decode", gdn, t, &d, &g, stream);
+}
+
+size_t amdc_gdn_prefill_ws(const amdc_gdn *g, uint32_t n_seq, uint32_t rows) {
+  if (!g || !g->n_k || !amdc_gdn_bytes(g->n_v, g->dk, g->dv, 1u) || g->n_v % g->n_k || !n_seq || n_seq > (1u << 20) || !rows || rows > (1u << 22)) return 0;
+  return 16u;
+}
+
+int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
+                     uint32_t T, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t as, uint32_t bs, uint32_t ys, const int32_t *cu, void *ws, size_t ws_bytes, void *stream) {
+  NEED_OPEN();
+  amdc_slots_dev d;
+  amdc_gdn_args g;
+  u32 rows = 0;
+  int rc = check_slots("gdn_prefill", slots, states, T, cu, 0, &d, &rows);
+  if (rc) return rc;
+  if ((rc = check_gdn("gdn_prefill", gdn, slots, states, q, k, v, a, b, y, t, rows, qs, ks, vs, as, bs, ys, &g))) return rc;
+  const size_t need = amdc_gdn_prefill_ws(gdn, slots->n_seq, rows);
+  if (!ws || !aligned16(ws) || ws_bytes < need) return fail(AMDC_EINVAL, "gdn_prefill: a workspace of %zu bytes (16-byte aligned, at least %zu)", ws ? ws_bytes : (size_t)0, need);
+  g.ws = ws;
+  return launch_rec("gdn_prefill", gdn, t, &d, &g, stream);
+}
+
+/* a row's byte stride: of n values of es bytes, a multiple of es */
+static int stride_ok(u32 T, u32 s, u32 n, u32 es) { return T <= 1u || (s % es == 0 && (u64)s >= (u64)n * es); }
+
+int amdc_norm_gate_q8(const void *x, int t, const float *w, const float *z, float *y, uint32_t n_h, uint32_t hd, float eps, int gate, uint8_t *q, uint32_t T, uint32_t xs,
+                      uint32_t zs, uint32_t ys, uint32_t qs, void *stream) {
+  NEED_OPEN();
+  if (!x || !w || !z || (!y && !q) || !T) return fail(AMDC_EINVAL, "norm_gate_q8: null pointer (x, w, z, or both y and q) or empty");
+  if (!type_ok(t)) return fail(AMDC_EINVAL, "norm_gate_q8: x of type %d", t);
+  if (gate != AMDC_GATE_SILU && gate != AMDC_GATE_SIGMOID) return fail(AMDC_EINVAL, "norm_gate_q8: gate %d", gate);
+  if ((hd != 32u && hd != 64u && hd != 128u && hd != 256u) || !n_h || n_h > 4096u) return fail(AMDC_EINVAL, "norm_gate_q8: %u heads of %u (1 to 4096 of 32, 64, 128 or 256)", n_h, hd);
+  const u32 n = n_h * hd, es = type_bytes(t);
+  if (T > 65535u) return fail(AMDC_EINVAL, "norm_gate_q8: T %u > 65535", T);
+  if (!vec_rows(x, 0, es) || !vec_rows(w, 0, 4u) || !vec_rows(z, 0, 4u) || !vec_rows(y, 0, 4u) || !vec_rows(q, 0, 4u))
+    return fail(AMDC_EINVAL, "norm_gate_q8: x, w, z and y must be aligned to their types, q to 4 bytes");
+  if (!stride_ok(T, xs, n, es) || !stride_ok(T, zs, n, 4u) || (y && !stride_ok(T, ys, n, 4u)) || (q && T > 1u && (qs % 4u || qs < 40u * (n / 32u))))
+    return fail(AMDC_EINVAL, "norm_gate_q8: strides xs %u, zs %u, ys %u, qs %u too small or unaligned for %u values", xs, zs, ys, qs, n);
+  const u32 vec = (vec_rows(x, T > 1u ? xs : 0u, 4u * es) ? 1u : 0u) | (vec_rows(z, T > 1u ? zs : 0u, 16u) ? 2u : 0u) | (aligned16(w) ? 4u : 0u) |
+                  (vec_rows(y, T > 1u ? ys : 0u, 16u) ? 8u : 0u);
+  amdc_norm_args a = {.x = x, .w = w, .z = z, .y = y, .q = q, .eps = eps, .n = n, .hd = hd, .xs = xs, .zs = zs, .ys = ys, .qs = qs, .gate = gate == AMDC_GATE_SIGMOID, .vec = vec};
+  void *args[] = {&a};
+  return launch(K_NORM_GATE + t, (n + 1023u) / 1024u, T, 0, stream, args);
+}
+
+int amdc_norm_res_q8(const float *x, const float *w1, float scale, const float *res, float *h, const float *w2, float *y, uint32_t n, float eps, uint8_t *q, uint32_t T,
+                     uint32_t xs, uint32_t rs, uint32_t hs, uint32_t ys, uint32_t qs, void *stream) {
+  NEED_OPEN();
+  if (!x || !res || !h || !w2 || (!y && !q) || !n || !T) return fail(AMDC_EINVAL, "norm_res_q8: null pointer (x, res, h, w2, or both y and q) or empty (n %u, T %u)", n, T);
+  if (n % 32u || n > 32768u) return fail(AMDC_EINVAL, "norm_res_q8: n %u (a multiple of 32, at most 32768)", n);
+  if (T > 65535u) return fail(AMDC_EINVAL, "norm_res_q8: T %u > 65535", T);
+  if (!vec_rows(x, 0, 4u) || !vec_rows(w1, 0, 4u) || !vec_rows(res, 0, 4u) || !vec_rows(h, 0, 4u) || !vec_rows(w2, 0, 4u) || !vec_rows(y, 0, 4u) || !vec_rows(q, 0, 4u))
+    return fail(AMDC_EINVAL, "norm_res_q8: every pointer must be 4-byte aligned");
+  if (!stride_ok(T, xs, n, 4u) || !stride_ok(T, rs, n, 4u) || !stride_ok(T, hs, n, 4u) || (y && !stride_ok(T, ys, n, 4u)) || (q && T > 1u && (qs % 4u || qs < 40u * (n / 32u))))
+    return fail(AMDC_EINVAL, "norm_res_q8: strides xs %u, rs %u, hs %u, ys %u, qs %u too small or unaligned for %u values", xs, rs, hs, ys, qs, n);
+  if (h == y || (h == res && T > 1u && hs != rs) || (h == x && T > 1u && hs != xs)) return fail(AMDC_EINVAL, "norm_res_q8: h cannot be y; in place (h = res or x) it needs its stride");
+  const u32 vec = (vec_rows(x, T > 1u ? xs : 0u, 16u) ? 1u : 0u) | (vec_rows(res, T > 1u ? rs : 0u, 16u) ? 2u : 0u) | (aligned16(w1) ? 4u : 0u) |
+                  (vec_rows(y, T > 1u ? ys : 0u, 16u) ? 8u : 0u) | (vec_rows(h, T > 1u ? hs : 0u, 16u) ? 16u : 0u) | (aligned16(w2) ? 32u : 0u);
+  amdc_norm_args a = {x, w1, res, w2, h, y, q, eps, scale, n, 0, xs, rs, hs, ys, qs, 0, vec};
+  /* few rows: a thread to four values, up to 1024; many: 256 threads, up to 32 values each */
+  const u32 fours = n / 4u, most = T >= 256u ? 256u : 1024u;
+  u32 nt = (fours + 63u) / 64u * 64u, nv = 0;
+  if (nt > most) nt = most;
+  if ((fours + nt - 1u) / nt > 8u) nt = 1024u;
+  while ((1u << nv) * nt < fours) nv++;
+  void *args[] = {&a};
+  return launch_nt(K_NORM_RES + (int)nv, 1, T, nt, 0, stream, args);
 }
 
 int amdc_probe_read(const void *src, size_t nbytes, void *scratch, uint32_t grid, void *stream) {

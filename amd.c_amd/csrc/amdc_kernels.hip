@@ -33,6 +33,8 @@
 //   amdc_kv_append_*, amdc_attn_dec_*, amdc_attn_pre_*, amdc_attn_join_*
 //                      the paged cache and the attention over it (amdc_attn.h)
 //   amdc_take_flag     amdc_kv_check's look at their error flag
+//   amdc_conv_*, amdc_gdn_*, amdc_norm_gate_*, amdc_norm_res_*
+//                      a linear-attention layer: short convolution, gated delta rule, norms (amdc_gdn.h)
 //   amdc_dots_{q4_0,q4_k,q8_0,q6_k}
 //                      the per-block int32 dot products (parity check)
 //   amdc_probe_read, amdc_probe_copy
@@ -4144,3 +4146,4 @@ __device__ __align__(256) u32 kv_bad_flag[64];
 extern "C" __global__ void amdc_take_flag(u32 *flag, u32 *to) { *to = __hip_atomic_exchange(flag, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 #include "amdc_attn.h"
+#include "amdc_gdn.h"

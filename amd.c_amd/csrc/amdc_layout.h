@@ -138,6 +138,42 @@ typedef struct {
 
 /* Where part i of n tiles in `parts` parts begins, floor(n i / parts): n i itself passes 32 bits (2^26 tiles in 64 parts). */
 AMDC_INLINE uint32_t amdc_part_at(uint32_t n, uint32_t i, uint32_t parts) { return n / parts * i + n % parts * i / parts; }
-enum { AMDC_BAD_PAGE = 1, AMDC_BAD_LEN = 2, AMDC_BAD_ROWS = 3 };
+enum { AMDC_BAD_PAGE = 1, AMDC_BAD_LEN = 2, AMDC_BAD_ROWS = 3, AMDC_BAD_SLOT = 4 };
+
+/* The operators of a linear-attention layer (amdc_gdn.h): the sequences and their slots as the kernels take them (amdc_slots of amdc_q4.h,
+ * with the rows of the call), and the arguments of each, by value. */
+typedef struct {
+  const int32_t *from, *to, *cu;
+  uint32_t *bad;
+  uint32_t n_seq, n_slots, T, each;
+} amdc_slots_dev;
+#define AMDC_CONV_ROWS 32u /* rows of a sequence that a thread of the convolution goes over */
+#define AMDC_LIN_MAX_T 16u /* the most new tokens of a sequence in a decode call, or whose states are kept one by one */
+typedef struct {
+  float *state;
+  const float *x, *w, *bias;
+  void *y;
+  uint32_t ch, xs, ys, cb /* workgroups to a row */, upb /* units to a sequence (cu NULL) */, act;
+  uint32_t vec; /* 1: rows of x and the state, 2: rows of y are aligned to four values */
+} amdc_conv_args;
+typedef struct {
+  float *s;
+  const void *q, *k, *v;
+  const float *a, *b, *A, *dt;
+  void *y;
+  uint8_t *ws;
+  float scale, eps;
+  uint32_t n_k, n_v, dv, G /* n_v / n_k */, tiled, qs, ks, vs, as, bs, ys;
+  uint32_t vec; /* 1: rows of v, 2: rows of y are aligned to four values */
+} amdc_gdn_args;
+typedef struct {
+  const void *x;
+  const float *w, *z, *w2;
+  float *h, *y;
+  uint8_t *q;
+  float eps, scale;
+  uint32_t n, hd, xs, zs, hs, ys, qs, gate;
+  uint32_t vec; /* aligned to four values: 1 x, 2 z, 4 w, 8 y, 16 h, 32 w2 */
+} amdc_norm_args;
 
 #endif

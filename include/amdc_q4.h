@@ -312,8 +312,8 @@ typedef struct {
 
 /* Bytes of each of the two pools; 0 for a geometry that is not supported. */
 size_t amdc_kv_bytes(int type, uint32_t n_kv, uint32_t hd, uint32_t page, uint32_t n_pages);
-/* Synchronizes the device; AMDC_EINVAL and a message if a call since the last check met a page, a length
- * or a row outside its bounds (see amdc_kv). One flag serves all caches and streams: the message is of one such call
+/* Synchronizes the device; AMDC_EINVAL and a message if a call since the last check met a page, a length,
+ * a row or a slot outside its bounds (see amdc_kv, amdc_slots). One flag serves all caches, states and streams: the message is of one such call
  * and does not say which; a report made while this runs is kept for the next check. */
 int amdc_kv_check(void);
 
@@ -360,6 +360,80 @@ int amdc_attn_decode(const amdc_kv *kv, const void *q, void *y, int t, uint32_t 
 size_t amdc_attn_prefill_ws(const amdc_kv *kv, uint32_t n_q, uint32_t rows);
 int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t n_q, uint32_t T, uint32_t qs, uint32_t ys, float scale,
                       uint32_t window, const int32_t *cu, uint8_t *q8, uint32_t q8s, void *ws, size_t ws_bytes, void *stream);
+
+/* ---------------------------------------------------------------- a linear-attention layer */
+
+/* What stands between the input and output matrices of a layer whose attention is a gated delta rule (the
+ * reference's GDN layers): the short convolution, the delta rule, the norm of its heads with the gate; and the norms around a block. They
+ * take the GEMVs' and GEMMs' f32 rows; between them rows have a type, AMDC_TYPE_F32, _F16 or _BF16. States are f32.
+ *
+ * A sequence's state is kept in a slot of a pool in device memory (one pool and slot numbering per layer is usual; the
+ * convolution and the delta rule have a pool each). A call starts sequence b from slot from[b] (-1: a state of zeros) and leaves its
+ * new state in slot to[b] (-1: nowhere; from[b] itself: in place). from and to are device memory, n_seq integers, so that a captured
+ * graph follows what the host writes there. With `each` not 0 (at most 16 new tokens a sequence, no cu) the state after every token is
+ * kept, for a verify step: to has n_seq T entries, token t of sequence b at b T + t. Several sequences may start from one slot; a
+ * slot that one sequence writes is not read or written by another in the same call, nor by another call at the same time.
+ * New tokens are rows as amdc_kv has them: T of each sequence, or with cu (n_seq + 1 device integers) those from cu[b] to cu[b + 1] - 1, at
+ * most T in all. A sequence without new tokens takes no part: its slots are not touched. A sequence that only fills up a batch has from
+ * and to -1.
+ * What only the device sees is checked there: a slot from outside the pool makes the sequence's rows NaN and nothing is written to its
+ * slots, a slot to outside the pool is not written, of rows outside 0 .. T none is; amdc_kv_check() reports them all. */
+typedef struct {
+  uint32_t n_seq, n_slots;
+  const int32_t *from, *to;
+} amdc_slots;
+
+/* The causal convolution over each of ch channels: with the inputs x_t of a sequence, before its first the state's,
+ *   y_t[c] = act(bias[c] + sum_j w[c width + j] x_{t - width + 1 + j}[c]),  width 2 to 4, bias may be NULL,
+ * in f32, rounded once to y's type t. states: amdc_conv_bytes() of f32, [n_slots][width - 1][ch]: the last width - 1 inputs, the oldest first.
+ * Rows of x and y are xs and ys values apart (x may be some columns of a matrix's output rows). y is not x. */
+enum { AMDC_ACT_NONE = 0, AMDC_ACT_SILU = 1 };
+size_t amdc_conv_bytes(uint32_t ch, uint32_t width, uint32_t n_slots);
+int amdc_conv(const amdc_slots *slots, float *states, const float *x, const float *w, const float *bias, void *y, int t, uint32_t ch, uint32_t width,
+              uint32_t T, uint32_t xs, uint32_t ys, const int32_t *cu, int each, int act, void *stream);
+
+/* The gated delta rule of a layer: n_k heads of queries and keys (dk = 64 or 128 values), n_v heads of values (dv: a multiple of 16, at
+ * most 256), n_v a multiple of n_k. Value head h reads key head h / (n_v / n_k) (AMDC_HEADS_GROUPED) or h % n_k (AMDC_HEADS_TILED). For every token,
+ * with rows q, k of the key head and v of the value head, and the f32 rows a and b (n_v values each) of the token,
+ *   k^ = k / sqrt(k.k + eps),  q^ = scale q / sqrt(q.q + eps),  beta = 1 / (1 + exp(-b[h])),
+ *   g = min(0, A[h] softplus(a[h] + dt[h])),
+ *   S <- exp(g) S,  u = beta (v - k^ S),  S <- S + k^T u,  y = q^ S
+ * where S is the head's dk x dv matrix of the state, f32, [n_slots][n_v][dv / 16][dk][16] in the pool: row i, column 16 e + c at [e][i][c]
+ * (amdc_gdn_bytes()). A and dt: n_v device floats (A is negative: -exp of what is learned). eps is above 0. All sums, states
+ * and gates are f32 or more, whatever the rows' type t (that of q, k, v and y): y is rounded once. Rows are qs, ks, vs, as, bs and ys
+ * values apart; y is none of the inputs. A q, k, v, a or b that is not finite makes NaN or infinite what the formula makes of it (a value its
+ * column alone); prompts: the rows of up to 63 tokens before it too. */
+enum { AMDC_HEADS_GROUPED = 0, AMDC_HEADS_TILED = 1 };
+typedef struct {
+  uint32_t n_k, n_v, dk, dv;
+  int order; /* AMDC_HEADS_* */
+  float scale, eps;
+  const float *A, *dt;
+} amdc_gdn;
+size_t amdc_gdn_bytes(uint32_t n_v, uint32_t dk, uint32_t dv, uint32_t n_slots);
+/* T new tokens of every sequence, at most 16: decode, or a verify step (each). No workspace; can be captured. */
+int amdc_gdn_decode(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
+                    uint32_t T, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t as, uint32_t bs, uint32_t ys, int each, void *stream);
+/* Any numbers of new tokens: prompts, or chunks of them, packed (cu) or T each. ws: amdc_gdn_prefill_ws(gdn, n_seq, rows) bytes of
+ * device memory (rows = T with cu, n_seq T without), 16-byte aligned, of any content; calls that share it must not overlap on the
+ * device. Nothing is allocated: every call can be captured. */
+size_t amdc_gdn_prefill_ws(const amdc_gdn *gdn, uint32_t n_seq, uint32_t rows);
+int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
+                     uint32_t T, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t as, uint32_t bs, uint32_t ys, const int32_t *cu, void *ws, size_t ws_bytes, void *stream);
+
+/* The norm of each of n_h heads of hd (32, 64, 128 or 256) values, times its gate: of T rows, with s = 1 / sqrt(sum x^2 / hd + eps) of a head,
+ *   y = x s w gate(z),  gate(z) = z / (1 + exp(-z)) (AMDC_GATE_SILU) or 1 / (1 + exp(-z)) (AMDC_GATE_SIGMOID)
+ * x has type t, w has hd floats that all heads share, z and y n_h hd floats a row; y or q may be NULL; q: the Q8 copy, bit for bit amdc_quant_q8 of
+ * y. Strides are bytes, as amdc_rmsnorm_q8's. y may be z, or x where that is f32, at the same stride. */
+enum { AMDC_GATE_SILU = 0, AMDC_GATE_SIGMOID = 1 };
+int amdc_norm_gate_q8(const void *x, int t, const float *w, const float *z, float *y, uint32_t n_h, uint32_t hd, float eps, int gate, uint8_t *q, uint32_t T, uint32_t xs,
+                      uint32_t zs, uint32_t ys, uint32_t qs, void *stream);
+/* Between two blocks: the norm behind the first (w1 NULL: none), the residual, and the norm before the second, of T rows of n (a multiple of
+ * 32, at most 32768) values:
+ *   h = res + scale x s1 w1,  y = h s2 w2,  s1 and s2 the factors 1 / sqrt(mean square + eps) of x and h
+ * and q the Q8 copy of y, bit for bit amdc_quant_q8's (y or q may be NULL). h may be res or x (at the same stride), y is not h. Strides are bytes. */
+int amdc_norm_res_q8(const float *x, const float *w1, float scale, const float *res, float *h, const float *w2, float *y, uint32_t n, float eps, uint8_t *q, uint32_t T,
+                     uint32_t xs, uint32_t rs, uint32_t hs, uint32_t ys, uint32_t qs, void *stream);
 
 /* Tuning knobs (0 = automatic): lanes per row of the GEMV (4..64, power of
  * two); the decode kernel (0: the pipelined one; 1 or 2: the multi-vector
