@@ -4,6 +4,8 @@
 //   amdc_conv_w{2,3,4}_{f32,f16,bf16}   the causal convolution over the channels, with its state
 //   amdc_gdn_rec_h{64,128}_{f32,f16,bf16}
 //                                       the delta rule, token after token
+//   amdc_gdn_prep_h{64,128}_{f32,f16,bf16}, amdc_gdn_scan_h{64,128}_{f32,f16,bf16}
+//                                       the delta rule in chunks of 64 tokens: what does not depend on the state, then the states
 //   amdc_norm_gate_{f32,f16,bf16}       the heads' norm times the gate, and the Q8 copy
 //   amdc_norm_res_{1,2,4,8}             norm, residual, norm, and the Q8 copy
 
@@ -278,6 +280,554 @@ __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amd
   extern "C" __global__ __launch_bounds__(256) void amdc_gdn_rec_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_rec_body<TY, H##u>(sl, g); }
 #define GDN_RECS(H) GDN_REC(H, f32, 0) GDN_REC(H, f16, 1) GDN_REC(H, bf16, 2)
 GDN_RECS(64) GDN_RECS(128)
+
+// ------------------------------------------------------------------ the gated delta rule in chunks of 64 tokens
+//
+// Inside a chunk, with G_i the sum of the log decays up to token i, the updates u_i = beta_i (v_i - k_i S_(i-1)) solve
+//   (I + L) U = R,  L_ij = beta_i e^(G_i - G_j) k_i.k_j (j < i),  R_i = beta_i (v_i - e^(G_i) k_i S)
+// for the state S before the chunk, and then
+//   y_i = e^(G_i) q_i S + sum_(j <= i) e^(G_i - G_j) q_i.k_j u_j,   S <- e^(G_63) S + sum_j e^(G_63 - G_j) k_j^T u_j.
+// Two launches: amdc_gdn_prep computes what does not depend on the state, for all chunks at once: M = (I + L)^-1 and the weights
+// A_ij = e^(G_i - G_j) q_i.k_j for each value head, and the normed keys and queries as operands; amdc_gdn_scan takes the chunks of a sequence
+// one after the other, 32 columns of a head's state to a workgroup.
+//
+// Exponents are of differences that are at most 0, and those are taken in 64 bits: after a strong decay the sums are large and
+// their differences small. |M_ij|, |A_ij| <= 1: (I - beta k^T k) shrinks whatever it multiplies, for beta <= 1 and |k| <= 1.
+//
+// All products are on the f16 matrix units with both operands in two parts, x = hi + lo with 11 bits each, and three products, hi hi +
+// hi lo + lo hi, which keeps 22 bits and so f32's accuracy (the errors against 64 bits are those of the recurrence in f32). What f16's
+// range needs: keys, queries, M and A are at most 1 and are multiplied by 2^8; columns of S, R and U by a power of two each, from the
+// column's largest value (S) or a bound of it (R: the largest v plus |S|; U: 64 times that).
+//
+// The operands' k index is permuted so that the results of one product, four rows of a tile in a lane, are the next product's operand in
+// the same lane: place (g, e) of 32, lane group g, element e, is k = 16 (e / 4) + 4 g + e % 4.
+
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+#define GDN_C 64u        // tokens of a chunk
+#define GDN_UP 256.0f    // what operands of size up to 1 are multiplied by
+#define GDN_P 68u        // words of a row of 64 in the LDS: four lane groups, four rows apart, are 16 banks apart
+
+__device__ __forceinline__ h8 join8(h4 a, h4 b) { return (h8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
+// four values in two parts each
+__device__ __forceinline__ void split4(v4f x, h4 &hi, h4 &lo) {
+  hi = __builtin_convertvector(x, h4);
+  lo = __builtin_convertvector(x - __builtin_convertvector(hi, v4f), h4);
+}
+__device__ __forceinline__ v4f mfma_f16(h8 a, h8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+// (a[0] + a[1]) (b[0] + b[1]) without the product of the low parts
+__device__ __forceinline__ v4f mfma3(const h8 (&a)[2], const h8 (&b)[2], v4f c) { return mfma_f16(a[0], b[0], mfma_f16(a[0], b[1], mfma_f16(a[1], b[0], c))); }
+// the wave's own LDS accesses stay in order
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+// The power of two that brings values of up to m under 2^15, and its inverse. Both are normal: of values under 2^-104 fewer bits are kept.
+__device__ __forceinline__ void pow2_of(float m, float &up, float &down) {
+  const u32 e = __builtin_bit_cast(u32, m) >> 23 & 255u;
+  const u32 f = 268u - e < 246u ? 268u - e : 246u;
+  up = __builtin_bit_cast(float, f << 23), down = __builtin_bit_cast(float, (254u - f) << 23);
+}
+__device__ __forceinline__ float max4(v4f x) { return __builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(x.x), __builtin_fabsf(x.y)), __builtin_fmaxf(__builtin_fabsf(x.z), __builtin_fabsf(x.w))); }
+// the largest of the four lanes that are 16 apart
+__device__ __forceinline__ float max_groups(float v) {
+  v = __builtin_fmaxf(v, __shfl_xor(v, 16));
+  return __builtin_fmaxf(v, __shfl_xor(v, 32));
+}
+
+// Where chunk slot s (of all sequences', in their order) lies: with cu, sequence b's chunks are the slots cu[b] / 64 + b on, which leaves room for
+// each one's last, partial chunk.
+__device__ __forceinline__ u32 gdn_base(const amdc_slots_dev &sl, u32 nc, u32 b) {
+  if (!sl.cu) return b * nc;
+  const int c = sl.cu[b];
+  return (c < 0 ? 0u : (u32)c) / GDN_C + b;
+}
+__device__ __forceinline__ u32 gdn_seq(const amdc_slots_dev &sl, u32 nc, u32 s) {
+  return sl.cu ? find_seq(sl.n_seq, s, [&](u32 i) { return gdn_base(sl, nc, i); }) : s / nc;
+}
+
+// The workspace: a chunk slot holds for every key head its keys, queries and transposed keys as operands (fragments of 1 KB: 16
+// rows, 32 of k, the lanes' 16 bytes in order; two parts each), then for every value head M and A (the 6 fragments that are not all above the
+// diagonal, in parts) and for each token the factors beta, beta e^G, e^G, e^(G_63 - G).
+__device__ __forceinline__ u32 gdn_tri(u32 i, u32 s) { return i < 2u ? i : 2u * (i - 1u) + s; }
+
+template <int TY, u32 DK>
+__device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
+  constexpr u32 KS = DK / 32u, SCR = 4u * 4u * 336u * 4u;
+  constexpr u32 FA = 64u * DK * 4u > SCR ? 64u * DK * 4u : SCR, FB = 2u * 64u * GDN_P * 4u > DK * GDN_P * 4u ? 2u * 64u * GDN_P * 4u : DK * GDN_P * 4u;
+  __shared__ __align__(16) uint8_t s_a[FA]; // the keys' fragments; then each wave's blocks
+  __shared__ __align__(16) uint8_t s_b[FB]; // the keys, transposed, two parts in a word; then k.k and q.k
+  __shared__ double s_G[4][64];
+  __shared__ float s_beta[4][64];
+  const u32 tid = threadIdx.x, lane = tid & 63u, w = uniform(tid >> 6), n = lane & 15u, gr = lane >> 4;
+  const u32 at = blockIdx.x / g.n_k, hk = blockIdx.x - at * g.n_k, slot = g.s0 + at;
+  const u32 b = gdn_seq(sl, g.nc, slot);
+  if (b >= sl.n_seq) return;
+  u32 row0;
+  const u32 m = uniform(slot_rows(sl, b, row0)), c = slot - uniform(gdn_base(sl, g.nc, b));
+  if (c >= (m + GDN_C - 1u) / GDN_C) return;
+  const u32 first = row0 + c * GDN_C, mc = m - c * GDN_C < GDN_C ? m - c * GDN_C : GDN_C;
+  uint8_t *ws = g.ws + (u64)at * g.sb, *wk = ws + (u64)hk * (3u * 64u * DK * 4u);
+
+  // keys and queries: wave w the rows 16 w .. + 15, as operands of the products along dk
+  h8 kf[KS][2], qf[KS][2];
+  {
+    const u32 r = 16u * w + n;
+    const bool on = r < mc;
+    const u64 row = first + (on ? r : mc - 1u);
+    v4f k[KS][2], q[KS][2];
+#pragma unroll
+    for (u32 s = 0; s < KS; s++)
+#pragma unroll
+      for (u32 p = 0; p < 2u; p++) {
+        k[s][p] = ld4<TY>(g.k, row * g.ks + hk * DK + 32u * s + 16u * p + 4u * gr, g.vec & 4u);
+        q[s][p] = ld4<TY>(g.q, row * g.qs + hk * DK + 32u * s + 16u * p + 4u * gr, g.vec & 8u);
+      }
+    v4f kk = splat(0.0f), qq = splat(0.0f);
+#pragma unroll
+    for (u32 s = 0; s < KS; s++)
+#pragma unroll
+      for (u32 p = 0; p < 2u; p++) kk = fma4(k[s][p], k[s][p], kk), qq = fma4(q[s][p], q[s][p], qq);
+    float sk = (kk.x + kk.y) + (kk.z + kk.w), sq = (qq.x + qq.y) + (qq.z + qq.w);
+    sk += __shfl_xor(sk, 16), sq += __shfl_xor(sq, 16);
+    sk += __shfl_xor(sk, 32), sq += __shfl_xor(sq, 32);
+    const float rk = GDN_UP / __builtin_sqrtf(sk + g.eps), rq = GDN_UP / __builtin_sqrtf(sq + g.eps);
+    u32 *kt = (u32 *)s_b;
+#pragma unroll
+    for (u32 s = 0; s < KS; s++) {
+      h4 hi[2], lo[2], qh[2], ql[2];
+#pragma unroll
+      for (u32 p = 0; p < 2u; p++) {
+        split4(on ? k[s][p] * rk : splat(0.0f), hi[p], lo[p]);
+        split4(on ? q[s][p] * rq : splat(0.0f), qh[p], ql[p]);
+#pragma unroll
+        for (u32 e = 0; e < 4u; e++) {
+          const _Float16 x = hi[p][e], y = lo[p][e];
+          kt[(32u * s + 16u * p + 4u * gr + e) * GDN_P + r] = (u32)__builtin_bit_cast(unsigned short, x) | (u32)__builtin_bit_cast(unsigned short, y) << 16;
+        }
+      }
+      kf[s][0] = join8(hi[0], hi[1]), kf[s][1] = join8(lo[0], lo[1]);
+      qf[s][0] = join8(qh[0], qh[1]), qf[s][1] = join8(ql[0], ql[1]);
+#pragma unroll
+      for (u32 p = 0; p < 2u; p++) {
+        const u32 f = 1024u * ((w * KS + s) * 2u + p) + 16u * lane;
+        *(h8 *)(s_a + f) = kf[s][p];
+        *(h8 *)(wk + f) = kf[s][p];
+        *(h8 *)(wk + 64u * DK * 4u + f) = qf[s][p];
+      }
+    }
+  }
+  __syncthreads();
+  // the transposed keys
+#pragma unroll
+  for (u32 i = 0; i < DK / 64u; i++) {
+    const u32 M = w + 4u * i;
+#pragma unroll
+    for (u32 s = 0; s < 2u; s++) {
+      const u32 *kt = (const u32 *)s_b + (16u * M + n) * GDN_P + 32u * s + 4u * gr;
+      const u32x4 x = *(const u32x4 *)kt, y = *(const u32x4 *)(kt + 16u);
+      const u32x4 hi = {__builtin_amdgcn_perm(x.y, x.x, 0x05040100u), __builtin_amdgcn_perm(x.w, x.z, 0x05040100u), __builtin_amdgcn_perm(y.y, y.x, 0x05040100u),
+                        __builtin_amdgcn_perm(y.w, y.z, 0x05040100u)};
+      const u32x4 lo = {__builtin_amdgcn_perm(x.y, x.x, 0x07060302u), __builtin_amdgcn_perm(x.w, x.z, 0x07060302u), __builtin_amdgcn_perm(y.y, y.x, 0x07060302u),
+                        __builtin_amdgcn_perm(y.w, y.z, 0x07060302u)};
+      const u32 f = 2u * 64u * DK * 4u + 1024u * ((M * 2u + s) * 2u) + 16u * lane;
+      *(u32x4 *)(wk + f) = hi;
+      *(u32x4 *)(wk + f + 1024u) = lo;
+    }
+  }
+  // k.k and q.k, the tiles up to the diagonal: a fragment of keys is either operand
+  v4f kk[4], qk[4];
+#pragma unroll
+  for (u32 j = 0; j < 4u; j++) {
+    kk[j] = qk[j] = splat(0.0f);
+    if (j <= w)
+#pragma unroll
+      for (u32 s = 0; s < KS; s++) {
+        const h8 bf[2] = {*(const h8 *)(s_a + 1024u * ((j * KS + s) * 2u) + 16u * lane), *(const h8 *)(s_a + 1024u * ((j * KS + s) * 2u + 1u) + 16u * lane)};
+        kk[j] = mfma3(kf[s], bf, kk[j]), qk[j] = mfma3(qf[s], bf, qk[j]);
+      }
+  }
+  __syncthreads();
+  float *KK = (float *)s_b, *QK = KK + 64u * GDN_P;
+#pragma unroll
+  for (u32 j = 0; j < 4u; j++)
+    if (j <= w)
+#pragma unroll
+      for (u32 e = 0; e < 4u; e++) {
+        const u32 f = (16u * w + 4u * gr + e) * GDN_P + 16u * j + n;
+        KK[f] = kk[j][e] * (1.0f / (GDN_UP * GDN_UP)), QK[f] = qk[j][e] * (1.0f / GDN_UP); // q.k stays multiplied by 2^8
+      }
+  __syncthreads();
+  // a value head to a wave
+  float *blk = (float *)(s_a + w * (SCR / 4u));
+  for (u32 v = w; v < g.G; v += 4u) {
+    const u32 h = g.tiled ? hk + v * g.n_k : hk * g.G + v;
+    uint8_t *wv = ws + (u64)g.n_k * (3u * 64u * DK * 4u) + (u64)h * AMDC_GDN_VB;
+    double G;
+    float beta;
+    {
+      float decay;
+      gdn_gates(g, first + (lane < mc ? lane : mc - 1u), h, decay, beta);
+      // e^-10000 is 0: an infinite decay makes no NaN of a difference
+      decay = lane < mc ? decay < -1e4f ? -1e4f : decay : 0.0f, beta = lane < mc ? beta : 0.0f;
+      G = (double)decay;
+#pragma unroll
+      for (u32 o = 1; o < 64u; o <<= 1) {
+        const double up = __shfl_up(G, o);
+        G += lane >= o ? up : 0.0;
+      }
+      s_G[w][lane] = G, s_beta[w][lane] = beta;
+      const float since = __builtin_expf((float)G), until = __builtin_expf((float)(__shfl(G, 63) - G));
+      float *cf = (float *)(wv + 24576u);
+      cf[lane] = beta, cf[64u + lane] = beta * since, cf[128u + lane] = since, cf[192u + lane] = until;
+    }
+    wave_order();
+    // L by blocks of 16 x 16, row n, columns 4 gr .. of a block in a lane; A's fragments on the way
+    v4f L[10];
+#pragma unroll
+    for (u32 i = 0; i < 4u; i++) {
+      const u32 r = 16u * i + n;
+      const double Gr = s_G[w][r];
+      const float be = s_beta[w][r];
+      h4 hi[4], lo[4];
+#pragma unroll
+      for (u32 j = 0; j < 4u; j++) {
+        if (j > i) {
+          hi[j] = lo[j] = (h4){0, 0, 0, 0};
+          continue;
+        }
+        const u32 cl = 16u * j + 4u * gr;
+        const v4f x = *(const v4f *)(KK + r * GDN_P + cl), y = *(const v4f *)(QK + r * GDN_P + cl);
+        v4f l, a;
+#pragma unroll
+        for (u32 e = 0; e < 4u; e++) {
+          const float d = __builtin_amdgcn_exp2f((float)(Gr - s_G[w][cl + e]) * 1.4426950408889634f);
+          l[e] = cl + e < r ? be * (x[e] * d) : 0.0f;
+          a[e] = cl + e <= r ? y[e] * d : 0.0f;
+        }
+        L[i * (i + 1u) / 2u + j] = l;
+        split4(a, hi[j], lo[j]);
+      }
+#pragma unroll
+      for (u32 s = 0; s < (i < 2u ? 1u : 2u); s++) {
+        uint8_t *f = wv + 12288u + 2048u * gdn_tri(i, s) + 16u * lane;
+        *(h8 *)f = join8(hi[2u * s], hi[2u * s + 1u]);
+        *(h8 *)(f + 1024u) = join8(lo[2u * s], lo[2u * s + 1u]);
+      }
+      // the diagonal block, for its inverse
+      *(v4f *)(blk + 336u * i + 20u * n + 4u * gr) = L[i * (i + 1u) / 2u + i];
+    }
+    wave_order();
+    // the inverses of the four diagonal blocks: block gr, column n in a lane
+    {
+      float t[16];
+      const float *lb = blk + 336u * gr;
+#pragma unroll
+      for (u32 r = 0; r < 16u; r++) {
+        float s = r == n ? 1.0f : 0.0f;
+#pragma unroll
+        for (u32 j0 = 0; j0 < r; j0 += 4u) {
+          const v4f x = *(const v4f *)(lb + 20u * r + j0);
+#pragma unroll
+          for (u32 e = 0; e < 4u; e++)
+            if (j0 + e < r) s = __builtin_fmaf(-x[e], t[j0 + e], s);
+        }
+        t[r] = s;
+      }
+      wave_order();
+#pragma unroll
+      for (u32 r = 0; r < 16u; r++) blk[336u * gr + 20u * r + n] = t[r];
+    }
+    wave_order();
+    v4f M[10], dg[4]; // M by blocks as L; the diagonal ones also column n, rows 4 gr .. in a lane, as results and right operands have them
+#pragma unroll
+    for (u32 i = 0; i < 4u; i++) {
+      M[i * (i + 1u) / 2u + i] = *(const v4f *)(blk + 336u * i + 20u * n + 4u * gr);
+#pragma unroll
+      for (u32 e = 0; e < 4u; e++) dg[i][e] = blk[336u * i + 20u * (4u * gr + e) + n];
+    }
+    wave_order();
+    // M_ij = -M_ii sum_m L_im M_mj, f32 matrix units
+#pragma unroll
+    for (u32 j = 0; j < 3u; j++) {
+      v4f col[4];
+      col[j] = dg[j];
+#pragma unroll
+      for (u32 i = j + 1u; i < 4u; i++) {
+        v4f x = splat(0.0f), y = splat(0.0f);
+#pragma unroll
+        for (u32 k = j; k < i; k++)
+#pragma unroll
+          for (u32 e = 0; e < 4u; e++) x = __builtin_amdgcn_mfma_f32_16x16x4f32(L[i * (i + 1u) / 2u + k][e], col[k][e], x, 0, 0, 0);
+#pragma unroll
+        for (u32 e = 0; e < 4u; e++) y = __builtin_amdgcn_mfma_f32_16x16x4f32(M[i * (i + 1u) / 2u + i][e], x[e], y, 0, 0, 0);
+        col[i] = -y;
+#pragma unroll
+        for (u32 e = 0; e < 4u; e++) blk[336u * i + 20u * (4u * gr + e) + n] = col[i][e];
+      }
+      wave_order();
+#pragma unroll
+      for (u32 i = j + 1u; i < 4u; i++) M[i * (i + 1u) / 2u + j] = *(const v4f *)(blk + 336u * i + 20u * n + 4u * gr);
+      wave_order();
+    }
+#pragma unroll
+    for (u32 i = 0; i < 4u; i++) {
+      h4 hi[4], lo[4];
+#pragma unroll
+      for (u32 j = 0; j < 4u; j++)
+        if (j <= i) split4(M[i * (i + 1u) / 2u + j] * GDN_UP, hi[j], lo[j]);
+        else hi[j] = lo[j] = (h4){0, 0, 0, 0};
+#pragma unroll
+      for (u32 s = 0; s < (i < 2u ? 1u : 2u); s++) {
+        uint8_t *f = wv + 2048u * gdn_tri(i, s) + 16u * lane;
+        *(h8 *)f = join8(hi[2u * s], hi[2u * s + 1u]);
+        *(h8 *)(f + 1024u) = join8(lo[2u * s], lo[2u * s + 1u]);
+      }
+    }
+  }
+}
+
+// The chunks of a sequence one after the other: a workgroup has 32 columns of a head's state (in its registers, as results of the
+// products), and for each chunk three products that wait for each other:
+//   R = beta v - beta e^G (K S), and Q S on the way;   U = M R;   y = e^G (Q S) + A U and S = e^(G_63) S + K^T (e^(G_63 - G) U).
+// Wave w has the 16 tokens' rows w of R, U and y, and 32 rows of S (dk = 64: of 16 columns), so that keys, queries, M and A are read once a
+// workgroup, straight into registers, and a chunk ahead; S, R and U go through the LDS, as right operands.
+template <int TY, u32 DK>
+__device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
+  constexpr u32 KS = DK / 32u, NS = DK / 64u; // column tiles of S that a wave has
+  __shared__ __align__(16) uint8_t s_S[KS * 4096u], s_R[8192], s_U[8192], s_W[8192];
+  __shared__ float s_down[KS][32], s_vmax[2][4][32];
+  const u32 tid = threadIdx.x, lane = tid & 63u, w = uniform(tid >> 6), n = lane & 15u, gr = lane >> 4;
+  const u32 nb = (g.dv + 31u) / 32u, per = g.G * nb;
+  // the workgroups of a key head are on one XCD (workgroups go round the 8 of them), where the group count allows it
+  u32 gi, in;
+  if (g.groups >= 8u) {
+    const u32 x = blockIdx.x & 7u, y = blockIdx.x >> 3;
+    gi = (y / per) * 8u + x, in = y % per;
+  } else gi = blockIdx.x / per, in = blockIdx.x % per;
+  if (gi >= g.groups) return;
+  const u32 b = gdn_seq(sl, g.nc, g.s0) + gi / g.n_k, hk = gi % g.n_k, v = in / nb, cb = in - v * nb;
+  if (b >= sl.n_seq) return;
+  u32 row0;
+  const u32 m = uniform(slot_rows(sl, b, row0)), base = uniform(gdn_base(sl, g.nc, b)), all = (m + GDN_C - 1u) / GDN_C, end = g.s0 + g.ns;
+  if (!m || base >= end || base + all <= g.s0) return;
+  const u32 h = g.tiled ? hk + v * g.n_k : hk * g.G + v;
+  const u32 c0 = base < g.s0 ? g.s0 - base : 0u, c1 = base + all < end ? all : end - base;
+  const u32 ks = DK == 128u ? w : w & 1u, nt0 = DK == 128u ? 0u : w >> 1, na = g.dv >> 4;
+  const u64 mat = (u64)DK * g.dv;
+
+  // the state: from the slot, or where the call's launches left off
+  bool bad = false;
+  v4f S[NS][2];
+  {
+    const int f = sl.from[b];
+    const bool have = slot_ok(sl, f, bad) && c0 == 0u;
+    const float *src = have ? g.s + ((u64)(u32)f * g.n_v + h) * mat : g.carry_in + (u64)h * mat;
+#pragma unroll
+    for (u32 t = 0; t < NS; t++)
+#pragma unroll
+      for (u32 p = 0; p < 2u; p++)
+#pragma unroll
+        for (u32 e = 0; e < 4u; e++) {
+          const u32 a = 2u * cb + nt0 + t;
+          const bool on = a < na && (have || c0);
+          S[t][p][e] = on ? src[((u64)a * DK + 32u * ks + 16u * p + 4u * gr + e) * 16u + n] : bad && !c0 ? nan_() : 0.0f;
+        }
+  }
+  const auto vload = [&](u32 c, v4f (&x)[2]) { // the values of rows 16 w + 4 gr .. of chunk c
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++)
+#pragma unroll
+      for (u32 e = 0; e < 4u; e++) {
+        const u32 r = c * GDN_C + 16u * w + 4u * gr + e, cl = 32u * cb + 16u * t + n;
+        const bool on = r < m && cl < g.dv;
+        const float y = ld1<TY>(g.v, (u64)(row0 + (r < m ? r : m - 1u)) * g.vs + h * g.dv + (cl < g.dv ? cl : 0u));
+        x[t][e] = on ? y : 0.0f;
+      }
+  };
+  const auto put_S = [&]() { // S as a right operand, its columns' factors
+#pragma unroll
+    for (u32 t = 0; t < NS; t++) {
+      float up, down;
+      pow2_of(max_groups(__builtin_fmaxf(max4(S[t][0]), max4(S[t][1]))), up, down);
+      h4 hi[2], lo[2];
+#pragma unroll
+      for (u32 p = 0; p < 2u; p++) split4(S[t][p] * up, hi[p], lo[p]);
+      uint8_t *f = s_S + 1024u * ((ks * 2u + nt0 + t) * 2u) + 16u * lane;
+      *(h8 *)f = join8(hi[0], hi[1]);
+      *(h8 *)(f + 1024u) = join8(lo[0], lo[1]);
+      if (gr == 0u) s_down[ks][16u * (nt0 + t) + n] = down;
+    }
+  };
+  const auto put_vmax = [&](const v4f (&x)[2], u32 at) {
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) {
+      const float y = max_groups(max4(x[t]));
+      if (gr == 0u) s_vmax[at][w][16u * t + n] = y;
+    }
+  };
+  const auto put16 = [&](uint8_t *to, u32 t, v4f x) { // 16 rows of a right operand of 64
+    h4 hi, lo;
+    split4(x, hi, lo);
+    uint8_t *f = to + 1024u * (((w >> 1) * 2u + t) * 2u) + 16u * lane + 8u * (w & 1u);
+    *(h4 *)f = hi;
+    *(h4 *)(f + 1024u) = lo;
+  };
+  const auto get = [&](const uint8_t *from, u32 s, u32 t, h8 (&x)[2]) {
+    const uint8_t *f = from + 1024u * ((s * 2u + t) * 2u) + 16u * lane;
+    x[0] = *(const h8 *)f, x[1] = *(const h8 *)(f + 1024u);
+  };
+  h8 kf[KS][2], qf[KS][2], tf[2][2][2], mf[2][2], af[2][2];
+  v4f beta, bs, since, until;
+  float whole = 0.0f;
+  const auto chunk_ws = [&](u32 c) { return g.ws + (u64)(base + (c < c1 ? c : c1 - 1u) - g.s0) * g.sb; };
+  const auto value_ws = [&](u32 c) { return chunk_ws(c) + (u64)g.n_k * (3u * 64u * DK * 4u) + (u64)h * AMDC_GDN_VB; };
+  const auto load_kq = [&](u32 c) {
+    const uint8_t *p = chunk_ws(c) + (u64)hk * (3u * 64u * DK * 4u) + 2048u * KS * w + 16u * lane;
+#pragma unroll
+    for (u32 s = 0; s < KS; s++)
+#pragma unroll
+      for (u32 i = 0; i < 2u; i++) kf[s][i] = *(const h8 *)(p + 1024u * (2u * s + i)), qf[s][i] = *(const h8 *)(p + 64u * DK * 4u + 1024u * (2u * s + i));
+    const float *cf = (const float *)(value_ws(c) + 24576u) + 16u * w + 4u * gr;
+    beta = *(const v4f *)cf, bs = *(const v4f *)(cf + 64u);
+  };
+  const auto load_m = [&](u32 c) {
+    const uint8_t *p = value_ws(c) + 2048u * gdn_tri(w, 0u) + 16u * lane;
+#pragma unroll
+    for (u32 s = 0; s < 2u; s++)
+      if (s == 0u || w >= 2u)
+#pragma unroll
+        for (u32 i = 0; i < 2u; i++) mf[s][i] = *(const h8 *)(p + 2048u * s + 1024u * i);
+  };
+  const auto load_at = [&](u32 c) {
+    const uint8_t *p = value_ws(c) + 12288u + 2048u * gdn_tri(w, 0u) + 16u * lane;
+#pragma unroll
+    for (u32 s = 0; s < 2u; s++)
+      if (s == 0u || w >= 2u)
+#pragma unroll
+        for (u32 i = 0; i < 2u; i++) af[s][i] = *(const h8 *)(p + 2048u * s + 1024u * i);
+    p = chunk_ws(c) + (u64)hk * (3u * 64u * DK * 4u) + 2u * 64u * DK * 4u + 16u * lane;
+#pragma unroll
+    for (u32 i = 0; i < 2u; i++)
+#pragma unroll
+      for (u32 s = 0; s < 2u; s++)
+#pragma unroll
+        for (u32 j = 0; j < 2u; j++) tf[i][s][j] = *(const h8 *)(p + 1024u * (((2u * ks + i) * 2u + s) * 2u + j));
+    const float *cf = (const float *)(value_ws(c) + 24576u);
+    since = *(const v4f *)(cf + 128u + 16u * w + 4u * gr), until = *(const v4f *)(cf + 192u + 16u * w + 4u * gr), whole = cf[128u + 63u];
+  };
+
+  v4f val[2];
+  vload(c0, val);
+  load_kq(c0), load_m(c0), load_at(c0);
+  put_S(), put_vmax(val, c0 & 1u);
+  for (u32 c = c0; c < c1; c++) {
+    __syncthreads(); // S is there
+    v4f P[2], Q[2];
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) P[t] = Q[t] = splat(0.0f);
+    float top[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (u32 s = 0; s < KS; s++)
+#pragma unroll
+      for (u32 t = 0; t < 2u; t++) {
+        h8 x[2];
+        get(s_S, s, t, x);
+        const float down = s_down[s][16u * t + n];
+        top[t] = __builtin_fmaxf(top[t], down);
+        P[t] = fma4(splat(down), mfma3(kf[s], x, splat(0.0f)), P[t]);
+        Q[t] = fma4(splat(down), mfma3(qf[s], x, splat(0.0f)), Q[t]);
+      }
+    float down_R[2], up_U[2], down_U[2];
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) {
+      const float(*vm)[32] = s_vmax[c & 1u];
+      const float v0 = __builtin_fmaxf(vm[0][16u * t + n], vm[1][16u * t + n]), v1 = __builtin_fmaxf(vm[2][16u * t + n], vm[3][16u * t + n]);
+      // |k S| <= sqrt(dk) times the column's largest value, which is under 2^15 of the factor
+      float up;
+      pow2_of(__builtin_fmaf(12.0f * 32768.0f, top[t], __builtin_fmaxf(v0, v1)), up, down_R[t]);
+      const v4f R = beta * val[t] - bs * (P[t] * (1.0f / GDN_UP));
+      put16(s_R, t, R * up);
+      up_U[t] = up * (1.0f / 64.0f), down_U[t] = down_R[t] * 64.0f;
+    }
+    load_kq(c + 1u);
+    vload(c + 1u < c1 ? c + 1u : c, val);
+    __syncthreads(); // R is there
+    v4f U[2];
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) {
+      h8 x[2];
+      get(s_R, 0u, t, x);
+      U[t] = mfma3(mf[0], x, splat(0.0f));
+      if (w >= 2u) {
+        get(s_R, 1u, t, x);
+        U[t] = mfma3(mf[1], x, U[t]);
+      }
+      U[t] = U[t] * (down_R[t] * (1.0f / GDN_UP));
+      put16(s_U, t, U[t] * up_U[t]);
+      put16(s_W, t, U[t] * until * up_U[t]);
+    }
+    load_m(c + 1u);
+    put_vmax(val, c + 1u & 1u);
+    __syncthreads(); // U is there
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) {
+      h8 x[2];
+      get(s_U, 0u, t, x);
+      v4f y = mfma3(af[0], x, splat(0.0f));
+      if (w >= 2u) {
+        get(s_U, 1u, t, x);
+        y = mfma3(af[1], x, y);
+      }
+      y = fma4(splat(down_U[t]), y, since * Q[t]) * (g.scale * (1.0f / GDN_UP));
+      const u32 cl = 32u * cb + 16u * t + n;
+#pragma unroll
+      for (u32 e = 0; e < 4u; e++) {
+        const u32 r = c * GDN_C + 16u * w + 4u * gr + e;
+        if (r < m && cl < g.dv) {
+          const u64 o = (u64)(row0 + r) * g.ys + h * g.dv + cl;
+          if constexpr (TY == 0) ((float *)g.y)[o] = y[e];
+          else ((unsigned short *)g.y)[o] = (unsigned short)pack2<TY == 2>(y[e], 0.0f);
+        }
+      }
+    }
+#pragma unroll
+    for (u32 t = 0; t < NS; t++) {
+      h8 x[2][2];
+      get(s_W, 0u, nt0 + t, x[0]), get(s_W, 1u, nt0 + t, x[1]);
+      const float down = (NS == 2u ? down_U[t] : nt0 ? down_U[1] : down_U[0]) * (1.0f / GDN_UP);
+#pragma unroll
+      for (u32 p = 0; p < 2u; p++) S[t][p] = fma4(splat(down), mfma3(tf[p][1], x[1], mfma3(tf[p][0], x[0], splat(0.0f))), S[t][p] * whole);
+    }
+    load_at(c + 1u);
+    if (c + 1u < c1) put_S();
+  }
+  // the state: into its slot, or for the launch that goes on
+  float *dst = g.carry_out + (u64)h * mat;
+  bool write = true;
+  if (c1 == all) {
+    const int o = sl.to[b];
+    bool worse;
+    const bool start_ok = sl.from[b] >= -1 && sl.from[b] < (int)sl.n_slots;
+    write = slot_ok(sl, o, worse) && start_ok;
+    dst = g.s + ((u64)(u32)(o < 0 ? 0 : o) * g.n_v + h) * mat;
+  }
+  if (!write) return;
+#pragma unroll
+  for (u32 t = 0; t < NS; t++) {
+    const u32 a = 2u * cb + nt0 + t;
+    if (a < na)
+#pragma unroll
+      for (u32 p = 0; p < 2u; p++)
+#pragma unroll
+        for (u32 e = 0; e < 4u; e++) dst[((u64)a * DK + 32u * ks + 16u * p + 4u * gr + e) * 16u + n] = S[t][p][e];
+  }
+}
+
+#define GDN_PRE(H, N, TY)                                                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void amdc_gdn_prep_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_prep_body<TY, H##u>(sl, g); }  \
+  extern "C" __global__ __launch_bounds__(256) void amdc_gdn_scan_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_scan_body<TY, H##u>(sl, g); }
+#define GDN_PRES(H) GDN_PRE(H, f32, 0) GDN_PRE(H, f16, 1) GDN_PRE(H, bf16, 2)
+GDN_PRES(64) GDN_PRES(128)
 
 // ------------------------------------------------------------------ the norms
 

@@ -296,7 +296,8 @@ enum {
   K_TAKE_FLAG = K_ATTN_JOIN + 3,
   K_CONV, /* amdc_conv_w2_f32, _f16, _bf16, then w3, w4 */
   K_GDN_REC = K_CONV + 9, /* amdc_gdn_rec_h64_f32, _f16, _bf16, then h128 */
-  K_NORM_GATE = K_GDN_REC + 6, /* amdc_norm_gate_f32, _f16, _bf16 */
+  K_GDN_PRE = K_GDN_REC + 6, /* amdc_gdn_prep_h64_f32, _f16, _bf16, then h128, then amdc_gdn_scan_* */
+  K_NORM_GATE = K_GDN_PRE + 12, /* amdc_norm_gate_f32, _f16, _bf16 */
   K_NORM_RES = K_NORM_GATE + 3, /* amdc_norm_res_1, _2, _4, _8 */
   K_N = K_NORM_RES + 4
 };
@@ -337,7 +338,8 @@ static const char *const kname[K_N] = {
     KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256"), KA2("attn_dec_h64"), KA2("attn_dec_h128"),
     KA("attn_pre_h64"), KA("attn_pre_h128"), KA("attn_pre_h256"),
     KN("attn_join_f32"), KN("attn_join_f16"), KN("attn_join_bf16"), KN("take_flag"),
-    KT("conv_w2"), KT("conv_w3"), KT("conv_w4"), KT("gdn_rec_h64"), KT("gdn_rec_h128"), KT("norm_gate"),
+    KT("conv_w2"), KT("conv_w3"), KT("conv_w4"), KT("gdn_rec_h64"), KT("gdn_rec_h128"), KT("gdn_prep_h64"), KT("gdn_prep_h128"),
+    KT("gdn_scan_h64"), KT("gdn_scan_h128"), KT("norm_gate"),
     KN("norm_res_1"), KN("norm_res_2"), KN("norm_res_4"), KN("norm_res_8")};
 
 static hipModule_t g_mod;
@@ -1889,17 +1891,11 @@ static int check_gdn(const char *op, const amdc_gdn *g, const amdc_slots *sl, fl
   if (y == q || y == k || y == v) return fail(AMDC_EINVAL, "%s: y cannot be q, k or v", op);
   if (rows > 1u && (qs < wk || ks < wk || vs < wv || ys < wv || as < g->n_v || bs < g->n_v))
     return fail(AMDC_EINVAL, "%s: strides qs %u, ks %u, vs %u, as %u, bs %u, ys %u under a row's values (%u, %u, %u)", op, qs, ks, vs, as, bs, ys, wk, wv, g->n_v);
-  const u32 vec = (vec4_rows(v, rows, vs, es) ? 1u : 0u) | (vec4_rows(y, rows, ys, es) ? 2u : 0u);
-  *d = (amdc_gdn_args){states, q, k, v, a, b, g->A, g->dt, y, NULL, g->scale, g->eps, g->n_k, g->n_v, g->dv, g->n_v / g->n_k, g->order == AMDC_HEADS_TILED, qs, ks, vs, as, bs, ys, vec};
+  const u32 vec = (vec4_rows(v, rows, vs, es) ? 1u : 0u) | (vec4_rows(y, rows, ys, es) ? 2u : 0u) | (vec4_rows(k, rows, ks, es) ? 4u : 0u) | (vec4_rows(q, rows, qs, es) ? 8u : 0u);
+  *d = (amdc_gdn_args){.s = states, .q = q, .k = k, .v = v, .a = a, .b = b, .A = g->A, .dt = g->dt, .y = y, .scale = g->scale, .eps = g->eps, .n_k = g->n_k, .n_v = g->n_v, .dv = g->dv,
+                       .G = g->n_v / g->n_k, .tiled = g->order == AMDC_HEADS_TILED, .qs = qs, .ks = ks, .vs = vs, .as = as, .bs = bs, .ys = ys, .vec = vec};
   return AMDC_OK;
 }
-static int launch_rec(const char *op, const amdc_gdn *g, int t, amdc_slots_dev *d, amdc_gdn_args *a, void *stream) {
-  const u64 waves = (u64)d->n_seq * g->n_v * (g->dv / 16u);
-  if (waves >= (1u << 25)) return fail(AMDC_EINVAL, "%s: %u sequences of %u heads of %u are too many for one call", op, d->n_seq, g->n_v, g->dv);
-  void *args[] = {d, a};
-  return launch(K_GDN_REC + (g->dk == 128u ? 3 : 0) + t, (unsigned)((waves + 3u) / 4u), 1, 0, stream, args);
-}
-
 int amdc_gdn_decode(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
                     uint32_t T, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t as, uint32_t bs, uint32_t ys, int each, void *stream) {
   NEED_OPEN();
@@ -1910,12 +1906,25 @@ int amdc_gdn_decode(const amdc_gdn *gdn, const amdc_slots *slots, float *states,
   if (rc) return rc;
   if (T > AMDC_LIN_MAX_T) return fail(AMDC_EINVAL, "gdn_decode: T %u (at most %u; more: gdn_prefill)", T, AMDC_LIN_MAX_T);
   if ((rc = check_gdn("gdn_decode", gdn, slots, states, q, k, v, a, b, y, t, rows, qs, ks, vs, as, bs, ys, &g))) return rc;
-  return launch_rec("gdn_decode", gdn, t, &d, &g, stream);
+  const u64 waves = (u64)d.n_seq * gdn->n_v * (gdn->dv / 16u);
+  if (waves >= (1u << 25)) return fail(AMDC_EINVAL, "gdn_decode: %u sequences of %u heads of %u are too many for one call", d.n_seq, gdn->n_v, gdn->dv);
+  void *args[] = {&d, &g};
+  return launch(K_GDN_REC + (gdn->dk == 128u ? 3 : 0) + t, (unsigned)((waves + 3u) / 4u), 1, 0, stream, args);
+}
+
+/* The workspace of a prompt: chunk slots of gdn_slot_bytes (amdc_gdn.h), and two states: of the sequence whose chunks go on from the launches before, and of
+ * the one whose chunks go on in the next.
+ * The slots of all sequences are numbered in their order, and a pair of launches takes gdn_slots of them: that bounds the workspace, and what the first launch
+ * writes is still in the last-level cache (256 MB) when the second one reads it. */
+static u64 gdn_slot_bytes(const amdc_gdn *g) { return (u64)g->n_k * 3u * AMDC_GDN_C * g->dk * 4u + (u64)g->n_v * AMDC_GDN_VB; }
+static u32 gdn_slots(const amdc_gdn *g, u64 total) {
+  const u64 most = AMDC_GDN_WS / gdn_slot_bytes(g) + 1u;
+  return (u32)(total < most ? total : most);
 }
 
 size_t amdc_gdn_prefill_ws(const amdc_gdn *g, uint32_t n_seq, uint32_t rows) {
   if (!g || !g->n_k || !amdc_gdn_bytes(g->n_v, g->dk, g->dv, 1u) || g->n_v % g->n_k || !n_seq || n_seq > (1u << 20) || !rows || rows > (1u << 22)) return 0;
-  return 16u;
+  return (size_t)(gdn_slots(g, (u64)rows / AMDC_GDN_C + n_seq) * gdn_slot_bytes(g) + (u64)g->n_v * g->dk * g->dv * 8u);
 }
 
 int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
@@ -1929,8 +1938,25 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
   if ((rc = check_gdn("gdn_prefill", gdn, slots, states, q, k, v, a, b, y, t, rows, qs, ks, vs, as, bs, ys, &g))) return rc;
   const size_t need = amdc_gdn_prefill_ws(gdn, slots->n_seq, rows);
   if (!ws || !aligned16(ws) || ws_bytes < need) return fail(AMDC_EINVAL, "gdn_prefill: a workspace of %zu bytes (16-byte aligned, at least %zu)", ws ? ws_bytes : (size_t)0, need);
-  g.ws = ws;
-  return launch_rec("gdn_prefill", gdn, t, &d, &g, stream);
+  g.sb = gdn_slot_bytes(gdn), g.nc = (T + AMDC_GDN_C - 1u) / AMDC_GDN_C;
+  const u32 total = cu ? rows / AMDC_GDN_C + slots->n_seq : slots->n_seq * g.nc, most = gdn_slots(gdn, (u64)rows / AMDC_GDN_C + slots->n_seq);
+  const u64 state = (u64)gdn->n_v * gdn->dk * gdn->dv;
+  float *in = ws, *out = in + state;
+  g.ws = (uint8_t *)(out + state);
+  const int kern = K_GDN_PRE + (gdn->dk == 128u ? 3 : 0) + t;
+  for (g.s0 = 0; g.s0 < total; g.s0 += most) {
+    g.ns = total - g.s0 < most ? total - g.s0 : most;
+    /* the sequences with chunks in these slots: one for each slot, and the one that goes on */
+    const u32 seqs = slots->n_seq < g.ns + 1u ? slots->n_seq : g.ns + 1u, per = g.G * ((g.dv + 31u) / 32u);
+    g.groups = seqs * g.n_k;
+    g.carry_in = in, g.carry_out = out;
+    float *swap = in;
+    in = out, out = swap;
+    void *args[] = {&d, &g};
+    if ((rc = launch(kern, g.ns * g.n_k, 1, 0, stream, args))) return rc;
+    if ((rc = launch(kern + 6, g.groups >= 8u ? (g.groups + 7u) / 8u * 8u * per : g.groups * per, 1, 0, stream, args))) return rc;
+  }
+  return AMDC_OK;
 }
 
 /* a row's byte stride: of n values of es bytes, a multiple of es */

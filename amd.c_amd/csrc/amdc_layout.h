@@ -162,10 +162,16 @@ typedef struct {
   const float *a, *b, *A, *dt;
   void *y;
   uint8_t *ws;
+  float *carry_in, *carry_out; /* prompts: the state of the sequence that the launches before left unfinished, and of the one that these leave */
+  uint64_t sb;  /* prompts: bytes of a chunk slot of the workspace */
   float scale, eps;
   uint32_t n_k, n_v, dv, G /* n_v / n_k */, tiled, qs, ks, vs, as, bs, ys;
-  uint32_t vec; /* 1: rows of v, 2: rows of y are aligned to four values */
+  uint32_t vec; /* rows that are aligned to four values: 1 v, 2 y, 4 k, 8 q */
+  uint32_t nc, s0, ns, groups; /* prompts: chunks of a sequence (cu NULL), the launch's first chunk slot and their number, sequences times key heads */
 } amdc_gdn_args;
+#define AMDC_GDN_C 64u      /* tokens of a chunk */
+#define AMDC_GDN_VB 25600u  /* bytes of a value head in a chunk slot */
+#define AMDC_GDN_WS (256u << 20) /* bytes of chunk slots that a prompt's launches take at a time, about */
 typedef struct {
   const void *x;
   const float *w, *z, *w2;

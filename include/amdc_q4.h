@@ -377,7 +377,8 @@ int amdc_attn_prefill(const amdc_kv *kv, const void *q, void *y, int t, uint32_t
  * most T in all. A sequence without new tokens takes no part: its slots are not touched. A sequence that only fills up a batch has from
  * and to -1.
  * What only the device sees is checked there: a slot from outside the pool makes the sequence's rows NaN and nothing is written to its
- * slots, a slot to outside the pool is not written, of rows outside 0 .. T none is; amdc_kv_check() reports them all. */
+ * slots, a slot to outside the pool is not written, of a sequence with rows outside 0 .. T no row is (where cu decreases the others'
+ * rows are not to be relied on either); amdc_kv_check() reports them all. */
 typedef struct {
   uint32_t n_seq, n_slots;
   const int32_t *from, *to;

@@ -123,9 +123,9 @@ class Layer:
           u = beta (v - ..): 4 roundings                                                                                     4 u (|v| + n)
           e S + k^T u: 3                                                                                                      3 u (n + |u|), |u| <= |v| + n
         under 48 u n + 8 u |v| with room; the error before it is multiplied by e |I - beta k k^T| <= 1. y: the same once more from q, of
-        |q^| = scale. In chunks the tokens' updates come out of a product with the inverse of a triangular matrix instead (rows of up to `chunk` terms of
-        size up to 1, in parts as well): up to sqrt(chunk) times the rounding of a term, for `chunk` tokens at once: 4 chunk u of
-        the largest |v| + n so far in the chunk more, a token.
+        |q^| = scale. In chunks the tokens' updates come out of a product with the inverse of a triangular matrix instead, and a row of y out of one
+        with a matrix of weights (rows of up to `chunk` terms of size up to 1, in parts of 2 x 11 bits, 2^-22 a part and the product that is left out:
+        12 u a term, of either sign): 12 sqrt(chunk) u of the largest |v| + n so far in the chunk more, a token.
         """
         m = sl.stop - sl.start
         n_k, n_v, dk, dv = self.n_k, self.n_v, self.dk, self.dv
@@ -151,8 +151,8 @@ class Layer:
             S = S + k[t][:, :, None] * u[:, None, :]
             ys[t] = np.einsum("hk,hkd->hd", q[t], S)
             most = np.maximum(most, n + np.abs(v[t]))
-            E = np.exp(g[t])[:, None] * E + U * (48 * n + 8 * np.abs(v[t])) + (4 * chunk * U * most if chunk > 1 else 0)
-            ey[t] = qn * (E + 32 * U * (n + np.abs(u)) + (4 * chunk * U * most if chunk > 1 else 0))
+            E = np.exp(g[t])[:, None] * E + U * (48 * n + 8 * np.abs(v[t])) + (12 * chunk ** 0.5 * U * most if chunk > 1 else 0)
+            ey[t] = qn * (E + 32 * U * (n + np.abs(u)) + (12 * chunk ** 0.5 * U * most if chunk > 1 else 0))
             states.append(S)
             es.append(np.broadcast_to(E[:, None, :], S.shape))
         return ys, ey, states, es
