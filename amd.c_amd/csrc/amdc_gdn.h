@@ -296,8 +296,8 @@ GDN_RECS(64) GDN_RECS(128)
 //
 // All products are on the f16 matrix units with both operands in two parts, x = hi + lo with 11 bits each, and three products, hi hi +
 // hi lo + lo hi, which keeps 22 bits and so f32's accuracy (the errors against 64 bits are those of the recurrence in f32). What f16's
-// range needs: keys, queries, M and A are at most 1 and are multiplied by 2^8; columns of S, R and U by a power of two each, from the
-// column's largest value (S) or a bound of it (R: the largest v plus |S|; U: 64 times that).
+// range needs: M is at most 1 (its parts end at 2^-25, f32's accuracy of the 1s on its diagonal), keys, queries and A are and are multiplied by 2^8;
+// columns of S, R and U by a power of two each, from a bound of the column's values.
 //
 // The operands' k index is permuted so that the results of one product, four rows of a tile in a lane, are the next product's operand in
 // the same lane: place (g, e) of 32, lane group g, element e, is k = 16 (e / 4) + 4 g + e % 4.
@@ -311,7 +311,8 @@ __device__ __forceinline__ h8 join8(h4 a, h4 b) { return (h8){a[0], a[1], a[2], 
 // four values in two parts each
 __device__ __forceinline__ void split4(v4f x, h4 &hi, h4 &lo) {
   hi = __builtin_convertvector(x, h4);
-  lo = __builtin_convertvector(x - __builtin_convertvector(hi, v4f), h4);
+#pragma unroll
+  for (u32 e = 0; e < 4u; e++) lo[e] = (_Float16)__builtin_fmaf((float)hi[e], -1.0f, x[e]);
 }
 __device__ __forceinline__ v4f mfma_f16(h8 a, h8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 // (a[0] + a[1]) (b[0] + b[1]) without the product of the low parts
@@ -330,8 +331,12 @@ __device__ __forceinline__ void pow2_of(float m, float &up, float &down) {
 __device__ __forceinline__ float max4(v4f x) { return __builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(x.x), __builtin_fabsf(x.y)), __builtin_fmaxf(__builtin_fabsf(x.z), __builtin_fabsf(x.w))); }
 // the largest of the four lanes that are 16 apart
 __device__ __forceinline__ float max_groups(float v) {
-  v = __builtin_fmaxf(v, __shfl_xor(v, 16));
-  return __builtin_fmaxf(v, __shfl_xor(v, 32));
+  auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(u32, v), __builtin_bit_cast(u32, v), false, false);
+  u32 x = r[0], y = r[1];
+  v = __builtin_fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+  r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(u32, v), __builtin_bit_cast(u32, v), false, false);
+  x = r[0], y = r[1];
+  return __builtin_fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
 }
 
 // Where chunk slot s (of all sequences', in their order) lies: with cu, sequence b's chunks are the slots cu[b] / 64 + b on, which leaves room for
@@ -347,7 +352,7 @@ __device__ __forceinline__ u32 gdn_seq(const amdc_slots_dev &sl, u32 nc, u32 s) 
 
 // The workspace: a chunk slot holds for every key head its keys, queries and transposed keys as operands (fragments of 1 KB: 16
 // rows, 32 of k, the lanes' 16 bytes in order; two parts each), then for every value head M and A (the 6 fragments that are not all above the
-// diagonal, in parts) and for each token the factors beta, beta e^G, e^G, e^(G_63 - G).
+// diagonal, in parts) and for each token the factors beta, 2^-8 beta e^G, e^G, e^(G_63 - G).
 __device__ __forceinline__ u32 gdn_tri(u32 i, u32 s) { return i < 2u ? i : 2u * (i - 1u) + s; }
 
 template <int TY, u32 DK>
@@ -478,7 +483,7 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
       s_G[w][lane] = G, s_beta[w][lane] = beta;
       const float since = __builtin_expf((float)G), until = __builtin_expf((float)(__shfl(G, 63) - G));
       float *cf = (float *)(wv + 24576u);
-      cf[lane] = beta, cf[64u + lane] = beta * since, cf[128u + lane] = since, cf[192u + lane] = until;
+      cf[lane] = beta, cf[64u + lane] = beta * since * (1.0f / GDN_UP), cf[128u + lane] = since, cf[192u + lane] = until;
     }
     wave_order();
     // L by blocks of 16 x 16, row n, columns 4 gr .. of a block in a lane; A's fragments on the way
@@ -574,7 +579,7 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
       h4 hi[4], lo[4];
 #pragma unroll
       for (u32 j = 0; j < 4u; j++)
-        if (j <= i) split4(M[i * (i + 1u) / 2u + j] * GDN_UP, hi[j], lo[j]);
+        if (j <= i) split4(M[i * (i + 1u) / 2u + j], hi[j], lo[j]);
         else hi[j] = lo[j] = (h4){0, 0, 0, 0};
 #pragma unroll
       for (u32 s = 0; s < (i < 2u ? 1u : 2u); s++) {
@@ -591,11 +596,13 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
 //   R = beta v - beta e^G (K S), and Q S on the way;   U = M R;   y = e^G (Q S) + A U and S = e^(G_63) S + K^T (e^(G_63 - G) U).
 // Wave w has the 16 tokens' rows w of R, U and y, and 32 rows of S (dk = 64: of 16 columns), so that keys, queries, M and A are read once a
 // workgroup, straight into registers, and a chunk ahead; S, R and U go through the LDS, as right operands.
+// A column's R, U and its next S are under 12 max |S| + 65 max |beta v| of the chunk (a token adds at most beta |v| to the column's norm, and the rest of
+// its step shrinks it): the power of two of this bound brings them into f16's range, and as they share it U needs no scaling.
 template <int TY, u32 DK>
 __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
-  constexpr u32 KS = DK / 32u, NS = DK / 64u; // column tiles of S that a wave has
+  constexpr u32 KS = DK / 32u, NS = DK / 64u, ES = TY ? 2u : 4u; // NS: column tiles of S that a wave has
   __shared__ __align__(16) uint8_t s_S[KS * 4096u], s_R[8192], s_U[8192], s_W[8192];
-  __shared__ float s_down[KS][32], s_vmax[2][4][32];
+  __shared__ float s_smax[KS][32], s_vmax[2][4][32];
   const u32 tid = threadIdx.x, lane = tid & 63u, w = uniform(tid >> 6), n = lane & 15u, gr = lane >> 4;
   const u32 nb = (g.dv + 31u) / 32u, per = g.G * nb;
   // the workgroups of a key head are on one XCD (workgroups go round the 8 of them), where the group count allows it
@@ -605,12 +612,13 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     gi = (y / per) * 8u + x, in = y % per;
   } else gi = blockIdx.x / per, in = blockIdx.x % per;
   if (gi >= g.groups) return;
-  const u32 b = gdn_seq(sl, g.nc, g.s0) + gi / g.n_k, hk = gi % g.n_k, v = in / nb, cb = in - v * nb;
+  const u32 b = gdn_seq(sl, g.nc, g.s0) + gi / g.n_k, hk = gi % g.n_k, vh = in / nb, cb = in - vh * nb;
   if (b >= sl.n_seq) return;
   u32 row0;
   const u32 m = uniform(slot_rows(sl, b, row0)), base = uniform(gdn_base(sl, g.nc, b)), all = (m + GDN_C - 1u) / GDN_C, end = g.s0 + g.ns;
+  row0 = uniform(row0);
   if (!m || base >= end || base + all <= g.s0) return;
-  const u32 h = g.tiled ? hk + v * g.n_k : hk * g.G + v;
+  const u32 h = g.tiled ? hk + vh * g.n_k : hk * g.G + vh;
   const u32 c0 = base < g.s0 ? g.s0 - base : 0u, c1 = base + all < end ? all : end - base;
   const u32 ks = DK == 128u ? w : w & 1u, nt0 = DK == 128u ? 0u : w >> 1, na = g.dv >> 4;
   const u64 mat = (u64)DK * g.dv;
@@ -633,36 +641,23 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
           S[t][p][e] = on ? src[((u64)a * DK + 32u * ks + 16u * p + 4u * gr + e) * 16u + n] : bad && !c0 ? nan_() : 0.0f;
         }
   }
-  const auto vload = [&](u32 c, v4f (&x)[2]) { // the values of rows 16 w + 4 gr .. of chunk c
-#pragma unroll
-    for (u32 t = 0; t < 2u; t++)
-#pragma unroll
-      for (u32 e = 0; e < 4u; e++) {
-        const u32 r = c * GDN_C + 16u * w + 4u * gr + e, cl = 32u * cb + 16u * t + n;
-        const bool on = r < m && cl < g.dv;
-        const float y = ld1<TY>(g.v, (u64)(row0 + (r < m ? r : m - 1u)) * g.vs + h * g.dv + (cl < g.dv ? cl : 0u));
-        x[t][e] = on ? y : 0.0f;
-      }
-  };
-  const auto put_S = [&]() { // S as a right operand, its columns' factors
+  const auto put_smax = [&]() {
 #pragma unroll
     for (u32 t = 0; t < NS; t++) {
-      float up, down;
-      pow2_of(max_groups(__builtin_fmaxf(max4(S[t][0]), max4(S[t][1]))), up, down);
+      const float x = max_groups(__builtin_fmaxf(max4(S[t][0]), max4(S[t][1])));
+      if (gr == 0u) s_smax[ks][16u * (nt0 + t) + n] = x;
+    }
+  };
+  const auto put_S = [&](const float(&up)[2]) { // S as a right operand
+#pragma unroll
+    for (u32 t = 0; t < NS; t++) {
+      const float x = NS == 2u ? up[t] : nt0 ? up[1] : up[0];
       h4 hi[2], lo[2];
 #pragma unroll
-      for (u32 p = 0; p < 2u; p++) split4(S[t][p] * up, hi[p], lo[p]);
+      for (u32 p = 0; p < 2u; p++) split4(S[t][p] * x, hi[p], lo[p]);
       uint8_t *f = s_S + 1024u * ((ks * 2u + nt0 + t) * 2u) + 16u * lane;
       *(h8 *)f = join8(hi[0], hi[1]);
       *(h8 *)(f + 1024u) = join8(lo[0], lo[1]);
-      if (gr == 0u) s_down[ks][16u * (nt0 + t) + n] = down;
-    }
-  };
-  const auto put_vmax = [&](const v4f (&x)[2], u32 at) {
-#pragma unroll
-    for (u32 t = 0; t < 2u; t++) {
-      const float y = max_groups(max4(x[t]));
-      if (gr == 0u) s_vmax[at][w][16u * t + n] = y;
     }
   };
   const auto put16 = [&](uint8_t *to, u32 t, v4f x) { // 16 rows of a right operand of 64
@@ -676,19 +671,60 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     const uint8_t *f = from + 1024u * ((s * 2u + t) * 2u) + 16u * lane;
     x[0] = *(const h8 *)f, x[1] = *(const h8 *)(f + 1024u);
   };
-  h8 kf[KS][2], qf[KS][2], tf[2][2][2], mf[2][2], af[2][2];
-  v4f beta, bs, since, until;
+  // what a chunk begins with is loaded while the chunk before it is computed, the rest once the last chunk's has been used
+  struct Head {
+    h8 k[KS][2], q[KS][2];
+    v4f beta, bs, val[2]; // val: the values, then beta times them
+  } even, odd;
+  h8 tf[2][2][2], mf[2][2], af[2][2];
+  v4f since, until;
   float whole = 0.0f;
   const auto chunk_ws = [&](u32 c) { return g.ws + (u64)(base + (c < c1 ? c : c1 - 1u) - g.s0) * g.sb; };
   const auto value_ws = [&](u32 c) { return chunk_ws(c) + (u64)g.n_k * (3u * 64u * DK * 4u) + (u64)h * AMDC_GDN_VB; };
-  const auto load_kq = [&](u32 c) {
+  // rows and columns that are not there are beyond the end of these buffers: loads give 0, stores nothing
+  const auto rows_of = [&](const void *p, u32 c, u32 stride) {
+    const u32 left = c < c1 ? m - c * GDN_C : 0u;
+    return rsrc((const uint8_t *)p + (u64)(row0 + c * GDN_C) * stride * ES, (left < GDN_C ? left : GDN_C) * stride * ES);
+  };
+  u32 voff[4], yoff[4];
+#pragma unroll
+  for (u32 e = 0; e < 4u; e++) {
+    const u32 r = 16u * w + 4u * gr + e, cl = h * g.dv + 32u * cb + n;
+    voff[e] = 32u * cb + n < g.dv ? (r * g.vs + cl) * ES : 0xC0000000u, yoff[e] = 32u * cb + n < g.dv ? (r * g.ys + cl) * ES : 0xC0000000u;
+  }
+  const bool two = 32u * cb + 16u < g.dv;
+  const auto load_head = [&](u32 c, Head &x) {
+    const __amdgpu_buffer_rsrc_t r = rows_of(g.v, c, g.vs);
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++)
+#pragma unroll
+      for (u32 e = 0; e < 4u; e++) {
+        if (t && !two) x.val[t][e] = 0.0f;
+        else if constexpr (TY == 0) x.val[t][e] = __builtin_bit_cast(float, (u32)__builtin_amdgcn_raw_buffer_load_b32(r, voff[e] + 16u * ES * t, 0, 0));
+        else x.val[t][e] = __builtin_bit_cast(float, (u32)__builtin_amdgcn_raw_buffer_load_b16(r, voff[e] + 16u * ES * t, 0, 0));
+      }
     const uint8_t *p = chunk_ws(c) + (u64)hk * (3u * 64u * DK * 4u) + 2048u * KS * w + 16u * lane;
+    const float *cf = (const float *)(value_ws(c) + 24576u) + 16u * w + 4u * gr;
+    x.beta = *(const v4f *)cf, x.bs = *(const v4f *)(cf + 64u);
 #pragma unroll
     for (u32 s = 0; s < KS; s++)
 #pragma unroll
-      for (u32 i = 0; i < 2u; i++) kf[s][i] = *(const h8 *)(p + 1024u * (2u * s + i)), qf[s][i] = *(const h8 *)(p + 64u * DK * 4u + 1024u * (2u * s + i));
-    const float *cf = (const float *)(value_ws(c) + 24576u) + 16u * w + 4u * gr;
-    beta = *(const v4f *)cf, bs = *(const v4f *)(cf + 64u);
+      for (u32 i = 0; i < 2u; i++) x.k[s][i] = *(const h8 *)(p + 1024u * (2u * s + i)), x.q[s][i] = *(const h8 *)(p + 64u * DK * 4u + 1024u * (2u * s + i));
+  };
+  const auto put_vmax = [&](Head &x, u32 at) {
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) {
+      if constexpr (TY != 0)
+#pragma unroll
+        for (u32 e = 0; e < 4u; e++) {
+          const float raw = x.val[t][e];
+          const u32 u = __builtin_bit_cast(u32, raw);
+          x.val[t][e] = TY == 2 ? __builtin_bit_cast(float, u << 16) : h2f(u);
+        }
+      x.val[t] = x.val[t] * x.beta;
+      const float y = max_groups(max4(x.val[t]));
+      if (gr == 0u) s_vmax[at][w][16u * t + n] = y;
+    }
   };
   const auto load_m = [&](u32 c) {
     const uint8_t *p = value_ws(c) + 2048u * gdn_tri(w, 0u) + 16u * lane;
@@ -715,91 +751,127 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     const float *cf = (const float *)(value_ws(c) + 24576u);
     since = *(const v4f *)(cf + 128u + 16u * w + 4u * gr), until = *(const v4f *)(cf + 192u + 16u * w + 4u * gr), whole = cf[128u + 63u];
   };
-
-  v4f val[2];
-  vload(c0, val);
-  load_kq(c0), load_m(c0), load_at(c0);
-  put_S(), put_vmax(val, c0 & 1u);
-  for (u32 c = c0; c < c1; c++) {
-    __syncthreads(); // S is there
-    v4f P[2], Q[2];
+  const auto top_S = [&](u32 t) { // the largest |S| of a column
+    float x = s_smax[0][16u * t + n];
 #pragma unroll
-    for (u32 t = 0; t < 2u; t++) P[t] = Q[t] = splat(0.0f);
-    float top[2] = {0.0f, 0.0f};
+    for (u32 s = 1; s < KS; s++) x = __builtin_fmaxf(x, s_smax[s][16u * t + n]);
+    return x;
+  };
+
+  load_head(c0, even), load_m(c0), load_at(c0);
+  put_smax(), put_vmax(even, c0 & 1u);
+  __syncthreads();
+  float up[2], down_S[2], down[2]; // the factor of R, U and the next S, and the inverses of S's and of that
+#pragma unroll
+  for (u32 t = 0; t < 2u; t++) pow2_of(top_S(t), up[t], down_S[t]);
+  put_S(up);
+  const auto step = [&](u32 c, const Head &now, Head &next) {
+    __syncthreads(); // S is there
+    load_head(c + 1u, next);
+    h8 x[KS][2][2];
 #pragma unroll
     for (u32 s = 0; s < KS; s++)
 #pragma unroll
-      for (u32 t = 0; t < 2u; t++) {
-        h8 x[2];
-        get(s_S, s, t, x);
-        const float down = s_down[s][16u * t + n];
-        top[t] = __builtin_fmaxf(top[t], down);
-        P[t] = fma4(splat(down), mfma3(kf[s], x, splat(0.0f)), P[t]);
-        Q[t] = fma4(splat(down), mfma3(qf[s], x, splat(0.0f)), Q[t]);
-      }
-    float down_R[2], up_U[2], down_U[2];
+      for (u32 t = 0; t < 2u; t++) get(s_S, s, t, x[s][t]);
+    float top[2];
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
       const float(*vm)[32] = s_vmax[c & 1u];
       const float v0 = __builtin_fmaxf(vm[0][16u * t + n], vm[1][16u * t + n]), v1 = __builtin_fmaxf(vm[2][16u * t + n], vm[3][16u * t + n]);
-      // |k S| <= sqrt(dk) times the column's largest value, which is under 2^15 of the factor
-      float up;
-      pow2_of(__builtin_fmaf(12.0f * 32768.0f, top[t], __builtin_fmaxf(v0, v1)), up, down_R[t]);
-      const v4f R = beta * val[t] - bs * (P[t] * (1.0f / GDN_UP));
-      put16(s_R, t, R * up);
-      up_U[t] = up * (1.0f / 64.0f), down_U[t] = down_R[t] * 64.0f;
+      top[t] = __builtin_fmaf(12.0f, top_S(t), 65.0f * __builtin_fmaxf(v0, v1));
     }
-    load_kq(c + 1u);
-    vload(c + 1u < c1 ? c + 1u : c, val);
-    __syncthreads(); // R is there
-    v4f U[2];
+    v4f P[2] = {splat(0.0f), splat(0.0f)}, Q[2] = {splat(0.0f), splat(0.0f)};
+#pragma unroll
+    for (u32 s = 0; s < KS; s++)
+#pragma unroll
+      for (u32 i = 0; i < 3u; i++)
+#pragma unroll
+        for (u32 t = 0; t < 2u; t++) P[t] = mfma_f16(now.k[s][i == 0u], x[s][t][i == 1u], P[t]);
+#pragma unroll
+    for (u32 s = 0; s < KS; s++)
+#pragma unroll
+      for (u32 i = 0; i < 3u; i++)
+#pragma unroll
+        for (u32 t = 0; t < 2u; t++) Q[t] = mfma_f16(now.q[s][i == 0u], x[s][t][i == 1u], Q[t]);
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
-      h8 x[2];
-      get(s_R, 0u, t, x);
-      U[t] = mfma3(mf[0], x, splat(0.0f));
-      if (w >= 2u) {
-        get(s_R, 1u, t, x);
-        U[t] = mfma3(mf[1], x, U[t]);
+      pow2_of(top[t], up[t], down[t]);
+      put16(s_R, t, fma4(-now.bs, P[t] * down_S[t], now.val[t]) * up[t]);
+    }
+    __syncthreads(); // R is there
+    {
+      h8 r[2][2][2];
+      v4f U[2] = {splat(0.0f), splat(0.0f)};
+#pragma unroll
+      for (u32 s = 0; s < 2u; s++)
+        if (s == 0u || w >= 2u) {
+          get(s_R, s, 0u, r[s][0]), get(s_R, s, 1u, r[s][1]);
+#pragma unroll
+          for (u32 i = 0; i < 3u; i++)
+#pragma unroll
+            for (u32 t = 0; t < 2u; t++) U[t] = mfma_f16(mf[s][i == 0u], r[s][t][i == 1u], U[t]);
+        }
+#pragma unroll
+      for (u32 t = 0; t < 2u; t++) {
+        put16(s_W, t, U[t] * until);
+        put16(s_U, t, U[t]);
       }
-      U[t] = U[t] * (down_R[t] * (1.0f / GDN_UP));
-      put16(s_U, t, U[t] * up_U[t]);
-      put16(s_W, t, U[t] * until * up_U[t]);
     }
     load_m(c + 1u);
-    put_vmax(val, c + 1u & 1u);
     __syncthreads(); // U is there
+    v4f y[2] = {splat(0.0f), splat(0.0f)};
+    {
+      h8 r[2][2][2], z[2][NS][2];
+      v4f d[NS][2];
+#pragma unroll
+      for (u32 s = 0; s < 2u; s++)
+#pragma unroll
+        for (u32 t = 0; t < NS; t++) get(s_W, s, nt0 + t, z[s][t]), d[t][0] = d[t][1] = splat(0.0f);
+#pragma unroll
+      for (u32 s = 0; s < 2u; s++)
+        if (s == 0u || w >= 2u) get(s_U, s, 0u, r[s][0]), get(s_U, s, 1u, r[s][1]);
+#pragma unroll
+      for (u32 s = 0; s < 2u; s++)
+#pragma unroll
+        for (u32 i = 0; i < 3u; i++)
+#pragma unroll
+          for (u32 t = 0; t < NS; t++)
+#pragma unroll
+            for (u32 p = 0; p < 2u; p++) d[t][p] = mfma_f16(tf[p][s][i == 0u], z[s][t][i == 1u], d[t][p]);
+#pragma unroll
+      for (u32 s = 0; s < 2u; s++)
+        if (s == 0u || w >= 2u)
+#pragma unroll
+          for (u32 i = 0; i < 3u; i++)
+#pragma unroll
+            for (u32 t = 0; t < 2u; t++) y[t] = mfma_f16(af[s][i == 0u], r[s][t][i == 1u], y[t]);
+#pragma unroll
+      for (u32 t = 0; t < NS; t++) {
+        const float x1 = (NS == 2u ? down[t] : nt0 ? down[1] : down[0]) * (1.0f / GDN_UP);
+#pragma unroll
+        for (u32 p = 0; p < 2u; p++) S[t][p] = fma4(splat(x1), d[t][p], S[t][p] * whole);
+      }
+    }
+    if (c + 1u < c1) put_S(up), put_smax(), put_vmax(next, (c + 1u) & 1u);
+    const __amdgpu_buffer_rsrc_t ry = rows_of(g.y, c, g.ys);
+    const float sc = g.scale * (1.0f / GDN_UP);
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
-      h8 x[2];
-      get(s_U, 0u, t, x);
-      v4f y = mfma3(af[0], x, splat(0.0f));
-      if (w >= 2u) {
-        get(s_U, 1u, t, x);
-        y = mfma3(af[1], x, y);
-      }
-      y = fma4(splat(down_U[t]), y, since * Q[t]) * (g.scale * (1.0f / GDN_UP));
-      const u32 cl = 32u * cb + 16u * t + n;
+      y[t] = fma4(splat(down[t] * sc), y[t], since * (down_S[t] * sc) * Q[t]);
+      down_S[t] = down[t];
+      if (t && !two) break;
 #pragma unroll
       for (u32 e = 0; e < 4u; e++) {
-        const u32 r = c * GDN_C + 16u * w + 4u * gr + e;
-        if (r < m && cl < g.dv) {
-          const u64 o = (u64)(row0 + r) * g.ys + h * g.dv + cl;
-          if constexpr (TY == 0) ((float *)g.y)[o] = y[e];
-          else ((unsigned short *)g.y)[o] = (unsigned short)pack2<TY == 2>(y[e], 0.0f);
-        }
+        const float o = y[t][e];
+        if constexpr (TY == 0) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, o), ry, yoff[e] + 16u * ES * t, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)pack2<TY == 2>(o, 0.0f), ry, yoff[e] + 16u * ES * t, 0, 0);
       }
     }
-#pragma unroll
-    for (u32 t = 0; t < NS; t++) {
-      h8 x[2][2];
-      get(s_W, 0u, nt0 + t, x[0]), get(s_W, 1u, nt0 + t, x[1]);
-      const float down = (NS == 2u ? down_U[t] : nt0 ? down_U[1] : down_U[0]) * (1.0f / GDN_UP);
-#pragma unroll
-      for (u32 p = 0; p < 2u; p++) S[t][p] = fma4(splat(down), mfma3(tf[p][1], x[1], mfma3(tf[p][0], x[0], splat(0.0f))), S[t][p] * whole);
-    }
     load_at(c + 1u);
-    if (c + 1u < c1) put_S();
+  };
+  for (u32 c = c0; c < c1; c += 2u) {
+    step(c, even, odd);
+    if (c + 1u < c1) step(c + 1u, odd, even);
   }
   // the state: into its slot, or for the launch that goes on
   float *dst = g.carry_out + (u64)h * mat;
@@ -825,7 +897,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 
 #define GDN_PRE(H, N, TY)                                                                                                             \
   extern "C" __global__ __launch_bounds__(256) void amdc_gdn_prep_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_prep_body<TY, H##u>(sl, g); }  \
-  extern "C" __global__ __launch_bounds__(256) void amdc_gdn_scan_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_scan_body<TY, H##u>(sl, g); }
+  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void amdc_gdn_scan_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_scan_body<TY, H##u>(sl, g); }
 #define GDN_PRES(H) GDN_PRE(H, f32, 0) GDN_PRE(H, f16, 1) GDN_PRE(H, bf16, 2)
 GDN_PRES(64) GDN_PRES(128)
 

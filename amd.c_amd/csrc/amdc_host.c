@@ -1936,6 +1936,7 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
   int rc = check_slots("gdn_prefill", slots, states, T, cu, 0, &d, &rows);
   if (rc) return rc;
   if ((rc = check_gdn("gdn_prefill", gdn, slots, states, q, k, v, a, b, y, t, rows, qs, ks, vs, as, bs, ys, &g))) return rc;
+  if (vs >= (1u << 23) || ys >= (1u << 23)) return fail(AMDC_EINVAL, "gdn_prefill: strides vs %u, ys %u (under 2^23)", vs, ys); /* 64 rows in a buffer of 2^31 bytes */
   const size_t need = amdc_gdn_prefill_ws(gdn, slots->n_seq, rows);
   if (!ws || !aligned16(ws) || ws_bytes < need) return fail(AMDC_EINVAL, "gdn_prefill: a workspace of %zu bytes (16-byte aligned, at least %zu)", ws ? ws_bytes : (size_t)0, need);
   g.sb = gdn_slot_bytes(gdn), g.nc = (T + AMDC_GDN_C - 1u) / AMDC_GDN_C;

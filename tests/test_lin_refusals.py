@@ -28,7 +28,7 @@ BAD = {
                                              dict(y=8194), dict(y=4096), dict(act=2), dict(act=-1), dict(xs=129), dict(ys=129), dict(each=1, T=17), dict(each=1, cu=4096), dict(cu=4098),
                                              dict(cu=4096, T=(1 << 22) + 1), dict(T=1 << 21, ch=1 << 20, xs=1 << 20, ys=1 << 20))],
     "gdn_decode": GDN_BAD + [(None, dict(T=17)), (None, dict(T=17, each=1))],
-    "gdn_prefill": GDN_BAD + [(None, c) for c in (dict(cu=4098), dict(cu=4096, T=(1 << 22) + 1), dict(ws=None), dict(ws=4104), dict(ws_bytes=15))],
+    "gdn_prefill": GDN_BAD + [(None, c) for c in (dict(cu=4098), dict(cu=4096, T=(1 << 22) + 1), dict(ws=None), dict(ws=4104), dict(ws_bytes=15), dict(vs=1 << 23), dict(ys=1 << 23))],
     "norm_gate_q8": [(None, c) for c in (dict(x=None), dict(w=None), dict(z=None), dict(y=None, q=None), dict(T=0), dict(T=65536), dict(type=3), dict(gate=2), dict(gate=-1), dict(hd=16), dict(hd=96),
                                          dict(hd=512), dict(n_h=0), dict(n_h=4097), dict(x=4097), dict(w=4098), dict(z=8194), dict(y=16386), dict(q=32770), dict(xs=382), dict(xs=385), dict(zs=764),
                                          dict(zs=770), dict(ys=764), dict(ys=769), dict(qs=236), dict(qs=242))],
