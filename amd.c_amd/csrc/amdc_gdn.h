@@ -594,16 +594,17 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
 // The chunks of a sequence one after the other: a workgroup has 32 columns of a head's state (in its registers, as results of the
 // products), and for each chunk three products that wait for each other:
 //   R = beta v - beta e^G (K S), and Q S on the way;   U = M R;   y = e^G (Q S) + A U and S = e^(G_63) S + K^T (e^(G_63 - G) U).
-// Wave w has the 16 tokens' rows w of R, U and y, and 32 rows of S (dk = 64: of 16 columns), so that keys, queries, M and A are read once a
-// workgroup, straight into registers, and a chunk ahead; S, R and U go through the LDS, as right operands.
+// Eight waves, in two roles, two to a SIMD: a wave alone has every wait to itself. Waves 0 to 3 go along that chain for 16 tokens' rows each: R, then U. Waves
+// 4 to 7 have the same rows of y: A U of the last chunk while R is made, Q S while U is. All eight update S, 16 rows of it each (dk = 64: of 16 columns). So keys,
+// queries, M and A are read once a workgroup, straight into registers and a chunk ahead; S, R and U go through the LDS, as right operands.
 // A column's R, U and its next S are under 12 max |S| + 65 max |beta v| of the chunk (a token adds at most beta |v| to the column's norm, and the rest of
 // its step shrinks it): the power of two of this bound brings them into f16's range, and as they share it U needs no scaling.
 template <int TY, u32 DK>
 __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
-  constexpr u32 KS = DK / 32u, NS = DK / 64u, ES = TY ? 2u : 4u; // NS: column tiles of S that a wave has
+  constexpr u32 KS = DK / 32u, NS = DK / 64u, NM = DK / 16u, ES = TY ? 2u : 4u; // NS: column tiles of S that a wave has
   __shared__ __align__(16) uint8_t s_S[KS * 4096u], s_R[8192], s_U[8192], s_W[8192];
-  __shared__ float s_smax[KS][32], s_vmax[2][4][32];
-  const u32 tid = threadIdx.x, lane = tid & 63u, w = uniform(tid >> 6), n = lane & 15u, gr = lane >> 4;
+  __shared__ float s_smax[NM][32], s_vmax[2][4][32];
+  const u32 tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), w = wave & 3u, n = lane & 15u, gr = lane >> 4;
   const u32 nb = (g.dv + 31u) / 32u, per = g.G * nb;
   // the workgroups of a key head are on one XCD (workgroups go round the 8 of them), where the group count allows it
   u32 gi, in;
@@ -620,12 +621,12 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   if (!m || base >= end || base + all <= g.s0) return;
   const u32 h = g.tiled ? hk + vh * g.n_k : hk * g.G + vh;
   const u32 c0 = base < g.s0 ? g.s0 - base : 0u, c1 = base + all < end ? all : end - base;
-  const u32 ks = DK == 128u ? w : w & 1u, nt0 = DK == 128u ? 0u : w >> 1, na = g.dv >> 4;
+  const u32 mt = DK == 128u ? wave : w, nt0 = DK == 128u ? 0u : wave >> 2, na = g.dv >> 4; // S: 16 rows, first column tile
   const u64 mat = (u64)DK * g.dv;
 
   // the state: from the slot, or where the call's launches left off
   bool bad = false;
-  v4f S[NS][2];
+  v4f S[NS];
   {
     const int f = sl.from[b];
     const bool have = slot_ok(sl, f, bad) && c0 == 0u;
@@ -633,51 +634,38 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 #pragma unroll
     for (u32 t = 0; t < NS; t++)
 #pragma unroll
-      for (u32 p = 0; p < 2u; p++)
-#pragma unroll
-        for (u32 e = 0; e < 4u; e++) {
-          const u32 a = 2u * cb + nt0 + t;
-          const bool on = a < na && (have || c0);
-          S[t][p][e] = on ? src[((u64)a * DK + 32u * ks + 16u * p + 4u * gr + e) * 16u + n] : bad && !c0 ? nan_() : 0.0f;
-        }
+      for (u32 e = 0; e < 4u; e++) {
+        const u32 a = 2u * cb + nt0 + t;
+        const bool on = a < na && (have || c0);
+        S[t][e] = on ? src[((u64)a * DK + 16u * mt + 4u * gr + e) * 16u + n] : bad && !c0 ? nan_() : 0.0f;
+      }
   }
   const auto put_smax = [&]() {
 #pragma unroll
     for (u32 t = 0; t < NS; t++) {
-      const float x = max_groups(__builtin_fmaxf(max4(S[t][0]), max4(S[t][1])));
-      if (gr == 0u) s_smax[ks][16u * (nt0 + t) + n] = x;
+      const float x = max_groups(max4(S[t]));
+      if (gr == 0u) s_smax[mt][16u * (nt0 + t) + n] = x;
     }
   };
-  const auto put_S = [&](const float(&up)[2]) { // S as a right operand
-#pragma unroll
-    for (u32 t = 0; t < NS; t++) {
-      const float x = NS == 2u ? up[t] : nt0 ? up[1] : up[0];
-      h4 hi[2], lo[2];
-#pragma unroll
-      for (u32 p = 0; p < 2u; p++) split4(S[t][p] * x, hi[p], lo[p]);
-      uint8_t *f = s_S + 1024u * ((ks * 2u + nt0 + t) * 2u) + 16u * lane;
-      *(h8 *)f = join8(hi[0], hi[1]);
-      *(h8 *)(f + 1024u) = join8(lo[0], lo[1]);
-    }
-  };
-  const auto put16 = [&](uint8_t *to, u32 t, v4f x) { // 16 rows of a right operand of 64
+  const auto put = [&](uint8_t *to, u32 tile, u32 t, v4f x) { // 16 rows of a right operand
     h4 hi, lo;
     split4(x, hi, lo);
-    uint8_t *f = to + 1024u * (((w >> 1) * 2u + t) * 2u) + 16u * lane + 8u * (w & 1u);
+    uint8_t *f = to + 1024u * (((tile >> 1) * 2u + t) * 2u) + 16u * lane + 8u * (tile & 1u);
     *(h4 *)f = hi;
     *(h4 *)(f + 1024u) = lo;
+  };
+  const auto put_S = [&](const float(&up)[2]) {
+#pragma unroll
+    for (u32 t = 0; t < NS; t++) put(s_S, mt, nt0 + t, S[t] * (NS == 2u ? up[t] : nt0 ? up[1] : up[0]));
   };
   const auto get = [&](const uint8_t *from, u32 s, u32 t, h8 (&x)[2]) {
     const uint8_t *f = from + 1024u * ((s * 2u + t) * 2u) + 16u * lane;
     x[0] = *(const h8 *)f, x[1] = *(const h8 *)(f + 1024u);
   };
-  // what a chunk begins with is loaded while the chunk before it is computed, the rest once the last chunk's has been used
-  struct Head {
-    h8 k[KS][2], q[KS][2];
-    v4f beta, bs, val[2]; // val: the values, then beta times them
-  } even, odd;
-  h8 tf[2][2][2], mf[2][2], af[2][2];
-  v4f since, until;
+  // the next chunk's of each is loaded once this one's has been used
+  h8 kq[KS][2], tf[2][2], mf[2][2]; // keys or queries; K^T; M or A
+  v4f beta, bs, val[2];             // val: the values, then beta times them
+  v4f coef; // until or since
   float whole = 0.0f;
   const auto chunk_ws = [&](u32 c) { return g.ws + (u64)(base + (c < c1 ? c : c1 - 1u) - g.s0) * g.sb; };
   const auto value_ws = [&](u32 c) { return chunk_ws(c) + (u64)g.n_k * (3u * 64u * DK * 4u) + (u64)h * AMDC_GDN_VB; };
@@ -693,185 +681,181 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     voff[e] = 32u * cb + n < g.dv ? (r * g.vs + cl) * ES : 0xC0000000u, yoff[e] = 32u * cb + n < g.dv ? (r * g.ys + cl) * ES : 0xC0000000u;
   }
   const bool two = 32u * cb + 16u < g.dv;
-  const auto load_head = [&](u32 c, Head &x) {
+  const auto load_val = [&](u32 c) {
     const __amdgpu_buffer_rsrc_t r = rows_of(g.v, c, g.vs);
 #pragma unroll
     for (u32 t = 0; t < 2u; t++)
 #pragma unroll
       for (u32 e = 0; e < 4u; e++) {
-        if (t && !two) x.val[t][e] = 0.0f;
-        else if constexpr (TY == 0) x.val[t][e] = __builtin_bit_cast(float, (u32)__builtin_amdgcn_raw_buffer_load_b32(r, voff[e] + 16u * ES * t, 0, 0));
-        else x.val[t][e] = __builtin_bit_cast(float, (u32)__builtin_amdgcn_raw_buffer_load_b16(r, voff[e] + 16u * ES * t, 0, 0));
+        if (t && !two) val[t][e] = 0.0f;
+        else if constexpr (TY == 0) val[t][e] = __builtin_bit_cast(float, (u32)__builtin_amdgcn_raw_buffer_load_b32(r, voff[e] + 16u * ES * t, 0, 0));
+        else val[t][e] = __builtin_bit_cast(float, (u32)__builtin_amdgcn_raw_buffer_load_b16(r, voff[e] + 16u * ES * t, 0, 0));
       }
-    const uint8_t *p = chunk_ws(c) + (u64)hk * (3u * 64u * DK * 4u) + 2048u * KS * w + 16u * lane;
     const float *cf = (const float *)(value_ws(c) + 24576u) + 16u * w + 4u * gr;
-    x.beta = *(const v4f *)cf, x.bs = *(const v4f *)(cf + 64u);
+    beta = *(const v4f *)cf, bs = *(const v4f *)(cf + 64u);
+  };
+  const auto load_kq = [&](u32 c, u32 q) {
+    const uint8_t *p = chunk_ws(c) + (u64)hk * (3u * 64u * DK * 4u) + q * (64u * DK * 4u) + 2048u * KS * w + 16u * lane;
 #pragma unroll
     for (u32 s = 0; s < KS; s++)
 #pragma unroll
-      for (u32 i = 0; i < 2u; i++) x.k[s][i] = *(const h8 *)(p + 1024u * (2u * s + i)), x.q[s][i] = *(const h8 *)(p + 64u * DK * 4u + 1024u * (2u * s + i));
+      for (u32 i = 0; i < 2u; i++) kq[s][i] = *(const h8 *)(p + 1024u * (2u * s + i));
   };
-  const auto put_vmax = [&](Head &x, u32 at) {
+  const auto put_vmax = [&](u32 at) {
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
       if constexpr (TY != 0)
 #pragma unroll
         for (u32 e = 0; e < 4u; e++) {
-          const float raw = x.val[t][e];
+          const float raw = val[t][e];
           const u32 u = __builtin_bit_cast(u32, raw);
-          x.val[t][e] = TY == 2 ? __builtin_bit_cast(float, u << 16) : h2f(u);
+          val[t][e] = TY == 2 ? __builtin_bit_cast(float, u << 16) : h2f(u);
         }
-      x.val[t] = x.val[t] * x.beta;
-      const float y = max_groups(max4(x.val[t]));
+      val[t] = val[t] * beta;
+      const float y = max_groups(max4(val[t]));
       if (gr == 0u) s_vmax[at][w][16u * t + n] = y;
     }
   };
-  const auto load_m = [&](u32 c) {
-    const uint8_t *p = value_ws(c) + 2048u * gdn_tri(w, 0u) + 16u * lane;
+  const auto load_ma = [&](u32 c, u32 a) { // M and until, or A and since
+    const uint8_t *p = value_ws(c) + 12288u * a + 2048u * gdn_tri(w, 0u) + 16u * lane;
 #pragma unroll
     for (u32 s = 0; s < 2u; s++)
       if (s == 0u || w >= 2u)
 #pragma unroll
         for (u32 i = 0; i < 2u; i++) mf[s][i] = *(const h8 *)(p + 2048u * s + 1024u * i);
+    coef = *(const v4f *)((const float *)(value_ws(c) + 24576u) + (a ? 128u : 192u) + 16u * w + 4u * gr);
   };
-  const auto load_at = [&](u32 c) {
-    const uint8_t *p = value_ws(c) + 12288u + 2048u * gdn_tri(w, 0u) + 16u * lane;
+  const auto load_t = [&](u32 c) {
+    const uint8_t *p = chunk_ws(c) + (u64)hk * (3u * 64u * DK * 4u) + 2u * 64u * DK * 4u + 4096u * mt + 16u * lane;
 #pragma unroll
     for (u32 s = 0; s < 2u; s++)
-      if (s == 0u || w >= 2u)
 #pragma unroll
-        for (u32 i = 0; i < 2u; i++) af[s][i] = *(const h8 *)(p + 2048u * s + 1024u * i);
-    p = chunk_ws(c) + (u64)hk * (3u * 64u * DK * 4u) + 2u * 64u * DK * 4u + 16u * lane;
-#pragma unroll
-    for (u32 i = 0; i < 2u; i++)
-#pragma unroll
-      for (u32 s = 0; s < 2u; s++)
-#pragma unroll
-        for (u32 j = 0; j < 2u; j++) tf[i][s][j] = *(const h8 *)(p + 1024u * (((2u * ks + i) * 2u + s) * 2u + j));
-    const float *cf = (const float *)(value_ws(c) + 24576u);
-    since = *(const v4f *)(cf + 128u + 16u * w + 4u * gr), until = *(const v4f *)(cf + 192u + 16u * w + 4u * gr), whole = cf[128u + 63u];
+      for (u32 j = 0; j < 2u; j++) tf[s][j] = *(const h8 *)(p + 1024u * (2u * s + j));
+    whole = ((const float *)(value_ws(c) + 24576u))[128u + 63u];
   };
   const auto top_S = [&](u32 t) { // the largest |S| of a column
     float x = s_smax[0][16u * t + n];
 #pragma unroll
-    for (u32 s = 1; s < KS; s++) x = __builtin_fmaxf(x, s_smax[s][16u * t + n]);
+    for (u32 s = 1; s < NM; s++) x = __builtin_fmaxf(x, s_smax[s][16u * t + n]);
     return x;
   };
 
-  load_head(c0, even), load_m(c0), load_at(c0);
-  put_smax(), put_vmax(even, c0 & 1u);
-  __syncthreads();
-  float up[2], down_S[2], down[2]; // the factor of R, U and the next S, and the inverses of S's and of that
+  // 16 rows by the columns of both tiles: three products for each 32 of k
+  const auto times_S = [&](v4f(&o)[2]) {
+    h8 r[KS][2][2];
 #pragma unroll
-  for (u32 t = 0; t < 2u; t++) pow2_of(top_S(t), up[t], down_S[t]);
-  put_S(up);
-  const auto step = [&](u32 c, const Head &now, Head &next) {
-    __syncthreads(); // S is there
-    load_head(c + 1u, next);
-    h8 x[KS][2][2];
+    for (u32 s = 0; s < KS; s++) get(s_S, s, 0u, r[s][0]), get(s_S, s, 1u, r[s][1]);
+    o[0] = o[1] = splat(0.0f);
 #pragma unroll
     for (u32 s = 0; s < KS; s++)
 #pragma unroll
-      for (u32 t = 0; t < 2u; t++) get(s_S, s, t, x[s][t]);
-    float top[2];
+      for (u32 i = 0; i < 3u; i++)
+#pragma unroll
+        for (u32 t = 0; t < 2u; t++) o[t] = mfma_f16(kq[s][i == 0u], r[s][t][i == 1u], o[t]);
+  };
+  const auto times_64 = [&](const uint8_t *from, v4f(&o)[2]) {
+    h8 r[2][2][2];
+    o[0] = o[1] = splat(0.0f);
+#pragma unroll
+    for (u32 s = 0; s < 2u; s++)
+      if (s == 0u || w >= 2u) get(from, s, 0u, r[s][0]), get(from, s, 1u, r[s][1]);
+#pragma unroll
+    for (u32 s = 0; s < 2u; s++)
+      if (s == 0u || w >= 2u)
+#pragma unroll
+        for (u32 i = 0; i < 3u; i++)
+#pragma unroll
+          for (u32 t = 0; t < 2u; t++) o[t] = mfma_f16(mf[s][i == 0u], r[s][t][i == 1u], o[t]);
+  };
+  float up[2], down_S[2], down[2]; // the factor of R, U and the next S, and the inverses of S's and of that
+  const auto factors = [&](u32 c) {
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
       const float(*vm)[32] = s_vmax[c & 1u];
       const float v0 = __builtin_fmaxf(vm[0][16u * t + n], vm[1][16u * t + n]), v1 = __builtin_fmaxf(vm[2][16u * t + n], vm[3][16u * t + n]);
-      top[t] = __builtin_fmaf(12.0f, top_S(t), 65.0f * __builtin_fmaxf(v0, v1));
+      pow2_of(__builtin_fmaf(12.0f, top_S(t), 65.0f * __builtin_fmaxf(v0, v1)), up[t], down[t]);
     }
-    v4f P[2] = {splat(0.0f), splat(0.0f)}, Q[2] = {splat(0.0f), splat(0.0f)};
+  };
+  const auto next_S = [&](u32 c) {
+    h8 z[2][NS][2];
+    v4f d[NS];
 #pragma unroll
-    for (u32 s = 0; s < KS; s++)
+    for (u32 s = 0; s < 2u; s++)
+#pragma unroll
+      for (u32 t = 0; t < NS; t++) get(s_W, s, nt0 + t, z[s][t]), d[t] = splat(0.0f);
+#pragma unroll
+    for (u32 s = 0; s < 2u; s++)
 #pragma unroll
       for (u32 i = 0; i < 3u; i++)
 #pragma unroll
-        for (u32 t = 0; t < 2u; t++) P[t] = mfma_f16(now.k[s][i == 0u], x[s][t][i == 1u], P[t]);
+        for (u32 t = 0; t < NS; t++) d[t] = mfma_f16(tf[s][i == 0u], z[s][t][i == 1u], d[t]);
 #pragma unroll
-    for (u32 s = 0; s < KS; s++)
+    for (u32 t = 0; t < NS; t++) S[t] = fma4(splat((NS == 2u ? down[t] : nt0 ? down[1] : down[0]) * (1.0f / GDN_UP)), d[t], S[t] * whole);
+    load_t(c + 1u);
+    if (c + 1u < c1) put_S(up), put_smax();
+  };
+
+  const bool chain = wave < 4u;
+  if (chain) {
+    load_val(c0), load_kq(c0, 0u), load_ma(c0, 0u), load_t(c0);
+    put_vmax(c0 & 1u);
+  } else load_kq(c0, 1u), load_t(c0);
+  put_smax();
+  __syncthreads();
 #pragma unroll
-      for (u32 i = 0; i < 3u; i++)
+  for (u32 t = 0; t < 2u; t++) pow2_of(top_S(t), up[t], down_S[t]);
+  put_S(up);
+  if (chain) {
+    for (u32 c = c0; c < c1; c++) {
+      __syncthreads(); // S is there
+      v4f P[2];
+      times_S(P);
+      factors(c);
 #pragma unroll
-        for (u32 t = 0; t < 2u; t++) Q[t] = mfma_f16(now.q[s][i == 0u], x[s][t][i == 1u], Q[t]);
+      for (u32 t = 0; t < 2u; t++) put(s_R, w, t, fma4(-bs, P[t] * down_S[t], val[t]) * up[t]), down_S[t] = down[t];
+      load_val(c + 1u), load_kq(c + 1u, 0u);
+      __syncthreads(); // R is there
+      v4f U[2];
+      times_64(s_R, U);
 #pragma unroll
-    for (u32 t = 0; t < 2u; t++) {
-      pow2_of(top[t], up[t], down[t]);
-      put16(s_R, t, fma4(-now.bs, P[t] * down_S[t], now.val[t]) * up[t]);
+      for (u32 t = 0; t < 2u; t++) put(s_W, w, t, U[t] * coef), put(s_U, w, t, U[t]);
+      load_ma(c + 1u, 0u);
+      __syncthreads(); // U is there
+      next_S(c);
+      if (c + 1u < c1) put_vmax((c + 1u) & 1u);
     }
-    __syncthreads(); // R is there
-    {
-      h8 r[2][2][2];
-      v4f U[2] = {splat(0.0f), splat(0.0f)};
-#pragma unroll
-      for (u32 s = 0; s < 2u; s++)
-        if (s == 0u || w >= 2u) {
-          get(s_R, s, 0u, r[s][0]), get(s_R, s, 1u, r[s][1]);
-#pragma unroll
-          for (u32 i = 0; i < 3u; i++)
-#pragma unroll
-            for (u32 t = 0; t < 2u; t++) U[t] = mfma_f16(mf[s][i == 0u], r[s][t][i == 1u], U[t]);
-        }
+  } else {
+    v4f Q[2];
+    const auto result = [&](u32 c) { // y of chunk c
+      v4f y[2];
+      times_64(s_U, y);
+      const __amdgpu_buffer_rsrc_t ry = rows_of(g.y, c, g.ys);
+      const float sc = g.scale * (1.0f / GDN_UP);
 #pragma unroll
       for (u32 t = 0; t < 2u; t++) {
-        put16(s_W, t, U[t] * until);
-        put16(s_U, t, U[t]);
+        y[t] = fma4(splat(down[t] * sc), y[t], coef * (down_S[t] * sc) * Q[t]);
+        down_S[t] = down[t];
+        if (t && !two) break;
+#pragma unroll
+        for (u32 e = 0; e < 4u; e++) {
+          const float o = y[t][e];
+          if constexpr (TY == 0) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, o), ry, yoff[e] + 16u * ES * t, 0, 0);
+          else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)pack2<TY == 2>(o, 0.0f), ry, yoff[e] + 16u * ES * t, 0, 0);
+        }
       }
+    };
+    for (u32 c = c0; c < c1; c++) {
+      __syncthreads(); // S is there
+      if (c != c0) result(c - 1u);
+      load_ma(c, 1u);
+      factors(c);
+      __syncthreads(); // R is there
+      times_S(Q);
+      load_kq(c + 1u, 1u);
+      __syncthreads(); // U is there
+      next_S(c);
     }
-    load_m(c + 1u);
-    __syncthreads(); // U is there
-    v4f y[2] = {splat(0.0f), splat(0.0f)};
-    {
-      h8 r[2][2][2], z[2][NS][2];
-      v4f d[NS][2];
-#pragma unroll
-      for (u32 s = 0; s < 2u; s++)
-#pragma unroll
-        for (u32 t = 0; t < NS; t++) get(s_W, s, nt0 + t, z[s][t]), d[t][0] = d[t][1] = splat(0.0f);
-#pragma unroll
-      for (u32 s = 0; s < 2u; s++)
-        if (s == 0u || w >= 2u) get(s_U, s, 0u, r[s][0]), get(s_U, s, 1u, r[s][1]);
-#pragma unroll
-      for (u32 s = 0; s < 2u; s++)
-#pragma unroll
-        for (u32 i = 0; i < 3u; i++)
-#pragma unroll
-          for (u32 t = 0; t < NS; t++)
-#pragma unroll
-            for (u32 p = 0; p < 2u; p++) d[t][p] = mfma_f16(tf[p][s][i == 0u], z[s][t][i == 1u], d[t][p]);
-#pragma unroll
-      for (u32 s = 0; s < 2u; s++)
-        if (s == 0u || w >= 2u)
-#pragma unroll
-          for (u32 i = 0; i < 3u; i++)
-#pragma unroll
-            for (u32 t = 0; t < 2u; t++) y[t] = mfma_f16(af[s][i == 0u], r[s][t][i == 1u], y[t]);
-#pragma unroll
-      for (u32 t = 0; t < NS; t++) {
-        const float x1 = (NS == 2u ? down[t] : nt0 ? down[1] : down[0]) * (1.0f / GDN_UP);
-#pragma unroll
-        for (u32 p = 0; p < 2u; p++) S[t][p] = fma4(splat(x1), d[t][p], S[t][p] * whole);
-      }
-    }
-    if (c + 1u < c1) put_S(up), put_smax(), put_vmax(next, (c + 1u) & 1u);
-    const __amdgpu_buffer_rsrc_t ry = rows_of(g.y, c, g.ys);
-    const float sc = g.scale * (1.0f / GDN_UP);
-#pragma unroll
-    for (u32 t = 0; t < 2u; t++) {
-      y[t] = fma4(splat(down[t] * sc), y[t], since * (down_S[t] * sc) * Q[t]);
-      down_S[t] = down[t];
-      if (t && !two) break;
-#pragma unroll
-      for (u32 e = 0; e < 4u; e++) {
-        const float o = y[t][e];
-        if constexpr (TY == 0) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, o), ry, yoff[e] + 16u * ES * t, 0, 0);
-        else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)pack2<TY == 2>(o, 0.0f), ry, yoff[e] + 16u * ES * t, 0, 0);
-      }
-    }
-    load_at(c + 1u);
-  };
-  for (u32 c = c0; c < c1; c += 2u) {
-    step(c, even, odd);
-    if (c + 1u < c1) step(c + 1u, odd, even);
+    result(c1 - 1u);
   }
   // the state: into its slot, or for the launch that goes on
   float *dst = g.carry_out + (u64)h * mat;
@@ -889,15 +873,13 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     const u32 a = 2u * cb + nt0 + t;
     if (a < na)
 #pragma unroll
-      for (u32 p = 0; p < 2u; p++)
-#pragma unroll
-        for (u32 e = 0; e < 4u; e++) dst[((u64)a * DK + 32u * ks + 16u * p + 4u * gr + e) * 16u + n] = S[t][p][e];
+      for (u32 e = 0; e < 4u; e++) dst[((u64)a * DK + 16u * mt + 4u * gr + e) * 16u + n] = S[t][e];
   }
 }
 
 #define GDN_PRE(H, N, TY)                                                                                                             \
   extern "C" __global__ __launch_bounds__(256) void amdc_gdn_prep_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_prep_body<TY, H##u>(sl, g); }  \
-  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1, 1))) void amdc_gdn_scan_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_scan_body<TY, H##u>(sl, g); }
+  extern "C" __global__ __launch_bounds__(512) void amdc_gdn_scan_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_scan_body<TY, H##u>(sl, g); }
 #define GDN_PRES(H) GDN_PRE(H, f32, 0) GDN_PRE(H, f16, 1) GDN_PRE(H, bf16, 2)
 GDN_PRES(64) GDN_PRES(128)
 

@@ -1955,7 +1955,7 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
     in = out, out = swap;
     void *args[] = {&d, &g};
     if ((rc = launch(kern, g.ns * g.n_k, 1, 0, stream, args))) return rc;
-    if ((rc = launch(kern + 6, g.groups >= 8u ? (g.groups + 7u) / 8u * 8u * per : g.groups * per, 1, 0, stream, args))) return rc;
+    if ((rc = launch_nt(kern + 6, g.groups >= 8u ? (g.groups + 7u) / 8u * 8u * per : g.groups * per, 1, 512u, 0, stream, args))) return rc;
   }
   return AMDC_OK;
 }
