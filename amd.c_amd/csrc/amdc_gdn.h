@@ -4,7 +4,7 @@
 //   amdc_conv_w{2,3,4}_{f32,f16,bf16}   the causal convolution over the channels, with its state
 //   amdc_gdn_rec_h{64,128}_{f32,f16,bf16}
 //                                       the delta rule, token after token
-//   amdc_gdn_prep_h{64,128}_{f32,f16,bf16}, amdc_gdn_scan_h{64,128}_{f32,f16,bf16}
+//   amdc_gdn_prep_h{64,128}_{f32,f16,bf16}, amdc_gdn_scan_h{64,128}_{f32,f16,bf16,f16_odd,bf16_odd}
 //                                       the delta rule in chunks of 64 tokens: what does not depend on the state, then the states
 //   amdc_norm_gate_{f32,f16,bf16}       the heads' norm times the gate, and the Q8 copy
 //   amdc_norm_res_{1,2,4,8}             norm, residual, norm, and the Q8 copy
@@ -594,16 +594,17 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
 // The chunks of a sequence one after the other: a workgroup has 32 columns of a head's state (in its registers, as results of the
 // products), and for each chunk three products that wait for each other:
 //   R = beta v - beta e^G (K S), and Q S on the way;   U = M R;   y = e^G (Q S) + A U and S = e^(G_63) S + K^T (e^(G_63 - G) U).
-// Eight waves, in two roles, two to a SIMD: a wave alone has every wait to itself. Waves 0 to 3 go along that chain for 16 tokens' rows each: R, then U. Waves
-// 4 to 7 have the same rows of y: A U of the last chunk while R is made, Q S while U is. All eight update S, 16 rows of it each (dk = 64: of 16 columns). So keys,
-// queries, M and A are read once a workgroup, straight into registers and a chunk ahead; S, R and U go through the LDS, as right operands.
+// Eight waves, in two roles, two to a SIMD: a wave alone has every wait to itself. Waves 0 to 3 make R and then U, for 16 tokens' rows each. Waves 4 to 7
+// have 32 rows of S (dk = 64: 16), which they bring on behind U, and 16 rows of y: A U of the last chunk while R is made, Q S while U is. Keys, queries,
+// M and A are read once a workgroup, straight into registers; S, R and U go through the LDS, as right operands.
 // A column's R, U and its next S are under 12 max |S| + 65 max |beta v| of the chunk (a token adds at most beta |v| to the column's norm, and the rest of
 // its step shrinks it): the power of two of this bound brings them into f16's range, and as they share it U needs no scaling.
-template <int TY, u32 DK>
+// PAIR: two values side by side in v and y are aligned to both (32-bit ones need not be).
+template <int TY, u32 DK, bool PAIR>
 __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
-  constexpr u32 KS = DK / 32u, NS = DK / 64u, NM = DK / 16u, ES = TY ? 2u : 4u; // NS: column tiles of S that a wave has
+  constexpr u32 KS = DK / 32u, RT = DK / 64u, ES = TY ? 2u : 4u; // RT: row tiles of S that a wave has
   __shared__ __align__(16) uint8_t s_S[KS * 4096u], s_R[8192], s_U[8192], s_W[8192];
-  __shared__ float s_smax[NM][32], s_vmax[2][4][32];
+  __shared__ __align__(16) float s_smax[4][32], s_vmax[2][4][32], s_cf[4][4][64];
   const u32 tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), w = wave & 3u, n = lane & 15u, gr = lane >> 4;
   const u32 nb = (g.dv + 31u) / 32u, per = g.G * nb;
   // the workgroups of a key head are on one XCD (workgroups go round the 8 of them), where the group count allows it
@@ -621,54 +622,75 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   if (!m || base >= end || base + all <= g.s0) return;
   const u32 h = g.tiled ? hk + vh * g.n_k : hk * g.G + vh;
   const u32 c0 = base < g.s0 ? g.s0 - base : 0u, c1 = base + all < end ? all : end - base;
-  const u32 mt = DK == 128u ? wave : w, nt0 = DK == 128u ? 0u : wave >> 2, na = g.dv >> 4; // S: 16 rows, first column tile
+  const u32 col = 32u * cb + 2u * n; // the lane's columns: this one in the products' first column tile, the next in the second
   const u64 mat = (u64)DK * g.dv;
 
   // the state: from the slot, or where the call's launches left off
+  const bool chain = wave < 4u;
   bool bad = false;
-  v4f S[NS];
-  {
+  v4f S[2][RT];
+  const auto s_at = [&](u32 t, u32 p, u32 e) { return ((u64)((col + t) >> 4) * DK + 16u * (RT * w + p) + 4u * gr + e) * 16u + (col + t & 15u); };
+  if (!chain) {
     const int f = sl.from[b];
     const bool have = slot_ok(sl, f, bad) && c0 == 0u;
     const float *src = have ? g.s + ((u64)(u32)f * g.n_v + h) * mat : g.carry_in + (u64)h * mat;
+    const bool on = col < g.dv && (have || c0);
 #pragma unroll
-    for (u32 t = 0; t < NS; t++)
+    for (u32 t = 0; t < 2u; t++)
 #pragma unroll
-      for (u32 e = 0; e < 4u; e++) {
-        const u32 a = 2u * cb + nt0 + t;
-        const bool on = a < na && (have || c0);
-        S[t][e] = on ? src[((u64)a * DK + 16u * mt + 4u * gr + e) * 16u + n] : bad && !c0 ? nan_() : 0.0f;
-      }
+      for (u32 p = 0; p < RT; p++)
+#pragma unroll
+        for (u32 e = 0; e < 4u; e++) S[t][p][e] = on ? src[s_at(t, p, e)] : bad && !c0 ? nan_() : 0.0f;
   }
   const auto put_smax = [&]() {
 #pragma unroll
-    for (u32 t = 0; t < NS; t++) {
-      const float x = max_groups(max4(S[t]));
-      if (gr == 0u) s_smax[mt][16u * (nt0 + t) + n] = x;
+    for (u32 t = 0; t < 2u; t++) {
+      const float x = max_groups(RT == 2u ? __builtin_fmaxf(max4(S[t][0]), max4(S[t][RT - 1u])) : max4(S[t][0]));
+      if (gr == 0u) s_smax[w][16u * t + n] = x;
     }
   };
-  const auto put = [&](uint8_t *to, u32 tile, u32 t, v4f x) { // 16 rows of a right operand
+  const auto put_S = [&](const float(&up)[2]) { // S as a right operand
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) {
+      h4 hi[RT], lo[RT];
+#pragma unroll
+      for (u32 p = 0; p < RT; p++) split4(S[t][p] * up[t], hi[p], lo[p]);
+      if constexpr (RT == 2u) {
+        uint8_t *f = s_S + 1024u * ((w * 2u + t) * 2u) + 16u * lane;
+        *(h8 *)f = join8(hi[0], hi[1]);
+        *(h8 *)(f + 1024u) = join8(lo[0], lo[1]);
+      } else {
+        uint8_t *f = s_S + 1024u * (((w >> 1) * 2u + t) * 2u) + 16u * lane + 8u * (w & 1u);
+        *(h4 *)f = hi[0];
+        *(h4 *)(f + 1024u) = lo[0];
+      }
+    }
+  };
+  const auto put = [&](uint8_t *to, u32 t, v4f x) { // 16 rows of a right operand of 64
     h4 hi, lo;
     split4(x, hi, lo);
-    uint8_t *f = to + 1024u * (((tile >> 1) * 2u + t) * 2u) + 16u * lane + 8u * (tile & 1u);
+    uint8_t *f = to + 1024u * (((w >> 1) * 2u + t) * 2u) + 16u * lane + 8u * (w & 1u);
     *(h4 *)f = hi;
     *(h4 *)(f + 1024u) = lo;
-  };
-  const auto put_S = [&](const float(&up)[2]) {
-#pragma unroll
-    for (u32 t = 0; t < NS; t++) put(s_S, mt, nt0 + t, S[t] * (NS == 2u ? up[t] : nt0 ? up[1] : up[0]));
   };
   const auto get = [&](const uint8_t *from, u32 s, u32 t, h8 (&x)[2]) {
     const uint8_t *f = from + 1024u * ((s * 2u + t) * 2u) + 16u * lane;
     x[0] = *(const h8 *)f, x[1] = *(const h8 *)(f + 1024u);
   };
-  // the next chunk's of each is loaded once this one's has been used
-  h8 kq[KS][2], tf[2][2], mf[2][2]; // keys or queries; K^T; M or A
-  v4f beta, bs, val[2];             // val: the values, then beta times them
-  v4f coef; // until or since
-  float whole = 0.0f;
-  const auto chunk_ws = [&](u32 c) { return g.ws + (u64)(base + (c < c1 ? c : c1 - 1u) - g.s0) * g.sb; };
-  const auto value_ws = [&](u32 c) { return chunk_ws(c) + (u64)g.n_k * (3u * 64u * DK * 4u) + (u64)h * AMDC_GDN_VB; };
+  // Loads go where they hold up no wave that others wait for: 128 KB a chunk come at 64 bytes a cycle, and a wave whose loads find the queue
+  // full waits. That is behind U for the first four waves, and ahead of U for the others.
+  h8 kq[KS][2], tf[RT][2][2], mf[2][2]; // keys or queries; K^T; M or A
+  v4f raw[2], val[2];                   // the values; beta times them
+  float factor = 0.0f;
+  // a chunk's slot of the workspace (under 2^31 bytes), where key head and value head begin in it, and the lane's 16 bytes of a fragment. A line
+  // of 128 bytes is asked for by one load of the workgroup: a second one while it is on its way would stop the cache until it is there.
+  const auto chunk_ws = [&](u32 c) { return rsrc(g.ws + (u64)(base + (c < c1 ? c : c1 - 1u) - g.s0) * g.sb, (u32)g.sb); };
+  const u32 ok = hk * (3u * 64u * DK * 4u), ov = g.n_k * (3u * 64u * DK * 4u) + h * AMDC_GDN_VB;
+  const auto frag = [&](__amdgpu_buffer_rsrc_t r, u32 at) { return __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(r, 16u * lane, at, 0)); };
+  // the tokens' factors, 64 of each of four kinds: a wave's load each, in the LDS from the chunk before to the one behind
+  const auto load_factor = [&](u32 c) { factor = __builtin_bit_cast(float, (u32)__builtin_amdgcn_raw_buffer_load_b32(chunk_ws(c), 4u * lane, ov + 24576u + 256u * w, 0)); };
+  const auto put_factor = [&](u32 c) { s_cf[c & 3u][w][lane] = factor; };
+  const auto four = [&](u32 c, u32 i) { return *(const v4f *)&s_cf[c & 3u][i][16u * w + 4u * gr]; };
   // rows and columns that are not there are beyond the end of these buffers: loads give 0, stores nothing
   const auto rows_of = [&](const void *p, u32 c, u32 stride) {
     const u32 left = c < c1 ? m - c * GDN_C : 0u;
@@ -677,66 +699,67 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   u32 voff[4], yoff[4];
 #pragma unroll
   for (u32 e = 0; e < 4u; e++) {
-    const u32 r = 16u * w + 4u * gr + e, cl = h * g.dv + 32u * cb + n;
-    voff[e] = 32u * cb + n < g.dv ? (r * g.vs + cl) * ES : 0xC0000000u, yoff[e] = 32u * cb + n < g.dv ? (r * g.ys + cl) * ES : 0xC0000000u;
+    const u32 r = 16u * w + 4u * gr + e;
+    voff[e] = col < g.dv ? (r * g.vs + h * g.dv + col) * ES : 0xC0000000u, yoff[e] = col < g.dv ? (r * g.ys + h * g.dv + col) * ES : 0xC0000000u;
   }
-  const bool two = 32u * cb + 16u < g.dv;
   const auto load_val = [&](u32 c) {
     const __amdgpu_buffer_rsrc_t r = rows_of(g.v, c, g.vs);
 #pragma unroll
-    for (u32 t = 0; t < 2u; t++)
-#pragma unroll
-      for (u32 e = 0; e < 4u; e++) {
-        if (t && !two) val[t][e] = 0.0f;
-        else if constexpr (TY == 0) val[t][e] = __builtin_bit_cast(float, (u32)__builtin_amdgcn_raw_buffer_load_b32(r, voff[e] + 16u * ES * t, 0, 0));
-        else val[t][e] = __builtin_bit_cast(float, (u32)__builtin_amdgcn_raw_buffer_load_b16(r, voff[e] + 16u * ES * t, 0, 0));
-      }
-    const float *cf = (const float *)(value_ws(c) + 24576u) + 16u * w + 4u * gr;
-    beta = *(const v4f *)cf, bs = *(const v4f *)(cf + 64u);
+    for (u32 e = 0; e < 4u; e++) {
+      u32 x, y = 0u;
+      if constexpr (TY == 0) {
+        const u32x2 p = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, voff[e], 0, 0));
+        x = p.x, y = p.y;
+      } else if constexpr (PAIR) x = (u32)__builtin_amdgcn_raw_buffer_load_b32(r, voff[e], 0, 0); // both halves
+      else x = (u32)__builtin_amdgcn_raw_buffer_load_b16(r, voff[e], 0, 0), y = (u32)__builtin_amdgcn_raw_buffer_load_b16(r, voff[e] + 2u, 0, 0);
+      raw[0][e] = __builtin_bit_cast(float, x), raw[1][e] = __builtin_bit_cast(float, y);
+    }
   };
   const auto load_kq = [&](u32 c, u32 q) {
-    const uint8_t *p = chunk_ws(c) + (u64)hk * (3u * 64u * DK * 4u) + q * (64u * DK * 4u) + 2048u * KS * w + 16u * lane;
+    const __amdgpu_buffer_rsrc_t r = chunk_ws(c);
 #pragma unroll
     for (u32 s = 0; s < KS; s++)
 #pragma unroll
-      for (u32 i = 0; i < 2u; i++) kq[s][i] = *(const h8 *)(p + 1024u * (2u * s + i));
+      for (u32 i = 0; i < 2u; i++) kq[s][i] = frag(r, ok + q * (64u * DK * 4u) + 1024u * ((KS * w + s) * 2u + i));
   };
-  const auto put_vmax = [&](u32 at) {
+  const auto put_vmax = [&](u32 c) {
+    const v4f beta = four(c, 0u);
+#pragma unroll
+    for (u32 e = 0; e < 4u; e++) {
+      const float x = raw[0][e], y = raw[1][e];
+      const u32 u = __builtin_bit_cast(u32, x), v = __builtin_bit_cast(u32, y), z = PAIR ? u >> 16 : v;
+      val[0][e] = beta[e] * (TY == 0 ? x : TY == 2 ? __builtin_bit_cast(float, u << 16) : h2f(u));
+      val[1][e] = beta[e] * (TY == 0 ? y : TY == 2 ? __builtin_bit_cast(float, z << 16) : h2f(z));
+    }
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
-      if constexpr (TY != 0)
-#pragma unroll
-        for (u32 e = 0; e < 4u; e++) {
-          const float raw = val[t][e];
-          const u32 u = __builtin_bit_cast(u32, raw);
-          val[t][e] = TY == 2 ? __builtin_bit_cast(float, u << 16) : h2f(u);
-        }
-      val[t] = val[t] * beta;
       const float y = max_groups(max4(val[t]));
-      if (gr == 0u) s_vmax[at][w][16u * t + n] = y;
+      if (gr == 0u) s_vmax[c & 1u][w][16u * t + n] = y;
     }
   };
-  const auto load_ma = [&](u32 c, u32 a) { // M and until, or A and since
-    const uint8_t *p = value_ws(c) + 12288u * a + 2048u * gdn_tri(w, 0u) + 16u * lane;
+  const u32 upper = w < 2u ? 0xC0000000u : 16u * lane; // the fragments above the diagonal are not there: beyond the end, 0
+  const auto load_ma = [&](u32 c, u32 a) { // M or A
+    const __amdgpu_buffer_rsrc_t r = chunk_ws(c);
 #pragma unroll
-    for (u32 s = 0; s < 2u; s++)
-      if (s == 0u || w >= 2u)
-#pragma unroll
-        for (u32 i = 0; i < 2u; i++) mf[s][i] = *(const h8 *)(p + 2048u * s + 1024u * i);
-    coef = *(const v4f *)((const float *)(value_ws(c) + 24576u) + (a ? 128u : 192u) + 16u * w + 4u * gr);
+    for (u32 i = 0; i < 2u; i++) {
+      const u32 at = ov + 12288u * a + 2048u * gdn_tri(w, 0u) + 1024u * i;
+      mf[0][i] = frag(r, at);
+      mf[1][i] = __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(r, upper, at + 2048u, 0));
+    }
   };
   const auto load_t = [&](u32 c) {
-    const uint8_t *p = chunk_ws(c) + (u64)hk * (3u * 64u * DK * 4u) + 2u * 64u * DK * 4u + 4096u * mt + 16u * lane;
+    const __amdgpu_buffer_rsrc_t r = chunk_ws(c);
 #pragma unroll
-    for (u32 s = 0; s < 2u; s++)
+    for (u32 i = 0; i < RT; i++)
 #pragma unroll
-      for (u32 j = 0; j < 2u; j++) tf[s][j] = *(const h8 *)(p + 1024u * (2u * s + j));
-    whole = ((const float *)(value_ws(c) + 24576u))[128u + 63u];
+      for (u32 s = 0; s < 2u; s++)
+#pragma unroll
+        for (u32 j = 0; j < 2u; j++) tf[i][s][j] = frag(r, ok + 2u * 64u * DK * 4u + 1024u * (((RT * w + i) * 2u + s) * 2u + j));
   };
   const auto top_S = [&](u32 t) { // the largest |S| of a column
     float x = s_smax[0][16u * t + n];
 #pragma unroll
-    for (u32 s = 1; s < NM; s++) x = __builtin_fmaxf(x, s_smax[s][16u * t + n]);
+    for (u32 s = 1; s < 4u; s++) x = __builtin_fmaxf(x, s_smax[s][16u * t + n]);
     return x;
   };
 
@@ -744,14 +767,17 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   const auto times_S = [&](v4f(&o)[2]) {
     h8 r[KS][2][2];
 #pragma unroll
-    for (u32 s = 0; s < KS; s++) get(s_S, s, 0u, r[s][0]), get(s_S, s, 1u, r[s][1]);
+    for (u32 s = 0; s < 2u; s++) get(s_S, s, 0u, r[s][0]), get(s_S, s, 1u, r[s][1]);
     o[0] = o[1] = splat(0.0f);
 #pragma unroll
-    for (u32 s = 0; s < KS; s++)
+    for (u32 s = 0; s < KS; s++) {
+      if (s + 2u < KS) get(s_S, s + 2u, 0u, r[s + 2u][0]), get(s_S, s + 2u, 1u, r[s + 2u][1]);
 #pragma unroll
       for (u32 i = 0; i < 3u; i++)
 #pragma unroll
         for (u32 t = 0; t < 2u; t++) o[t] = mfma_f16(kq[s][i == 0u], r[s][t][i == 1u], o[t]);
+      if (s + 1u < KS) __builtin_amdgcn_sched_barrier(0); // not all of S's operands at once: the registers
+    }
   };
   const auto times_64 = [&](const uint8_t *from, v4f(&o)[2]) {
     h8 r[2][2][2];
@@ -776,87 +802,96 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       pow2_of(__builtin_fmaf(12.0f, top_S(t), 65.0f * __builtin_fmaxf(v0, v1)), up[t], down[t]);
     }
   };
-  const auto next_S = [&](u32 c) {
-    h8 z[2][NS][2];
-    v4f d[NS];
-#pragma unroll
-    for (u32 s = 0; s < 2u; s++)
-#pragma unroll
-      for (u32 t = 0; t < NS; t++) get(s_W, s, nt0 + t, z[s][t]), d[t] = splat(0.0f);
-#pragma unroll
-    for (u32 s = 0; s < 2u; s++)
-#pragma unroll
-      for (u32 i = 0; i < 3u; i++)
-#pragma unroll
-        for (u32 t = 0; t < NS; t++) d[t] = mfma_f16(tf[s][i == 0u], z[s][t][i == 1u], d[t]);
-#pragma unroll
-    for (u32 t = 0; t < NS; t++) S[t] = fma4(splat((NS == 2u ? down[t] : nt0 ? down[1] : down[0]) * (1.0f / GDN_UP)), d[t], S[t] * whole);
-    load_t(c + 1u);
-    if (c + 1u < c1) put_S(up), put_smax();
-  };
-
-  const bool chain = wave < 4u;
   if (chain) {
-    load_val(c0), load_kq(c0, 0u), load_ma(c0, 0u), load_t(c0);
-    put_vmax(c0 & 1u);
-  } else load_kq(c0, 1u), load_t(c0);
-  put_smax();
+    load_factor(c0), put_factor(c0), load_factor(c0 + 1u), put_factor(c0 + 1u);
+    load_kq(c0, 0u), load_ma(c0, 0u), load_val(c0);
+  } else put_smax();
   __syncthreads();
 #pragma unroll
   for (u32 t = 0; t < 2u; t++) pow2_of(top_S(t), up[t], down_S[t]);
-  put_S(up);
   if (chain) {
+    put_vmax(c0), load_val(c0 + 1u), load_factor(c0 + 2u);
     for (u32 c = c0; c < c1; c++) {
       __syncthreads(); // S is there
       v4f P[2];
       times_S(P);
       factors(c);
+      const v4f bs = four(c, 1u);
 #pragma unroll
-      for (u32 t = 0; t < 2u; t++) put(s_R, w, t, fma4(-bs, P[t] * down_S[t], val[t]) * up[t]), down_S[t] = down[t];
-      load_val(c + 1u), load_kq(c + 1u, 0u);
+      for (u32 t = 0; t < 2u; t++) put(s_R, t, fma4(-bs, P[t] * down_S[t], val[t]) * up[t]), down_S[t] = down[t];
       __syncthreads(); // R is there
       v4f U[2];
       times_64(s_R, U);
+      const v4f until = four(c, 3u);
 #pragma unroll
-      for (u32 t = 0; t < 2u; t++) put(s_W, w, t, U[t] * coef), put(s_U, w, t, U[t]);
-      load_ma(c + 1u, 0u);
+      for (u32 t = 0; t < 2u; t++) put(s_W, t, U[t] * until), put(s_U, t, U[t]);
+      put_factor(c + 2u);
       __syncthreads(); // U is there
-      next_S(c);
-      if (c + 1u < c1) put_vmax((c + 1u) & 1u);
+      put_vmax(c + 1u);
+      load_kq(c + 1u, 0u), load_ma(c + 1u, 0u), load_factor(c + 3u), load_val(c + 2u);
     }
-  } else {
-    v4f Q[2];
-    const auto result = [&](u32 c) { // y of chunk c
-      v4f y[2];
-      times_64(s_U, y);
-      const __amdgpu_buffer_rsrc_t ry = rows_of(g.y, c, g.ys);
-      const float sc = g.scale * (1.0f / GDN_UP);
-#pragma unroll
-      for (u32 t = 0; t < 2u; t++) {
-        y[t] = fma4(splat(down[t] * sc), y[t], coef * (down_S[t] * sc) * Q[t]);
-        down_S[t] = down[t];
-        if (t && !two) break;
-#pragma unroll
-        for (u32 e = 0; e < 4u; e++) {
-          const float o = y[t][e];
-          if constexpr (TY == 0) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(u32, o), ry, yoff[e] + 16u * ES * t, 0, 0);
-          else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)pack2<TY == 2>(o, 0.0f), ry, yoff[e] + 16u * ES * t, 0, 0);
-        }
-      }
-    };
-    for (u32 c = c0; c < c1; c++) {
-      __syncthreads(); // S is there
-      if (c != c0) result(c - 1u);
-      load_ma(c, 1u);
-      factors(c);
-      __syncthreads(); // R is there
-      times_S(Q);
-      load_kq(c + 1u, 1u);
-      __syncthreads(); // U is there
-      next_S(c);
-    }
-    result(c1 - 1u);
+    return;
   }
+  put_S(up);
+  v4f Q[2];
+  const auto result = [&](u32 c) { // y of chunk c
+    v4f y[2];
+    times_64(s_U, y);
+    const __amdgpu_buffer_rsrc_t ry = rows_of(g.y, c, g.ys);
+    const float sc = g.scale * (1.0f / GDN_UP);
+    const v4f since = four(c, 2u);
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) {
+      y[t] = fma4(splat(down[t] * sc), y[t], since * (down_S[t] * sc) * Q[t]);
+      down_S[t] = down[t];
+    }
+#pragma unroll
+    for (u32 e = 0; e < 4u; e++) {
+      const float o = y[0][e], z = y[1][e];
+      const u32 u = __builtin_bit_cast(u32, o), v = __builtin_bit_cast(u32, z);
+      if constexpr (TY == 0) __builtin_amdgcn_raw_buffer_store_b64((u32x2){u, v}, ry, yoff[e], 0, 0);
+      else {
+        const u32 x = pack2<TY == 2>(o, z);
+        if constexpr (PAIR) __builtin_amdgcn_raw_buffer_store_b32(x, ry, yoff[e], 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)x, ry, yoff[e], 0, 0), __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(x >> 16), ry, yoff[e] + 2u, 0, 0);
+      }
+    }
+  };
+  for (u32 c = c0; c < c1; c++) {
+    __syncthreads(); // S is there
+    load_kq(c, 1u), load_t(c);
+    if (c != c0) result(c - 1u);
+    load_ma(c, 1u);
+    factors(c);
+    __syncthreads(); // R is there
+    times_S(Q);
+    const float whole = s_cf[c & 3u][2][63];
+    __syncthreads(); // U is there
+    h8 z[2][2][2];
+    v4f d[2][RT];
+#pragma unroll
+    for (u32 s = 0; s < 2u; s++)
+#pragma unroll
+      for (u32 t = 0; t < 2u; t++) get(s_W, s, t, z[s][t]);
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++)
+#pragma unroll
+      for (u32 p = 0; p < RT; p++) d[t][p] = splat(0.0f);
+#pragma unroll
+    for (u32 s = 0; s < 2u; s++)
+#pragma unroll
+      for (u32 i = 0; i < 3u; i++)
+#pragma unroll
+        for (u32 t = 0; t < 2u; t++)
+#pragma unroll
+          for (u32 p = 0; p < RT; p++) d[t][p] = mfma_f16(tf[p][s][i == 0u], z[s][t][i == 1u], d[t][p]);
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++)
+#pragma unroll
+      for (u32 p = 0; p < RT; p++) S[t][p] = fma4(splat(down[t] * (1.0f / GDN_UP)), d[t][p], S[t][p] * whole);
+    put_S(up), put_smax();
+  }
+  result(c1 - 1u);
   // the state: into its slot, or for the launch that goes on
   float *dst = g.carry_out + (u64)h * mat;
   bool write = true;
@@ -867,20 +902,22 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     write = slot_ok(sl, o, worse) && start_ok;
     dst = g.s + ((u64)(u32)(o < 0 ? 0 : o) * g.n_v + h) * mat;
   }
-  if (!write) return;
+  if (!write || col >= g.dv) return;
 #pragma unroll
-  for (u32 t = 0; t < NS; t++) {
-    const u32 a = 2u * cb + nt0 + t;
-    if (a < na)
+  for (u32 t = 0; t < 2u; t++)
 #pragma unroll
-      for (u32 e = 0; e < 4u; e++) dst[((u64)a * DK + 16u * mt + 4u * gr + e) * 16u + n] = S[t][e];
-  }
+    for (u32 p = 0; p < RT; p++)
+#pragma unroll
+      for (u32 e = 0; e < 4u; e++) dst[s_at(t, p, e)] = S[t][p][e];
 }
 
-#define GDN_PRE(H, N, TY)                                                                                                             \
-  extern "C" __global__ __launch_bounds__(256) void amdc_gdn_prep_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_prep_body<TY, H##u>(sl, g); }  \
-  extern "C" __global__ __launch_bounds__(512) void amdc_gdn_scan_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_scan_body<TY, H##u>(sl, g); }
-#define GDN_PRES(H) GDN_PRE(H, f32, 0) GDN_PRE(H, f16, 1) GDN_PRE(H, bf16, 2)
+#define GDN_PREP(H, N, TY)                                                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void amdc_gdn_prep_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_prep_body<TY, H##u>(sl, g); }
+#define GDN_SCAN(H, N, TY, PAIR)                                                                                                       \
+  extern "C" __global__ __launch_bounds__(512) void amdc_gdn_scan_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_scan_body<TY, H##u, PAIR>(sl, g); }
+#define GDN_PRES(H)                                                                                                                    \
+  GDN_PREP(H, f32, 0) GDN_PREP(H, f16, 1) GDN_PREP(H, bf16, 2)                                                                         \
+  GDN_SCAN(H, f32, 0, true) GDN_SCAN(H, f16, 1, true) GDN_SCAN(H, bf16, 2, true) GDN_SCAN(H, f16_odd, 1, false) GDN_SCAN(H, bf16_odd, 2, false)
 GDN_PRES(64) GDN_PRES(128)
 
 // ------------------------------------------------------------------ the norms

@@ -296,8 +296,9 @@ enum {
   K_TAKE_FLAG = K_ATTN_JOIN + 3,
   K_CONV, /* amdc_conv_w2_f32, _f16, _bf16, then w3, w4 */
   K_GDN_REC = K_CONV + 9, /* amdc_gdn_rec_h64_f32, _f16, _bf16, then h128 */
-  K_GDN_PRE = K_GDN_REC + 6, /* amdc_gdn_prep_h64_f32, _f16, _bf16, then h128, then amdc_gdn_scan_* */
-  K_NORM_GATE = K_GDN_PRE + 12, /* amdc_norm_gate_f32, _f16, _bf16 */
+  K_GDN_PREP = K_GDN_REC + 6, /* amdc_gdn_prep_h64_f32, _f16, _bf16, then h128 */
+  K_GDN_SCAN = K_GDN_PREP + 6, /* amdc_gdn_scan_h64_f32, _f16, _bf16, _f16_odd, _bf16_odd, then h128 */
+  K_NORM_GATE = K_GDN_SCAN + 10, /* amdc_norm_gate_f32, _f16, _bf16 */
   K_NORM_RES = K_NORM_GATE + 3, /* amdc_norm_res_1, _2, _4, _8 */
   K_N = K_NORM_RES + 4
 };
@@ -339,7 +340,8 @@ static const char *const kname[K_N] = {
     KA("attn_pre_h64"), KA("attn_pre_h128"), KA("attn_pre_h256"),
     KN("attn_join_f32"), KN("attn_join_f16"), KN("attn_join_bf16"), KN("take_flag"),
     KT("conv_w2"), KT("conv_w3"), KT("conv_w4"), KT("gdn_rec_h64"), KT("gdn_rec_h128"), KT("gdn_prep_h64"), KT("gdn_prep_h128"),
-    KT("gdn_scan_h64"), KT("gdn_scan_h128"), KT("norm_gate"),
+    KT("gdn_scan_h64"), KN("gdn_scan_h64_f16_odd"), KN("gdn_scan_h64_bf16_odd"),
+    KT("gdn_scan_h128"), KN("gdn_scan_h128_f16_odd"), KN("gdn_scan_h128_bf16_odd"), KT("norm_gate"),
     KN("norm_res_1"), KN("norm_res_2"), KN("norm_res_4"), KN("norm_res_8")};
 
 static hipModule_t g_mod;
@@ -1891,7 +1893,8 @@ static int check_gdn(const char *op, const amdc_gdn *g, const amdc_slots *sl, fl
   if (y == q || y == k || y == v) return fail(AMDC_EINVAL, "%s: y cannot be q, k or v", op);
   if (rows > 1u && (qs < wk || ks < wk || vs < wv || ys < wv || as < g->n_v || bs < g->n_v))
     return fail(AMDC_EINVAL, "%s: strides qs %u, ks %u, vs %u, as %u, bs %u, ys %u under a row's values (%u, %u, %u)", op, qs, ks, vs, as, bs, ys, wk, wv, g->n_v);
-  const u32 vec = (vec4_rows(v, rows, vs, es) ? 1u : 0u) | (vec4_rows(y, rows, ys, es) ? 2u : 0u) | (vec4_rows(k, rows, ks, es) ? 4u : 0u) | (vec4_rows(q, rows, qs, es) ? 8u : 0u);
+  const u32 vec = (vec4_rows(v, rows, vs, es) ? 1u : 0u) | (vec4_rows(y, rows, ys, es) ? 2u : 0u) | (vec4_rows(k, rows, ks, es) ? 4u : 0u) | (vec4_rows(q, rows, qs, es) ? 8u : 0u) |
+                  (!(((uintptr_t)v | (rows > 1u ? (u64)vs * es : 0u)) & (2u * es - 1u)) ? 16u : 0u) | (!(((uintptr_t)y | (rows > 1u ? (u64)ys * es : 0u)) & (2u * es - 1u)) ? 32u : 0u);
   *d = (amdc_gdn_args){.s = states, .q = q, .k = k, .v = v, .a = a, .b = b, .A = g->A, .dt = g->dt, .y = y, .scale = g->scale, .eps = g->eps, .n_k = g->n_k, .n_v = g->n_v, .dv = g->dv,
                        .G = g->n_v / g->n_k, .tiled = g->order == AMDC_HEADS_TILED, .qs = qs, .ks = ks, .vs = vs, .as = as, .bs = bs, .ys = ys, .vec = vec};
   return AMDC_OK;
@@ -1924,7 +1927,7 @@ static u32 gdn_slots(const amdc_gdn *g, u64 total) {
 
 size_t amdc_gdn_prefill_ws(const amdc_gdn *g, uint32_t n_seq, uint32_t rows) {
   if (!g || !g->n_k || !amdc_gdn_bytes(g->n_v, g->dk, g->dv, 1u) || g->n_v % g->n_k || !n_seq || n_seq > (1u << 20) || !rows || rows > (1u << 22)) return 0;
-  return (size_t)(gdn_slots(g, (u64)rows / AMDC_GDN_C + n_seq) * gdn_slot_bytes(g) + (u64)g->n_v * g->dk * g->dv * 8u);
+  return (size_t)(gdn_slots(g, (u64)rows / AMDC_GDN_C + n_seq) * gdn_slot_bytes(g) + (u64)g->n_v * g->dk * g->dv * 8u + 128u);
 }
 
 int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
@@ -1942,9 +1945,9 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
   g.sb = gdn_slot_bytes(gdn), g.nc = (T + AMDC_GDN_C - 1u) / AMDC_GDN_C;
   const u32 total = cu ? rows / AMDC_GDN_C + slots->n_seq : slots->n_seq * g.nc, most = gdn_slots(gdn, (u64)rows / AMDC_GDN_C + slots->n_seq);
   const u64 state = (u64)gdn->n_v * gdn->dk * gdn->dv;
-  float *in = ws, *out = in + state;
+  float *in = (float *)(((uintptr_t)ws + 127u) & ~(uintptr_t)127u), *out = in + state; /* slots begin with a line */
   g.ws = (uint8_t *)(out + state);
-  const int kern = K_GDN_PRE + (gdn->dk == 128u ? 3 : 0) + t;
+  const int prep = K_GDN_PREP + (gdn->dk == 128u ? 3 : 0) + t, scan = K_GDN_SCAN + (gdn->dk == 128u ? 5 : 0) + (t == AMDC_TYPE_F32 || (g.vec & 16u && g.vec & 32u) ? t : t + 2);
   for (g.s0 = 0; g.s0 < total; g.s0 += most) {
     g.ns = total - g.s0 < most ? total - g.s0 : most;
     /* the sequences with chunks in these slots: one for each slot, and the one that goes on */
@@ -1954,8 +1957,8 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
     float *swap = in;
     in = out, out = swap;
     void *args[] = {&d, &g};
-    if ((rc = launch(kern, g.ns * g.n_k, 1, 0, stream, args))) return rc;
-    if ((rc = launch_nt(kern + 6, g.groups >= 8u ? (g.groups + 7u) / 8u * 8u * per : g.groups * per, 1, 512u, 0, stream, args))) return rc;
+    if ((rc = launch(prep, g.ns * g.n_k, 1, 0, stream, args))) return rc;
+    if ((rc = launch_nt(scan, g.groups >= 8u ? (g.groups + 7u) / 8u * 8u * per : g.groups * per, 1, 512u, 0, stream, args))) return rc;
   }
   return AMDC_OK;
 }

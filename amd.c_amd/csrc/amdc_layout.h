@@ -166,7 +166,7 @@ typedef struct {
   uint64_t sb;  /* prompts: bytes of a chunk slot of the workspace */
   float scale, eps;
   uint32_t n_k, n_v, dv, G /* n_v / n_k */, tiled, qs, ks, vs, as, bs, ys;
-  uint32_t vec; /* rows that are aligned to four values: 1 v, 2 y, 4 k, 8 q */
+  uint32_t vec; /* rows that are aligned to four values: 1 v, 2 y, 4 k, 8 q; to two: 16 v, 32 y */
   uint32_t nc, s0, ns, groups; /* prompts: chunks of a sequence (cu NULL), the launch's first chunk slot and their number, sequences times key heads */
 } amdc_gdn_args;
 #define AMDC_GDN_C 64u      /* tokens of a chunk */
