@@ -747,14 +747,13 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       mf[1][i] = __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(r, upper, at + 2048u, 0));
     }
   };
-  const auto load_t = [&](u32 c) {
+  const auto load_t = [&](u32 c, u32 k) { // part k of KS
     const __amdgpu_buffer_rsrc_t r = chunk_ws(c);
 #pragma unroll
-    for (u32 i = 0; i < RT; i++)
-#pragma unroll
-      for (u32 s = 0; s < 2u; s++)
-#pragma unroll
-        for (u32 j = 0; j < 2u; j++) tf[i][s][j] = frag(r, ok + 2u * 64u * DK * 4u + 1024u * (((RT * w + i) * 2u + s) * 2u + j));
+    for (u32 j = 0; j < 2u; j++) {
+      const u32 i = RT == 2u ? k >> 1 : 0u, s = k & 1u;
+      tf[i][s][j] = frag(r, ok + 2u * 64u * DK * 4u + 1024u * (((RT * w + i) * 2u + s) * 2u + j));
+    }
   };
   const auto top_S = [&](u32 t) { // the largest |S| of a column
     float x = s_smax[0][16u * t + n];
@@ -764,7 +763,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   };
 
   // 16 rows by the columns of both tiles: three products for each 32 of k
-  const auto times_S = [&](v4f(&o)[2]) {
+  const auto times_S = [&](v4f(&o)[2], auto between) {
     h8 r[KS][2][2];
 #pragma unroll
     for (u32 s = 0; s < 2u; s++) get(s_S, s, 0u, r[s][0]), get(s_S, s, 1u, r[s][1]);
@@ -776,6 +775,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       for (u32 i = 0; i < 3u; i++)
 #pragma unroll
         for (u32 t = 0; t < 2u; t++) o[t] = mfma_f16(kq[s][i == 0u], r[s][t][i == 1u], o[t]);
+      between(s);
       if (s + 1u < KS) __builtin_amdgcn_sched_barrier(0); // not all of S's operands at once: the registers
     }
   };
@@ -813,10 +813,10 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     put_vmax(c0), load_val(c0 + 1u), load_factor(c0 + 2u);
     for (u32 c = c0; c < c1; c++) {
       __syncthreads(); // S is there
-      v4f P[2];
-      times_S(P);
       factors(c);
       const v4f bs = four(c, 1u);
+      v4f P[2];
+      times_S(P, [](u32) {});
 #pragma unroll
       for (u32 t = 0; t < 2u; t++) put(s_R, t, fma4(-bs, P[t] * down_S[t], val[t]) * up[t]), down_S[t] = down[t];
       __syncthreads(); // R is there
@@ -827,8 +827,9 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       for (u32 t = 0; t < 2u; t++) put(s_W, t, U[t] * until), put(s_U, t, U[t]);
       put_factor(c + 2u);
       __syncthreads(); // U is there
+      load_kq(c + 1u, 0u), load_ma(c + 1u, 0u), load_factor(c + 3u);
       put_vmax(c + 1u);
-      load_kq(c + 1u, 0u), load_ma(c + 1u, 0u), load_factor(c + 3u), load_val(c + 2u);
+      load_val(c + 2u);
     }
     return;
   }
@@ -859,12 +860,12 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   };
   for (u32 c = c0; c < c1; c++) {
     __syncthreads(); // S is there
-    load_kq(c, 1u), load_t(c);
+    load_kq(c, 1u);
     if (c != c0) result(c - 1u);
     load_ma(c, 1u);
     factors(c);
     __syncthreads(); // R is there
-    times_S(Q);
+    times_S(Q, [&](u32 s) { load_t(c, s); });
     const float whole = s_cf[c & 3u][2][63];
     __syncthreads(); // U is there
     h8 z[2][2][2];
