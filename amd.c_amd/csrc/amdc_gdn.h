@@ -322,10 +322,10 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
-// The power of two that brings values of up to m under 2^15, and its inverse. Both are normal: of values under 2^-104 fewer bits are kept.
+// The power of two that brings values of up to m under 2^7, and its inverse. Both are normal: of values under 2^-112 fewer bits are kept.
 __device__ __forceinline__ void pow2_of(float m, float &up, float &down) {
   const u32 e = __builtin_bit_cast(u32, m) >> 23 & 255u;
-  const u32 f = 268u - e < 246u ? 268u - e : 246u;
+  const u32 f = 260u - e < 246u ? 260u - e : 246u;
   up = __builtin_bit_cast(float, f << 23), down = __builtin_bit_cast(float, (254u - f) << 23);
 }
 __device__ __forceinline__ float max4(v4f x) { return __builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(x.x), __builtin_fabsf(x.y)), __builtin_fmaxf(__builtin_fabsf(x.z), __builtin_fabsf(x.w))); }
@@ -594,16 +594,17 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
 // The chunks of a sequence one after the other: a workgroup has 32 columns of a head's state (in its registers, as results of the
 // products), and for each chunk three products that wait for each other:
 //   R = beta v - beta e^G (K S), and Q S on the way;   U = M R;   y = e^G (Q S) + A U and S = e^(G_63) S + K^T (e^(G_63 - G) U).
-// Eight waves, in two roles, two to a SIMD: a wave alone has every wait to itself. Waves 0 to 3 make R and then U, for 16 tokens' rows each. Waves 4 to 7
-// have 32 rows of S (dk = 64: 16), which they bring on behind U, and 16 rows of y: A U of the last chunk while R is made, Q S while U is. Keys, queries,
-// M and A are read once a workgroup, straight into registers; S, R and U go through the LDS, as right operands.
+// Eight waves, in two roles, two to a SIMD: a wave alone has every wait to itself. Waves 0 to 3 have 16 tokens' rows each: they make R, then U, and y while the
+// others bring S on. Waves 4 to 7 have 32 rows of S (dk = 64: 16), and of Q S what 16 tokens need, which they make beside U. Keys, queries, M and A are read
+// once a workgroup, straight into registers; S, R, U and Q S go through the LDS.
 // A column's R, U and its next S are under 12 max |S| + 65 max |beta v| of the chunk (a token adds at most beta |v| to the column's norm, and the rest of
-// its step shrinks it): the power of two of this bound brings them into f16's range, and as they share it U needs no scaling.
+// its step shrinks it): the power of two of this bound brings them into f16's range, and as they share it U needs no scaling. S is kept as
+// 2^8 times that, as the products with K^T give it: they add to it.
 // PAIR: two values side by side in v and y are aligned to both (32-bit ones need not be).
 template <int TY, u32 DK, bool PAIR>
 __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
   constexpr u32 KS = DK / 32u, RT = DK / 64u, ES = TY ? 2u : 4u; // RT: row tiles of S that a wave has
-  __shared__ __align__(16) uint8_t s_S[KS * 4096u], s_R[8192], s_U[8192], s_W[8192];
+  __shared__ __align__(16) uint8_t s_S[KS * 4096u], s_R[8192], s_U[8192], s_W[8192], s_Q[8192];
   __shared__ __align__(16) float s_smax[4][32], s_vmax[2][4][32], s_cf[4][4][64];
   const u32 tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), w = wave & 3u, n = lane & 15u, gr = lane >> 4;
   const u32 nb = (g.dv + 31u) / 32u, per = g.G * nb;
@@ -642,19 +643,19 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 #pragma unroll
         for (u32 e = 0; e < 4u; e++) S[t][p][e] = on ? src[s_at(t, p, e)] : bad && !c0 ? nan_() : 0.0f;
   }
-  const auto put_smax = [&]() {
+  const auto put_smax = [&](const float(&by)[2]) {
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
       const float x = max_groups(RT == 2u ? __builtin_fmaxf(max4(S[t][0]), max4(S[t][RT - 1u])) : max4(S[t][0]));
-      if (gr == 0u) s_smax[w][16u * t + n] = x;
+      if (gr == 0u) s_smax[w][16u * t + n] = x * by[t];
     }
   };
-  const auto put_S = [&](const float(&up)[2]) { // S as a right operand
+  const auto put_S = [&]() { // S as a right operand
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
       h4 hi[RT], lo[RT];
 #pragma unroll
-      for (u32 p = 0; p < RT; p++) split4(S[t][p] * up[t], hi[p], lo[p]);
+      for (u32 p = 0; p < RT; p++) split4(S[t][p], hi[p], lo[p]);
       if constexpr (RT == 2u) {
         uint8_t *f = s_S + 1024u * ((w * 2u + t) * 2u) + 16u * lane;
         *(h8 *)f = join8(hi[0], hi[1]);
@@ -679,7 +680,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   };
   // Loads go where they hold up no wave that others wait for: 128 KB a chunk come at 64 bytes a cycle, and a wave whose loads find the queue
   // full waits. That is behind U for the first four waves, and ahead of U for the others.
-  h8 kq[KS][2], tf[RT][2][2], mf[2][2]; // keys or queries; K^T; M or A
+  h8 kq[KS][2], tf[RT][2][2], mf[2][2], af[2][2]; // keys or queries; K^T; M; A
   v4f raw[2], val[2];                   // the values; beta times them
   float factor = 0.0f;
   // a chunk's slot of the workspace (under 2^31 bytes), where key head and value head begin in it, and the lane's 16 bytes of a fragment. A line
@@ -715,12 +716,10 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       raw[0][e] = __builtin_bit_cast(float, x), raw[1][e] = __builtin_bit_cast(float, y);
     }
   };
-  const auto load_kq = [&](u32 c, u32 q) {
+  const auto load_kq = [&](u32 c, u32 q, u32 s) { // the part along 32 of dk
     const __amdgpu_buffer_rsrc_t r = chunk_ws(c);
 #pragma unroll
-    for (u32 s = 0; s < KS; s++)
-#pragma unroll
-      for (u32 i = 0; i < 2u; i++) kq[s][i] = frag(r, ok + q * (64u * DK * 4u) + 1024u * ((KS * w + s) * 2u + i));
+    for (u32 i = 0; i < 2u; i++) kq[s][i] = frag(r, ok + q * (64u * DK * 4u) + 1024u * ((KS * w + s) * 2u + i));
   };
   const auto put_vmax = [&](u32 c) {
     const v4f beta = four(c, 0u);
@@ -737,23 +736,34 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       if (gr == 0u) s_vmax[c & 1u][w][16u * t + n] = y;
     }
   };
+  // A line from the memory takes as long as half a chunk. So each of the workgroups that share a key head (per of them) or a value head (nb)
+  // asks for its part of a chunk two ahead, a line to a lane, which brings it into the L2.
+  u32 ahead = 0u;
+  const u32 lines_k = (3u * 64u * DK * 4u / 128u + per - 1u) / per, lines_v = (AMDC_GDN_VB / 128u + nb - 1u) / nb;
+  const auto prefetch = [&](u32 c) {
+    const bool keys = w == 0u;
+    const u32 i = 64u * (keys ? 0u : w - 1u) + lane, lines = keys ? lines_k : lines_v, at = (keys ? in : cb) * lines + i;
+    const u32 off = c < c1 && i < lines && at < (keys ? 3u * 64u * DK * 4u : AMDC_GDN_VB) / 128u ? (keys ? ok : ov) + 128u * at : 0xC0000000u;
+    ahead = (u32)__builtin_amdgcn_raw_buffer_load_b32(chunk_ws(c), off, 0, 0);
+  };
   const u32 upper = w < 2u ? 0xC0000000u : 16u * lane; // the fragments above the diagonal are not there: beyond the end, 0
-  const auto load_ma = [&](u32 c, u32 a) { // M or A
+  const auto load_ma = [&](u32 c, u32 a, h8(&x)[2][2]) { // M or A
     const __amdgpu_buffer_rsrc_t r = chunk_ws(c);
 #pragma unroll
     for (u32 i = 0; i < 2u; i++) {
       const u32 at = ov + 12288u * a + 2048u * gdn_tri(w, 0u) + 1024u * i;
-      mf[0][i] = frag(r, at);
-      mf[1][i] = __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(r, upper, at + 2048u, 0));
+      x[0][i] = frag(r, at);
+      x[1][i] = __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(r, upper, at + 2048u, 0));
     }
   };
-  const auto load_t = [&](u32 c, u32 k) { // part k of KS
+  const auto load_t = [&](u32 c) {
     const __amdgpu_buffer_rsrc_t r = chunk_ws(c);
 #pragma unroll
-    for (u32 j = 0; j < 2u; j++) {
-      const u32 i = RT == 2u ? k >> 1 : 0u, s = k & 1u;
-      tf[i][s][j] = frag(r, ok + 2u * 64u * DK * 4u + 1024u * (((RT * w + i) * 2u + s) * 2u + j));
-    }
+    for (u32 s = 0; s < 2u; s++)
+#pragma unroll
+      for (u32 i = 0; i < RT; i++)
+#pragma unroll
+        for (u32 j = 0; j < 2u; j++) tf[i][s][j] = frag(r, ok + 2u * 64u * DK * 4u + 1024u * (((RT * w + i) * 2u + s) * 2u + j));
   };
   const auto top_S = [&](u32 t) { // the largest |S| of a column
     float x = s_smax[0][16u * t + n];
@@ -763,7 +773,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   };
 
   // 16 rows by the columns of both tiles: three products for each 32 of k
-  const auto times_S = [&](v4f(&o)[2], auto between) {
+  const auto times_S = [&](v4f(&o)[2]) {
     h8 r[KS][2][2];
 #pragma unroll
     for (u32 s = 0; s < 2u; s++) get(s_S, s, 0u, r[s][0]), get(s_S, s, 1u, r[s][1]);
@@ -775,11 +785,10 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       for (u32 i = 0; i < 3u; i++)
 #pragma unroll
         for (u32 t = 0; t < 2u; t++) o[t] = mfma_f16(kq[s][i == 0u], r[s][t][i == 1u], o[t]);
-      between(s);
       if (s + 1u < KS) __builtin_amdgcn_sched_barrier(0); // not all of S's operands at once: the registers
     }
   };
-  const auto times_64 = [&](const uint8_t *from, v4f(&o)[2]) {
+  const auto times_64 = [&](const h8(&f)[2][2], const uint8_t *from, v4f(&o)[2]) {
     h8 r[2][2][2];
     o[0] = o[1] = splat(0.0f);
 #pragma unroll
@@ -791,7 +800,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 #pragma unroll
         for (u32 i = 0; i < 3u; i++)
 #pragma unroll
-          for (u32 t = 0; t < 2u; t++) o[t] = mfma_f16(mf[s][i == 0u], r[s][t][i == 1u], o[t]);
+          for (u32 t = 0; t < 2u; t++) o[t] = mfma_f16(f[s][i == 0u], r[s][t][i == 1u], o[t]);
   };
   float up[2], down_S[2], down[2]; // the factor of R, U and the next S, and the inverses of S's and of that
   const auto factors = [&](u32 c) {
@@ -804,8 +813,13 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   };
   if (chain) {
     load_factor(c0), put_factor(c0), load_factor(c0 + 1u), put_factor(c0 + 1u);
-    load_kq(c0, 0u), load_ma(c0, 0u), load_val(c0);
-  } else put_smax();
+#pragma unroll
+    for (u32 s = 0; s < KS; s++) load_kq(c0, 0u, s);
+    load_ma(c0, 0u, mf), load_ma(c0, 1u, af), load_val(c0);
+  } else {
+    const float one[2] = {1.0f, 1.0f};
+    put_smax(one);
+  }
   __syncthreads();
 #pragma unroll
   for (u32 t = 0; t < 2u; t++) pow2_of(top_S(t), up[t], down_S[t]);
@@ -816,68 +830,82 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       factors(c);
       const v4f bs = four(c, 1u);
       v4f P[2];
-      times_S(P, [](u32) {});
+      times_S(P);
 #pragma unroll
-      for (u32 t = 0; t < 2u; t++) put(s_R, t, fma4(-bs, P[t] * down_S[t], val[t]) * up[t]), down_S[t] = down[t];
+      for (u32 t = 0; t < 2u; t++) put(s_R, t, fma4(-bs, P[t] * (down_S[t] * (1.0f / GDN_UP)), val[t]) * up[t]);
       __syncthreads(); // R is there
       v4f U[2];
-      times_64(s_R, U);
+      times_64(mf, s_R, U);
+      load_kq(c + 1u, 0u, 0u);
       const v4f until = four(c, 3u);
 #pragma unroll
-      for (u32 t = 0; t < 2u; t++) put(s_W, t, U[t] * until), put(s_U, t, U[t]);
+      for (u32 t = 0; t < 2u; t++) {
+        put(s_W, t, U[t] * until);
+        if (t == 0u || KS == 4u) load_kq(c + 1u, 0u, 1u + t); // a load takes its time: between the others
+        put(s_U, t, U[t]);
+        if (t == 0u && KS == 4u) load_kq(c + 1u, 0u, KS - 1u);
+      }
       put_factor(c + 2u);
-      __syncthreads(); // U is there
-      load_kq(c + 1u, 0u), load_ma(c + 1u, 0u), load_factor(c + 3u);
+      __syncthreads(); // U and Q S are there
+      load_ma(c + 1u, 0u, mf), load_factor(c + 3u);
       put_vmax(c + 1u);
-      load_val(c + 2u);
+      asm volatile("" ::"v"(ahead));
+      load_val(c + 2u), prefetch(c + 2u);
+      v4f y[2];
+      times_64(af, s_U, y);
+      load_ma(c + 1u, 1u, af);
+      const __amdgpu_buffer_rsrc_t ry = rows_of(g.y, c, g.ys);
+      const float sc = g.scale * (1.0f / GDN_UP);
+      const v4f since = four(c, 2u);
+#pragma unroll
+      for (u32 t = 0; t < 2u; t++) {
+        const v4f q = *(const v4f *)(s_Q + 2048u * w + 1024u * t + 16u * lane);
+        y[t] = fma4(splat(down[t] * sc), y[t], since * (down_S[t] * sc * (1.0f / GDN_UP)) * q);
+        down_S[t] = down[t];
+      }
+#pragma unroll
+      for (u32 e = 0; e < 4u; e++) {
+        const float o = y[0][e], z = y[1][e];
+        const u32 u = __builtin_bit_cast(u32, o), v = __builtin_bit_cast(u32, z);
+        if constexpr (TY == 0) __builtin_amdgcn_raw_buffer_store_b64((u32x2){u, v}, ry, yoff[e], 0, 0);
+        else {
+          const u32 x = pack2<TY == 2>(o, z);
+          if constexpr (PAIR) __builtin_amdgcn_raw_buffer_store_b32(x, ry, yoff[e], 0, 0);
+          else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)x, ry, yoff[e], 0, 0), __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(x >> 16), ry, yoff[e] + 2u, 0, 0);
+        }
+      }
     }
     return;
   }
-  put_S(up);
-  v4f Q[2];
-  const auto result = [&](u32 c) { // y of chunk c
-    v4f y[2];
-    times_64(s_U, y);
-    const __amdgpu_buffer_rsrc_t ry = rows_of(g.y, c, g.ys);
-    const float sc = g.scale * (1.0f / GDN_UP);
-    const v4f since = four(c, 2u);
 #pragma unroll
-    for (u32 t = 0; t < 2u; t++) {
-      y[t] = fma4(splat(down[t] * sc), y[t], since * (down_S[t] * sc) * Q[t]);
-      down_S[t] = down[t];
-    }
+  for (u32 t = 0; t < 2u; t++)
 #pragma unroll
-    for (u32 e = 0; e < 4u; e++) {
-      const float o = y[0][e], z = y[1][e];
-      const u32 u = __builtin_bit_cast(u32, o), v = __builtin_bit_cast(u32, z);
-      if constexpr (TY == 0) __builtin_amdgcn_raw_buffer_store_b64((u32x2){u, v}, ry, yoff[e], 0, 0);
-      else {
-        const u32 x = pack2<TY == 2>(o, z);
-        if constexpr (PAIR) __builtin_amdgcn_raw_buffer_store_b32(x, ry, yoff[e], 0, 0);
-        else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)x, ry, yoff[e], 0, 0), __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(x >> 16), ry, yoff[e] + 2u, 0, 0);
-      }
-    }
-  };
+    for (u32 p = 0; p < RT; p++) S[t][p] *= up[t] * GDN_UP;
+  put_S();
   for (u32 c = c0; c < c1; c++) {
     __syncthreads(); // S is there
-    load_kq(c, 1u);
-    if (c != c0) result(c - 1u);
-    load_ma(c, 1u);
+#pragma unroll
+    for (u32 s = 0; s < KS; s++) load_kq(c, 1u, s);
+    load_t(c);
     factors(c);
-    __syncthreads(); // R is there
-    times_S(Q, [&](u32 s) { load_t(c, s); });
     const float whole = s_cf[c & 3u][2][63];
-    __syncthreads(); // U is there
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) {
+#pragma unroll
+      for (u32 p = 0; p < RT; p++) S[t][p] = S[t][p] * down_S[t] * whole * up[t];
+      down_S[t] = down[t];
+    }
+    __syncthreads(); // R is there
+    v4f Q[2];
+    times_S(Q);
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++) *(v4f *)(s_Q + 2048u * w + 1024u * t + 16u * lane) = Q[t];
+    __syncthreads(); // U and Q S are there
     h8 z[2][2][2];
-    v4f d[2][RT];
 #pragma unroll
     for (u32 s = 0; s < 2u; s++)
 #pragma unroll
       for (u32 t = 0; t < 2u; t++) get(s_W, s, t, z[s][t]);
-#pragma unroll
-    for (u32 t = 0; t < 2u; t++)
-#pragma unroll
-      for (u32 p = 0; p < RT; p++) d[t][p] = splat(0.0f);
 #pragma unroll
     for (u32 s = 0; s < 2u; s++)
 #pragma unroll
@@ -885,14 +913,11 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 #pragma unroll
         for (u32 t = 0; t < 2u; t++)
 #pragma unroll
-          for (u32 p = 0; p < RT; p++) d[t][p] = mfma_f16(tf[p][s][i == 0u], z[s][t][i == 1u], d[t][p]);
-#pragma unroll
-    for (u32 t = 0; t < 2u; t++)
-#pragma unroll
-      for (u32 p = 0; p < RT; p++) S[t][p] = fma4(splat(down[t] * (1.0f / GDN_UP)), d[t][p], S[t][p] * whole);
-    put_S(up), put_smax();
+          for (u32 p = 0; p < RT; p++) S[t][p] = mfma_f16(tf[p][s][i == 0u], z[s][t][i == 1u], S[t][p]);
+    put_S();
+    const float by[2] = {down[0] * (1.0f / GDN_UP), down[1] * (1.0f / GDN_UP)};
+    put_smax(by);
   }
-  result(c1 - 1u);
   // the state: into its slot, or for the launch that goes on
   float *dst = g.carry_out + (u64)h * mat;
   bool write = true;
@@ -909,7 +934,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 #pragma unroll
     for (u32 p = 0; p < RT; p++)
 #pragma unroll
-      for (u32 e = 0; e < 4u; e++) dst[s_at(t, p, e)] = S[t][p][e];
+      for (u32 e = 0; e < 4u; e++) dst[s_at(t, p, e)] = S[t][p][e] * (down[t] * (1.0f / GDN_UP));
 }
 
 #define GDN_PREP(H, N, TY)                                                                                                             \
