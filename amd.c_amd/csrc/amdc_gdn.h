@@ -297,7 +297,7 @@ GDN_RECS(64) GDN_RECS(128)
 // All products are on the f16 matrix units with both operands in two parts, x = hi + lo with 11 bits each, and three products, hi hi +
 // hi lo + lo hi, which keeps 22 bits and so f32's accuracy (the errors against 64 bits are those of the recurrence in f32). What f16's
 // range needs: M is at most 1 (its parts end at 2^-25, f32's accuracy of the 1s on its diagonal), keys, queries and A are and are multiplied by 2^8;
-// columns of S, R and U by a power of two each, from a bound of the column's values.
+// columns of S, R and U by a power of two each, from a bound of the column's values. For S += K^T U both sides have 2^4.
 //
 // The operands' k index is permuted so that the results of one product, four rows of a tile in a lane, are the next product's operand in
 // the same lane: place (g, e) of 32, lane group g, element e, is k = 16 (e / 4) + 4 g + e % 4.
@@ -305,6 +305,7 @@ GDN_RECS(64) GDN_RECS(128)
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 #define GDN_C 64u        // tokens of a chunk
 #define GDN_UP 256.0f    // what operands of size up to 1 are multiplied by
+#define GDN_UT 16.0f     // and those of the product that adds to S, on either side: S is in the square of this
 #define GDN_P 68u        // words of a row of 64 in the LDS: four lane groups, four rows apart, are 16 banks apart
 
 __device__ __forceinline__ h8 join8(h4 a, h4 b) { return (h8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}; }
@@ -329,14 +330,14 @@ __device__ __forceinline__ void pow2_of(float m, float &up, float &down) {
   up = __builtin_bit_cast(float, f << 23), down = __builtin_bit_cast(float, (254u - f) << 23);
 }
 __device__ __forceinline__ float max4(v4f x) { return __builtin_fmaxf(__builtin_fmaxf(__builtin_fabsf(x.x), __builtin_fabsf(x.y)), __builtin_fmaxf(__builtin_fabsf(x.z), __builtin_fabsf(x.w))); }
-// the largest of the four lanes that are 16 apart
+// The largest of the four lanes that are 16 apart, of values that are not negative: their bits are in their order, NaN the largest
 __device__ __forceinline__ float max_groups(float v) {
-  auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(u32, v), __builtin_bit_cast(u32, v), false, false);
-  u32 x = r[0], y = r[1];
-  v = __builtin_fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
-  r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(u32, v), __builtin_bit_cast(u32, v), false, false);
-  x = r[0], y = r[1];
-  return __builtin_fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+  u32 u = __builtin_bit_cast(u32, v);
+  auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = r[0] > r[1] ? r[0] : r[1];
+  r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  u = r[0] > r[1] ? r[0] : r[1];
+  return __builtin_bit_cast(float, u);
 }
 
 // Where chunk slot s (of all sequences', in their order) lies: with cu, sequence b's chunks are the slots cu[b] / 64 + b on, which leaves room for
@@ -352,7 +353,7 @@ __device__ __forceinline__ u32 gdn_seq(const amdc_slots_dev &sl, u32 nc, u32 s) 
 
 // The workspace: a chunk slot holds for every key head its keys, queries and transposed keys as operands (fragments of 1 KB: 16
 // rows, 32 of k, the lanes' 16 bytes in order; two parts each), then for every value head M and A (the 6 fragments that are not all above the
-// diagonal, in parts) and for each token the factors beta, 2^-8 beta e^G, e^G, e^(G_63 - G).
+// diagonal, in parts) and for each token the factors beta, 2^-8 beta e^G, e^G, 2^-4 e^(G_63 - G).
 __device__ __forceinline__ u32 gdn_tri(u32 i, u32 s) { return i < 2u ? i : 2u * (i - 1u) + s; }
 
 template <int TY, u32 DK>
@@ -435,8 +436,8 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
       const u32x4 lo = {__builtin_amdgcn_perm(x.y, x.x, 0x07060302u), __builtin_amdgcn_perm(x.w, x.z, 0x07060302u), __builtin_amdgcn_perm(y.y, y.x, 0x07060302u),
                         __builtin_amdgcn_perm(y.w, y.z, 0x07060302u)};
       const u32 f = 2u * 64u * DK * 4u + 1024u * ((M * 2u + s) * 2u) + 16u * lane;
-      *(u32x4 *)(wk + f) = hi;
-      *(u32x4 *)(wk + f + 1024u) = lo;
+      *(h8 *)(wk + f) = __builtin_bit_cast(h8, hi) * (_Float16)(GDN_UT / GDN_UP);
+      *(h8 *)(wk + f + 1024u) = __builtin_bit_cast(h8, lo) * (_Float16)(GDN_UT / GDN_UP);
     }
   }
   // k.k and q.k, the tiles up to the diagonal: a fragment of keys is either operand
@@ -483,7 +484,7 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
       s_G[w][lane] = G, s_beta[w][lane] = beta;
       const float since = __builtin_expf((float)G), until = __builtin_expf((float)(__shfl(G, 63) - G));
       float *cf = (float *)(wv + 24576u);
-      cf[lane] = beta, cf[64u + lane] = beta * since * (1.0f / GDN_UP), cf[128u + lane] = since, cf[192u + lane] = until;
+      cf[lane] = beta, cf[64u + lane] = beta * since * (1.0f / GDN_UP), cf[128u + lane] = since, cf[192u + lane] = until * (GDN_UT / GDN_UP);
     }
     wave_order();
     // L by blocks of 16 x 16, row n, columns 4 gr .. of a block in a lane; A's fragments on the way
@@ -598,14 +599,14 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
 // others bring S on. Waves 4 to 7 have 32 rows of S (dk = 64: 16), and of Q S what 16 tokens need, which they make beside U. Keys, queries, M and A are read
 // once a workgroup, straight into registers; S, R, U and Q S go through the LDS.
 // A column's R, U and its next S are under 12 max |S| + 65 max |beta v| of the chunk (a token adds at most beta |v| to the column's norm, and the rest of
-// its step shrinks it): the power of two of this bound brings them into f16's range, and as they share it U needs no scaling. S is kept as
-// 2^8 times that, as the products with K^T give it: they add to it.
+// its step shrinks it): the power of two of this bound brings them into f16's range, and as they share it U needs no scaling. max |S| is not waited for:
+// what it was a chunk before bounds it, by the same rule. S is kept as the products with K^T give it: they add to it.
 // PAIR: two values side by side in v and y are aligned to both (32-bit ones need not be).
 template <int TY, u32 DK, bool PAIR>
 __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
   constexpr u32 KS = DK / 32u, RT = DK / 64u, ES = TY ? 2u : 4u; // RT: row tiles of S that a wave has
   __shared__ __align__(16) uint8_t s_S[KS * 4096u], s_R[8192], s_U[8192], s_W[8192], s_Q[8192];
-  __shared__ __align__(16) float s_smax[4][32], s_vmax[2][4][32], s_cf[4][4][64];
+  __shared__ __align__(16) float s_smax[2][4][32], s_vmax[2][4][32], s_cf[4][4][64];
   const u32 tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), w = wave & 3u, n = lane & 15u, gr = lane >> 4;
   const u32 nb = (g.dv + 31u) / 32u, per = g.G * nb;
   // the workgroups of a key head are on one XCD (workgroups go round the 8 of them), where the group count allows it
@@ -643,12 +644,9 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 #pragma unroll
         for (u32 e = 0; e < 4u; e++) S[t][p][e] = on ? src[s_at(t, p, e)] : bad && !c0 ? nan_() : 0.0f;
   }
-  const auto put_smax = [&](const float(&by)[2]) {
+  const auto put_smax = [&](u32 c, const float(&by)[2]) {
 #pragma unroll
-    for (u32 t = 0; t < 2u; t++) {
-      const float x = max_groups(RT == 2u ? __builtin_fmaxf(max4(S[t][0]), max4(S[t][RT - 1u])) : max4(S[t][0]));
-      if (gr == 0u) s_smax[w][16u * t + n] = x * by[t];
-    }
+    for (u32 t = 0; t < 2u; t++) s_smax[c & 1u][w][16u * t + n] = by[t] * max_groups(RT == 2u ? __builtin_fmaxf(max4(S[t][0]), max4(S[t][RT - 1u])) : max4(S[t][0]));
   };
   const auto put_S = [&]() { // S as a right operand
 #pragma unroll
@@ -732,8 +730,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     }
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
-      const float y = max_groups(max4(val[t]));
-      if (gr == 0u) s_vmax[c & 1u][w][16u * t + n] = y;
+      s_vmax[c & 1u][w][16u * t + n] = max_groups(max4(val[t]));
     }
   };
   // A line from the memory takes as long as half a chunk. So each of the workgroups that share a key head (per of them) or a value head (nb)
@@ -756,24 +753,27 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       x[1][i] = __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(r, upper, at + 2048u, 0));
     }
   };
-  const auto load_t = [&](u32 c) {
+  const auto load_t = [&](u32 c, u32 k) { // part k of KS
     const __amdgpu_buffer_rsrc_t r = chunk_ws(c);
 #pragma unroll
-    for (u32 s = 0; s < 2u; s++)
-#pragma unroll
-      for (u32 i = 0; i < RT; i++)
-#pragma unroll
-        for (u32 j = 0; j < 2u; j++) tf[i][s][j] = frag(r, ok + 2u * 64u * DK * 4u + 1024u * (((RT * w + i) * 2u + s) * 2u + j));
+    for (u32 j = 0; j < 2u; j++) {
+      const u32 i = RT == 2u ? k & 1u : 0u, s = RT == 2u ? k >> 1 : k;
+      tf[i][s][j] = frag(r, ok + 2u * 64u * DK * 4u + 1024u * (((RT * w + i) * 2u + s) * 2u + j));
+    }
   };
-  const auto top_S = [&](u32 t) { // the largest |S| of a column
-    float x = s_smax[0][16u * t + n];
-#pragma unroll
-    for (u32 s = 1; s < 4u; s++) x = __builtin_fmaxf(x, s_smax[s][16u * t + n]);
-    return x;
+  struct Tops { // of a column: what the waves say of |S| a chunk ago and of |beta v|, and that chunk's whole decay
+    float s[2][4], v[2][4], whole;
   };
-
+  const auto get_tops = [&](u32 c, Tops &x) {
+#pragma unroll
+    for (u32 t = 0; t < 2u; t++)
+#pragma unroll
+      for (u32 i = 0; i < 4u; i++) x.s[t][i] = s_smax[(c - 1u) & 1u][i][16u * t + n], x.v[t][i] = s_vmax[c & 1u][i][16u * t + n];
+    x.whole = s_cf[(c - 1u) & 3u][2][63];
+  };
+  const auto top = [](const float(&x)[4]) { return __builtin_fmaxf(__builtin_fmaxf(x[0], x[1]), __builtin_fmaxf(x[2], x[3])); };
   // 16 rows by the columns of both tiles: three products for each 32 of k
-  const auto times_S = [&](v4f(&o)[2]) {
+  const auto times_S = [&](v4f(&o)[2], auto between) {
     h8 r[KS][2][2];
 #pragma unroll
     for (u32 s = 0; s < 2u; s++) get(s_S, s, 0u, r[s][0]), get(s_S, s, 1u, r[s][1]);
@@ -785,6 +785,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       for (u32 i = 0; i < 3u; i++)
 #pragma unroll
         for (u32 t = 0; t < 2u; t++) o[t] = mfma_f16(kq[s][i == 0u], r[s][t][i == 1u], o[t]);
+      between(s);
       if (s + 1u < KS) __builtin_amdgcn_sched_barrier(0); // not all of S's operands at once: the registers
     }
   };
@@ -802,13 +803,14 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 #pragma unroll
           for (u32 t = 0; t < 2u; t++) o[t] = mfma_f16(f[s][i == 0u], r[s][t][i == 1u], o[t]);
   };
-  float up[2], down_S[2], down[2]; // the factor of R, U and the next S, and the inverses of S's and of that
-  const auto factors = [&](u32 c) {
+  // bounds of |S| and |beta v|; the factor of R, U and the next S, and the inverses of S's and of that
+  float most[2], vmost[2], up[2], down_S[2], down[2];
+  const auto factors = [&](u32 c, const Tops &x) {
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
-      const float(*vm)[32] = s_vmax[c & 1u];
-      const float v0 = __builtin_fmaxf(vm[0][16u * t + n], vm[1][16u * t + n]), v1 = __builtin_fmaxf(vm[2][16u * t + n], vm[3][16u * t + n]);
-      pow2_of(__builtin_fmaf(12.0f, top_S(t), 65.0f * __builtin_fmaxf(v0, v1)), up[t], down[t]);
+      if (c != c0) most[t] = __builtin_fmaf(12.0f * x.whole, top(x.s[t]), 65.0f * vmost[t]);
+      vmost[t] = top(x.v[t]);
+      pow2_of(__builtin_fmaf(12.0f, most[t], 65.0f * vmost[t]), up[t], down[t]);
     }
   };
   if (chain) {
@@ -818,35 +820,43 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     load_ma(c0, 0u, mf), load_ma(c0, 1u, af), load_val(c0);
   } else {
     const float one[2] = {1.0f, 1.0f};
-    put_smax(one);
+    put_smax(c0 + 1u, one);
   }
   __syncthreads();
 #pragma unroll
-  for (u32 t = 0; t < 2u; t++) pow2_of(top_S(t), up[t], down_S[t]);
+  for (u32 t = 0; t < 2u; t++) {
+    float x[4];
+#pragma unroll
+    for (u32 i = 0; i < 4u; i++) x[i] = s_smax[(c0 + 1u) & 1u][i][16u * t + n];
+    most[t] = top(x), vmost[t] = 0.0f;
+    pow2_of(most[t], up[t], down_S[t]);
+  }
   if (chain) {
     put_vmax(c0), load_val(c0 + 1u), load_factor(c0 + 2u);
     for (u32 c = c0; c < c1; c++) {
       __syncthreads(); // S is there
-      factors(c);
+      Tops tops;
+      get_tops(c, tops);
       const v4f bs = four(c, 1u);
       v4f P[2];
-      times_S(P);
+      times_S(P, [](u32) {});
+      factors(c, tops);
 #pragma unroll
-      for (u32 t = 0; t < 2u; t++) put(s_R, t, fma4(-bs, P[t] * (down_S[t] * (1.0f / GDN_UP)), val[t]) * up[t]);
+      for (u32 t = 0; t < 2u; t++) put(s_R, t, fma4(-bs, P[t] * (down_S[t] * (1.0f / GDN_UP)), val[t]) * (up[t] * GDN_UP));
       __syncthreads(); // R is there
       v4f U[2];
       times_64(mf, s_R, U);
-      load_kq(c + 1u, 0u, 0u);
       const v4f until = four(c, 3u);
 #pragma unroll
       for (u32 t = 0; t < 2u; t++) {
         put(s_W, t, U[t] * until);
-        if (t == 0u || KS == 4u) load_kq(c + 1u, 0u, 1u + t); // a load takes its time: between the others
+        load_kq(c + 1u, 0u, t); // a load takes its time: between the others
         put(s_U, t, U[t]);
-        if (t == 0u && KS == 4u) load_kq(c + 1u, 0u, KS - 1u);
       }
       put_factor(c + 2u);
       __syncthreads(); // U and Q S are there
+#pragma unroll
+      for (u32 s = 2; s < KS; s++) load_kq(c + 1u, 0u, s);
       load_ma(c + 1u, 0u, mf), load_factor(c + 3u);
       put_vmax(c + 1u);
       asm volatile("" ::"v"(ahead));
@@ -855,12 +865,12 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
       times_64(af, s_U, y);
       load_ma(c + 1u, 1u, af);
       const __amdgpu_buffer_rsrc_t ry = rows_of(g.y, c, g.ys);
-      const float sc = g.scale * (1.0f / GDN_UP);
+      const float sc = g.scale * (1.0f / GDN_UP / GDN_UP);
       const v4f since = four(c, 2u);
 #pragma unroll
       for (u32 t = 0; t < 2u; t++) {
         const v4f q = *(const v4f *)(s_Q + 2048u * w + 1024u * t + 16u * lane);
-        y[t] = fma4(splat(down[t] * sc), y[t], since * (down_S[t] * sc * (1.0f / GDN_UP)) * q);
+        y[t] = fma4(splat(down[t] * sc), y[t], since * (down_S[t] * sc) * q);
         down_S[t] = down[t];
       }
 #pragma unroll
@@ -886,8 +896,11 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     __syncthreads(); // S is there
 #pragma unroll
     for (u32 s = 0; s < KS; s++) load_kq(c, 1u, s);
-    load_t(c);
-    factors(c);
+    const float by[2] = {down_S[0] * (1.0f / GDN_UP), down_S[1] * (1.0f / GDN_UP)};
+    put_smax(c, by);
+    Tops tops;
+    get_tops(c, tops);
+    factors(c, tops);
     const float whole = s_cf[c & 3u][2][63];
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) {
@@ -897,7 +910,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     }
     __syncthreads(); // R is there
     v4f Q[2];
-    times_S(Q);
+    times_S(Q, [&](u32 s) { load_t(c, s); });
 #pragma unroll
     for (u32 t = 0; t < 2u; t++) *(v4f *)(s_Q + 2048u * w + 1024u * t + 16u * lane) = Q[t];
     __syncthreads(); // U and Q S are there
@@ -915,8 +928,6 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 #pragma unroll
           for (u32 p = 0; p < RT; p++) S[t][p] = mfma_f16(tf[p][s][i == 0u], z[s][t][i == 1u], S[t][p]);
     put_S();
-    const float by[2] = {down[0] * (1.0f / GDN_UP), down[1] * (1.0f / GDN_UP)};
-    put_smax(by);
   }
   // the state: into its slot, or for the launch that goes on
   float *dst = g.carry_out + (u64)h * mat;

@@ -153,6 +153,8 @@ class Layer:
             most = np.maximum(most, n + np.abs(v[t]))
             E = np.exp(g[t])[:, None] * E + U * (48 * n + 8 * np.abs(v[t])) + (12 * chunk ** 0.5 * U * most if chunk > 1 else 0)
             ey[t] = qn * (E + 32 * U * (n + np.abs(u)) + (12 * chunk ** 0.5 * U * most if chunk > 1 else 0))
+            if m > 1000 and states:  # the last alone
+                states.pop(), es.pop()
             states.append(S)
             es.append(np.broadcast_to(E[:, None, :], S.shape))
         return ys, ey, states, es

@@ -1,11 +1,13 @@
 """amdc_gdn_prefill against the recurrence in 64 bits: lengths around the chunks of 64, ragged packing, all head sizes, types and
 orders; states in place, shared, from zeros; sequences that go on from one pair of launches to the next; and that it agrees with
 amdc_gdn_decode."""
+import copy
+
 import numpy as np
 import pytest
 
-from attncase import BF16, F16, F32
-from lincase import U, pool_of
+from attncase import BF16, F16, F32, TINY, ULP, from16
+from lincase import U, near, pool_of, state_of
 from test_gdn_decode import HEADS, Call as Both
 
 pytestmark = pytest.mark.gpu
@@ -122,9 +124,19 @@ def test_decode_goes_on(dev):
     assert (np.abs(got.astype(np.float64) - whole) <= 2 * err.reshape(n + more, -1) + 2 * U * np.abs(whole)).all()
 
 
+def some_heads(L, heads):
+    """The layer of some value heads of L alone, each with a key head of its own."""
+    c = copy.copy(L)
+    c.n_k = c.n_v = len(heads)
+    hk = [h % L.n_k if L.tiled else h * L.n_k // L.n_v for h in heads]
+    col = [np.arange(o + h * d, o + (h + 1) * d) for o, hs, d in ((0, hk, L.dk), (L.n_k * L.dk, hk, L.dk), (2 * L.n_k * L.dk, heads, L.dv)) for h in hs]
+    c.x, c.ab = L.x[:, np.concatenate(col)], L.ab[:, list(heads) + [L.n_v + h for h in heads]]
+    c.A, c.dt, c.tiled = L.A[list(heads)], L.dt[list(heads)], False
+    return c
+
+
 def test_sequences_over_launches(dev):
-    """More chunk slots than a pair of launches takes: sequences that begin in one and go on in the next, over several, in place; the same
-    bits as each alone where it fits one."""
+    """More chunk slots than a pair of launches takes: sequences that begin in one and go on in the next, over several, in place."""
     n_k, n_v, dk, dv = 16, 64, 128, 16
     per = n_k * 3 * 64 * 128 * 4 + n_v * 25600
     most = (256 << 20) // per + 1  # slots of a pair of launches
@@ -132,26 +144,15 @@ def test_sequences_over_launches(dev):
     c = Call(dev, 1158, new, n_k, n_v, dk, dv, tiled=True, t=BF16, start=(0, -1, 2, 3, 4, -1, 6), to=(0, 1, 2, 3, 4, 5, -1)).upload().launch()
     dev.kv_check()
     raw, pool = c.results()
-    pool = pool.reshape(c.s.n_slots, -1)
-    s = c.s
-    assert np.array_equal(pool[6:], pool_of(c.S).reshape(s.n_slots, -1)[6:])  # the last one's starting slot too
-    # each by itself, in pieces of under a launch's slots: the state goes through a slot instead
-    start, piece = pool_of(c.S), 64 * (most // 2)
-    es, L = c.L.raw.itemsize, c.L
-    work, one, two = dev.DevBuf(start.nbytes // s.n_slots * 2), dev.DevBuf(4), dev.DevBuf(4)
-    y = dev.DevBuf(piece * c.ys * es)
-    for b, m in enumerate(new):
-        if s.start[b] >= 0:
-            work.upload(start[s.start[b]])
-        at = int(s.cu[b])
-        for t in range(0, m, piece):
-            k = min(piece, m - t)
-            one.upload(np.array([-1 if t == 0 and s.start[b] < 0 else 0], np.int32)), two.upload(np.zeros(1, np.int32))
-            ptr = [p + (at + t) * (es * L.w if i < 3 else 4 * (2 * n_v + 1)) for i, p in enumerate(L.args())]
-            dev.gdn_prefill(L.gdn, dev.Slots(1, 2, one, two), work, *ptr, y, BF16, k, *L.strides(), c.ys, c.ws, c.ws.nbytes)
-            assert np.array_equal(y.download(np.uint16, k * c.ys).reshape(k, -1), raw[at + t:at + t + k]), (b, t)
+    s, heads = c.s, [3, 50]
+    pool = state_of(pool.reshape(s.n_slots, n_v, dv // 16, dk, 16)).astype(np.float64)
+    assert np.array_equal(pool[6:], c.S[6:])  # the last one's starting slot too
+    y, L = from16(raw, BF16).reshape(-1, n_v, dv)[:, heads], some_heads(c.L, heads)
+    for b in range(s.n):
+        want, err, st, es = L.run64(s.at(b), c.S[s.start[b]][heads] if s.start[b] >= 0 else np.zeros((2, dk, dv)), chunk=64)
+        near(y[s.at(b)], want, err * (1 + ULP[BF16]) + ULP[BF16] * np.abs(want) + TINY[BF16], f"sequence {b}")
         if s.to[b] >= 0:
-            assert np.array_equal(work.download(np.float32, pool.shape[1]), pool[s.to[b]]), b
+            near(pool[s.to[b]][heads], st[-1], es[-1], f"state {b}")
 
 
 def test_not_finite(dev):
