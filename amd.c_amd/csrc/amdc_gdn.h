@@ -734,15 +734,17 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     }
   };
   // A line from the memory takes as long as half a chunk. So each of the workgroups that share a key head (per of them) or a value head (nb)
-  // asks for its part of a chunk two ahead, a line to a lane, which brings it into the L2.
-  u32 ahead = 0u;
-  const u32 lines_k = (3u * 64u * DK * 4u / 128u + per - 1u) / per, lines_v = (AMDC_GDN_VB / 128u + nb - 1u) / nb;
-  const auto prefetch = [&](u32 c) {
-    const bool keys = w == 0u;
-    const u32 i = 64u * (keys ? 0u : w - 1u) + lane, lines = keys ? lines_k : lines_v, at = (keys ? in : cb) * lines + i;
-    const u32 off = c < c1 && i < lines && at < (keys ? 3u * 64u * DK * 4u : AMDC_GDN_VB) / 128u ? (keys ? ok : ov) + 128u * at : 0xC0000000u;
-    ahead = (u32)__builtin_amdgcn_raw_buffer_load_b32(chunk_ws(c), off, 0, 0);
-  };
+  // asks for its part of a chunk two ahead, a line to a lane, which brings it into the L2: where that is an eighth of what it loads at most (12000 tokens,
+  // 48 heads of 128 on 16: 262 -> 242 us a launch; heads of 64, two to a key head, a third of it: 82 -> 95, so not there).
+  constexpr u32 LK = 3u * 64u * DK * 4u / 128u, LV = AMDC_GDN_VB / 128u;
+  const u32 lines_k = (LK + per - 1u) / per, lines_v = (LV + nb - 1u) / nb;
+  u32 ahead = 0u, line = 0xC0000000u; // where the lane's line is in a slot
+  if (8u * (lines_k + lines_v) <= LK + LV) {
+    const u32 i = 64u * w + lane;
+    if (i < lines_k && in * lines_k + i < LK) line = ok + 128u * (in * lines_k + i);
+    else if (i >= lines_k && i < lines_k + lines_v && cb * lines_v + i - lines_k < LV) line = ov + 128u * (cb * lines_v + i - lines_k);
+  }
+  const auto prefetch = [&](u32 c) { ahead = (u32)__builtin_amdgcn_raw_buffer_load_b32(chunk_ws(c), line, 0, 0); };
   const u32 upper = w < 2u ? 0xC0000000u : 16u * lane; // the fragments above the diagonal are not there: beyond the end, 0
   const auto load_ma = [&](u32 c, u32 a, h8(&x)[2][2]) { // M or A
     const __amdgpu_buffer_rsrc_t r = chunk_ws(c);

@@ -171,7 +171,7 @@ typedef struct {
 } amdc_gdn_args;
 #define AMDC_GDN_C 64u      /* tokens of a chunk */
 #define AMDC_GDN_VB 25600u  /* bytes of a value head in a chunk slot */
-#define AMDC_GDN_WS (256u << 20) /* bytes of chunk slots that a prompt's launches take at a time, about */
+#define AMDC_GDN_WS (512u << 20) /* bytes of chunk slots that a prompt's launches take at a time, about */
 typedef struct {
   const void *x;
   const float *w, *z, *w2;

@@ -137,14 +137,14 @@ def some_heads(L, heads):
 
 def test_sequences_over_launches(dev):
     """More chunk slots than a pair of launches takes: sequences that begin in one and go on in the next, over several, in place."""
-    n_k, n_v, dk, dv = 16, 64, 128, 16
+    n_k, n_v, dk, dv = 32, 128, 128, 16
     per = n_k * 3 * 64 * 128 * 4 + n_v * 25600
-    most = (256 << 20) // per + 1  # slots of a pair of launches
+    most = (512 << 20) // per + 1  # slots of a pair of launches
     new = [64 * (most - 2) + 5, 64 * 3, 7, 64 * (2 * most) + 1, 64, 64 * most, 10]
     c = Call(dev, 1158, new, n_k, n_v, dk, dv, tiled=True, t=BF16, start=(0, -1, 2, 3, 4, -1, 6), to=(0, 1, 2, 3, 4, 5, -1)).upload().launch()
     dev.kv_check()
     raw, pool = c.results()
-    s, heads = c.s, [3, 50]
+    s, heads = c.s, [3, 100]
     pool = state_of(pool.reshape(s.n_slots, n_v, dv // 16, dk, 16)).astype(np.float64)
     assert np.array_equal(pool[6:], c.S[6:])  # the last one's starting slot too
     y, L = from16(raw, BF16).reshape(-1, n_v, dv)[:, heads], some_heads(c.L, heads)
