@@ -1,7 +1,8 @@
 // amdc_gdn.h -- the device code of a linear-attention layer (amdc_slots and amdc_gdn of amdc_q4.h): the short convolution,
 // the gated delta rule, and the norms around them; part of amdc_kernels.hip's translation unit.
 //
-//   amdc_conv_w{2,3,4}_{f32,f16,bf16}   the causal convolution over the channels, with its state
+//   amdc_conv_w{2,3,4}_{f32,f16,bf16}[_odd]
+//                                       the causal convolution over the channels, with its state
 //   amdc_gdn_rec_h{64,128}_{f32,f16,bf16}
 //                                       the delta rule, token after token
 //   amdc_gdn_prep_h{64,128}_{f32,f16,bf16}, amdc_gdn_scan_h{64,128}_{f32,f16,bf16,f16_odd,bf16_odd}
@@ -11,7 +12,10 @@
 
 // ------------------------------------------------------------------ helpers
 
-// a value of a row of type TY (AMDC_TYPE_*), and four side by side (vec: aligned to four values)
+// A value of a row of type TY (AMDC_TYPE_*), and four side by side, aligned to one: the memory takes them at any
+// address, and a branch on the alignment would keep the loads behind it from being in flight together.
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short u4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <int TY>
 __device__ __forceinline__ float ld1(const void *p, u64 i) {
   if constexpr (TY == 0) return ((const float *)p)[i];
@@ -19,31 +23,36 @@ __device__ __forceinline__ float ld1(const void *p, u64 i) {
   else return __builtin_bit_cast(float, (u32)((const unsigned short *)p)[i] << 16);
 }
 template <int TY>
-__device__ __forceinline__ v4f ld4(const void *p, u64 i, bool vec) {
-  if (!vec) return (v4f){ld1<TY>(p, i), ld1<TY>(p, i + 1u), ld1<TY>(p, i + 2u), ld1<TY>(p, i + 3u)};
-  if constexpr (TY == 0) return *(const v4f *)((const float *)p + i);
-  else {
-    const u32x2 u = *(const u32x2 *)((const unsigned short *)p + i);
-    return (v4f){lo16<TY == 2>(u.x), hi16<TY == 2>(u.x), lo16<TY == 2>(u.y), hi16<TY == 2>(u.y)};
+__device__ __forceinline__ v4f ld4(const void *p, u64 i) {
+  if constexpr (TY == 0) {
+    const f4_any v = *(const f4_any *)((const float *)p + i);
+    return (v4f){v.x, v.y, v.z, v.w};
+  } else {
+    const u4_any u = *(const u4_any *)((const unsigned short *)p + i);
+    return TY == 1 ? (v4f){h2f(u.x), h2f(u.y), h2f(u.z), h2f(u.w)}
+                   : (v4f){__builtin_bit_cast(float, (u32)u.x << 16), __builtin_bit_cast(float, (u32)u.y << 16), __builtin_bit_cast(float, (u32)u.z << 16),
+                           __builtin_bit_cast(float, (u32)u.w << 16)};
   }
 }
-// the first n (1 to 4) of them
 template <int TY>
-__device__ __forceinline__ void st4(void *p, u64 i, v4f v, bool vec, u32 n = 4u) {
-  if constexpr (TY == 0) {
-    if (vec) *(v4f *)((float *)p + i) = v;
-    else
-#pragma unroll
-      for (u32 e = 0; e < 4u; e++)
-        if (e < n) ((float *)p)[i + e] = v[e];
-  } else {
-    const u32x2 u = {pack2<TY == 2>(v.x, v.y), pack2<TY == 2>(v.z, v.w)};
-    if (vec) *(u32x2 *)((unsigned short *)p + i) = u;
-    else
-#pragma unroll
-      for (u32 e = 0; e < 4u; e++)
-        if (e < n) ((unsigned short *)p)[i + e] = (unsigned short)(u[e >> 1] >> (16u * (e & 1u)));
+__device__ __forceinline__ void st4(void *p, u64 i, v4f v) {
+  if constexpr (TY == 0) *(f4_any *)((float *)p + i) = (f4_any){v.x, v.y, v.z, v.w};
+  else {
+    const u32 a = pack2<TY == 2>(v.x, v.y), b = pack2<TY == 2>(v.z, v.w);
+    *(u4_any *)((unsigned short *)p + i) = (u4_any){(unsigned short)a, (unsigned short)(a >> 16), (unsigned short)b, (unsigned short)(b >> 16)};
   }
+}
+// C (4 or 1) of them: the others are 0
+template <int TY, u32 C>
+__device__ __forceinline__ v4f ldc(const void *p, u64 i) {
+  if constexpr (C == 4u) return ld4<TY>(p, i);
+  else return (v4f){ld1<TY>(p, i), 0.0f, 0.0f, 0.0f};
+}
+template <int TY, u32 C>
+__device__ __forceinline__ void stc(void *p, u64 i, v4f v) {
+  if constexpr (C == 4u) st4<TY>(p, i, v);
+  else if constexpr (TY == 0) ((float *)p)[i] = v.x;
+  else ((unsigned short *)p)[i] = (unsigned short)pack2<TY == 2>(v.x, 0.0f);
 }
 
 __device__ __forceinline__ v4f splat(float x) { return (v4f){x, x, x, x}; }
@@ -79,13 +88,13 @@ __device__ __forceinline__ float sigmoid_fast(float v) { return __builtin_amdgcn
 
 // ------------------------------------------------------------------ the short convolution
 
-// Reading and writing bound it. A thread has four channels of up to AMDC_CONV_ROWS rows of a sequence: the window of the last W - 1
+// Reading and writing bound it. A thread has four channels (one, where their number is no multiple of four: _odd) of up to AMDC_CONV_ROWS rows of a sequence: the window of the last W - 1
 // inputs stays in its registers, the next eight rows are in flight while it goes over them, and a row is read again only by the unit
 // behind it (W - 1 of 32). The unit of a sequence's first rows reads the state and, after that, writes it: from x where the sequence has rows enough, and
 // else from what it has read, so that a slot may be read and written by the same call.
-template <u32 W, int TY>
+template <u32 W, int TY, u32 C>
 __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_conv_args &a) {
-  const u32 ct = blockIdx.x % a.cb, u = blockIdx.x / a.cb, c = 4u * (ct * blockDim.x + threadIdx.x);
+  const u32 ct = blockIdx.x % a.cb, u = blockIdx.x / a.cb, c = C * (ct * blockDim.x + threadIdx.x);
   u32 b, first;
   if (sl.cu) {
     const auto base = [&](u32 i) { const int s = sl.cu[i]; return (s < 0 ? 0u : (u32)s) / AMDC_CONV_ROWS + i; };
@@ -95,27 +104,18 @@ __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_c
   u32 row0;
   const u32 m = slot_rows(sl, b, row0), t0 = (u - first) * AMDC_CONV_ROWS;
   if (t0 >= m) return;
-  const u32 n = c >= a.ch ? 0u : a.ch - c < 4u ? a.ch - c : 4u, t1 = m - t0 < AMDC_CONV_ROWS ? m : t0 + AMDC_CONV_ROWS;
-  if (!n) return;
-  const bool vec = a.vec & 1u, vecy = a.vec & 2u;
-  const auto row = [&](const float *p, u64 i) { // n values of a row
-    v4f v = splat(0.0f);
-    if (vec) v = *(const v4f *)(p + i);
-    else
-#pragma unroll
-      for (u32 e = 0; e < 4u; e++)
-        if (e < n) v[e] = p[i + e];
-    return v;
-  };
+  const u32 t1 = m - t0 < AMDC_CONV_ROWS ? m : t0 + AMDC_CONV_ROWS;
+  if (c >= a.ch) return;
+  const auto row = [](const float *p, u64 i) { return ldc<0, C>(p, i); };
   const float *x = a.x + c + (u64)row0 * a.xs;
   v4f w[W], bias = splat(0.0f), win[W - 1u];
 #pragma unroll
-  for (u32 e = 0; e < 4u; e++) {
-    const u32 ce = c + (e < n ? e : 0u);
+  for (u32 j = 0; j < W; j++) w[j] = splat(0.0f);
 #pragma unroll
-    for (u32 j = 0; j < W; j++) w[j][e] = a.w[(u64)ce * W + j];
-    if (a.bias) bias[e] = a.bias[ce];
-  }
+  for (u32 e = 0; e < C; e++)
+#pragma unroll
+    for (u32 j = 0; j < W; j++) w[j][e] = a.w[(u64)(c + e) * W + j];
+  if (a.bias) bias = row(a.bias, c);
   if (t0 == 0u) {
     const int f = sl.from[b];
     bool bad;
@@ -136,7 +136,7 @@ __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_c
           s[j] = at < W - 1u ? old : row(x, (u64)(at - (W - 1u)) * a.xs);
         }
 #pragma unroll
-        for (u32 j = 0; j < W - 1u; j++) st4<0>(a.state, ((u64)(u32)o * (W - 1u) + j) * a.ch + c, s[j], vec, n);
+        for (u32 j = 0; j < W - 1u; j++) stc<0, C>(a.state, ((u64)(u32)o * (W - 1u) + j) * a.ch + c, s[j]);
       }
     }
   } else {
@@ -164,33 +164,36 @@ __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_c
         if (a.act)
 #pragma unroll
           for (u32 e = 0; e < 4u; e++) s[e] *= sigmoid_fast(s[e]);
-        st4<TY>(a.y, (u64)(row0 + t + i) * a.ys + c, s, vecy, n);
+        stc<TY, C>(a.y, (u64)(row0 + t + i) * a.ys + c, s);
         if (keep) {
           const int o = sl.to[row0 + t + i];
           bool bad;
           if (slot_ok(sl, o, bad) && !(sl.from[b] < -1 || (sl.from[b] >= 0 && (u32)sl.from[b] >= sl.n_slots)))
 #pragma unroll
-            for (u32 j = 0; j < W - 1u; j++) st4<0>(a.state, ((u64)(u32)o * (W - 1u) + j) * a.ch + c, win[j], vec, n);
+            for (u32 j = 0; j < W - 1u; j++) stc<0, C>(a.state, ((u64)(u32)o * (W - 1u) + j) * a.ch + c, win[j]);
         }
       }
     }
   }
 }
 
-#define CONV(W, N, TY)                                                                                                             \
-  extern "C" __global__ __launch_bounds__(256) void amdc_conv_w##W##_##N(const amdc_slots_dev sl, const amdc_conv_args a) { conv_body<W##u, TY>(sl, a); }
-#define CONVS(W) CONV(W, f32, 0) CONV(W, f16, 1) CONV(W, bf16, 2)
+#define CONV(W, N, TY, C)                                                                                                          \
+  extern "C" __global__ __launch_bounds__(256) void amdc_conv_w##W##_##N(const amdc_slots_dev sl, const amdc_conv_args a) { conv_body<W##u, TY, C##u>(sl, a); }
+#define CONVS(W) CONV(W, f32, 0, 4) CONV(W, f16, 1, 4) CONV(W, bf16, 2, 4) CONV(W, f32_odd, 0, 1) CONV(W, f16_odd, 1, 1) CONV(W, bf16_odd, 2, 1)
 CONVS(2) CONVS(3) CONVS(4)
 
 // ------------------------------------------------------------------ the gated delta rule, token after token
 
-// log decay (at most 0, NaN kept) and rate of value head h at a row
-__device__ __forceinline__ void gdn_gates(const amdc_gdn_args &g, u64 row, u32 h, float &decay, float &rate) {
-  const float x = g.a[row * g.as + h] + g.dt[h];
-  const float v = g.A[h] * ((x > 0.0f ? x : 0.0f) + log1pf(__builtin_expf(-__builtin_fabsf(x))));
-  decay = v > 0.0f ? 0.0f : v;
-  rate = 1.0f / (1.0f + __builtin_expf(-g.b[row * g.bs + h]));
-}
+// What the gates of value head h at a row are made of; its log decay (at most 0, NaN kept) and rate
+struct GdnGates {
+  float a, b, A, dt;
+  __device__ __forceinline__ GdnGates(const amdc_gdn_args &g, u64 row, u32 h) : a(g.a[row * g.as + h]), b(g.b[row * g.bs + h]), A(g.A[h]), dt(g.dt[h]) {}
+  __device__ __forceinline__ void get(float &decay, float &rate) const {
+    const float x = a + dt, v = A * ((x > 0.0f ? x : 0.0f) + log1pf(__builtin_expf(-__builtin_fabsf(x))));
+    decay = v > 0.0f ? 0.0f : v;
+    rate = 1.0f / (1.0f + __builtin_expf(-b));
+  }
+};
 __device__ __forceinline__ u32 gdn_key_head(const amdc_gdn_args &g, u32 h) { return g.tiled ? h % g.n_k : h / g.G; }
 __device__ __forceinline__ float lane_of(float v, u32 l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), (int)l)); }
 
@@ -235,12 +238,12 @@ __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amd
     const u64 row = row0 + t;
 #pragma unroll
     for (u32 i = 0; i < NI; i++) k[i] = ld1<TY>(g.k, row * g.ks + hk * DK + 16u * i + r), q[i] = ld1<TY>(g.q, row * g.qs + hk * DK + 16u * i + r);
-    v = ld4<TY>(g.v, row * g.vs + h * g.dv + c + 4u * c4, g.vec & 1u);
+    v = ld4<TY>(g.v, row * g.vs + h * g.dv + c + 4u * c4);
   };
   load(0u);
   float decay = 0.0f, rate = 0.0f;
   for (u32 t = 0; t < m; t++) {
-    if (!(t & 63u)) gdn_gates(g, row0 + (t + lane < m ? t + lane : m - 1u), h, decay, rate), decay = __builtin_expf(decay); // those of 64 tokens
+    if (!(t & 63u)) GdnGates(g, row0 + (t + lane < m ? t + lane : m - 1u), h).get(decay, rate), decay = __builtin_expf(decay); // those of 64 tokens
     const float e = lane_of(decay, t & 63u), be = lane_of(rate, t & 63u);
     float kk = 0.0f, qq = 0.0f, kq = 0.0f;
     v4f kS = splat(0.0f), qS = splat(0.0f), vt = v;
@@ -263,7 +266,7 @@ __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amd
       y[j] = rq * __builtin_fmaf(kq * rk, u[j], e * qS[j]);
       u[j] *= rk;
     }
-    if (r == 0u) st4<TY>(g.y, (u64)(row0 + t) * g.ys + h * g.dv + c + 4u * c4, y, g.vec & 2u);
+    if (r == 0u) st4<TY>(g.y, (u64)(row0 + t) * g.ys + h * g.dv + c + 4u * c4, y);
 #pragma unroll
     for (u32 i = 0; i < NI; i++) S[i] = fma4(splat(kt[i]), u, S[i] * e);
     if (sl.each || t + 1u == m) {
@@ -374,9 +377,30 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
   const u32 first = row0 + c * GDN_C, mc = m - c * GDN_C < GDN_C ? m - c * GDN_C : GDN_C;
   uint8_t *ws = g.ws + (u64)at * g.sb, *wk = ws + (u64)hk * (3u * 64u * DK * 4u);
 
+  // the gates of a value head, a token to a lane: the sums of its log decays into the LDS, the tokens' factors into the workspace
+  const auto head = [&](u32 v) { return g.tiled ? hk + v * g.n_k : hk * g.G + v; };
+  const auto raw_gates = [&](u32 v) { return GdnGates(g, first + (lane < mc ? lane : mc - 1u), head(v < g.G ? v : 0u)); };
+  const auto gates = [&](u32 v, const GdnGates &raw) {
+    const u32 h = head(v);
+    float decay, beta;
+    raw.get(decay, beta);
+    // e^-10000 is 0: an infinite decay makes no NaN of a difference
+    decay = lane < mc ? decay < -1e4f ? -1e4f : decay : 0.0f, beta = lane < mc ? beta : 0.0f;
+    double G = (double)decay;
+#pragma unroll
+    for (u32 o = 1; o < 64u; o <<= 1) {
+      const double up = __shfl_up(G, o);
+      G += lane >= o ? up : 0.0;
+    }
+    s_G[w][lane] = G, s_beta[w][lane] = beta;
+    const float since = __builtin_expf((float)G), until = __builtin_expf((float)(__shfl(G, 63) - G));
+    float *cf = (float *)(ws + (u64)g.n_k * (3u * 64u * DK * 4u) + (u64)h * AMDC_GDN_VB + 24576u);
+    cf[lane] = beta, cf[64u + lane] = beta * since * (1.0f / GDN_UP), cf[128u + lane] = since, cf[192u + lane] = until * (GDN_UT / GDN_UP);
+  };
   // keys and queries: wave w the rows 16 w .. + 15, as operands of the products along dk
   h8 kf[KS][2], qf[KS][2];
   {
+    const GdnGates raw = raw_gates(w); // asked for ahead of the others, and used while they are on their way
     const u32 r = 16u * w + n;
     const bool on = r < mc;
     const u64 row = first + (on ? r : mc - 1u);
@@ -385,9 +409,10 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
     for (u32 s = 0; s < KS; s++)
 #pragma unroll
       for (u32 p = 0; p < 2u; p++) {
-        k[s][p] = ld4<TY>(g.k, row * g.ks + hk * DK + 32u * s + 16u * p + 4u * gr, g.vec & 4u);
-        q[s][p] = ld4<TY>(g.q, row * g.qs + hk * DK + 32u * s + 16u * p + 4u * gr, g.vec & 8u);
+        k[s][p] = ld4<TY>(g.k, row * g.ks + hk * DK + 32u * s + 16u * p + 4u * gr);
+        q[s][p] = ld4<TY>(g.q, row * g.qs + hk * DK + 32u * s + 16u * p + 4u * gr);
       }
+    if (w < g.G) gates(w, raw);
     v4f kk = splat(0.0f), qq = splat(0.0f);
 #pragma unroll
     for (u32 s = 0; s < KS; s++)
@@ -396,15 +421,15 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
     float sk = (kk.x + kk.y) + (kk.z + kk.w), sq = (qq.x + qq.y) + (qq.z + qq.w);
     sk += __shfl_xor(sk, 16), sq += __shfl_xor(sq, 16);
     sk += __shfl_xor(sk, 32), sq += __shfl_xor(sq, 32);
-    const float rk = GDN_UP / __builtin_sqrtf(sk + g.eps), rq = GDN_UP / __builtin_sqrtf(sq + g.eps);
+    const float rk = on ? GDN_UP / __builtin_sqrtf(sk + g.eps) : 0.0f, rq = on ? GDN_UP / __builtin_sqrtf(sq + g.eps) : 0.0f;
     u32 *kt = (u32 *)s_b;
 #pragma unroll
     for (u32 s = 0; s < KS; s++) {
       h4 hi[2], lo[2], qh[2], ql[2];
 #pragma unroll
       for (u32 p = 0; p < 2u; p++) {
-        split4(on ? k[s][p] * rk : splat(0.0f), hi[p], lo[p]);
-        split4(on ? q[s][p] * rq : splat(0.0f), qh[p], ql[p]);
+        split4(k[s][p] * rk, hi[p], lo[p]);
+        split4(q[s][p] * rq, qh[p], ql[p]);
 #pragma unroll
         for (u32 e = 0; e < 4u; e++) {
           const _Float16 x = hi[p][e], y = lo[p][e];
@@ -466,26 +491,9 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
   // a value head to a wave
   float *blk = (float *)(s_a + w * (SCR / 4u));
   for (u32 v = w; v < g.G; v += 4u) {
-    const u32 h = g.tiled ? hk + v * g.n_k : hk * g.G + v;
+    const u32 h = head(v);
     uint8_t *wv = ws + (u64)g.n_k * (3u * 64u * DK * 4u) + (u64)h * AMDC_GDN_VB;
-    double G;
-    float beta;
-    {
-      float decay;
-      gdn_gates(g, first + (lane < mc ? lane : mc - 1u), h, decay, beta);
-      // e^-10000 is 0: an infinite decay makes no NaN of a difference
-      decay = lane < mc ? decay < -1e4f ? -1e4f : decay : 0.0f, beta = lane < mc ? beta : 0.0f;
-      G = (double)decay;
-#pragma unroll
-      for (u32 o = 1; o < 64u; o <<= 1) {
-        const double up = __shfl_up(G, o);
-        G += lane >= o ? up : 0.0;
-      }
-      s_G[w][lane] = G, s_beta[w][lane] = beta;
-      const float since = __builtin_expf((float)G), until = __builtin_expf((float)(__shfl(G, 63) - G));
-      float *cf = (float *)(wv + 24576u);
-      cf[lane] = beta, cf[64u + lane] = beta * since * (1.0f / GDN_UP), cf[128u + lane] = since, cf[192u + lane] = until * (GDN_UT / GDN_UP);
-    }
+    if (v >= 4u) gates(v, raw_gates(v));
     wave_order();
     // L by blocks of 16 x 16, row n, columns 4 gr .. of a block in a lane; A's fragments on the way
     v4f L[10];
@@ -968,8 +976,8 @@ __device__ __forceinline__ void norm_gate_body(const amdc_norm_args &a) {
   const u32 i0 = 4u * (blockIdx.x * NT + threadIdx.x), n = a.n;
   const bool on = i0 < n; // whole heads, and whole blocks of 32, at once
   const u32 i = on ? i0 : n - 4u;
-  const v4f x = ld4<TY>((const uint8_t *)a.x + (u64)blockIdx.y * a.xs, i, a.vec & 1u), z = ld4<0>((const uint8_t *)a.z + (u64)blockIdx.y * a.zs, i, a.vec & 2u);
-  const v4f w = ld4<0>(a.w, i & (a.hd - 1u), a.vec & 4u);
+  const v4f x = ld4<TY>((const uint8_t *)a.x + (u64)blockIdx.y * a.xs, i), z = ld4<0>((const uint8_t *)a.z + (u64)blockIdx.y * a.zs, i);
+  const v4f w = ld4<0>(a.w, i & (a.hd - 1u));
   const float ss = seg_sum((x.x * x.x + x.y * x.y) + (x.z * x.z + x.w * x.w), a.hd >> 2);
   const float s = 1.0f / __builtin_sqrtf(ss / (float)a.hd + a.eps);
   v4f y;
@@ -978,7 +986,7 @@ __device__ __forceinline__ void norm_gate_body(const amdc_norm_args &a) {
     const float g = sigmoid_fast(z[j]);
     y[j] = x[j] * s * w[j] * (a.gate ? g : z[j] * g);
   }
-  if (on && a.y) st4<0>((uint8_t *)a.y + (u64)blockIdx.y * a.ys, i, y, a.vec & 8u);
+  if (on && a.y) st4<0>((uint8_t *)a.y + (u64)blockIdx.y * a.ys, i, y);
   if (a.q) quant_vec4(y, i >> 5, on, a.q + (u64)blockIdx.y * a.qs, n >> 5);
 }
 extern "C" __global__ __launch_bounds__(256) void amdc_norm_gate_f32(const amdc_norm_args a) { norm_gate_body<0>(a); }
@@ -1013,16 +1021,16 @@ __device__ __forceinline__ void norm_res_body(const amdc_norm_args &a) {
 #pragma unroll
   for (u32 j = 0; j < NV; j++) {
     const u32 i = 4u * threadIdx.x + j * step;
-    x[j] = i < n ? ld4<0>(px, i, a.vec & 1u) : splat(0.0f), h[j] = i < n ? ld4<0>(pr, i, a.vec & 2u) : splat(0.0f);
+    x[j] = i < n ? ld4<0>(px, i) : splat(0.0f), h[j] = i < n ? ld4<0>(pr, i) : splat(0.0f);
   }
   const float s1 = a.w ? row_scale<NV>(x, rn, a.eps, part[0]) : 1.0f;
 #pragma unroll
   for (u32 j = 0; j < NV; j++) {
     const u32 i = 4u * threadIdx.x + j * step;
     if (i < n) {
-      if (a.w) x[j] = x[j] * s1 * ld4<0>(a.w, i, a.vec & 4u);
+      if (a.w) x[j] = x[j] * s1 * ld4<0>(a.w, i);
       h[j] = fma4(splat(a.scale), x[j], h[j]);
-      st4<0>((uint8_t *)a.h + (u64)blockIdx.y * a.hs, i, h[j], a.vec & 16u);
+      st4<0>((uint8_t *)a.h + (u64)blockIdx.y * a.hs, i, h[j]);
     }
   }
   const float s2 = row_scale<NV>(h, rn, a.eps, part[1]);
@@ -1030,8 +1038,8 @@ __device__ __forceinline__ void norm_res_body(const amdc_norm_args &a) {
   for (u32 j = 0; j < NV; j++) {
     const u32 i = 4u * threadIdx.x + j * step;
     const bool on = i < n;
-    const v4f y = h[j] * s2 * ld4<0>(a.w2, on ? i : 0u, a.vec & 32u);
-    if (on && a.y) st4<0>((uint8_t *)a.y + (u64)blockIdx.y * a.ys, i, y, a.vec & 8u);
+    const v4f y = h[j] * s2 * ld4<0>(a.w2, on ? i : 0u);
+    if (on && a.y) st4<0>((uint8_t *)a.y + (u64)blockIdx.y * a.ys, i, y);
     if (a.q) quant_vec4(y, (on ? i : 0u) >> 5, on, a.q + (u64)blockIdx.y * a.qs, n >> 5);
   }
 }

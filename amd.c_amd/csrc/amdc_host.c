@@ -294,8 +294,8 @@ enum {
   K_ATTN_PRE = K_ATTN_DEC2 + 8, /* amdc_attn_pre_h64_f16, .. */
   K_ATTN_JOIN = K_ATTN_PRE + 12, /* amdc_attn_join_f32, _f16, _bf16: in the order of AMDC_TYPE_* */
   K_TAKE_FLAG = K_ATTN_JOIN + 3,
-  K_CONV, /* amdc_conv_w2_f32, _f16, _bf16, then w3, w4 */
-  K_GDN_REC = K_CONV + 9, /* amdc_gdn_rec_h64_f32, _f16, _bf16, then h128 */
+  K_CONV, /* amdc_conv_w2_f32, _f16, _bf16, _f32_odd, _f16_odd, _bf16_odd, then w3, w4 */
+  K_GDN_REC = K_CONV + 18, /* amdc_gdn_rec_h64_f32, _f16, _bf16, then h128 */
   K_GDN_PREP = K_GDN_REC + 6, /* amdc_gdn_prep_h64_f32, _f16, _bf16, then h128 */
   K_GDN_SCAN = K_GDN_PREP + 6, /* amdc_gdn_scan_h64_f32, _f16, _bf16, _f16_odd, _bf16_odd, then h128 */
   K_NORM_GATE = K_GDN_SCAN + 10, /* amdc_norm_gate_f32, _f16, _bf16 */
@@ -307,6 +307,7 @@ enum {
 #define KA2(s) KN(s "_f16_n2"), KN(s "_f16_f32_n2"), KN(s "_bf16_n2"), KN(s "_bf16_f32_n2")
 #define KA(s) KN(s "_f16"), KN(s "_f16_f32"), KN(s "_bf16"), KN(s "_bf16_f32")
 #define KT(s) KN(s "_f32"), KN(s "_f16"), KN(s "_bf16")
+#define KC(s) KT(s), KN(s "_f32_odd"), KN(s "_f16_odd"), KN(s "_bf16_odd")
 #define GW(s) "amdc_gemmw_" s
 static const char *const kname[K_N] = {
     "amdc_quant_q8",           "amdc_dots_q4_0",          "amdc_dots_q4_k",          "amdc_gemm_q4_k_n128",
@@ -339,7 +340,7 @@ static const char *const kname[K_N] = {
     KA("attn_dec_h64"), KA("attn_dec_h128"), KA("attn_dec_h256"), KA2("attn_dec_h64"), KA2("attn_dec_h128"),
     KA("attn_pre_h64"), KA("attn_pre_h128"), KA("attn_pre_h256"),
     KN("attn_join_f32"), KN("attn_join_f16"), KN("attn_join_bf16"), KN("take_flag"),
-    KT("conv_w2"), KT("conv_w3"), KT("conv_w4"), KT("gdn_rec_h64"), KT("gdn_rec_h128"), KT("gdn_prep_h64"), KT("gdn_prep_h128"),
+    KC("conv_w2"), KC("conv_w3"), KC("conv_w4"), KT("gdn_rec_h64"), KT("gdn_rec_h128"), KT("gdn_prep_h64"), KT("gdn_prep_h128"),
     KT("gdn_scan_h64"), KN("gdn_scan_h64_f16_odd"), KN("gdn_scan_h64_bf16_odd"),
     KT("gdn_scan_h128"), KN("gdn_scan_h128_f16_odd"), KN("gdn_scan_h128_bf16_odd"), KT("norm_gate"),
     KN("norm_res_1"), KN("norm_res_2"), KN("norm_res_4"), KN("norm_res_8")};
@@ -1837,9 +1838,6 @@ static int check_slots(const char *op, const amdc_slots *sl, const void *states,
 }
 static int type_ok(int t) { return t == AMDC_TYPE_F32 || t == AMDC_TYPE_F16 || t == AMDC_TYPE_BF16; }
 static u32 type_bytes(int t) { return t == AMDC_TYPE_F32 ? 4u : 2u; }
-/* rows of s values of es bytes, aligned to four values */
-static int vec4_rows(const void *p, u32 rows, u32 s, u32 es) { return (((uintptr_t)p | (rows > 1u ? (u64)s * es : 0u)) & (4u * es - 1u)) == 0; }
-
 size_t amdc_conv_bytes(uint32_t ch, uint32_t width, uint32_t n_slots) {
   if (!ch || ch > (1u << 20) || width < 2u || width > 4u || !n_slots || n_slots > 0x7FFFFFFFu) return 0;
   return (size_t)n_slots * (width - 1u) * ch * sizeof(float);
@@ -1862,12 +1860,11 @@ int amdc_conv(const amdc_slots *slots, float *states, const float *x, const floa
   /* workgroups of one wave while the call's are few: they spread over the CUs */
   const u32 upb = (T + AMDC_CONV_ROWS - 1u) / AMDC_CONV_ROWS;
   const u64 units = cu ? (u64)rows / AMDC_CONV_ROWS + slots->n_seq : (u64)slots->n_seq * upb;
-  const u32 cols = (ch + 3u) / 4u, nt = units * ((cols + 255u) / 256u) < 4u * (u64)(g_cus > 0 ? g_cus : 256) ? 64u : 256u, cb = (cols + nt - 1u) / nt;
+  const u32 cols = ch % 4u ? ch : ch / 4u, nt = units * ((cols + 255u) / 256u) < 4u * (u64)(g_cus > 0 ? g_cus : 256) ? 64u : 256u, cb = (cols + nt - 1u) / nt;
   if (units * cb >= (1u << 24)) return fail(AMDC_EINVAL, "conv: %u rows of %u sequences and %u channels are too many for one call", rows, slots->n_seq, ch);
-  const u32 vec = (ch % 4u == 0 && vec4_rows(x, rows, xs, 4u) ? 1u : 0u) | (ch % 4u == 0 && vec4_rows(y, rows, ys, type_bytes(t)) ? 2u : 0u);
-  amdc_conv_args a = {states, x, w, bias, y, ch, xs, ys, cb, upb, (u32)act, vec};
+  amdc_conv_args a = {states, x, w, bias, y, ch, xs, ys, cb, upb, (u32)act};
   void *args[] = {&d, &a};
-  return launch_nt(K_CONV + 3 * (int)(width - 2u) + t, (unsigned)(units * cb), 1, nt, 0, stream, args);
+  return launch_nt(K_CONV + 6 * (int)(width - 2u) + (ch % 4u ? 3 : 0) + t, (unsigned)(units * cb), 1, nt, 0, stream, args);
 }
 
 size_t amdc_gdn_bytes(uint32_t n_v, uint32_t dk, uint32_t dv, uint32_t n_slots) {
@@ -1893,10 +1890,8 @@ static int check_gdn(const char *op, const amdc_gdn *g, const amdc_slots *sl, fl
   if (y == q || y == k || y == v) return fail(AMDC_EINVAL, "%s: y cannot be q, k or v", op);
   if (rows > 1u && (qs < wk || ks < wk || vs < wv || ys < wv || as < g->n_v || bs < g->n_v))
     return fail(AMDC_EINVAL, "%s: strides qs %u, ks %u, vs %u, as %u, bs %u, ys %u under a row's values (%u, %u, %u)", op, qs, ks, vs, as, bs, ys, wk, wv, g->n_v);
-  const u32 vec = (vec4_rows(v, rows, vs, es) ? 1u : 0u) | (vec4_rows(y, rows, ys, es) ? 2u : 0u) | (vec4_rows(k, rows, ks, es) ? 4u : 0u) | (vec4_rows(q, rows, qs, es) ? 8u : 0u) |
-                  (!(((uintptr_t)v | (rows > 1u ? (u64)vs * es : 0u)) & (2u * es - 1u)) ? 16u : 0u) | (!(((uintptr_t)y | (rows > 1u ? (u64)ys * es : 0u)) & (2u * es - 1u)) ? 32u : 0u);
   *d = (amdc_gdn_args){.s = states, .q = q, .k = k, .v = v, .a = a, .b = b, .A = g->A, .dt = g->dt, .y = y, .scale = g->scale, .eps = g->eps, .n_k = g->n_k, .n_v = g->n_v, .dv = g->dv,
-                       .G = g->n_v / g->n_k, .tiled = g->order == AMDC_HEADS_TILED, .qs = qs, .ks = ks, .vs = vs, .as = as, .bs = bs, .ys = ys, .vec = vec};
+                       .G = g->n_v / g->n_k, .tiled = g->order == AMDC_HEADS_TILED, .qs = qs, .ks = ks, .vs = vs, .as = as, .bs = bs, .ys = ys};
   return AMDC_OK;
 }
 int amdc_gdn_decode(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
@@ -1947,7 +1942,9 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
   const u64 state = (u64)gdn->n_v * gdn->dk * gdn->dv;
   float *in = (float *)(((uintptr_t)ws + 127u) & ~(uintptr_t)127u), *out = in + state; /* slots begin with a line */
   g.ws = (uint8_t *)(out + state);
-  const int prep = K_GDN_PREP + (gdn->dk == 128u ? 3 : 0) + t, scan = K_GDN_SCAN + (gdn->dk == 128u ? 5 : 0) + (t == AMDC_TYPE_F32 || (g.vec & 16u && g.vec & 32u) ? t : t + 2);
+  /* two 16-bit values side by side in rows of v and y are aligned to both */
+  const int pair = (((uintptr_t)v | (uintptr_t)y | (rows > 1u ? 2u * (vs | ys) : 0u)) & 3u) == 0;
+  const int prep = K_GDN_PREP + (gdn->dk == 128u ? 3 : 0) + t, scan = K_GDN_SCAN + (gdn->dk == 128u ? 5 : 0) + (t == AMDC_TYPE_F32 || pair ? t : t + 2);
   for (g.s0 = 0; g.s0 < total; g.s0 += most) {
     g.ns = total - g.s0 < most ? total - g.s0 : most;
     /* the sequences with chunks in these slots: one for each slot, and the one that goes on */
@@ -1979,9 +1976,7 @@ int amdc_norm_gate_q8(const void *x, int t, const float *w, const float *z, floa
     return fail(AMDC_EINVAL, "norm_gate_q8: x, w, z and y must be aligned to their types, q to 4 bytes");
   if (!stride_ok(T, xs, n, es) || !stride_ok(T, zs, n, 4u) || (y && !stride_ok(T, ys, n, 4u)) || (q && T > 1u && (qs % 4u || qs < 40u * (n / 32u))))
     return fail(AMDC_EINVAL, "norm_gate_q8: strides xs %u, zs %u, ys %u, qs %u too small or unaligned for %u values", xs, zs, ys, qs, n);
-  const u32 vec = (vec_rows(x, T > 1u ? xs : 0u, 4u * es) ? 1u : 0u) | (vec_rows(z, T > 1u ? zs : 0u, 16u) ? 2u : 0u) | (aligned16(w) ? 4u : 0u) |
-                  (vec_rows(y, T > 1u ? ys : 0u, 16u) ? 8u : 0u);
-  amdc_norm_args a = {.x = x, .w = w, .z = z, .y = y, .q = q, .eps = eps, .n = n, .hd = hd, .xs = xs, .zs = zs, .ys = ys, .qs = qs, .gate = gate == AMDC_GATE_SIGMOID, .vec = vec};
+  amdc_norm_args a = {.x = x, .w = w, .z = z, .y = y, .q = q, .eps = eps, .n = n, .hd = hd, .xs = xs, .zs = zs, .ys = ys, .qs = qs, .gate = gate == AMDC_GATE_SIGMOID};
   void *args[] = {&a};
   return launch(K_NORM_GATE + t, (n + 1023u) / 1024u, T, 0, stream, args);
 }
@@ -1997,9 +1992,7 @@ int amdc_norm_res_q8(const float *x, const float *w1, float scale, const float *
   if (!stride_ok(T, xs, n, 4u) || !stride_ok(T, rs, n, 4u) || !stride_ok(T, hs, n, 4u) || (y && !stride_ok(T, ys, n, 4u)) || (q && T > 1u && (qs % 4u || qs < 40u * (n / 32u))))
     return fail(AMDC_EINVAL, "norm_res_q8: strides xs %u, rs %u, hs %u, ys %u, qs %u too small or unaligned for %u values", xs, rs, hs, ys, qs, n);
   if (h == y || (h == res && T > 1u && hs != rs) || (h == x && T > 1u && hs != xs)) return fail(AMDC_EINVAL, "norm_res_q8: h cannot be y; in place (h = res or x) it needs its stride");
-  const u32 vec = (vec_rows(x, T > 1u ? xs : 0u, 16u) ? 1u : 0u) | (vec_rows(res, T > 1u ? rs : 0u, 16u) ? 2u : 0u) | (aligned16(w1) ? 4u : 0u) |
-                  (vec_rows(y, T > 1u ? ys : 0u, 16u) ? 8u : 0u) | (vec_rows(h, T > 1u ? hs : 0u, 16u) ? 16u : 0u) | (aligned16(w2) ? 32u : 0u);
-  amdc_norm_args a = {x, w1, res, w2, h, y, q, eps, scale, n, 0, xs, rs, hs, ys, qs, 0, vec};
+  amdc_norm_args a = {x, w1, res, w2, h, y, q, eps, scale, n, 0, xs, rs, hs, ys, qs, 0};
   /* few rows: a thread to four values, up to 1024; many: 256 threads, up to 32 values each */
   const u32 fours = n / 4u, most = T >= 256u ? 256u : 1024u;
   u32 nt = (fours + 63u) / 64u * 64u, nv = 0;

@@ -154,7 +154,6 @@ typedef struct {
   const float *x, *w, *bias;
   void *y;
   uint32_t ch, xs, ys, cb /* workgroups to a row */, upb /* units to a sequence (cu NULL) */, act;
-  uint32_t vec; /* 1: rows of x and the state, 2: rows of y are aligned to four values */
 } amdc_conv_args;
 typedef struct {
   float *s;
@@ -166,7 +165,6 @@ typedef struct {
   uint64_t sb;  /* prompts: bytes of a chunk slot of the workspace */
   float scale, eps;
   uint32_t n_k, n_v, dv, G /* n_v / n_k */, tiled, qs, ks, vs, as, bs, ys;
-  uint32_t vec; /* rows that are aligned to four values: 1 v, 2 y, 4 k, 8 q; to two: 16 v, 32 y */
   uint32_t nc, s0, ns, groups; /* prompts: chunks of a sequence (cu NULL), the launch's first chunk slot and their number, sequences times key heads */
 } amdc_gdn_args;
 #define AMDC_GDN_C 64u      /* tokens of a chunk */
@@ -179,7 +177,6 @@ typedef struct {
   uint8_t *q;
   float eps, scale;
   uint32_t n, hd, xs, zs, hs, ys, qs, gate;
-  uint32_t vec; /* aligned to four values: 1 x, 2 z, 4 w, 8 y, 16 h, 32 w2 */
 } amdc_norm_args;
 
 #endif
