@@ -1857,14 +1857,13 @@ int amdc_conv(const amdc_slots *slots, float *states, const float *x, const floa
   if (!vec_rows(x, 0, 4u) || !vec_rows(w, 0, 4u) || !vec_rows(bias, 0, 4u) || !vec_rows(y, 0, type_bytes(t))) return fail(AMDC_EINVAL, "conv: x, w, bias and y must be aligned to their types");
   if ((const void *)x == y) return fail(AMDC_EINVAL, "conv: y cannot be x");
   if (rows > 1u && (xs < ch || ys < ch)) return fail(AMDC_EINVAL, "conv: strides xs %u, ys %u under a row's %u values", xs, ys, ch);
-  /* workgroups of one wave while the call's are few: they spread over the CUs */
-  const u32 upb = (T + AMDC_CONV_ROWS - 1u) / AMDC_CONV_ROWS;
+  const u32 upb = each ? 1u : (T + AMDC_CONV_ROWS - 1u) / AMDC_CONV_ROWS;
   const u64 units = cu ? (u64)rows / AMDC_CONV_ROWS + slots->n_seq : (u64)slots->n_seq * upb;
-  const u32 cols = ch % 4u ? ch : ch / 4u, nt = units * ((cols + 255u) / 256u) < 4u * (u64)(g_cus > 0 ? g_cus : 256) ? 64u : 256u, cb = (cols + nt - 1u) / nt;
-  if (units * cb >= (1u << 24)) return fail(AMDC_EINVAL, "conv: %u rows of %u sequences and %u channels are too many for one call", rows, slots->n_seq, ch);
+  const u32 cb = ((ch % 4u ? ch : ch / 4u) + 63u) / 64u;
+  if (units * cb >= (1u << 26)) return fail(AMDC_EINVAL, "conv: %u rows of %u sequences and %u channels are too many for one call", rows, slots->n_seq, ch);
   amdc_conv_args a = {states, x, w, bias, y, ch, xs, ys, cb, upb, (u32)act};
   void *args[] = {&d, &a};
-  return launch_nt(K_CONV + 6 * (int)(width - 2u) + (ch % 4u ? 3 : 0) + t, (unsigned)(units * cb), 1, nt, 0, stream, args);
+  return launch_nt(K_CONV + 6 * (int)(width - 2u) + (ch % 4u ? 3 : 0) + t, (unsigned)(units * cb), 1, 64u, 0, stream, args);
 }
 
 size_t amdc_gdn_bytes(uint32_t n_v, uint32_t dk, uint32_t dv, uint32_t n_slots) {

@@ -147,7 +147,7 @@ typedef struct {
   uint32_t *bad;
   uint32_t n_seq, n_slots, T, each;
 } amdc_slots_dev;
-#define AMDC_CONV_ROWS 32u /* rows of a sequence that a thread of the convolution goes over */
+#define AMDC_CONV_ROWS 8u /* rows of a sequence that a thread of the convolution goes over */
 #define AMDC_LIN_MAX_T 16u /* the most new tokens of a sequence in a decode call, or whose states are kept one by one */
 typedef struct {
   float *state;
