@@ -403,7 +403,9 @@ int amdc_conv(const amdc_slots *slots, float *states, const float *x, const floa
  * (amdc_gdn_bytes()). A and dt: n_v device floats (A is negative: -exp of what is learned). eps is above 0. All sums, states
  * and gates are f32 or more, whatever the rows' type t (that of q, k, v and y): y is rounded once. Rows are qs, ks, vs, as, bs and ys
  * values apart; y is none of the inputs. A q, k, v, a or b that is not finite makes NaN or infinite what the formula makes of it (a value its
- * column alone); prompts: the rows of up to 63 tokens before it too. */
+ * column alone); prompts: the rows of up to 63 tokens before it too. Token after token a row is off by roundings of its own size; prompts
+ * are worked in chunks of 64 tokens, and a column of a chunk is off by up to about 2^-26 of its largest |v| and |S| in that chunk and the
+ * one before, however small the row itself. */
 enum { AMDC_HEADS_GROUPED = 0, AMDC_HEADS_TILED = 1 };
 typedef struct {
   uint32_t n_k, n_v, dk, dv;
@@ -416,7 +418,7 @@ size_t amdc_gdn_bytes(uint32_t n_v, uint32_t dk, uint32_t dv, uint32_t n_slots);
 int amdc_gdn_decode(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
                     uint32_t T, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t as, uint32_t bs, uint32_t ys, int each, void *stream);
 /* Any numbers of new tokens: prompts, or chunks of them, packed (cu) or T each. vs and ys are under 2^23. ws: amdc_gdn_prefill_ws(gdn, n_seq, rows) bytes of
- * device memory (rows = T with cu, n_seq T without), 16-byte aligned, of any content; calls that share it must not overlap on the
+ * device memory (rows = T with cu, n_seq T without; longer prompts go through it part by part, so that it is hardly over half a GB), 16-byte aligned, of any content; calls that share it must not overlap on the
  * device. Nothing is allocated: every call can be captured. */
 size_t amdc_gdn_prefill_ws(const amdc_gdn *gdn, uint32_t n_seq, uint32_t rows);
 int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
