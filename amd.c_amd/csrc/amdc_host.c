@@ -1992,12 +1992,11 @@ int amdc_norm_res_q8(const float *x, const float *w1, float scale, const float *
     return fail(AMDC_EINVAL, "norm_res_q8: strides xs %u, rs %u, hs %u, ys %u, qs %u too small or unaligned for %u values", xs, rs, hs, ys, qs, n);
   if (h == y || (h == res && T > 1u && hs != rs) || (h == x && T > 1u && hs != xs)) return fail(AMDC_EINVAL, "norm_res_q8: h cannot be y; in place (h = res or x) it needs its stride");
   amdc_norm_args a = {x, w1, res, w2, h, y, q, eps, scale, n, 0, xs, rs, hs, ys, qs, 0};
-  /* few rows: a thread to four values, up to 1024; many: 256 threads, up to 32 values each */
-  const u32 fours = n / 4u, most = T >= 256u ? 256u : 1024u;
-  u32 nt = (fours + 63u) / 64u * 64u, nv = 0;
-  if (nt > most) nt = most;
-  if ((fours + nt - 1u) / nt > 8u) nt = 1024u;
-  while ((1u << nv) * nt < fours) nv++;
+  /* fours to a thread, a power of two, of at most 1024 threads; then as few threads as that takes */
+  const u32 fours = n / 4u;
+  u32 nv = 0;
+  while ((1024u << nv) < fours) nv++;
+  const u32 nt = (((fours + (1u << nv) - 1u) >> nv) + 63u) / 64u * 64u;
   void *args[] = {&a};
   return launch_nt(K_NORM_RES + (int)nv, 1, T, nt, 0, stream, args);
 }
