@@ -1016,18 +1016,21 @@ __device__ __forceinline__ void norm_res_body(const amdc_norm_args &a) {
   const u32 n = a.n, step = 4u * blockDim.x;
   const float rn = 1.0f / (float)n;
   const uint8_t *px = (const uint8_t *)a.x + (u64)blockIdx.y * a.xs, *pr = (const uint8_t *)a.z + (u64)blockIdx.y * a.zs;
-  v4f x[NV], h[NV];
+  constexpr bool EARLY = NV <= 2u; // the weights beside the rows; more do not fit the registers
+  v4f x[NV], h[NV], w1[EARLY ? NV : 1u], w2[EARLY ? NV : 1u];
 #pragma unroll
   for (u32 j = 0; j < NV; j++) {
-    const u32 i = 4u * threadIdx.x + j * step;
-    x[j] = i < n ? ld4<0>(px, i) : splat(0.0f), h[j] = i < n ? ld4<0>(pr, i) : splat(0.0f);
+    const u32 i = 4u * threadIdx.x + j * step, k = i < n ? i : n - 4u;
+    x[j] = ld4<0>(px, k), h[j] = ld4<0>(pr, k);
+    if (i >= n) x[j] = h[j] = splat(0.0f);
+    if constexpr (EARLY) w1[j] = a.w ? ld4<0>(a.w, k) : splat(1.0f), w2[j] = ld4<0>(a.w2, k);
   }
   const float s1 = a.w ? row_scale<NV>(x, rn, a.eps, part[0]) : 1.0f;
 #pragma unroll
   for (u32 j = 0; j < NV; j++) {
     const u32 i = 4u * threadIdx.x + j * step;
     if (i < n) {
-      if (a.w) x[j] = x[j] * s1 * ld4<0>(a.w, i);
+      if (a.w) x[j] = x[j] * s1 * (EARLY ? w1[EARLY ? j : 0u] : ld4<0>(a.w, i));
       h[j] = fma4(splat(a.scale), x[j], h[j]);
       st4<0>((uint8_t *)a.h + (u64)blockIdx.y * a.hs, i, h[j]);
     }
@@ -1037,7 +1040,7 @@ __device__ __forceinline__ void norm_res_body(const amdc_norm_args &a) {
   for (u32 j = 0; j < NV; j++) {
     const u32 i = 4u * threadIdx.x + j * step;
     const bool on = i < n;
-    const v4f y = h[j] * s2 * ld4<0>(a.w2, on ? i : 0u);
+    const v4f y = h[j] * s2 * (EARLY ? w2[EARLY ? j : 0u] : ld4<0>(a.w2, on ? i : 0u));
     if (on && a.y) st4<0>((uint8_t *)a.y + (u64)blockIdx.y * a.ys, i, y);
     if (a.q) quant_vec4(y, (on ? i : 0u) >> 5, on, a.q + (u64)blockIdx.y * a.qs, n >> 5);
   }
