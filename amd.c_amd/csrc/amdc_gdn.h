@@ -92,9 +92,9 @@ __device__ __forceinline__ float sigmoid_fast(float v) { return __builtin_amdgcn
 // AMDC_CONV_ROWS rows of a sequence, which are all in flight at once, with the W - 1 inputs before them. The unit of a sequence's first
 // rows reads the state and, after that, writes it: from x where the sequence has rows enough, and else from what it has read, so that a
 // slot may be read and written by the same call; with `each` one unit has all rows of a sequence, eight after eight, for the same
-// reason. Workgroups of one wave; 8192 channels, 9 prompts of 1100 tokens into bf16: units of
-// 8 rows 85 us (5.7 TB/s), of 4 90 us, of 32 with 8 rows in flight 105 us; 256 threads 87 us; units that follow each other on one XCD
-// 87 us (the rows that two units read come from the last-level cache). One token of 10240 channels: 3.3 us.
+// reason. Workgroups of one wave. 8192 channels, 9 prompts of 1100 tokens, into bf16: units of 8 rows 85 us (5.7 TB/s), of 4 90 us, of 32 with 8
+// rows in flight 105 us; 256 threads 87 us; units that follow each other on one XCD 87 us (the rows that two units read come from
+// the last-level cache). One token of 10240 channels: 3.2 us.
 template <u32 W, int TY, u32 C>
 __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_conv_args &a) {
   const u32 ct = blockIdx.x % a.cb, u = blockIdx.x / a.cb, c = C * (ct * blockDim.x + threadIdx.x);
@@ -212,8 +212,9 @@ __device__ __forceinline__ float sum16(float v) {
 // goes through the sequence's tokens alone, without the LDS and without a barrier: lane l has the rows 16 i + l / 4 of the columns 4 (l % 4) .. + 3.
 // With k and q of norm 1 (their factors rk, rq) and the state as it is before the token's decay e,
 //   u = rate (v - e rk k S),  S' = e S + rk k^T u,  y = rq q S' = rq (e q S + rk (q.k) u),
-// so that k S, q S, k.k, q.q and k.q go through one reduction a token. Reading and writing the states bounds it for batches; a single
-// sequence waits for two dependent loads (its slot, the state).
+// so that k S, q S, k.k, q.q and k.q go through one reduction a token. Reading and writing the states bounds it for batches: 96
+// sequences of 32 heads of 128 x 128, 405 MB, in 84 us (4.8 TB/s, a copy's rate here); 8 of 48 heads and 5 tokens, a state kept after each,
+// 154 MB in 35 us. A single sequence waits for two dependent loads (its slot, the state): 4.6 us.
 template <int TY, u32 DK>
 __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
   constexpr u32 NI = DK / 16u;
@@ -291,7 +292,10 @@ GDN_RECS(64) GDN_RECS(128)
 //   y_i = e^(G_i) q_i S + sum_(j <= i) e^(G_i - G_j) q_i.k_j u_j,   S <- e^(G_63) S + sum_j e^(G_63 - G_j) k_j^T u_j.
 // Two launches: amdc_gdn_prep computes what does not depend on the state, for all chunks at once: M = (I + L)^-1 and the weights
 // A_ij = e^(G_i - G_j) q_i.k_j for each value head, and the normed keys and queries as operands; amdc_gdn_scan takes the chunks of a sequence
-// one after the other, 32 columns of a head's state to a workgroup.
+// one after the other, 32 columns of a head's state to a workgroup. A prompt of 12000 tokens, 16 heads of keys and 48 of values of 128: 0.58 ms, 0.14 of
+// it amdc_gdn_prep's, which writes 0.51 GB of operands (4.4 TB/s with what it reads); token after token it takes 11.1 ms. Prompts go through
+// the workspace in parts of AMDC_GDN_WS bytes: 48 MB 0.77 ms, 96 MB 0.68, 160 MB 0.64, 256 MB 0.61, 512 MB 0.58 (a launch of the scan begins and
+// ends with all its workgroups).
 //
 // Exponents are of differences that are at most 0, and those are taken in 64 bits: after a strong decay the sums are large and
 // their differences small. |M_ij|, |A_ij| <= 1: (I - beta k^T k) shrinks whatever it multiplies, for beta <= 1 and |k| <= 1.
@@ -608,6 +612,9 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
 // A column's R, U and its next S are under 12 max |S| + 65 max |beta v| of the chunk (a token adds at most beta |v| to the column's norm, and the rest of
 // its step shrinks it): the power of two of this bound brings them into f16's range, and as they share it U needs no scaling. max |S| is not waited for:
 // what it was a chunk before bounds it, by the same rule. S is kept as the products with K^T give it: they add to it.
+// A chunk takes 2.3 to 2.5 us, waits of many kinds: matrix units 28 % busy, vector units 37 %, the LDS 35 %; without its products it
+// would take 92 % of that, without its reads of the workspace 93 %. 16 columns a workgroup would read the workspace twice as
+// often, 64 leave half of the CUs idle.
 // PAIR: two values side by side in v and y are aligned to both (32-bit ones need not be).
 template <int TY, u32 DK, bool PAIR>
 __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
@@ -616,7 +623,8 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   __shared__ __align__(16) float s_smax[2][4][32], s_vmax[2][4][32], s_cf[4][4][64];
   const u32 tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), w = wave & 3u, n = lane & 15u, gr = lane >> 4;
   const u32 nb = (g.dv + 31u) / 32u, per = g.G * nb;
-  // the workgroups of a key head are on one XCD (workgroups go round the 8 of them), where the group count allows it
+  // the workgroups of a key head are on one XCD (workgroups go round the 8 of them), where the group count allows it: 12000 tokens 578 us, as they
+  // come 666; 77 tokens 22.3 and 24.2
   u32 gi, in;
   if (g.groups >= 8u) {
     const u32 x = blockIdx.x & 7u, y = blockIdx.x >> 3;
@@ -969,7 +977,7 @@ GDN_PRES(64) GDN_PRES(128)
 // ------------------------------------------------------------------ the norms
 
 // y = x s w gate(z), s = 1 / sqrt(sum x^2 / hd + eps) over a head, and its Q8 copy. Reading and writing bound it. Four values a lane, hd / 4 lanes a
-// head. Grid (ceil(n / 1024), T).
+// head. Grid (ceil(n / 1024), T). 4097 rows of 32 heads of 128 from bf16: 168 MB in 31 us (5.4 TB/s); one row of 48 heads 2.4 us.
 template <int TY>
 __device__ __forceinline__ void norm_gate_body(const amdc_norm_args &a) {
   const u32 i0 = 4u * (blockIdx.x * NT + threadIdx.x), n = a.n;
@@ -1009,7 +1017,9 @@ __device__ __forceinline__ float row_scale(const v4f (&x)[NV], float rn, float e
 }
 
 // h = res + scale (x s1 w1, or x itself), y = h s2 w2 and its Q8 copy: a row to a workgroup, which keeps it in its registers between the two
-// norms. h may be res: a thread reads and writes the same places. Grid (1, T).
+// norms. h may be res: a thread reads and writes the same places. Grid (1, T). Reading and writing bound it: 3001 rows of 4096, 197 MB, in 41 us
+// (4.8 TB/s, a copy's rate); one row of 5120 3.5 us. 256 threads of more values each: 45 and 4.8 us (1024 rows of 4096, which the caches
+// hold, 12.3 against 12.6).
 template <u32 NV>
 __device__ __forceinline__ void norm_res_body(const amdc_norm_args &a) {
   __shared__ float part[2][16];
