@@ -1886,7 +1886,7 @@ static int check_gdn(const char *op, const amdc_gdn *g, const amdc_slots *sl, fl
   if (!vec_rows(q, 0, es) || !vec_rows(k, 0, es) || !vec_rows(v, 0, es) || !vec_rows(y, 0, es) || !vec_rows(a, 0, 4u) || !vec_rows(b, 0, 4u) || !vec_rows(g->A, 0, 4u) ||
       !vec_rows(g->dt, 0, 4u))
     return fail(AMDC_EINVAL, "%s: q, k, v, y, a, b, A and dt must be aligned to their types", op);
-  if (y == q || y == k || y == v) return fail(AMDC_EINVAL, "%s: y cannot be q, k or v", op);
+  if (y == q || y == k || y == v || y == a || y == b) return fail(AMDC_EINVAL, "%s: y cannot be q, k, v, a or b", op);
   if (rows > 1u && (qs < wk || ks < wk || vs < wv || ys < wv || as < g->n_v || bs < g->n_v))
     return fail(AMDC_EINVAL, "%s: strides qs %u, ks %u, vs %u, as %u, bs %u, ys %u under a row's values (%u, %u, %u)", op, qs, ks, vs, as, bs, ys, wk, wv, g->n_v);
   *d = (amdc_gdn_args){.s = states, .q = q, .k = k, .v = v, .a = a, .b = b, .A = g->A, .dt = g->dt, .y = y, .scale = g->scale, .eps = g->eps, .n_k = g->n_k, .n_v = g->n_v, .dv = g->dv,
@@ -1975,6 +1975,8 @@ int amdc_norm_gate_q8(const void *x, int t, const float *w, const float *z, floa
     return fail(AMDC_EINVAL, "norm_gate_q8: x, w, z and y must be aligned to their types, q to 4 bytes");
   if (!stride_ok(T, xs, n, es) || !stride_ok(T, zs, n, 4u) || (y && !stride_ok(T, ys, n, 4u)) || (q && T > 1u && (qs % 4u || qs < 40u * (n / 32u))))
     return fail(AMDC_EINVAL, "norm_gate_q8: strides xs %u, zs %u, ys %u, qs %u too small or unaligned for %u values", xs, zs, ys, qs, n);
+  if ((y == z && T > 1u && ys != zs) || ((const void *)y == x && (t != AMDC_TYPE_F32 || (T > 1u && ys != xs))))
+    return fail(AMDC_EINVAL, "norm_gate_q8: y in place of z, or of an f32 x, needs its stride");
   amdc_norm_args a = {.x = x, .w = w, .z = z, .y = y, .q = q, .eps = eps, .n = n, .hd = hd, .xs = xs, .zs = zs, .ys = ys, .qs = qs, .gate = gate == AMDC_GATE_SIGMOID};
   void *args[] = {&a};
   return launch(K_NORM_GATE + t, (n + 1023u) / 1024u, T, 0, stream, args);
@@ -1990,7 +1992,8 @@ int amdc_norm_res_q8(const float *x, const float *w1, float scale, const float *
     return fail(AMDC_EINVAL, "norm_res_q8: every pointer must be 4-byte aligned");
   if (!stride_ok(T, xs, n, 4u) || !stride_ok(T, rs, n, 4u) || !stride_ok(T, hs, n, 4u) || (y && !stride_ok(T, ys, n, 4u)) || (q && T > 1u && (qs % 4u || qs < 40u * (n / 32u))))
     return fail(AMDC_EINVAL, "norm_res_q8: strides xs %u, rs %u, hs %u, ys %u, qs %u too small or unaligned for %u values", xs, rs, hs, ys, qs, n);
-  if (h == y || (h == res && T > 1u && hs != rs) || (h == x && T > 1u && hs != xs)) return fail(AMDC_EINVAL, "norm_res_q8: h cannot be y; in place (h = res or x) it needs its stride");
+  if (h == y || (T > 1u && ((h == res && hs != rs) || (h == x && hs != xs) || (y == res && ys != rs) || (y == x && ys != xs))))
+    return fail(AMDC_EINVAL, "norm_res_q8: h cannot be y; in place of res or x, h and y need its stride");
   amdc_norm_args a = {x, w1, res, w2, h, y, q, eps, scale, n, 0, xs, rs, hs, ys, qs, 0};
   /* fours to a thread, a power of two, of at most 1024 threads; then as few threads as that takes */
   const u32 fours = n / 4u;

@@ -427,14 +427,14 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
 /* The norm of each of n_h heads of hd (32, 64, 128 or 256) values, times its gate: of T rows, with s = 1 / sqrt(sum x^2 / hd + eps) of a head,
  *   y = x s w gate(z),  gate(z) = z / (1 + exp(-z)) (AMDC_GATE_SILU) or 1 / (1 + exp(-z)) (AMDC_GATE_SIGMOID)
  * x has type t, w has hd floats that all heads share, z and y n_h hd floats a row; y or q may be NULL; q: the Q8 copy, bit for bit amdc_quant_q8 of
- * y. Strides are bytes, as amdc_rmsnorm_q8's. y may be z, or x where that is f32, at the same stride. */
+ * y. T is up to 65535, strides are bytes, as amdc_rmsnorm_q8's. y may be z, or x where that is f32, at the same stride. */
 enum { AMDC_GATE_SILU = 0, AMDC_GATE_SIGMOID = 1 };
 int amdc_norm_gate_q8(const void *x, int t, const float *w, const float *z, float *y, uint32_t n_h, uint32_t hd, float eps, int gate, uint8_t *q, uint32_t T, uint32_t xs,
                       uint32_t zs, uint32_t ys, uint32_t qs, void *stream);
 /* Between two blocks: the norm behind the first (w1 NULL: none), the residual, and the norm before the second, of T rows of n (a multiple of
  * 32, at most 32768) values:
  *   h = res + scale x s1 w1,  y = h s2 w2,  s1 and s2 the factors 1 / sqrt(mean square + eps) of x and h
- * and q the Q8 copy of y, bit for bit amdc_quant_q8's (y or q may be NULL). h may be res or x (at the same stride), y is not h. Strides are bytes. */
+ * and q the Q8 copy of y, bit for bit amdc_quant_q8's (y or q may be NULL). h and y may be res or x (at the same stride), y is not h. T is up to 65535, strides are bytes. */
 int amdc_norm_res_q8(const float *x, const float *w1, float scale, const float *res, float *h, const float *w2, float *y, uint32_t n, float eps, uint8_t *q, uint32_t T,
                      uint32_t xs, uint32_t rs, uint32_t hs, uint32_t ys, uint32_t qs, void *stream);
 

@@ -104,3 +104,19 @@ def test_bytes():
     for n_seq, rows in ((0, 1), (1, 0), (1, (1 << 22) + 1), ((1 << 20) + 1, 5)):
         with pytest.raises(amdc.AmdcError):
             amdc.gdn_prefill_ws(amdc.Gdn(**GDN), n_seq, rows)
+
+
+ALIASED = {"gdn_decode": [dict(a=8192), dict(b=8192)], "gdn_prefill": [dict(a=8192), dict(b=8192)],
+           "norm_gate_q8": [dict(y=8192, ys=772), dict(y=8192, zs=772), dict(y=4096), dict(y=4096, type=0, xs=772), dict(y=4096, T=1)],
+           "norm_res_q8": [dict(y=8192, ys=388), dict(y=4096, xs=388), dict(y=4096, h=4096)]}
+IN_PLACE = {"norm_gate_q8": [dict(y=8192), dict(y=4096, type=0, xs=768), dict(y=8192, T=1, ys=0)], "norm_res_q8": [dict(y=8192), dict(y=4096), dict(y=8192, T=1, ys=0), dict(y=4096, h=8192)]}
+
+
+@pytest.mark.parametrize("op", sorted(ALIASED))
+def test_aliases(stub, op):  # noqa: F811
+    """An output in an input's place is taken where a thread reads what it writes, and refused elsewhere."""
+    for change, (err, launches, _) in zip(ALIASED[op], calls(stub, op, [(None, c) for c in ALIASED[op]])):
+        assert err.startswith(op) and launches == 0, (change, err)
+    if op in IN_PLACE:
+        for change, (err, launches, _) in zip(IN_PLACE[op], calls(stub, op, [(None, c) for c in IN_PLACE[op]])):
+            assert err == "" and launches == 1, (change, err)
