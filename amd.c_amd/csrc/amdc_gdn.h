@@ -216,7 +216,7 @@ __device__ __forceinline__ float sum16(float v) {
 // sequences of 32 heads of 128 x 128, 405 MB, in 84 us (4.8 TB/s, a copy's rate here); 8 of 48 heads and 5 tokens, a state kept after each,
 // 154 MB in 35 us. A single sequence waits for two dependent loads (its slot, the state): 4.6 us.
 template <int TY, u32 DK>
-__device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amdc_gdn_args &g) {
+__device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amdc_gdn_args &g, u32 most) {
   constexpr u32 NI = DK / 16u;
   const u32 lane = threadIdx.x & 63u, ng = g.dv >> 4, w = uniform(4u * blockIdx.x + (threadIdx.x >> 6));
   if (w >= sl.n_seq * g.n_v * ng) return;
@@ -224,7 +224,7 @@ __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amd
   const u32 r = lane >> 2, c4 = lane & 3u;
   u32 row0;
   const u32 m = uniform(slot_rows(sl, b, row0));
-  if (!m) return;
+  if (!m || m > most) return;
   const int f = sl.from[b];
   bool bad;
   const bool have = slot_ok(sl, f, bad);
@@ -280,7 +280,7 @@ __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amd
 }
 
 #define GDN_REC(H, N, TY)                                                                                                            \
-  extern "C" __global__ __launch_bounds__(256) void amdc_gdn_rec_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_rec_body<TY, H##u>(sl, g); }
+  extern "C" __global__ __launch_bounds__(256) void amdc_gdn_rec_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_rec_body<TY, H##u>(sl, g, AMDC_LIN_MAX_T); }
 #define GDN_RECS(H) GDN_REC(H, f32, 0) GDN_REC(H, f16, 1) GDN_REC(H, bf16, 2)
 GDN_RECS(64) GDN_RECS(128)
 
@@ -292,7 +292,9 @@ GDN_RECS(64) GDN_RECS(128)
 //   y_i = e^(G_i) q_i S + sum_(j <= i) e^(G_i - G_j) q_i.k_j u_j,   S <- e^(G_63) S + sum_j e^(G_63 - G_j) k_j^T u_j.
 // Two launches: amdc_gdn_prep computes what does not depend on the state, for all chunks at once: M = (I + L)^-1 and the weights
 // A_ij = e^(G_i - G_j) q_i.k_j for each value head, and the normed keys and queries as operands; amdc_gdn_scan takes the chunks of a sequence
-// one after the other, 32 columns of a head's state to a workgroup. A prompt of 12000 tokens, 16 heads of keys and 48 of values of 128: 0.58 ms, 0.14 of
+// one after the other, 32 columns of a head's state to a workgroup. Of packed prompts the sequences of up to AMDC_LIN_MAX_T rows (decode steps
+// beside prompts) go token after token, in workgroups of amdc_gdn_prep's launch ahead of its own: 96 of one token, 48 heads of 128, in 152 us, as chunks 522; 32 of 5 tokens 80
+// and 171, of 16 162 and 168. A prompt of 12000 tokens, 16 heads of keys and 48 of values of 128: 0.58 ms, 0.14 of
 // it amdc_gdn_prep's, which writes 0.51 GB of operands (4.4 TB/s with what it reads); token after token it takes 11.1 ms. Prompts go through
 // the workspace in parts of AMDC_GDN_WS bytes: 48 MB 0.77 ms, 96 MB 0.68, 160 MB 0.64, 256 MB 0.61, 512 MB 0.58 (a launch of the scan begins and
 // ends with all its workgroups).
@@ -371,12 +373,12 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
   __shared__ double s_G[4][64];
   __shared__ float s_beta[4][64];
   const u32 tid = threadIdx.x, lane = tid & 63u, w = uniform(tid >> 6), n = lane & 15u, gr = lane >> 4;
-  const u32 at = blockIdx.x / g.n_k, hk = blockIdx.x - at * g.n_k, slot = g.s0 + at;
+  const u32 wg = blockIdx.x - g.rec, at = wg / g.n_k, hk = wg - at * g.n_k, slot = g.s0 + at;
   const u32 b = gdn_seq(sl, g.nc, slot);
   if (b >= sl.n_seq) return;
   u32 row0;
   const u32 m = uniform(slot_rows(sl, b, row0)), c = slot - uniform(gdn_base(sl, g.nc, b));
-  if (c >= (m + GDN_C - 1u) / GDN_C) return;
+  if (m <= g.few || c >= (m + GDN_C - 1u) / GDN_C) return;
   const u32 first = row0 + c * GDN_C, mc = m - c * GDN_C < GDN_C ? m - c * GDN_C : GDN_C;
   uint8_t *ws = g.ws + (u64)at * g.sb, *wk = ws + (u64)hk * (3u * 64u * DK * 4u);
 
@@ -636,7 +638,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
   u32 row0;
   const u32 m = uniform(slot_rows(sl, b, row0)), base = uniform(gdn_base(sl, g.nc, b)), all = (m + GDN_C - 1u) / GDN_C, end = g.s0 + g.ns;
   row0 = uniform(row0);
-  if (!m || base >= end || base + all <= g.s0) return;
+  if (m <= g.few || !m || base >= end || base + all <= g.s0) return;
   const u32 h = g.tiled ? hk + vh * g.n_k : hk * g.G + vh;
   const u32 c0 = base < g.s0 ? g.s0 - base : 0u, c1 = base + all < end ? all : end - base;
   const u32 col = 32u * cb + 2u * n; // the lane's columns: this one in the products' first column tile, the next in the second
@@ -966,7 +968,10 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 }
 
 #define GDN_PREP(H, N, TY)                                                                                                             \
-  extern "C" __global__ __launch_bounds__(256) void amdc_gdn_prep_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_prep_body<TY, H##u>(sl, g); }
+  extern "C" __global__ __launch_bounds__(256) void amdc_gdn_prep_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { \
+    if (blockIdx.x < g.rec) gdn_rec_body<TY, H##u>(sl, g, g.few);                                                                       \
+    else gdn_prep_body<TY, H##u>(sl, g);                                                                                               \
+  }
 #define GDN_SCAN(H, N, TY, PAIR)                                                                                                       \
   extern "C" __global__ __launch_bounds__(512) void amdc_gdn_scan_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { gdn_scan_body<TY, H##u, PAIR>(sl, g); }
 #define GDN_PRES(H)                                                                                                                    \

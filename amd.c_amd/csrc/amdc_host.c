@@ -1936,6 +1936,13 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
   if (vs >= (1u << 23) || ys >= (1u << 23)) return fail(AMDC_EINVAL, "gdn_prefill: strides vs %u, ys %u (under 2^23)", vs, ys); /* 64 rows in a buffer of 2^31 bytes */
   const size_t need = amdc_gdn_prefill_ws(gdn, slots->n_seq, rows);
   if (!ws || !aligned16(ws) || ws_bytes < need) return fail(AMDC_EINVAL, "gdn_prefill: a workspace of %zu bytes (16-byte aligned, at least %zu)", ws ? ws_bytes : (size_t)0, need);
+  const u64 waves = (u64)d.n_seq * gdn->n_v * (gdn->dv / 16u);
+  const int few = waves < (1u << 25);
+  if (!cu && T <= AMDC_LIN_MAX_T && few) {
+    void *args[] = {&d, &g};
+    return launch(K_GDN_REC + (gdn->dk == 128u ? 3 : 0) + t, (unsigned)((waves + 3u) / 4u), 1, 0, stream, args);
+  }
+  if (cu && few) g.few = AMDC_LIN_MAX_T, g.rec = (u32)((waves + 3u) / 4u);
   g.sb = gdn_slot_bytes(gdn), g.nc = (T + AMDC_GDN_C - 1u) / AMDC_GDN_C;
   const u32 total = cu ? rows / AMDC_GDN_C + slots->n_seq : slots->n_seq * g.nc, most = gdn_slots(gdn, (u64)rows / AMDC_GDN_C + slots->n_seq);
   const u64 state = (u64)gdn->n_v * gdn->dk * gdn->dv;
@@ -1953,7 +1960,8 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
     float *swap = in;
     in = out, out = swap;
     void *args[] = {&d, &g};
-    if ((rc = launch(prep, g.ns * g.n_k, 1, 0, stream, args))) return rc;
+    if ((rc = launch(prep, g.rec + g.ns * g.n_k, 1, 0, stream, args))) return rc;
+    g.rec = 0;
     if ((rc = launch_nt(scan, g.groups >= 8u ? (g.groups + 7u) / 8u * 8u * per : g.groups * per, 1, 512u, 0, stream, args))) return rc;
   }
   return AMDC_OK;

@@ -165,6 +165,7 @@ typedef struct {
   uint64_t sb;  /* prompts: bytes of a chunk slot of the workspace */
   float scale, eps;
   uint32_t n_k, n_v, dv, G /* n_v / n_k */, tiled, qs, ks, vs, as, bs, ys;
+  uint32_t few, rec; /* prompts: sequences of up to few rows go token after token, in the first rec workgroups of amdc_gdn_prep */
   uint32_t nc, s0, ns, groups; /* prompts: chunks of a sequence (cu NULL), the launch's first chunk slot and their number, sequences times key heads */
 } amdc_gdn_args;
 #define AMDC_GDN_C 64u      /* tokens of a chunk */

@@ -241,3 +241,20 @@ def test_same_bits(dev):
         c.launch()
         y2, p2 = c.results()
         assert np.array_equal(y, y2) and np.array_equal(p, p2)
+
+
+@pytest.mark.parametrize("t", (F32, BF16))
+@pytest.mark.parametrize("new", [(1,) * 20 + (70, 16, 17, 1, 0, 200, 15), (16, 17), (130, 1), (1, 2, 3), (0, 0, 5)])
+def test_mixed(dev, new, t):
+    """Decode steps beside prompts: the sequences of a few rows go token after token, the others in chunks."""
+    Call(dev, 1170, new, 2, 6, 128, 64, True, t, ragged=True, room=3).upload().launch().check()
+
+
+def test_few_as_decode(dev):
+    """T rows of every sequence, few of them: decode's bits, packed or not."""
+    d = Both(dev, 1171, (5,) * 9, 2, 4, 64, 48).upload().launch()
+    y, p = d.results()
+    for ragged in (False, True):
+        c = Call(dev, 1171, (5,) * 9, 2, 4, 64, 48, ragged=ragged).upload().launch()
+        y2, p2 = c.results()
+        assert np.array_equal(y, y2) and np.array_equal(p, p2)
