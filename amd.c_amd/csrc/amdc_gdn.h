@@ -359,6 +359,29 @@ __device__ __forceinline__ u32 gdn_seq(const amdc_slots_dev &sl, u32 nc, u32 s) 
   return sl.cu ? find_seq(sl.n_seq, s, [&](u32 i) { return gdn_base(sl, nc, i); }) : s / nc;
 }
 
+// What amdc_gdn_scan has to know of packed sequences, 64 to a wave (block k) of amdc_gdn_prep's launch: of those with chunks in this launch, from the one
+// of its first slot on, the number, first row, rows (0: no chunk here) and first slot; of each 64 in the order of their chunks here, the
+// most first, so that those which take longest begin first. Without it each of the scan's
+// workgroups searches for its sequence: 90 sequences of up to 150 tokens, 32 heads of 128, 262 us, 294 without; 40 of up to 900, 16 heads of 64, 78 and 92.
+// A single sequence needs none (77 tokens: 22.0 us, 23.7 with it).
+__device__ __forceinline__ void gdn_table(const amdc_slots_dev &sl, const amdc_gdn_args &g, u32 k) {
+  const u32 lane = threadIdx.x, seqs = g.groups / g.n_k, n = seqs - 64u * k < 64u ? seqs - 64u * k : 64u;
+  if (lane >= 64u) return;
+  const u32 b = gdn_seq(sl, g.nc, g.s0) + 64u * k + lane, end = g.s0 + g.ns;
+  u32 row0 = 0u, m = 0u, base = 0u, len = 0u;
+  if (lane < n && b < sl.n_seq) {
+    m = slot_rows(sl, b, row0), base = gdn_base(sl, g.nc, b);
+    const u32 to = base + (m + GDN_C - 1u) / GDN_C, x = base > g.s0 ? base : g.s0, y = to < end ? to : end;
+    len = m > g.few && y > x ? y - x : 0u;
+  }
+  u32 rank = 0u;
+  for (u32 j = 0; j < n; j++) {
+    const u32 other = (u32)__builtin_amdgcn_readlane((int)len, (int)j);
+    rank += other > len || (other == len && j < lane);
+  }
+  if (lane < n) g.table[64u * k + rank] = (amdc_gdn_seq){b, row0, len ? m : 0u, base};
+}
+
 // The workspace: a chunk slot holds for every key head its keys, queries and transposed keys as operands (fragments of 1 KB: 16
 // rows, 32 of k, the lanes' 16 bytes in order; two parts each), then for every value head M and A (the 6 fragments that are not all above the
 // diagonal, in parts) and for each token the factors beta, 2^-8 beta e^G, e^G, 2^-4 e^(G_63 - G).
@@ -373,7 +396,7 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
   __shared__ double s_G[4][64];
   __shared__ float s_beta[4][64];
   const u32 tid = threadIdx.x, lane = tid & 63u, w = uniform(tid >> 6), n = lane & 15u, gr = lane >> 4;
-  const u32 wg = blockIdx.x - g.rec, at = wg / g.n_k, hk = wg - at * g.n_k, slot = g.s0 + at;
+  const u32 wg = blockIdx.x - g.rec - g.tabs, at = wg / g.n_k, hk = wg - at * g.n_k, slot = g.s0 + at;
   const u32 b = gdn_seq(sl, g.nc, slot);
   if (b >= sl.n_seq) return;
   u32 row0;
@@ -633,12 +656,19 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
     gi = (y / per) * 8u + x, in = y % per;
   } else gi = blockIdx.x / per, in = blockIdx.x % per;
   if (gi >= g.groups) return;
-  const u32 b = gdn_seq(sl, g.nc, g.s0) + gi / g.n_k, hk = gi % g.n_k, vh = in / nb, cb = in - vh * nb;
-  if (b >= sl.n_seq) return;
-  u32 row0;
-  const u32 m = uniform(slot_rows(sl, b, row0)), base = uniform(gdn_base(sl, g.nc, b)), all = (m + GDN_C - 1u) / GDN_C, end = g.s0 + g.ns;
-  row0 = uniform(row0);
-  if (m <= g.few || !m || base >= end || base + all <= g.s0) return;
+  const u32 i = gi / g.n_k, hk = gi % g.n_k, vh = in / nb, cb = in - vh * nb;
+  u32 b, row0, m, base;
+  if (g.packed) {
+    const amdc_gdn_seq e = g.table[i];
+    b = uniform(e.b), row0 = uniform(e.row0), m = uniform(e.m), base = uniform(e.base);
+  } else { // all of one length, or a single one
+    b = sl.cu ? 0u : g.s0 / g.nc + i;
+    if (b >= sl.n_seq) return;
+    m = uniform(slot_rows(sl, b, row0)), row0 = uniform(row0), base = uniform(gdn_base(sl, g.nc, b));
+    if (m <= g.few) return;
+  }
+  const u32 all = (m + GDN_C - 1u) / GDN_C, end = g.s0 + g.ns;
+  if (!m || base >= end || base + all <= g.s0) return;
   const u32 h = g.tiled ? hk + vh * g.n_k : hk * g.G + vh;
   const u32 c0 = base < g.s0 ? g.s0 - base : 0u, c1 = base + all < end ? all : end - base;
   const u32 col = 32u * cb + 2u * n; // the lane's columns: this one in the products' first column tile, the next in the second
@@ -970,6 +1000,7 @@ __device__ __forceinline__ void gdn_scan_body(const amdc_slots_dev &sl, const am
 #define GDN_PREP(H, N, TY)                                                                                                             \
   extern "C" __global__ __launch_bounds__(256) void amdc_gdn_prep_h##H##_##N(const amdc_slots_dev sl, const amdc_gdn_args g) { \
     if (blockIdx.x < g.rec) gdn_rec_body<TY, H##u>(sl, g, g.few);                                                                       \
+    else if (blockIdx.x < g.rec + g.tabs) gdn_table(sl, g, blockIdx.x - g.rec);                                                         \
     else gdn_prep_body<TY, H##u>(sl, g);                                                                                               \
   }
 #define GDN_SCAN(H, N, TY, PAIR)                                                                                                       \

@@ -1909,7 +1909,7 @@ int amdc_gdn_decode(const amdc_gdn *gdn, const amdc_slots *slots, float *states,
   return launch(K_GDN_REC + (gdn->dk == 128u ? 3 : 0) + t, (unsigned)((waves + 3u) / 4u), 1, 0, stream, args);
 }
 
-/* The workspace of a prompt: chunk slots of gdn_slot_bytes (amdc_gdn.h), and two states: of the sequence whose chunks go on from the launches before, and of
+/* The workspace of a prompt: chunk slots of gdn_slot_bytes (amdc_gdn.h), the table of packed sequences, and two states: of the sequence whose chunks go on from the launches before, and of
  * the one whose chunks go on in the next.
  * The slots of all sequences are numbered in their order, and a pair of launches takes gdn_slots of them, which bounds the workspace (12000 tokens of
  * 16 / 48 heads of 128 in launches of 48, 96, 160, 256, 512 MB: 771, 677, 638, 611, 582 us). */
@@ -1919,9 +1919,13 @@ static u32 gdn_slots(const amdc_gdn *g, u64 total) {
   return (u32)(total < most ? total : most);
 }
 
+/* of the sequences that may have chunks in these slots: one for each, and the one that goes on */
+static u64 gdn_table_bytes(u32 slots) { return ((u64)slots + 1u + 63u) / 64u * 64u * sizeof(amdc_gdn_seq); }
+
 size_t amdc_gdn_prefill_ws(const amdc_gdn *g, uint32_t n_seq, uint32_t rows) {
   if (!g || !g->n_k || !amdc_gdn_bytes(g->n_v, g->dk, g->dv, 1u) || g->n_v % g->n_k || !n_seq || n_seq > (1u << 20) || !rows || rows > (1u << 22)) return 0;
-  return (size_t)(gdn_slots(g, (u64)rows / AMDC_GDN_C + n_seq) * gdn_slot_bytes(g) + (u64)g->n_v * g->dk * g->dv * 8u + 128u);
+  const u32 slots = gdn_slots(g, (u64)rows / AMDC_GDN_C + n_seq);
+  return (size_t)(slots * gdn_slot_bytes(g) + gdn_table_bytes(slots) + (u64)g->n_v * g->dk * g->dv * 8u + 128u);
 }
 
 int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
@@ -1942,12 +1946,14 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
     void *args[] = {&d, &g};
     return launch(K_GDN_REC + (gdn->dk == 128u ? 3 : 0) + t, (unsigned)((waves + 3u) / 4u), 1, 0, stream, args);
   }
+  g.packed = cu && d.n_seq > 1u;
   if (cu && few) g.few = AMDC_LIN_MAX_T, g.rec = (u32)((waves + 3u) / 4u);
   g.sb = gdn_slot_bytes(gdn), g.nc = (T + AMDC_GDN_C - 1u) / AMDC_GDN_C;
   const u32 total = cu ? rows / AMDC_GDN_C + slots->n_seq : slots->n_seq * g.nc, most = gdn_slots(gdn, (u64)rows / AMDC_GDN_C + slots->n_seq);
   const u64 state = (u64)gdn->n_v * gdn->dk * gdn->dv;
   float *in = (float *)(((uintptr_t)ws + 127u) & ~(uintptr_t)127u), *out = in + state; /* slots begin with a line */
-  g.ws = (uint8_t *)(out + state);
+  g.table = (amdc_gdn_seq *)(out + state);
+  g.ws = (uint8_t *)g.table + gdn_table_bytes(most);
   /* two 16-bit values side by side in rows of v and y are aligned to both */
   const int pair = (((uintptr_t)v | (uintptr_t)y | (rows > 1u ? 2u * (vs | ys) : 0u)) & 3u) == 0;
   const int prep = K_GDN_PREP + (gdn->dk == 128u ? 3 : 0) + t, scan = K_GDN_SCAN + (gdn->dk == 128u ? 5 : 0) + (t == AMDC_TYPE_F32 || pair ? t : t + 2);
@@ -1955,12 +1961,12 @@ int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states
     g.ns = total - g.s0 < most ? total - g.s0 : most;
     /* the sequences with chunks in these slots: one for each slot, and the one that goes on */
     const u32 seqs = slots->n_seq < g.ns + 1u ? slots->n_seq : g.ns + 1u, per = g.G * ((g.dv + 31u) / 32u);
-    g.groups = seqs * g.n_k;
+    g.groups = seqs * g.n_k, g.tabs = g.packed ? (seqs + 63u) / 64u : 0u;
     g.carry_in = in, g.carry_out = out;
     float *swap = in;
     in = out, out = swap;
     void *args[] = {&d, &g};
-    if ((rc = launch(prep, g.rec + g.ns * g.n_k, 1, 0, stream, args))) return rc;
+    if ((rc = launch(prep, g.rec + g.tabs + g.ns * g.n_k, 1, 0, stream, args))) return rc;
     g.rec = 0;
     if ((rc = launch_nt(scan, g.groups >= 8u ? (g.groups + 7u) / 8u * 8u * per : g.groups * per, 1, 512u, 0, stream, args))) return rc;
   }

@@ -156,6 +156,9 @@ typedef struct {
   uint32_t ch, xs, ys, cb /* workgroups to a row */, upb /* units to a sequence (cu NULL) */, act;
 } amdc_conv_args;
 typedef struct {
+  uint32_t b, row0, m, base;
+} amdc_gdn_seq; /* a packed sequence of a prompt's launches: its number, first row, rows and first chunk slot */
+typedef struct {
   float *s;
   const void *q, *k, *v;
   const float *a, *b, *A, *dt;
@@ -165,6 +168,8 @@ typedef struct {
   uint64_t sb;  /* prompts: bytes of a chunk slot of the workspace */
   float scale, eps;
   uint32_t n_k, n_v, dv, G /* n_v / n_k */, tiled, qs, ks, vs, as, bs, ys;
+  amdc_gdn_seq *table;
+  uint32_t packed, tabs; /* prompts: whether there is a table, and the workgroups of amdc_gdn_prep that write it */
   uint32_t few, rec; /* prompts: sequences of up to few rows go token after token, in the first rec workgroups of amdc_gdn_prep */
   uint32_t nc, s0, ns, groups; /* prompts: chunks of a sequence (cu NULL), the launch's first chunk slot and their number, sequences times key heads */
 } amdc_gdn_args;
