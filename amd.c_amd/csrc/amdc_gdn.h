@@ -213,8 +213,9 @@ __device__ __forceinline__ float sum16(float v) {
 // With k and q of norm 1 (their factors rk, rq) and the state as it is before the token's decay e,
 //   u = rate (v - e rk k S),  S' = e S + rk k^T u,  y = rq q S' = rq (e q S + rk (q.k) u),
 // so that k S, q S, k.k, q.q and k.q go through one reduction a token. Reading and writing the states bounds it for batches: 96
-// sequences of 32 heads of 128 x 128, 405 MB, in 84 us (4.8 TB/s, a copy's rate here); 8 of 48 heads and 5 tokens, a state kept after each,
-// 154 MB in 35 us. A single sequence waits for two dependent loads (its slot, the state): 4.6 us.
+// sequences of 32 heads of 128 x 128, 405 MB, in 81 us (5.0 TB/s, a copy's rate here); 8 of 48 heads and 5 tokens, a state kept after each,
+// 154 MB in 34 us. A single sequence waits for two dependent loads (its slot, the state): 4.3 us, and 0.8 a token more, which a wave's
+// instructions take. Rows and gates are loaded ahead of the state, which waits for its slot: behind it, 84, 35 and 4.6 us.
 template <int TY, u32 DK>
 __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amdc_gdn_args &g, u32 most) {
   constexpr u32 NI = DK / 16u;
@@ -226,12 +227,7 @@ __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amd
   const u32 m = uniform(slot_rows(sl, b, row0));
   if (!m || m > most) return;
   const int f = sl.from[b];
-  bool bad;
-  const bool have = slot_ok(sl, f, bad);
-  const u64 mat = (u64)DK * g.dv, part = (u64)h * mat + (u64)c * DK + 16u * r + 4u * c4;
-  v4f S[NI];
-#pragma unroll
-  for (u32 i = 0; i < NI; i++) S[i] = have ? *(const v4f *)(g.s + (u64)(u32)f * g.n_v * mat + part + 256u * i) : splat(bad ? nan_() : 0.0f);
+  const GdnGates gates(g, row0 + (lane < m ? lane : m - 1u), h); // a token to a lane: all of them are loaded beside the state
   float k[NI], q[NI];
   v4f v;
   const auto load = [&](u32 t) {
@@ -241,10 +237,20 @@ __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amd
     v = ld4<TY>(g.v, row * g.vs + h * g.dv + c + 4u * c4);
   };
   load(0u);
-  float decay = 0.0f, rate = 0.0f;
+  bool bad;
+  const bool have = slot_ok(sl, f, bad);
+  const u64 mat = (u64)DK * g.dv, part = (u64)h * mat + (u64)c * DK + 16u * r + 4u * c4;
+  v4f S[NI];
+#pragma unroll
+  for (u32 i = 0; i < NI; i++) S[i] = splat(bad ? nan_() : 0.0f);
+  if (have)
+#pragma unroll
+    for (u32 i = 0; i < NI; i++) S[i] = *(const v4f *)(g.s + (u64)(u32)f * g.n_v * mat + part + 256u * i);
+  float decay, rate;
+  gates.get(decay, rate);
+  decay = __builtin_expf(decay);
   for (u32 t = 0; t < m; t++) {
-    if (!(t & 63u)) GdnGates(g, row0 + (t + lane < m ? t + lane : m - 1u), h).get(decay, rate), decay = __builtin_expf(decay); // those of 64 tokens
-    const float e = lane_of(decay, t & 63u), be = lane_of(rate, t & 63u);
+    const float e = lane_of(decay, t), be = lane_of(rate, t);
     float kk = 0.0f, qq = 0.0f, kq = 0.0f;
     v4f kS = splat(0.0f), qS = splat(0.0f), vt = v;
     float kt[NI];
