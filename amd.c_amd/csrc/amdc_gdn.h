@@ -90,11 +90,11 @@ __device__ __forceinline__ float sigmoid_fast(float v) { return __builtin_amdgcn
 
 // Reading and writing bound it. A thread has four channels (one, where their number is no multiple of four: _odd) of a unit of up to
 // AMDC_CONV_ROWS rows of a sequence, which are all in flight at once, with the W - 1 inputs before them. The unit of a sequence's first
-// rows reads the state and, after that, writes it: from x where the sequence has rows enough, and else from what it has read, so that a
+// rows reads the state and, after that, writes it: the window behind its rows, or from x where the sequence has more, so that a
 // slot may be read and written by the same call; with `each` one unit has all rows of a sequence, eight after eight, for the same
 // reason. Workgroups of one wave. 8192 channels, 9 prompts of 1100 tokens, into bf16: units of 8 rows 85 us (5.7 TB/s), of 4 90 us, of 32 with 8
 // rows in flight 105 us; 256 threads 87 us; units that follow each other on one XCD 87 us (the rows that two units read come from
-// the last-level cache). One token of 10240 channels: 3.2 us.
+// the last-level cache). One token of 10240 channels: 2.8 us.
 template <u32 W, int TY, u32 C>
 __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_conv_args &a) {
   const u32 ct = blockIdx.x % a.cb, u = blockIdx.x / a.cb, c = C * (ct * blockDim.x + threadIdx.x);
@@ -112,7 +112,14 @@ __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_c
   if (c >= a.ch) return;
   const auto row = [](const float *p, u64 i) { return ldc<0, C>(p, i); };
   const float *x = a.x + c + (u64)row0 * a.xs;
-  v4f w[W], bias = splat(0.0f), win[W - 1u];
+  const bool first_rows = t0 == 0u;
+  v4f w[W], bias = splat(0.0f), win[W - 1u], in[AMDC_CONV_ROWS];
+  const auto rows = [&](u32 t) {
+#pragma unroll
+    for (u32 i = 0; i < AMDC_CONV_ROWS; i++) in[i] = row(x, (u64)(t + i < t1 ? t + i : t1 - 1u) * a.xs);
+  };
+  const int f = sl.from[b], o = sl.to[keep ? row0 : b]; // no branch around them: all these loads are in flight together
+  rows(t0);
 #pragma unroll
   for (u32 j = 0; j < W; j++) w[j] = splat(0.0f);
 #pragma unroll
@@ -120,37 +127,25 @@ __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_c
 #pragma unroll
     for (u32 j = 0; j < W; j++) w[j][e] = a.w[(u64)(c + e) * W + j];
   if (a.bias) bias = row(a.bias, c);
-  if (t0 == 0u) {
-    const int f = sl.from[b];
-    bool bad;
+  bool bad = false;
+  if (first_rows) {
     const bool have = slot_ok(sl, f, bad);
 #pragma unroll
-    for (u32 j = 0; j < W - 1u; j++) win[j] = have ? row(a.state, ((u64)(u32)f * (W - 1u) + j) * a.ch + c) : splat(bad ? nan_() : 0.0f);
-    if (!keep) {
-      const int o = sl.to[b];
-      bool worse;
-      if (slot_ok(sl, o, worse) && !bad) {
-        v4f s[W - 1u]; // all of it, before the first is written
+    for (u32 j = 0; j < W - 1u; j++) win[j] = splat(bad ? nan_() : 0.0f);
+    if (have)
 #pragma unroll
-        for (u32 j = 0; j < W - 1u; j++) {
-          const u32 at = m + j; // of the W - 1 old inputs and the m new ones, those from m on
-          v4f old = win[W - 2u];
-#pragma unroll
-          for (u32 i = 0; i + 1u < W; i++) old = at == i ? win[i] : old;
-          s[j] = at < W - 1u ? old : row(x, (u64)(at - (W - 1u)) * a.xs);
-        }
-#pragma unroll
-        for (u32 j = 0; j < W - 1u; j++) stc<0, C>(a.state, ((u64)(u32)o * (W - 1u) + j) * a.ch + c, s[j]);
-      }
-    }
+      for (u32 j = 0; j < W - 1u; j++) win[j] = row(a.state, ((u64)(u32)f * (W - 1u) + j) * a.ch + c);
   } else {
 #pragma unroll
     for (u32 j = 0; j < W - 1u; j++) win[j] = row(x, (u64)(t0 + j - (W - 1u)) * a.xs);
   }
-  for (u32 t = t0; t < t1; t += AMDC_CONV_ROWS) {
-    v4f in[AMDC_CONV_ROWS];
+  const auto put_state = [&](int slot) { // the window
+    bool worse;
+    if (slot_ok(sl, slot, worse) && !bad)
 #pragma unroll
-    for (u32 i = 0; i < AMDC_CONV_ROWS; i++) in[i] = row(x, (u64)(t + i < t1 ? t + i : t1 - 1u) * a.xs);
+      for (u32 j = 0; j < W - 1u; j++) stc<0, C>(a.state, ((u64)(u32)slot * (W - 1u) + j) * a.ch + c, win[j]);
+  };
+  for (u32 t = t0;;) {
 #pragma unroll
     for (u32 i = 0; i < AMDC_CONV_ROWS; i++) {
       if (t + i >= t1) break;
@@ -165,15 +160,17 @@ __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_c
 #pragma unroll
         for (u32 e = 0; e < C; e++) s[e] *= sigmoid_fast(s[e]);
       stc<TY, C>(a.y, (u64)(row0 + t + i) * a.ys + c, s);
-      if (keep) {
-        const int o = sl.to[row0 + t + i];
-        bool bad;
-        if (slot_ok(sl, o, bad) && !(sl.from[b] < -1 || (sl.from[b] >= 0 && (u32)sl.from[b] >= sl.n_slots)))
-#pragma unroll
-          for (u32 j = 0; j < W - 1u; j++) stc<0, C>(a.state, ((u64)(u32)o * (W - 1u) + j) * a.ch + c, win[j]);
-      }
+      if (keep) put_state(sl.to[row0 + t + i]);
     }
+    t += AMDC_CONV_ROWS;
+    if (t >= t1) break;
+    rows(t);
   }
+  if (!first_rows || keep) return;
+  if (t1 < m) // the last rows are other units'
+#pragma unroll
+    for (u32 j = 0; j < W - 1u; j++) win[j] = row(x, (u64)(m + j - (W - 1u)) * a.xs);
+  put_state(o);
 }
 
 #define CONV(W, N, TY, C)                                                                                                          \
