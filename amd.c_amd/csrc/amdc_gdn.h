@@ -296,11 +296,11 @@ GDN_RECS(64) GDN_RECS(128)
 // Two launches: amdc_gdn_prep computes what does not depend on the state, for all chunks at once: M = (I + L)^-1 and the weights
 // A_ij = e^(G_i - G_j) q_i.k_j for each value head, and the normed keys and queries as operands; amdc_gdn_scan takes the chunks of a sequence
 // one after the other, 32 columns of a head's state to a workgroup. Of packed prompts the sequences of up to AMDC_LIN_MAX_T rows (decode steps
-// beside prompts) go token after token, in workgroups of amdc_gdn_prep's launch ahead of its own: 96 of one token, 48 heads of 128, in 152 us, as chunks 522; 32 of 5 tokens 80
-// and 171, of 16 162 and 168. A prompt of 12000 tokens, 16 heads of keys and 48 of values of 128: 0.58 ms, 0.14 of
-// it amdc_gdn_prep's, which writes 0.51 GB of operands (4.4 TB/s with what it reads); token after token it takes 11.1 ms. Prompts go through
-// the workspace in parts of AMDC_GDN_WS bytes: 48 MB 0.77 ms, 96 MB 0.68, 160 MB 0.64, 256 MB 0.61, 512 MB 0.58 (a launch of the scan begins and
-// ends with all its workgroups).
+// beside prompts) go token after token, in workgroups of amdc_gdn_prep's launch ahead of its own: 96 of one token, 48 heads of 128, in 152 us,
+// as chunks 522; 32 of 5 tokens 80 and 171, of 16 162 and 168. A prompt of 12000 tokens, 16 heads of keys and 48 of values of 128: 0.58 ms,
+// 0.14 of it amdc_gdn_prep's, which writes 0.51 GB of operands (4.4 TB/s with what it reads); token after token it takes 11.1 ms. Prompts go
+// through the workspace in parts of AMDC_GDN_WS bytes: 48 MB 0.77 ms, 96 MB 0.68, 160 MB 0.64, 256 MB 0.61, 512 MB 0.58 (a launch of the scan
+// begins and ends with all its workgroups).
 //
 // Exponents are of differences that are at most 0, and those are taken in 64 bits: after a strong decay the sums are large and
 // their differences small. |M_ij|, |A_ij| <= 1: (I - beta k^T k) shrinks whatever it multiplies, for beta <= 1 and |k| <= 1.
