@@ -1889,6 +1889,7 @@ static int check_gdn(const char *op, const amdc_gdn *g, const amdc_slots *sl, fl
   if (y == q || y == k || y == v || y == a || y == b) return fail(AMDC_EINVAL, "%s: y cannot be q, k, v, a or b", op);
   if (rows > 1u && (qs < wk || ks < wk || vs < wv || ys < wv || as < g->n_v || bs < g->n_v))
     return fail(AMDC_EINVAL, "%s: strides qs %u, ks %u, vs %u, as %u, bs %u, ys %u under a row's values (%u, %u, %u)", op, qs, ks, vs, as, bs, ys, wk, wv, g->n_v);
+  if (rows == 1u) vs = ys = wv; /* any strides were taken, and the chunked form ends its buffers behind whole rows */
   *d = (amdc_gdn_args){.s = states, .q = q, .k = k, .v = v, .a = a, .b = b, .A = g->A, .dt = g->dt, .y = y, .scale = g->scale, .eps = g->eps, .n_k = g->n_k, .n_v = g->n_v, .dv = g->dv,
                        .G = g->n_v / g->n_k, .tiled = g->order == AMDC_HEADS_TILED, .qs = qs, .ks = ks, .vs = vs, .as = as, .bs = bs, .ys = ys};
   return AMDC_OK;
