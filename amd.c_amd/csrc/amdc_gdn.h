@@ -127,11 +127,12 @@ __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_c
 #pragma unroll
     for (u32 j = 0; j < W; j++) w[j][e] = a.w[(u64)(c + e) * W + j];
   if (a.bias) bias = row(a.bias, c);
-  bool bad = false;
+  bool bad;
+  const bool have = slot_ok(sl, f, bad);
+  if (bad) bias = splat(nan_()); // all rows, also those that see nothing of the state
   if (first_rows) {
-    const bool have = slot_ok(sl, f, bad);
 #pragma unroll
-    for (u32 j = 0; j < W - 1u; j++) win[j] = splat(bad ? nan_() : 0.0f);
+    for (u32 j = 0; j < W - 1u; j++) win[j] = splat(0.0f);
     if (have)
 #pragma unroll
       for (u32 j = 0; j < W - 1u; j++) win[j] = row(a.state, ((u64)(u32)f * (W - 1u) + j) * a.ch + c);
