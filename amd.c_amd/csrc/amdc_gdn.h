@@ -75,6 +75,12 @@ __device__ __forceinline__ u32 slot_rows(const amdc_slots_dev &sl, u32 b, u32 &r
   row0 = (u32)c0;
   return (u32)(c1 - c0);
 }
+// Sequence i's rows, for the report alone: where cu decreases, the searches below may come upon no row of a sequence that is at fault. `part`: 0
+// for one workgroup of each i.
+__device__ __forceinline__ void check_rows(const amdc_slots_dev &sl, u32 i, u32 part) {
+  u32 row0;
+  if (part == 0u && i < sl.n_seq) slot_rows(sl, i, row0);
+}
 // Whether a slot is to be read or written: -1 is none, any other outside the pool is reported (bad).
 __device__ __forceinline__ bool slot_ok(const amdc_slots_dev &sl, int s, bool &bad) {
   bad = s < -1 || (s >= 0 && (u32)s >= sl.n_slots);
@@ -100,6 +106,7 @@ __device__ __forceinline__ void conv_body(const amdc_slots_dev &sl, const amdc_c
   const u32 ct = blockIdx.x % a.cb, u = blockIdx.x / a.cb, c = C * (ct * blockDim.x + threadIdx.x);
   u32 b, first;
   if (sl.cu) {
+    check_rows(sl, u, ct); // a unit for each sequence at least
     const auto base = [&](u32 i) { const int s = sl.cu[i]; return (s < 0 ? 0u : (u32)s) / AMDC_CONV_ROWS + i; };
     b = find_seq(sl.n_seq, u, base), first = base(b);
     if (first > u) return;
@@ -401,6 +408,7 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
   __shared__ float s_beta[4][64];
   const u32 tid = threadIdx.x, lane = tid & 63u, w = uniform(tid >> 6), n = lane & 15u, gr = lane >> 4;
   const u32 wg = blockIdx.x - g.rec - g.tabs, at = wg / g.n_k, hk = wg - at * g.n_k, slot = g.s0 + at;
+  if (sl.cu && !g.few) check_rows(sl, slot, hk); // else the waves that go token after token have
   const u32 b = gdn_seq(sl, g.nc, slot);
   if (b >= sl.n_seq) return;
   u32 row0;

@@ -85,3 +85,23 @@ def test_one_row(dev, strides):
 def test_rows(dev):
     """Sequences of one, a few and more than a chunk's rows, far apart: in different launches."""
     case(dev, 1402, {0: 1, 7: 66, 700: 16, 2047: 3}, {7: 0, 2047: 1}, {7: 0, 2047: 1}, [2, 1000])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("at", (None, 10, 500, 1001, 1500, 2000))
+def test_rows_outside(dev, at):
+    """A sequence whose rows decrease is reported, wherever it stands: its chunks' numbers decrease too, by more than a launch takes."""
+    rows = 1920
+    L = Layer(np.random.default_rng(1403), 1, N_K, N_V, DK, DV).upload(dev)
+    s = Seqs(dev, 1403, [0] * N_SEQ, start=[-1] * N_SEQ, to=[-1] * N_SEQ, ragged=True)
+    s.cu[1:] = rows
+    s.cu[at or N_SEQ:N_SEQ] = 0
+    s.upload()
+    x, ab, y, dS = dev.DevBuf(4 * rows * W), dev.DevBuf(4 * rows * 2 * N_V), dev.DevBuf(4 * rows * N_V * DV), dev.DevBuf(4)
+    x.fill(0), ab.fill(0)
+    ws = dev.DevBuf(dev.gdn_prefill_ws(L.gdn, N_SEQ, rows))
+    dev.gdn_prefill(L.gdn, s.slots, dS, x.ptr, x.ptr + 4 * DK, x.ptr + 8 * DK, ab.ptr, ab.ptr + 4 * N_V, y, F32, rows, W, W, W, 2 * N_V, 2 * N_V, N_V * DV, ws, ws.nbytes, cu=s.dcu)
+    if at:
+        with pytest.raises(dev.AmdcError, match="rows outside"):
+            dev.kv_check()
+    dev.kv_check()
