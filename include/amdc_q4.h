@@ -398,14 +398,17 @@ int amdc_conv(const amdc_slots *slots, float *states, const float *x, const floa
  * with rows q, k of the key head and v of the value head, and the f32 rows a and b (n_v values each) of the token,
  *   k^ = k / sqrt(k.k + eps),  q^ = scale q / sqrt(q.q + eps),  beta = 1 / (1 + exp(-b[h])),
  *   g = min(0, A[h] softplus(a[h] + dt[h])),
- *   S <- exp(g) S,  u = beta (v - k^ S),  S <- S + k^T u,  y = q^ S
+ *   S <- exp(g) S,  u = beta (v - k^ S),  S <- S + (k^ transposed) u,  y = q^ S
  * where S is the head's dk x dv matrix of the state, f32, [n_slots][n_v][dv / 16][dk][16] in the pool: row i, column 16 e + c at [e][i][c]
  * (amdc_gdn_bytes()). A and dt: n_v device floats (A is negative: -exp of what is learned). eps is above 0. All sums, states
  * and gates are f32 or more, whatever the rows' type t (that of q, k, v and y): y is rounded once. Rows are qs, ks, vs, as, bs and ys
  * values apart; y is none of the inputs. A q, k, v, a or b that is not finite makes NaN or infinite what the formula makes of it (a value its
- * column alone); prompts: the rows of up to 63 tokens before it too. Token after token a row is off by roundings of its own size; prompts
- * are worked in chunks of 64 tokens, and a column of a chunk is off by up to about 2^-26 of its largest |v| and |S| in that chunk and the
- * one before, however small the row itself. */
+ * column alone); prompts: the rows of up to 63 tokens before it too.
+ * Errors: token after token they are f32's, of the sizes of the terms. Prompts are worked in chunks of 64 tokens with products of 22-bit operands and
+ * f32 sums: a row of y is off by |scale| times, and the state by, a part of the column's largest |v| and |S| in that chunk and the one before, however
+ * small the row itself: a root mean square of up to 2^-23, and 2^-20 at most, of random rows, which is what a recurrence in f32 has; errors go on
+ * with the state and shrink with its decay. To that comes 2^-125, which tells below |v| and |S| of about 2^-100. Sums stay in f32's range for norms of
+ * q and k rows up to 2^40 and norms of v rows and of columns of S up to 2^80. */
 enum { AMDC_HEADS_GROUPED = 0, AMDC_HEADS_TILED = 1 };
 typedef struct {
   uint32_t n_k, n_v, dk, dv;
