@@ -307,8 +307,9 @@ GDN_RECS(64) GDN_RECS(128)
 // beside prompts) go token after token, in workgroups of amdc_gdn_prep's launch ahead of its own: 96 of one token, 48 heads of 128, in 152 us,
 // as chunks 522; 32 of 5 tokens 80 and 171, of 16 162 and 168. A prompt of 12000 tokens, 16 heads of keys and 48 of values of 128: 0.58 ms,
 // 0.14 of it amdc_gdn_prep's, which writes 0.51 GB of operands (4.4 TB/s with what it reads); token after token it takes 11.1 ms. Prompts go
-// through the workspace in parts of AMDC_GDN_WS bytes: 48 MB 0.77 ms, 96 MB 0.68, 160 MB 0.64, 256 MB 0.61, 512 MB 0.58 (a launch of the scan
-// begins and ends with all its workgroups).
+// through the workspace in parts of AMDC_GDN_WS bytes (a launch of the scan begins and ends with all its workgroups): 12000, 24000 and 48000 tokens in parts of
+// 64 MB 0.68, 1.35, 2.70 ms, 128 MB 0.63, 1.25, 2.50, 256 MB 0.61, 1.21, 2.43, 512 MB 0.58, 1.15, 2.32, 1 GB 0.58, 1.13, 2.28; 4 of 6000 1.34, 1.23, 1.20, 1.22,
+// 1.06 (192 workgroups a sequence on 256 CUs: two sequences in a part are two rounds, four in one are three).
 //
 // Exponents are of differences that are at most 0, and those are taken in 64 bits: after a strong decay the sums are large and
 // their differences small. |M_ij|, |A_ij| <= 1: (I - beta k^T k) shrinks whatever it multiplies, for beta <= 1 and |k| <= 1.

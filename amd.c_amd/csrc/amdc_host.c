@@ -1912,8 +1912,8 @@ int amdc_gdn_decode(const amdc_gdn *gdn, const amdc_slots *slots, float *states,
 
 /* The workspace of a prompt: chunk slots of gdn_slot_bytes (amdc_gdn.h), the table of packed sequences, and two states: of the sequence whose chunks go on from the launches before, and of
  * the one whose chunks go on in the next.
- * The slots of all sequences are numbered in their order, and a pair of launches takes gdn_slots of them, which bounds the workspace (12000 tokens of
- * 16 / 48 heads of 128 in launches of 48, 96, 160, 256, 512 MB: 771, 677, 638, 611, 582 us). */
+ * The slots of all sequences are numbered in their order, and a pair of launches takes gdn_slots of them, which bounds the workspace (measured at
+ * amdc_gdn.h's chunked form). */
 static u64 gdn_slot_bytes(const amdc_gdn *g) { return (u64)g->n_k * 3u * AMDC_GDN_C * g->dk * 4u + (u64)g->n_v * AMDC_GDN_VB; }
 static u32 gdn_slots(const amdc_gdn *g, u64 total) {
   const u64 most = AMDC_GDN_WS / gdn_slot_bytes(g) + 1u;

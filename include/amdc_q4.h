@@ -420,9 +420,11 @@ size_t amdc_gdn_bytes(uint32_t n_v, uint32_t dk, uint32_t dv, uint32_t n_slots);
 /* T new tokens of every sequence, at most 16: decode, or a verify step (each). No workspace; can be captured. */
 int amdc_gdn_decode(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
                     uint32_t T, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t as, uint32_t bs, uint32_t ys, int each, void *stream);
-/* Any numbers of new tokens: prompts, chunks of them, and among them sequences of a few tokens (decode steps), packed (cu) or T each. vs and ys are under 2^23. ws: amdc_gdn_prefill_ws(gdn, n_seq, rows) bytes of
- * device memory (rows = T with cu, n_seq T without; longer prompts go through it part by part, so that it is hardly over half a GB), 16-byte aligned, of any content; calls that share it must not overlap on the
- * device. Nothing is allocated: every call can be captured. */
+/* Any numbers of new tokens: prompts, chunks of them, and among them sequences of a few tokens (decode steps), packed (cu) or T each. vs and ys are under 2^23.
+ * ws: amdc_gdn_prefill_ws(gdn, n_seq, rows) bytes of device memory (rows = T with cu, n_seq T without), 16-byte aligned, of any content; calls that share it
+ * must not overlap on the device. It holds a chunk's operands (n_k 768 dk + n_v 25600 bytes) for every 64 rows and one more for every sequence, of few rows
+ * too, up to 512 MB and one of them (what is longer goes through it part by part), two states, and 16 bytes a chunk. What is enough for some numbers of
+ * sequences and rows is for all smaller ones. Nothing is allocated: every call can be captured. */
 size_t amdc_gdn_prefill_ws(const amdc_gdn *gdn, uint32_t n_seq, uint32_t rows);
 int amdc_gdn_prefill(const amdc_gdn *gdn, const amdc_slots *slots, float *states, const void *q, const void *k, const void *v, const float *a, const float *b, void *y, int t,
                      uint32_t T, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t as, uint32_t bs, uint32_t ys, const int32_t *cu, void *ws, size_t ws_bytes, void *stream);
