@@ -218,8 +218,8 @@ __device__ __forceinline__ float sum16(float v) {
 // With k and q of norm 1 (their factors rk, rq) and the state as it is before the token's decay e,
 //   u = rate (v - e rk k S),  S' = e S + rk k^T u,  y = rq q S' = rq (e q S + rk (q.k) u),
 // so that k S, q S, k.k, q.q and k.q go through one reduction a token. Reading and writing the states bounds it for batches: 96
-// sequences of 32 heads of 128 x 128, 405 MB, in 81 us (5.0 TB/s, a copy's rate here); 8 of 48 heads and 5 tokens, a state kept after each,
-// 154 MB in 34 us. A single sequence waits for two dependent loads (its slot, the state): 4.3 us, and 0.8 a token more, which a wave's
+// sequences of 32 heads of 128 x 128, 405 MB, in 80 us (5.0 TB/s, a copy's rate here); 8 of 48 heads and 5 tokens, a state kept after each,
+// 154 MB in 33 us. A single sequence waits for two dependent loads (its slot, the state): 4.3 us, and 0.8 a token more, which a wave's
 // instructions take. Rows and gates are loaded ahead of the state, which waits for its slot: behind it, 84, 35 and 4.6 us.
 template <int TY, u32 DK>
 __device__ __forceinline__ void gdn_rec_body(const amdc_slots_dev &sl, const amdc_gdn_args &g, u32 most) {
@@ -372,8 +372,8 @@ __device__ __forceinline__ u32 gdn_seq(const amdc_slots_dev &sl, u32 nc, u32 s) 
 }
 
 // What amdc_gdn_scan has to know of packed sequences, 64 to a wave (block k) of amdc_gdn_prep's launch: of those with chunks in this launch, from the one
-// of its first slot on, the number, first row, rows (0: no chunk here) and first slot; of each 64 in the order of their chunks here, the
-// most first, so that those which take longest begin first. Without it each of the scan's
+// of its first slot on, the number, first row, rows (0: no chunk here) and first slot; of each 64 of them in the order of their chunks here, the
+// most first, so that of these those which take longest begin first. Without it each of the scan's
 // workgroups searches for its sequence: 90 sequences of up to 150 tokens, 32 heads of 128, 262 us, 294 without; 40 of up to 900, 16 heads of 64, 78 and 92.
 // A single sequence needs none (77 tokens: 22.0 us, 23.7 with it).
 __device__ __forceinline__ void gdn_table(const amdc_slots_dev &sl, const amdc_gdn_args &g, u32 k) {
@@ -650,7 +650,7 @@ __device__ __forceinline__ void gdn_prep_body(const amdc_slots_dev &sl, const am
 // A column's R, U and its next S are under 12 max |S| + 65 max |beta v| of the chunk (a token adds at most beta |v| to the column's norm, and the rest of
 // its step shrinks it): the power of two of this bound brings them into f16's range, and as they share it U needs no scaling. max |S| is not waited for:
 // what it was a chunk before bounds it, by the same rule. S is kept as the products with K^T give it: they add to it.
-// A chunk takes 2.3 to 2.5 us, waits of many kinds: matrix units 28 % busy, vector units 37 %, the LDS 35 %; without its products it
+// A chunk takes 2.3 to 2.5 us, waits of many kinds: matrix units 27 % busy, vector units 36 %, the LDS 34 %; without its products it
 // would take 92 % of that, without its reads of the workspace 93 %. 16 columns a workgroup would read the workspace twice as
 // often, 64 leave half of the CUs idle.
 // PAIR: two values side by side in v and y are aligned to both (32-bit ones need not be).
@@ -1026,7 +1026,8 @@ GDN_PRES(64) GDN_PRES(128)
 // ------------------------------------------------------------------ the norms
 
 // y = x s w gate(z), s = 1 / sqrt(sum x^2 / hd + eps) over a head, and its Q8 copy. Reading and writing bound it. Four values a lane, hd / 4 lanes a
-// head. Grid (ceil(n / 1024), T). 4097 rows of 32 heads of 128 from bf16: 168 MB in 31 us (5.4 TB/s); one row of 48 heads 2.4 us.
+// head. Grid (ceil(n / 1024), T). 4097 rows of 32 heads of 128 from bf16: 168 MB in 31 us (5.4 TB/s); one row of 48 heads 2.4 us. With the Q8 copy
+// alone, as the next matrix takes it: 122 MB in 27.6 us (4.4 TB/s; from f32 155 MB in 29.6, 5.2 TB/s), one row 2.5 us.
 template <int TY>
 __device__ __forceinline__ void norm_gate_body(const amdc_norm_args &a) {
   const u32 i0 = 4u * (blockIdx.x * NT + threadIdx.x), n = a.n;
@@ -1066,9 +1067,9 @@ __device__ __forceinline__ float row_scale(const v4f (&x)[NV], float rn, float e
 }
 
 // h = res + scale (x s1 w1, or x itself), y = h s2 w2 and its Q8 copy: a row to a workgroup, which keeps it in its registers between the two
-// norms. h may be res: a thread reads and writes the same places. Grid (1, T). Reading and writing bound it: 3001 rows of 4096, 197 MB, in 41 us
-// (4.8 TB/s, a copy's rate); one row of 5120 3.5 us. 256 threads of more values each: 45 and 4.8 us (1024 rows of 4096, which the caches
-// hold, 12.3 against 12.6).
+// norms. h may be res: a thread reads and writes the same places. Grid (1, T). Reading and writing bound it: 3001 rows of 4096, 197 MB, in 40 us
+// (4.9 TB/s, a copy's rate); one row of 5120 3.4 us. With the Q8 copy alone, as the next matrix takes it: 163 MB in 37 us (4.4 TB/s), one row
+// 4.5 us. 256 threads of more values each: 45 and 4.8 us, to y (1024 rows of 4096, which the caches hold, 12.3 against 12.6).
 template <u32 NV>
 __device__ __forceinline__ void norm_res_body(const amdc_norm_args &a) {
   __shared__ float part[2][16];
